@@ -319,6 +319,102 @@ NSC_API nsc_status nsc_metropolis_fwd_noalloc(const void* w_half, int w_dtype,
                                       int use_box, double eps, void* Wx,
                                       void* d_hat, void* stream);
 
+/* ---------------------------------------------------------------------
+ * Token attention: operators of the transformer layers that run beside the
+ * shift-window denoisers.  No counterpart in the reference.
+ *
+ * qk_norm_rotate.  For every head vector x of q (B, L, Hq, D) and of
+ * k (B, L, Hkv, D):
+ *     y = x * rsqrt(mean(x^2) + eps) * weight          (over D)
+ *     out = R(pos) y,  pos = positions[b, l], or l when positions is NULL
+ * where R turns the pairs (i, i + R/2) of the first R = rot_dim channels
+ * (adjacent == 0) or (2i, 2i + 1) (adjacent != 0) by the angle whose cosine
+ * and sine are cos[pos][i], sin[pos][i] (fp32, (rows, R/2) contiguous; fp64
+ * for fp64 inputs); channels past R are not turned.  A position outside
+ * [0, rows) gives NaN in the R turned channels.  q and k may be strided
+ * (element strides of b, l, h; unit stride in D); the outputs are
+ * contiguous.  q_weight / k_weight: (D) in `weight_dtype` (that of q, or
+ * fp32 with fp16 / bf16), or NULL for no weight.  D even, 2 <= D <= 512.
+ * Backward: grad_q_out / grad_k_out contiguous; grad_q, grad_k contiguous in
+ * the dtype of q; grad_*_weight in weight_dtype (NULL: not wanted).
+ * `workspace`: nsc_qk_norm_rotate_workspace(...) bytes, needed only when a
+ * weight gradient is wanted.  All sums in fp32 (fp64), in a fixed order.
+ * ------------------------------------------------------------------- */
+typedef struct nsc_norm_rotate {
+    int64_t B, L, Hq, Hkv, D, rot_dim, rows;
+    int64_t q_stride[3], k_stride[3];   /* b, l, h, in elements */
+    const void *q, *k, *q_weight, *k_weight, *cos, *sin;
+    const int32_t* positions;           /* (B, L) contiguous, or NULL */
+    int dtype, weight_dtype, adjacent;
+    double eps;
+} nsc_norm_rotate;
+
+NSC_API nsc_status nsc_qk_norm_rotate_fwd(const nsc_norm_rotate* a, void* q_out,
+                                  void* k_out, void* stream);
+NSC_API int64_t nsc_qk_norm_rotate_workspace(const nsc_norm_rotate* a);
+NSC_API nsc_status nsc_qk_norm_rotate_bwd(const nsc_norm_rotate* a,
+                                  const void* grad_q_out,
+                                  const void* grad_k_out, void* grad_q,
+                                  void* grad_k, void* grad_q_weight,
+                                  void* grad_k_weight, void* workspace,
+                                  void* stream);
+
+/* token_attention.  q (B, Lq, Hq, D), k and v (B, Lk, Hkv, D), Hq a multiple
+ * of Hkv (query head h reads key head h Hkv / Hq), any strides of b, l, h,
+ * unit stride in D; out (B, Lq, Hq, D) contiguous, lse (B, Hq, Lq) fp32
+ * (fp64).  Query i stands at position pos = i + n - Lq, n = Lk or lengths[b].
+ *     s(i, j) = c tanh(scale q_i.k_j / c) + table[buckets[clamp(j - pos, -reach,
+ *               reach) + reach], h]            (c = softcap; 0: no cap)
+ *     out_i   = sum_j softmax_j(s) v_j over the visible j,  lse_i = log sum_j e^s
+ * Visible are the keys j < n of the same document (documents: `docs` + 1
+ * ascending int32 bounds per batch entry, docs_stride apart, Lq == Lk; a token
+ * outside all of them sees nothing and is seen by none), and with `causal` of
+ * those j <= pos or j < start + prefix (start: that of the document; prefix:
+ * (B, docs) int32, or (B, 1) without documents, prefix_stride apart).  A query that sees nothing, or only scores
+ * of -inf, gives out = 0 and lse = -inf.  What is not visible is not part of
+ * any sum, whatever it holds.
+ * table: (n_buckets, Hq) contiguous in table_dtype (that of q, or fp32 with
+ * fp16 / bf16), buckets: 2 reach + 1 int32 (values outside [0, n_buckets) are
+ * taken as the nearest).  n_buckets <= 256, reach <= 1024.
+ * D <= 256 (fp64: 128).
+ * Backward: grad_out in the dtype and shape of out (its own strides), grad_lse (B, Hq, Lq) or
+ * NULL; grad_q, grad_k, grad_v contiguous in the dtype of q; grad_table
+ * (n_buckets, Hq) in table_dtype, or NULL.  No atomics: the same inputs give the
+ * same bits.  `workspace`: nsc_token_attention_bwd_workspace(a) bytes, 256-byte aligned.
+ * ------------------------------------------------------------------- */
+typedef struct nsc_attention {
+    int64_t B, Lq, Lk, Hq, Hkv, D;
+    int64_t q_stride[3], k_stride[3], v_stride[3];  /* b, l, h, in elements */
+    int64_t docs, docs_stride, prefix_stride, n_buckets, reach;
+    const void *q, *k, *v;
+    const int32_t *documents, *prefix, *lengths, *buckets;
+    const void* table;
+    double scale, softcap;
+    int dtype, table_dtype, causal;
+} nsc_attention;
+
+typedef struct nsc_attention_grad {
+    int64_t grad_out_stride[3];
+    const void *out, *lse, *grad_out, *grad_lse;
+    void *grad_q, *grad_k, *grad_v, *grad_table, *workspace;
+} nsc_attention_grad;
+
+NSC_API nsc_status nsc_token_attention_fwd(const nsc_attention* a, void* out,
+                                   void* lse, void* stream);
+NSC_API int64_t nsc_token_attention_bwd_workspace(const nsc_attention* a);
+NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
+                                   const nsc_attention_grad* g, void* stream);
+
+/* The form for the newest Lq tokens of ragged sequences: k and v are caches
+ * of Lk rows of which the first lengths[b] hold sequence b, the newest tokens'
+ * own keys among them; causal.  Rows past lengths[b] are not read.  The long
+ * axis is split over the GPU and joined.  `workspace`:
+ * nsc_token_attention_decode_workspace(a) bytes (may be 0), 256-byte aligned. */
+NSC_API int64_t nsc_token_attention_decode_workspace(const nsc_attention* a);
+NSC_API nsc_status nsc_token_attention_decode(const nsc_attention* a, void* out,
+                                      void* lse, void* workspace,
+                                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,12 @@ from .ops import (
     shift_gather,
 )
 from .metropolis import metropolis_aggregate
+from .token_attention import (
+    qk_norm_rotate,
+    relative_buckets,
+    token_attention,
+    token_attention_decode,
+)
 
 __version__ = "0.12.0+b200.1"
 
@@ -24,6 +30,10 @@ __all__ = [
     "accumulate_uz",
     "normalized_accumulate_uz",
     "metropolis_aggregate",
+    "qk_norm_rotate",
+    "token_attention",
+    "token_attention_decode",
+    "relative_buckets",
     "check_validation",
     "index_width_bits",
 ]

@@ -39,6 +39,38 @@ _L = ctypes.c_int64
 _D = ctypes.c_double
 _LP = ctypes.POINTER(ctypes.c_int64)
 
+class NormRotate(ctypes.Structure):
+    """nsc_norm_rotate of the header."""
+    _fields_ = [(n, _L) for n in ("B", "L", "Hq", "Hkv", "D", "rot_dim", "rows")] \
+        + [("q_stride", _L * 3), ("k_stride", _L * 3)] \
+        + [(n, _P) for n in ("q", "k", "q_weight", "k_weight", "cos", "sin",
+                             "positions")] \
+        + [("dtype", _I), ("weight_dtype", _I), ("adjacent", _I), ("eps", _D)]
+
+
+class Attention(ctypes.Structure):
+    """nsc_attention of the header."""
+    _fields_ = [(n, _L) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D")] \
+        + [("q_stride", _L * 3), ("k_stride", _L * 3), ("v_stride", _L * 3)] \
+        + [(n, _L) for n in ("docs", "docs_stride", "prefix_stride", "n_buckets",
+                             "reach")] \
+        + [(n, _P) for n in ("q", "k", "v", "documents", "prefix", "lengths",
+                             "buckets", "table")] \
+        + [("scale", _D), ("softcap", _D), ("dtype", _I), ("table_dtype", _I),
+           ("causal", _I)]
+
+
+class AttentionGrad(ctypes.Structure):
+    """nsc_attention_grad of the header."""
+    _fields_ = [("grad_out_stride", _L * 3)] \
+        + [(n, _P) for n in ("out", "lse", "grad_out", "grad_lse", "grad_q",
+                             "grad_k", "grad_v", "grad_table", "workspace")]
+
+
+_NR = ctypes.POINTER(NormRotate)
+_AT = ctypes.POINTER(Attention)
+_AG = ctypes.POINTER(AttentionGrad)
+
 # argument lists, in header order
 _SIGS = {
     "nsc_shift_gather_fwd": [_P, _I, _L, _L, _L, _L, _LP, _L, _L, _P, _P, _P],
@@ -72,10 +104,22 @@ _SIGS = {
     "nsc_nectr_fused_fwd": [_P, _P, _I, _L, _L, _L, _L, _L, _I,
                             ctypes.POINTER(ctypes.c_double), _L, _D, _D, _D, _D,
                             _LP, _L, _I, _P, _P, _P, _P],
+    "nsc_qk_norm_rotate_fwd": [_NR, _P, _P, _P],
+    "nsc_qk_norm_rotate_bwd": [_NR, _P, _P, _P, _P, _P, _P, _P, _P],
+    "nsc_token_attention_fwd": [_AT, _P, _P, _P],
+    "nsc_token_attention_bwd": [_AT, _AG, _P],
+    "nsc_token_attention_decode": [_AT, _P, _P, _P, _P],
+}
+
+# entry points that return a workspace size in bytes (negative: bad arguments)
+_SIZES = {
+    "nsc_qk_norm_rotate_workspace": [_NR],
+    "nsc_token_attention_bwd_workspace": [_AT],
+    "nsc_token_attention_decode_workspace": [_AT],
 }
 
 EXPORTED = ["nsc_index_width_bits", "nsc_version", "nsc_last_error_string",
-            "nsc_wait_timeouts", "nsc_test_wait_fault", *_SIGS]
+            "nsc_wait_timeouts", "nsc_test_wait_fault", *_SIGS, *_SIZES]
 
 
 def load() -> ctypes.CDLL:
@@ -98,6 +142,10 @@ def load() -> ctypes.CDLL:
                 fn = getattr(lib, name)
                 fn.argtypes = args
                 fn.restype = ctypes.c_int
+            for name, args in _SIZES.items():
+                fn = getattr(lib, name)
+                fn.argtypes = args
+                fn.restype = ctypes.c_int64
         except (OSError, AttributeError) as e:
             _load_error = e
             raise RuntimeError(
@@ -155,6 +203,16 @@ def call(name: str, *args) -> None:
     if st != 0:
         msg = lib.nsc_last_error_string().decode()
         raise RuntimeError(f"{msg} [{_STATUS.get(st, st)}]")
+
+
+def workspace(name: str, device, *args) -> Optional[torch.Tensor]:
+    """A buffer of the size that workspace query `name` gives (None for 0)."""
+    lib = load()
+    n = int(getattr(lib, name)(*args))
+    if n < 0:
+        raise RuntimeError(f"{lib.nsc_last_error_string().decode()} "
+                           f"[{_STATUS[1]}]")
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -1,0 +1,105 @@
+// token_attention.h -- what the token-attention kernels share: the call's
+// parameters as the kernels read them, the visible spans, and the launchers
+// of the kernel families behind the entry points in token_attention.cu.
+#pragma once
+
+#include "nsc_host.h"
+
+namespace nsc {
+namespace tok {
+
+struct Params {
+    const void *q, *k, *v;
+    int64_t qs[3], ks[3], vs[3];      // element strides of b, l, h
+    void* out;                        // contiguous (B, Lq, Hq, D)
+    void* lse;                        // contiguous (B, Hq, Lq), nullable
+    int B, Lq, Lk, Hq, Hkv, G, D;     // G = Hq / Hkv
+    int causal;
+    const int32_t *docs, *prefix, *lengths, *lut;
+    int64_t docs_stride, prefix_stride;
+    int n_docs, prefix_cols, nb, reach;
+    const void* table;
+    int table_dtype;
+    double scale, cap;
+};
+
+struct Grads {
+    const void *dout, *dlse;
+    int64_t dos[3];
+    void *dq, *dk, *dv;               // contiguous
+    void *delta;                      // (B, Hq, Lq): sum_d dout out - dlse
+    void* tab;                        // (Hq, n_part, nb) partial sums, or null
+    int n_part;
+};
+
+// Document [s, e) of position t: the last bound <= t opens it.  Bounds are
+// clamped to [0, n], so no call reads past a tensor whatever they hold.
+__device__ __forceinline__ bool find_doc(const Params& p, int b, int t, int n, int& s, int& e,
+                                         int& doc) {
+    const int32_t* d = p.docs + b * p.docs_stride;
+    int lo = 0, hi = p.n_docs + 1;    // bounds [0, lo) are <= t, [hi, ...) are > t
+    while (lo < hi) {
+        const int m = (lo + hi) >> 1;
+        if (__ldg(d + m) <= t) lo = m + 1; else hi = m;
+    }
+    doc = lo - 1;
+    if (doc < 0 || doc >= p.n_docs) return false;
+    s = min(max(__ldg(d + doc), 0), n);
+    e = min(max(__ldg(d + doc + 1), 0), n);
+    return true;
+}
+
+__device__ __forceinline__ int prefix_of(const Params& p, int b, int doc, int n) {
+    if (!p.prefix) return 0;
+    return min(max(__ldg(p.prefix + b * p.prefix_stride + doc), 0), n);
+}
+
+__device__ __forceinline__ int keys_of(const Params& p, int b) {
+    return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.Lk) : p.Lk;
+}
+
+// Every mask here is one interval of keys per query: keys [lo, hi) are
+// visible to query i (hi <= lo: none).  n = keys_of(p, b).
+__device__ __forceinline__ void key_span(const Params& p, int b, int i, int n, int& lo, int& hi) {
+    const int pos = i + n - p.Lq;
+    int s = 0, e = n, doc = 0;
+    if (p.docs && !find_doc(p, b, pos, n, s, e, doc)) { lo = hi = 0; return; }
+    lo = s;
+    hi = p.causal ? min(e, max(pos + 1, s + prefix_of(p, b, doc, n))) : e;
+}
+
+// The same relation from a key: queries [lo, hi) see key j (lengths is null).
+__device__ __forceinline__ void query_span(const Params& p, int b, int j, int& lo, int& hi) {
+    const int off = p.Lk - p.Lq;
+    int s = 0, e = p.Lk, doc = 0;
+    if (j >= p.Lk || (p.docs && !find_doc(p, b, j, p.Lk, s, e, doc))) { lo = hi = 0; return; }
+    const bool all = !p.causal || j < s + prefix_of(p, b, doc, p.Lk);
+    lo = all ? (p.docs ? s : 0) : max(0, j - off);
+    hi = p.docs ? e : p.Lq;
+}
+
+// Bias of bucket b for head h.
+template <typename A>
+__device__ __forceinline__ A table_at(const Params& p, int b, int h) {
+    b = min(max(b, 0), p.nb - 1);
+    const int64_t at = static_cast<int64_t>(b) * p.Hq + h;
+    switch (p.table_dtype) {
+        case NSC_F16: return __half2float(static_cast<const __half*>(p.table)[at]);
+        case NSC_BF16: return __bfloat162float(static_cast<const __nv_bfloat16*>(p.table)[at]);
+        case NSC_F32: return static_cast<const float*>(p.table)[at];
+    }
+    return static_cast<A>(static_cast<const double*>(p.table)[at]);
+}
+
+// Kernels for any type, strides and head width (token_attention_general.cu).
+nsc_status general_fwd(const Params& p, int dtype, cudaStream_t st);
+nsc_status general_bwd(const Params& p, const Grads& g, int dtype, cudaStream_t st);
+int general_tile(int dtype, int D);
+
+// delta (and its layout (B, Hq, Lq)) for a backward pass; joining of the
+// table-gradient partials.
+nsc_status launch_delta(const Params& p, const Grads& g, int dtype, cudaStream_t st);
+nsc_status launch_table_join(const Params& p, const Grads& g, void* grad_table, cudaStream_t st);
+
+}  // namespace tok
+}  // namespace nsc

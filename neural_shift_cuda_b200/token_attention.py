@@ -1,0 +1,445 @@
+"""Token attention on B200: the operators of the transformer layers that run
+beside the shift-window denoisers (token mixers over image patches, image
+language models, diffusion transformers).
+
+    qk_norm_rotate(q, k, q_weight, k_weight, cos, sin)      -> (q', k')
+    token_attention(q, k, v, ...)                           -> out
+    token_attention_decode(q, k_cache, v_cache, lengths)    -> out
+    relative_buckets(num_buckets, max_distance)             -> bucket map
+
+Where `normalized_accumulate_uz` is a softmax over a fixed window of shifts
+with given logits, `token_attention` is the softmax over all tokens whose
+logits are products of queries and keys, capped by a tanh, with a learned
+bias by buckets of distance, under causal, prefix and document masks.
+Tensors are (B, L, H, D) with any strides of B, L and H, so the slices of one
+projection are read in place; fp16, bf16, fp32 and fp64; sums and softmax
+statistics in fp32 (fp64).  CUDA tensors only, as the other ops.  Nothing here
+has a counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _require_cuda
+
+__all__ = ["qk_norm_rotate", "token_attention", "token_attention_decode",
+           "relative_buckets"]
+
+_byref = ctypes.byref
+
+
+# ---------------------------------------------------------------------------
+# argument handling
+# ---------------------------------------------------------------------------
+
+def _check_heads(op: str, name: str, t: torch.Tensor) -> None:
+    if t.dim() != 4:
+        raise RuntimeError(f"{op}: {name} must be (B, L, H, D); got "
+                           f"{tuple(t.shape)}")
+
+
+def _check_like(op: str, q: torch.Tensor, **others: torch.Tensor) -> None:
+    if q.dtype not in _lib._DTYPES:
+        raise TypeError(f"{op}: unsupported dtype {q.dtype}")
+    for name, t in others.items():
+        if t.dtype != q.dtype:
+            raise TypeError(f"{op}: {name} is {t.dtype}, q is {q.dtype}")
+        if t.device != q.device:
+            raise ValueError(f"{op}: {name} is on {t.device}, q on {q.device}")
+
+
+def _check_param(op: str, q: torch.Tensor, name: str, t: torch.Tensor) -> None:
+    """A learned parameter: the dtype of q, or fp32 beside fp16 / bf16."""
+    if t.device != q.device:
+        raise ValueError(f"{op}: {name} is on {t.device}, q on {q.device}")
+    if t.dtype != q.dtype and not (t.dtype == torch.float32
+                                   and q.dtype in (torch.float16, torch.bfloat16)):
+        raise TypeError(f"{op}: {name} is {t.dtype}; it has the dtype of q "
+                        f"({q.dtype}), or fp32 with fp16 / bf16")
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """t with unit stride in its last dimension."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _int32(op: str, name: str, t: torch.Tensor, device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{op}: {name} must be an int32 or int64 tensor")
+    if t.device != device:
+        raise ValueError(f"{op}: {name} is on {t.device}, q on {device}")
+    return t.to(torch.int32).contiguous()
+
+
+def _acc(dt: torch.dtype) -> torch.dtype:
+    return torch.float64 if dt == torch.float64 else torch.float32
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------
+# qk_norm_rotate
+# ---------------------------------------------------------------------------
+
+def _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps):
+    B, L, Hq, D = q.shape
+    a = _lib.NormRotate()
+    a.B, a.L, a.Hq, a.Hkv, a.D = B, L, Hq, k.shape[2], D
+    a.rot_dim, a.rows = 2 * cos.shape[1], cos.shape[0]
+    a.q_stride[:] = q.stride()[:3]
+    a.k_stride[:] = k.stride()[:3]
+    a.q, a.k, a.q_weight, a.k_weight = _addr(q), _addr(k), _addr(wq), _addr(wk)
+    a.cos, a.sin, a.positions = _addr(cos), _addr(sin), _addr(positions)
+    a.dtype = _lib.dtype_code(q.dtype)
+    w = wq if wq is not None else wk
+    a.weight_dtype = _lib.dtype_code(q.dtype if w is None else w.dtype)
+    a.adjacent, a.eps = int(adjacent), eps
+    return a
+
+
+def _rotate_fwd(q, k, wq, wk, cos, sin, positions, adjacent, eps):
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    a = _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps)
+    with torch.cuda.device(q.device):
+        _lib.call("nsc_qk_norm_rotate_fwd", _byref(a), _lib.ptr(qo),
+                  _lib.ptr(ko), _lib.stream_of(q))
+    return qo, ko
+
+
+class _RotateFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, adjacent, eps):
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        ctx.adjacent, ctx.eps = adjacent, eps
+        return _rotate_fwd(q, k, wq, wk, cos, sin, positions, adjacent, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        a = _rotate_args(q, k, wq, wk, cos, sin, positions, ctx.adjacent, ctx.eps)
+        gq, gk = gq.contiguous(), gk.contiguous()
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
+        dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
+        with torch.cuda.device(q.device):
+            ws = None
+            if dwq is not None or dwk is not None:
+                ws = _lib.workspace("nsc_qk_norm_rotate_workspace", q.device, _byref(a))
+            _lib.call("nsc_qk_norm_rotate_bwd", _byref(a), _lib.ptr(gq),
+                      _lib.ptr(gk), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dwq),
+                      _lib.ptr(dwk), _lib.ptr(ws), _lib.stream_of(q))
+        return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
+                   q_weight: Optional[torch.Tensor],
+                   k_weight: Optional[torch.Tensor], cos: torch.Tensor,
+                   sin: torch.Tensor, *, positions: Optional[torch.Tensor] = None,
+                   adjacent: bool = False,
+                   eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Root-mean-square norm of every head of q (B, L, Hq, D) and k
+    (B, L, Hkv, D), times the weights (D,) (None: no weight), then the
+    rotation by position, in one pass -> contiguous (q', k').
+
+    cos, sin: (rows, R/2), R <= D: pair i of the first R channels -- (i,
+    i + R/2), or (2i, 2i + 1) with adjacent=True -- turns by the angle of
+    row positions[b, l] (int (B, L) or (L,); default: row l).  Channels past
+    R are only normed.  Differentiable in q, k and the weights; the weight
+    gradients are summed in a fixed order."""
+    op = "qk_norm_rotate"
+    _check_heads(op, "q", q)
+    _check_heads(op, "k", k)
+    _check_like(op, q, k=k)
+    B, L, _, D = q.shape
+    if k.shape[0] != B or k.shape[1] != L or k.shape[3] != D:
+        raise RuntimeError(f"{op}: q {tuple(q.shape)} and k {tuple(k.shape)} "
+                           f"do not agree")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        _check_param(op, q, name, w)
+        if w.shape != (D,):
+            raise RuntimeError(f"{op}: {name} must be ({D},); got {tuple(w.shape)}")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError(f"{op}: q_weight is {q_weight.dtype}, k_weight "
+                        f"{k_weight.dtype}")
+    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > D:
+        raise RuntimeError(f"{op}: cos and sin must be (rows, R/2) with R <= {D}; got "
+                           f"{tuple(cos.shape)}, {tuple(sin.shape)}")
+    if cos.device != q.device or sin.device != q.device:
+        raise ValueError(f"{op}: cos and sin must be on {q.device}")
+    _require_cuda(op, q, k)
+    if positions is not None:
+        positions = _int32(op, "positions", positions, q.device)
+        if positions.shape == (L,):
+            positions = positions.expand(B, L).contiguous()
+        if positions.shape != (B, L):
+            raise RuntimeError(f"{op}: positions must be ({B}, {L}) or ({L},); got "
+                               f"{tuple(positions.shape)}")
+    elif cos.shape[0] < L:
+        raise RuntimeError(f"{op}: cos and sin have {cos.shape[0]} rows for "
+                           f"{L} positions")
+    acc = _acc(q.dtype)
+    cos, sin = cos.detach().to(acc).contiguous(), sin.detach().to(acc).contiguous()
+    wq = None if q_weight is None else q_weight.contiguous()
+    wk = None if k_weight is None else k_weight.contiguous()
+    args = (_unit(q), _unit(k), wq, wk, cos, sin, positions, bool(adjacent), float(eps))
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _RotateFn.apply(*args)
+    return _rotate_fwd(*args)
+
+
+# ---------------------------------------------------------------------------
+# token_attention
+# ---------------------------------------------------------------------------
+
+def relative_buckets(num_buckets: int, max_distance: int,
+                     bidirectional: bool = True, device=None) -> torch.Tensor:
+    """Bucket of every distance key - query in [-max_distance, max_distance]
+    ((2 max_distance + 1,) int32; farther distances take the ends' buckets).
+
+    Each sign has its own half of the buckets (bidirectional=False: keys past
+    the query share bucket 0 and the past has all buckets).  Half of a sign's
+    buckets hold one distance each, the others grow by a constant factor up to
+    max_distance."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    if n < 2 or num_buckets > 256:
+        raise ValueError(f"relative_buckets: num_buckets = {num_buckets}, need "
+                         f"{4 if bidirectional else 2}..256")
+    near = n // 2
+    if not near < max_distance <= 1024:
+        raise ValueError(f"relative_buckets: max_distance = {max_distance}, need "
+                         f"{near + 1}..1024 for {num_buckets} buckets")
+    rows = []
+    for d in range(-max_distance, max_distance + 1):
+        a = abs(d) if bidirectional else max(-d, 0)
+        u = a if a < near else min(n - 1, near + int(
+            math.log(a / near) / math.log(max_distance / near) * (n - near)))
+        rows.append(u + (n if bidirectional and d > 0 else 0))
+    return torch.tensor(rows, dtype=torch.int32, device=device)
+
+
+def _attention_args(q, k, v, documents, prefix, lengths, table, buckets, scale,
+                    cap, causal):
+    B, Lq, Hq, D = q.shape
+    a = _lib.Attention()
+    a.B, a.Lq, a.Lk, a.Hq, a.Hkv, a.D = B, Lq, k.shape[1], Hq, k.shape[2], D
+    a.q_stride[:] = q.stride()[:3]
+    a.k_stride[:] = k.stride()[:3]
+    a.v_stride[:] = v.stride()[:3]
+    a.q, a.k, a.v = _addr(q), _addr(k), _addr(v)
+    a.dtype = _lib.dtype_code(q.dtype)
+    if documents is not None:
+        a.documents, a.docs = _addr(documents), documents.shape[1] - 1
+        a.docs_stride = documents.stride(0)
+    if prefix is not None:
+        a.prefix, a.prefix_stride = _addr(prefix), prefix.stride(0)
+    if lengths is not None:
+        a.lengths = _addr(lengths)
+    if table is not None:
+        a.table, a.buckets = _addr(table), _addr(buckets)
+        a.table_dtype = _lib.dtype_code(table.dtype)
+        a.n_buckets, a.reach = table.shape[0], buckets.shape[0] // 2
+    a.scale, a.softcap, a.causal = scale, cap, int(causal)
+    return a
+
+
+def _attention_fwd(q, k, v, documents, prefix, table, buckets, scale, cap, causal,
+                   want_lse):
+    B, Lq, Hq, D = q.shape
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    lse = (torch.empty((B, Hq, Lq), dtype=_acc(q.dtype), device=q.device)
+           if want_lse else None)
+    a = _attention_args(q, k, v, documents, prefix, None, table, buckets, scale,
+                        cap, causal)
+    with torch.cuda.device(q.device):
+        _lib.call("nsc_token_attention_fwd", _byref(a), _lib.ptr(out),
+                  _lib.ptr(lse), _lib.stream_of(q))
+    return out, lse
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, documents, prefix, table, buckets, scale, cap, causal):
+        out, lse = _attention_fwd(q, k, v, documents, prefix, table, buckets,
+                                  scale, cap, causal, True)
+        ctx.save_for_backward(q, k, v, out, lse, documents, prefix, table, buckets)
+        ctx.scale, ctx.cap, ctx.causal = scale, cap, causal
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_lse):
+        q, k, v, out, lse, documents, prefix, table, buckets = ctx.saved_tensors
+        a = _attention_args(q, k, v, documents, prefix, None, table, buckets,
+                            ctx.scale, ctx.cap, ctx.causal)
+        grad_out = torch.zeros_like(out) if grad_out is None else _unit(grad_out)
+        if grad_lse is not None:
+            grad_lse = grad_lse.contiguous()
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        dt = (torch.empty_like(table) if table is not None and ctx.needs_input_grad[5]
+              else None)
+        g = _lib.AttentionGrad()
+        g.grad_out_stride[:] = grad_out.stride()[:3]
+        with torch.cuda.device(q.device):
+            ws = _lib.workspace("nsc_token_attention_bwd_workspace", q.device, _byref(a))
+            g.out, g.lse, g.grad_out, g.grad_lse = (
+                _addr(out), _addr(lse), _addr(grad_out), _addr(grad_lse))
+            g.grad_q, g.grad_k, g.grad_v = _addr(dq), _addr(dk), _addr(dv)
+            g.grad_table, g.workspace = _addr(dt), _addr(ws)
+            _lib.call("nsc_token_attention_bwd", _byref(a), _byref(g), _lib.stream_of(q))
+        return dq, dk, dv, None, None, dt, None, None, None, None
+
+
+def _check_qkv(op, q, k, v, kname="k", vname="v"):
+    _check_heads(op, "q", q)
+    _check_heads(op, kname, k)
+    _check_heads(op, vname, v)
+    _check_like(op, q, **{kname: k, vname: v})
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError(f"{op}: q {tuple(q.shape)}, {kname} {tuple(k.shape)} and "
+                           f"{vname} {tuple(v.shape)} do not agree")
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2] or q.shape[2] == 0:
+        raise RuntimeError(f"{op}: {q.shape[2]} query heads are not a multiple of "
+                           f"{k.shape[2]} key heads")
+
+
+def _check_bias(op, q, table, buckets):
+    if (table is None) != (buckets is None):
+        raise ValueError(f"{op}: a bias needs bias_table and bias_buckets")
+    if table is None:
+        return None, None
+    _check_param(op, q, "bias_table", table)
+    if table.dim() != 2 or table.shape[1] != q.shape[2]:
+        raise RuntimeError(f"{op}: bias_table must be (buckets, {q.shape[2]}); got "
+                           f"{tuple(table.shape)}")
+    buckets = _int32(op, "bias_buckets", buckets, q.device)
+    if buckets.dim() != 1 or buckets.shape[0] % 2 == 0:
+        raise RuntimeError(f"{op}: bias_buckets must have 2 reach + 1 entries; got "
+                           f"{tuple(buckets.shape)}")
+    return table.contiguous(), buckets
+
+
+def _numbers(q, scale, softcap):
+    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    return scale, 0.0 if softcap is None else float(softcap)
+
+
+def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                    scale: Optional[float] = None, softcap: Optional[float] = None,
+                    causal: bool = False, prefix=None,
+                    documents: Optional[torch.Tensor] = None,
+                    bias_table: Optional[torch.Tensor] = None,
+                    bias_buckets: Optional[torch.Tensor] = None,
+                    return_lse: bool = False):
+    """Softmax attention of q (B, Lq, Hq, D) over k, v (B, Lk, Hkv, D) ->
+    out (B, Lq, Hq, D), or (out, lse (B, Hq, Lq) fp32).
+
+    Query head h reads key head h Hkv // Hq; query i stands at key position
+    i + Lk - Lq.  scale defaults to D^-0.5; softcap c turns a score s into
+    c tanh(s / c); then bias_table[bias_buckets[distance], h] is added
+    (`relative_buckets`; distances past the map's ends take the ends').
+
+    causal: a query sees keys up to its own position.  prefix (an int, or an
+    int tensor (B,), or (B, documents)): and the first `prefix` keys of its row or
+    document.  documents: (B, n + 1) or (n + 1,) ascending bounds; tokens see
+    only their own document, tokens outside all documents see nothing.  A query
+    that sees nothing gives out = 0, lse = -inf.  What a query does not see has no
+    influence on it, even where it is not finite.
+
+    Differentiable in q, k, v and bias_table, through out and lse; the
+    gradients are summed in a fixed order."""
+    op = "token_attention"
+    _check_qkv(op, q, k, v)
+    B, Lq, Lk, dev = q.shape[0], q.shape[1], k.shape[1], q.device
+    table, buckets = _check_bias(op, q, bias_table, bias_buckets)
+    if prefix is not None and not causal:
+        raise ValueError(f"{op}: a prefix needs causal=True")
+    _require_cuda(op, q, k, v)
+    if documents is not None:
+        documents = _int32(op, "documents", documents, dev)
+        if documents.dim() == 1:
+            documents = documents.expand(B, -1)
+        if documents.dim() != 2 or documents.shape[0] != B or documents.shape[1] < 2:
+            raise RuntimeError(f"{op}: documents must be ({B}, n + 1) or (n + 1,) bounds; "
+                               f"got {tuple(documents.shape)}")
+        if Lq != Lk:
+            raise RuntimeError(f"{op}: documents need as many queries as keys; got "
+                               f"{Lq} and {Lk}")
+    if prefix is not None:
+        if isinstance(prefix, int):
+            prefix = torch.full((1,), prefix, dtype=torch.int32, device=dev).expand(B)
+        else:
+            prefix = _int32(op, "prefix", prefix, dev)
+        n = 1 if documents is None else documents.shape[1] - 1
+        if prefix.dim() == 1:
+            prefix = prefix[:, None].expand(-1, n) if n == 1 else \
+                prefix[:, None].expand(-1, n).contiguous()
+        if prefix.shape != (B, n):
+            raise RuntimeError(f"{op}: prefix must be ({B},) or ({B}, {n}); got "
+                               f"{tuple(prefix.shape)}")
+    scale, cap = _numbers(q, scale, softcap)
+    args = (_unit(q), _unit(k), _unit(v), documents, prefix, table, buckets, scale,
+            cap, bool(causal))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (table is not None and table.requires_grad)):
+        out, lse = _AttentionFn.apply(*args)
+    else:
+        out, lse = _attention_fwd(*args, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, lengths: torch.Tensor, *,
+                           scale: Optional[float] = None,
+                           softcap: Optional[float] = None,
+                           bias_table: Optional[torch.Tensor] = None,
+                           bias_buckets: Optional[torch.Tensor] = None,
+                           return_lse: bool = False):
+    """The newest T tokens of every sequence over its cache: q (B, T, Hq, D),
+    caches (B, rows, Hkv, D) whose first lengths[b] rows hold sequence b, the
+    new tokens' own keys among them -> out (B, T, Hq, D) (and lse (B, Hq, T)).
+
+    Token t stands at position lengths[b] - T + t and sees the keys up to it;
+    scores as in `token_attention`.  Rows past lengths[b] are not read.  For
+    serving: no gradient."""
+    op = "token_attention_decode"
+    _check_qkv(op, q, k_cache, v_cache, "k_cache", "v_cache")
+    table, buckets = _check_bias(op, q, bias_table, bias_buckets)
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k_cache, v_cache, table)):
+        raise RuntimeError(f"{op} has no backward; use token_attention, or "
+                           f"torch.no_grad()")
+    _require_cuda(op, q, k_cache, v_cache)
+    lengths = _int32(op, "lengths", lengths, q.device)
+    B, T, Hq, D = q.shape
+    if lengths.shape != (B,):
+        raise RuntimeError(f"{op}: lengths must be ({B},); got {tuple(lengths.shape)}")
+    scale, cap = _numbers(q, scale, softcap)
+    q, k_cache, v_cache = _unit(q), _unit(k_cache), _unit(v_cache)
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    lse = (torch.empty((B, Hq, T), dtype=_acc(q.dtype), device=q.device)
+           if return_lse else None)
+    a = _attention_args(q, k_cache, v_cache, None, None, lengths, table, buckets,
+                        scale, cap, True)
+    with torch.cuda.device(q.device):
+        ws = _lib.workspace("nsc_token_attention_decode_workspace", q.device, _byref(a))
+        _lib.call("nsc_token_attention_decode", _byref(a), _lib.ptr(out),
+                  _lib.ptr(lse), _lib.ptr(ws), _lib.stream_of(q))
+    return (out, lse) if return_lse else out
