@@ -376,7 +376,10 @@ NSC_API nsc_status nsc_qk_norm_rotate_bwd(const nsc_norm_rotate* a,
  * table: (n_buckets, Hq) contiguous in table_dtype (that of q, or fp32 with
  * fp16 / bf16), buckets: 2 reach + 1 int32 (values outside [0, n_buckets) are
  * taken as the nearest).  n_buckets <= 256, reach <= 1024.
- * D <= 256 (fp64: 128).
+ * D <= 256 (fp64: 128).  lse may be NULL; for a backward pass the forward writes
+ * `stats` (2, B, Hq, Lq) fp32 (fp64), the softmax statistics of its rows, and
+ * may write `residue` (like out): what rounding the output dropped, which
+ * makes the backward's row sums exact to fp32 (NULL: not wanted).
  * Backward: grad_out in the dtype and shape of out (its own strides), grad_lse (B, Hq, Lq) or
  * NULL; grad_q, grad_k, grad_v contiguous in the dtype of q; grad_table
  * (n_buckets, Hq) in table_dtype, or NULL.  No atomics: the same inputs give the
@@ -395,12 +398,13 @@ typedef struct nsc_attention {
 
 typedef struct nsc_attention_grad {
     int64_t grad_out_stride[3];
-    const void *out, *lse, *grad_out, *grad_lse;
+    const void *out, *stats, *residue, *grad_out, *grad_lse;
     void *grad_q, *grad_k, *grad_v, *grad_table, *workspace;
 } nsc_attention_grad;
 
 NSC_API nsc_status nsc_token_attention_fwd(const nsc_attention* a, void* out,
-                                   void* lse, void* stream);
+                                   void* lse, void* stats, void* residue,
+                                   void* stream);
 NSC_API int64_t nsc_token_attention_bwd_workspace(const nsc_attention* a);
 NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
                                    const nsc_attention_grad* g, void* stream);

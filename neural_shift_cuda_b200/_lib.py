@@ -63,8 +63,8 @@ class Attention(ctypes.Structure):
 class AttentionGrad(ctypes.Structure):
     """nsc_attention_grad of the header."""
     _fields_ = [("grad_out_stride", _L * 3)] \
-        + [(n, _P) for n in ("out", "lse", "grad_out", "grad_lse", "grad_q",
-                             "grad_k", "grad_v", "grad_table", "workspace")]
+        + [(n, _P) for n in ("out", "stats", "residue", "grad_out", "grad_lse",
+                             "grad_q", "grad_k", "grad_v", "grad_table", "workspace")]
 
 
 _NR = ctypes.POINTER(NormRotate)
@@ -106,7 +106,7 @@ _SIGS = {
                             _LP, _L, _I, _P, _P, _P, _P],
     "nsc_qk_norm_rotate_fwd": [_NR, _P, _P, _P],
     "nsc_qk_norm_rotate_bwd": [_NR, _P, _P, _P, _P, _P, _P, _P, _P],
-    "nsc_token_attention_fwd": [_AT, _P, _P, _P],
+    "nsc_token_attention_fwd": [_AT, _P, _P, _P, _P, _P],
     "nsc_token_attention_bwd": [_AT, _AG, _P],
     "nsc_token_attention_decode": [_AT, _P, _P, _P, _P],
 }

@@ -99,7 +99,7 @@ using namespace nsc;
 using namespace nsc::tok;
 
 extern "C" NSC_API nsc_status nsc_token_attention_fwd(const nsc_attention* a, void* out, void* lse,
-                                                      void* stream) {
+                                                      void* stats, void* residue, void* stream) {
     const char* op = "token_attention";
     nsc_status st = check(op, a, true);
     if (st != NSC_OK) return st;
@@ -110,6 +110,9 @@ extern "C" NSC_API nsc_status nsc_token_attention_fwd(const nsc_attention* a, vo
     Params p = params(a);
     p.out = out;
     p.lse = lse;
+    p.stats = stats;
+    p.residue = residue;
+    if (tc_fits(p, a->dtype)) return tc_fwd(p, a->dtype, as_stream(stream));
     return general_fwd(p, a->dtype, as_stream(stream));
 }
 
@@ -129,13 +132,14 @@ extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
     if (a->lengths)
         return fail(NSC_ERR_INVALID_ARG, "%s: lengths belong to the decode form", op);
     const bool rows = a->B && a->Lq, cols = a->B && a->Lk;
-    if ((rows && (!g->out || !g->lse || !g->grad_out || !g->grad_q || !g->workspace)) ||
+    if ((rows && (!g->out || !g->stats || !g->grad_out || !g->grad_q || !g->workspace)) ||
         (cols && (!g->grad_k || !g->grad_v)) || (g->grad_table && !a->table))
         return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
     cudaStream_t s = as_stream(stream);
     Params p = params(a);
     p.out = const_cast<void*>(g->out);
-    p.lse = const_cast<void*>(g->lse);
+    p.stats = const_cast<void*>(g->stats);
+    p.residue = const_cast<void*>(g->residue);
     Grads gr{};
     gr.dout = g->grad_out;
     gr.dlse = g->grad_lse;

@@ -13,6 +13,8 @@ struct Params {
     int64_t qs[3], ks[3], vs[3];      // element strides of b, l, h
     void* out;                        // contiguous (B, Lq, Hq, D)
     void* lse;                        // contiguous (B, Hq, Lq), nullable
+    void* stats;                      // (2, B, Hq, Lq), nullable: see row_stats
+    void* residue;                    // like out, nullable: what rounding out dropped
     int B, Lq, Lk, Hq, Hkv, G, D;     // G = Hq / Hkv
     int causal;
     const int32_t *docs, *prefix, *lengths, *lut;
@@ -91,10 +93,44 @@ __device__ __forceinline__ A table_at(const Params& p, int b, int h) {
     return static_cast<A>(static_cast<const double*>(p.table)[at]);
 }
 
+constexpr double kLog2e = 1.4426950408889634;
+constexpr double kLn2 = 0.6931471805599453;
+
+// Scores are held in units of log 2, s2 = s log2(e).  A finite bias is kept
+// within 1e37, so that the sum of a score and the lowest value of its type
+// stays finite (and a row that sees nothing else has a uniform softmax).
+template <typename A>
+__device__ __forceinline__ A bias2_at(const Params& p, int b, int h) {
+    const A t = table_at<A>(p, b, h);
+    if (!(t - t == A(0))) return t;   // infinities and NaN as they are
+    const A v = t * static_cast<A>(kLog2e);
+    return v < A(-1e37) ? A(-1e37) : (v > A(1e37) ? A(1e37) : v);
+}
+
+// What a forward leaves for its backward: the reference m and log2 of the sum
+// of 2^(s2 - m), apart (their sum would lose the sum's digits beside a large
+// m).  A row that sees nothing has m = -inf.
+template <typename A>
+__device__ __forceinline__ void row_stats(const Params& p, int64_t row, A m, A log2_sum, bool none) {
+    const int64_t n = static_cast<int64_t>(p.B) * p.Hq * p.Lq;
+    if (p.stats) {
+        static_cast<A*>(p.stats)[row] = none ? A(-INFINITY) : m;
+        static_cast<A*>(p.stats)[n + row] = none ? A(0) : log2_sum;
+    }
+    if (p.lse)
+        static_cast<A*>(p.lse)[row] =
+            none ? A(-INFINITY) : m * static_cast<A>(kLn2) + log2_sum * static_cast<A>(kLn2);
+}
+
 // Kernels for any type, strides and head width (token_attention_general.cu).
 nsc_status general_fwd(const Params& p, int dtype, cudaStream_t st);
 nsc_status general_bwd(const Params& p, const Grads& g, int dtype, cudaStream_t st);
 int general_tile(int dtype, int D);
+
+// Tensor-core kernels for fp16 / bf16 (token_attention_tc_*.cu); tc_fits: whether a
+// call's layout is one that their TMA boxes describe.
+bool tc_fits(const Params& p, int dtype);
+nsc_status tc_fwd(const Params& p, int dtype, cudaStream_t st);
 
 // delta (and its layout (B, Hq, Lq)) for a backward pass; joining of the
 // table-gradient partials.

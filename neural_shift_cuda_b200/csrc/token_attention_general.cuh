@@ -20,8 +20,10 @@ namespace tok {
 constexpr int kGenThreads = 256;
 
 template <typename A> __device__ __forceinline__ A ninf() { return -INFINITY; }
-__device__ __forceinline__ float exp_(float x) { return expf(x); }
-__device__ __forceinline__ double exp_(double x) { return exp(x); }
+__device__ __forceinline__ float exp2_(float x) { return exp2f(x); }
+__device__ __forceinline__ double exp2_(double x) { return exp2(x); }
+__device__ __forceinline__ float log2_(float x) { return log2f(x); }
+__device__ __forceinline__ double log2_(double x) { return log2(x); }
 __device__ __forceinline__ float tanh_(float x) { return tanhf(x); }
 __device__ __forceinline__ double tanh_(double x) { return tanh(x); }
 
@@ -133,7 +135,7 @@ __device__ __forceinline__ void mix_tile(const A* w, const A* b, int tx, int ty,
 template <typename A>
 __device__ __forceinline__ void load_bias(const Params& p, int h, A* bias) {
     for (int i = threadIdx.x; i <= 2 * p.reach; i += kGenThreads)
-        bias[i] = table_at<A>(p, __ldg(p.lut + i), h);
+        bias[i] = bias2_at<A>(p, __ldg(p.lut + i), h);
 }
 __device__ __forceinline__ int distance_at(const Params& p, int rel) {
     return min(max(rel, -p.reach), p.reach) + p.reach;

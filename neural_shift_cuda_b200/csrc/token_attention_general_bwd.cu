@@ -2,7 +2,7 @@
 // type, stride and head width, and the two small kernels around every
 // backward pass (see token_attention_general.cuh).
 //
-// With P = e^(s - lse), dP = dO V^T and delta_i = sum_d dO_id O_id - dlse_i:
+// With P the softmax weights, dP = dO V^T and delta_i = sum_d dO_id O_id - dlse_i:
 //     dz = P (dP - delta)                       (gradient at the biased score)
 //     dtable[u] = sum of dz over the pairs whose distance is in bucket u
 //     ds = dz (1 - tanh^2) scale                (gradient at q.k)
@@ -19,21 +19,21 @@ namespace nsc {
 namespace tok {
 namespace {
 
-// The softmax weight and score gradients of one pair.
+// The softmax weight and score gradients of one pair: s2 = unit x + bias with
+// x the product, or its tanh; m and ll are the forward's row statistics.
 template <typename A> struct Pair { A p, dz, ds; };
 
 template <typename A>
-__device__ __forceinline__ Pair<A> pair_grad(A dot, A dp, A bias, A lse, A delta, bool seen,
-                                             A scale, A cap, A icap) {
+__device__ __forceinline__ Pair<A> pair_grad(A dot, A dp, A bias, A m, A ll, A delta, bool seen,
+                                             A scale, A unit, A y1) {
     Pair<A> r{0, 0, 0};
-    if (!seen || lse == ninf<A>()) return r;
-    A x = dot * scale, slope = scale;
-    if (cap > 0) {
-        const A t = tanh_(x * icap);
-        x = cap * t;
-        slope = scale * (1 - t * t);
+    if (!seen || m == ninf<A>()) return r;
+    A x = dot, slope = scale;
+    if (y1 != A(0)) {
+        x = tanh_(dot * y1);
+        slope = scale * (1 - x * x);
     }
-    r.p = exp_(x + bias - lse);
+    r.p = exp2_(x * unit + bias - m - ll);
     r.dz = r.p * (dp - delta);
     r.ds = r.dz * slope;
     return r;
@@ -65,16 +65,18 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
     const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
 
     int lo[MI], hi[MI], slo = INT_MAX, shi = 0;
-    A lse[MI], delta[MI];
+    A m[MI], ll[MI], delta[MI];
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         const int row = q0 + ty + 16 * i;
         lo[i] = hi[i] = 0;
-        lse[i] = delta[i] = 0;
+        m[i] = ll[i] = delta[i] = 0;
         if (row < p.Lq) {
             key_span(p, b, row, p.Lk, lo[i], hi[i]);
-            lse[i] = static_cast<const A*>(p.lse)[static_cast<int64_t>(bh) * p.Lq + row];
-            delta[i] = static_cast<const A*>(gr.delta)[static_cast<int64_t>(bh) * p.Lq + row];
+            const int64_t at = static_cast<int64_t>(bh) * p.Lq + row;
+            m[i] = static_cast<const A*>(p.stats)[at];
+            ll[i] = static_cast<const A*>(p.stats)[BH * p.Lq + at];
+            delta[i] = static_cast<const A*>(gr.delta)[at];
         }
         if (hi[i] > lo[i]) { slo = min(slo, lo[i]); shi = max(shi, hi[i]); }
     }
@@ -92,7 +94,8 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
 #pragma unroll
             for (int e = 0; e < G::VEC; ++e) dq[i][g][e] = 0;
     A mine = 0;  // bucket threadIdx.x of the table gradient
-    const A scale = p.scale, cap = p.cap, icap = p.cap > 0 ? 1 / p.cap : 0;
+    const A scale = p.scale, unit = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
+    const A y1 = p.cap > 0 ? p.scale / p.cap : 0;
     for (int k0 = first / TL * TL; k0 < last; k0 += TL) {
         __syncthreads();
         const bool odd = load_tile<T, A, DP, TL>(Ks, k, p.ks[1], k0, first, last, p.D);
@@ -107,8 +110,8 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
             for (int j = 0; j < MI; ++j) {
                 const int key = k0 + tx + 16 * j;
                 const A bi = p.table ? bias[distance_at(p, key - (q0 + ty + 16 * i + off))] : A(0);
-                const Pair<A> r = pair_grad<A>(s[i][j], dp[i][j], bi, lse[i], delta[i],
-                                               key >= lo[i] && key < hi[i], scale, cap, icap);
+                const Pair<A> r = pair_grad<A>(s[i][j], dp[i][j], bi, m[i], ll[i], delta[i],
+                                               key >= lo[i] && key < hi[i], scale, unit, y1);
                 s[i][j] = r.ds;
                 Ps[(ty + 16 * i) * G::LP + tx + 16 * j] = gr.tab ? r.dz : r.ds;
             }
@@ -166,7 +169,7 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
     constexpr int MI = G::MI;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int box[2];
-    __shared__ A lses[TL], deltas[TL];
+    __shared__ A ms[TL], lls[TL], deltas[TL];
     A* Ks = reinterpret_cast<A*>(smem_raw);
     A* Vs = Ks + TL * G::LD;
     A* Qs = Vs + TL * G::LD;
@@ -201,7 +204,8 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
         for (int g = 0; g < G::NG; ++g)
 #pragma unroll
             for (int e = 0; e < G::VEC; ++e) dk[i][g][e] = dv[i][g][e] = 0;
-    const A scale = p.scale, cap = p.cap, icap = p.cap > 0 ? 1 / p.cap : 0;
+    const A scale = p.scale, unit = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
+    const A y1 = p.cap > 0 ? p.scale / p.cap : 0;
     for (int u = 0; u < p.G; ++u) {
         const int h = hk * p.G + u;
         const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2];
@@ -215,7 +219,10 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
             odd |= load_tile<T, A, DP, TL>(Os, go, gr.dos[1], q0, first, last, p.D);
             if (threadIdx.x < TL) {
                 const int row = q0 + threadIdx.x;
-                lses[threadIdx.x] = row < p.Lq ? static_cast<const A*>(p.lse)[row0 + row] : 0;
+                const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Lq;
+                ms[threadIdx.x] = row < p.Lq ? static_cast<const A*>(p.stats)[row0 + row] : 0;
+                lls[threadIdx.x] =
+                    row < p.Lq ? static_cast<const A*>(p.stats)[rows + row0 + row] : 0;
                 deltas[threadIdx.x] =
                     row < p.Lq ? static_cast<const A*>(gr.delta)[row0 + row] : 0;
             }
@@ -229,8 +236,8 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
                 for (int j = 0; j < MI; ++j) {
                     const int r = ty + 16 * i, c = tx + 16 * j, row = q0 + r;
                     const A bi = p.table ? bias[distance_at(p, k0 + c - (row + off))] : A(0);
-                    const Pair<A> g = pair_grad<A>(s[i][j], dp[i][j], bi, lses[r], deltas[r],
-                                                   row >= lo[j] && row < hi[j], scale, cap, icap);
+                    const Pair<A> g = pair_grad<A>(s[i][j], dp[i][j], bi, ms[r], lls[r], deltas[r],
+                                                   row >= lo[j] && row < hi[j], scale, unit, y1);
                     Ps[c * G::LP + r] = g.p;
                     Ss[c * G::LP + r] = g.ds;
                 }
@@ -266,9 +273,14 @@ __global__ __launch_bounds__(256) void delta_kernel(Params p, Grads gr) {
     const int h = static_cast<int>(w % p.Hq);
     const int64_t bl = w / p.Hq, b = bl / p.Lq, l = bl % p.Lq;
     const T* o = static_cast<const T*>(p.out) + w * p.D;
+    const T* lo = p.residue ? static_cast<const T*>(p.residue) + w * p.D : nullptr;
     const T* g = static_cast<const T*>(gr.dout) + b * gr.dos[0] + l * gr.dos[1] + h * gr.dos[2];
     A sum = 0;
-    for (int d = lane; d < p.D; d += 32) sum += static_cast<A>(to_acc(o[d])) * static_cast<A>(to_acc(g[d]));
+    for (int d = lane; d < p.D; d += 32) {
+        A x = to_acc(o[d]);
+        if (lo) x += to_acc(lo[d]);
+        sum += x * static_cast<A>(to_acc(g[d]));
+    }
 #pragma unroll
     for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
     if (lane == 0) {

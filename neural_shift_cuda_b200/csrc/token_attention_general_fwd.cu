@@ -3,7 +3,7 @@
 //
 // One block per (query tile, head, batch entry).  Keys pass tile by tile with
 // the running maximum and sum of a softmax: when the maximum m of a row moves
-// to m', its sum and its output row are scaled by e^(m - m').
+// to m', its sum and its output row are scaled by 2^(m - m').
 #include <climits>
 
 #include "token_attention_general.cuh"
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kGenThreads) void general_fwd_kernel(Params p) {
 #pragma unroll
             for (int e = 0; e < G::VEC; ++e) o[i][g][e] = 0;
     }
-    const A scale = p.scale, cap = p.cap, icap = p.cap > 0 ? 1 / p.cap : 0;
+    const A unit = (p.cap > 0 ? p.cap : p.scale) * kLog2e, y1 = p.cap > 0 ? p.scale / p.cap : 0;
     for (int k0 = first / TL * TL; k0 < last; k0 += TL) {
         __syncthreads();
         load_tile<T, A, DP, TL>(Ks, k, p.ks[1], k0, first, last, p.D);
@@ -73,8 +73,7 @@ __global__ __launch_bounds__(kGenThreads) void general_fwd_kernel(Params p) {
 #pragma unroll
             for (int j = 0; j < MI; ++j) {
                 const int key = k0 + tx + 16 * j;
-                A x = s[i][j] * scale;
-                if (cap > 0) x = cap * tanh_(x * icap);
+                A x = (p.cap > 0 ? tanh_(s[i][j] * y1) : s[i][j]) * unit;
                 if (p.table) x += bias[distance_at(p, rel0 + 16 * j)];
                 s[i][j] = key >= lo[i] && key < hi[i] ? x : ninf<A>();
                 top = s[i][j] > top || s[i][j] != s[i][j] ? s[i][j] : top;
@@ -86,11 +85,11 @@ __global__ __launch_bounds__(kGenThreads) void general_fwd_kernel(Params p) {
             }
             const A mn = m[i] > top ? m[i] : top;
             const A ref = mn == ninf<A>() ? A(0) : mn;
-            const A corr = exp_(m[i] - ref);
+            const A corr = exp2_(m[i] - ref);
             A sum = 0;
 #pragma unroll
             for (int j = 0; j < MI; ++j) {
-                const A e = exp_(s[i][j] - ref);
+                const A e = exp2_(s[i][j] - ref);
                 sum += e;
                 Ps[(ty + 16 * i) * G::LP + tx + 16 * j] = e;
             }
@@ -111,18 +110,22 @@ __global__ __launch_bounds__(kGenThreads) void general_fwd_kernel(Params p) {
         const int row = q0 + ty + 16 * i;
         if (row >= p.Lq) continue;
         const A inv = l[i] == A(0) ? A(0) : 1 / l[i];
-        T* dst = static_cast<T*>(p.out) +
-                 ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
+        const int64_t at = ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
+        T* dst = static_cast<T*>(p.out) + at;
 #pragma unroll
         for (int g = 0; g < G::NG; ++g)
 #pragma unroll
             for (int e = 0; e < G::VEC; ++e) {
                 const int d = (g * 16 + tx) * G::VEC + e;
-                if (d < p.D) dst[d] = store_as<T>(o[i][g][e] * inv);
+                if (d >= p.D) continue;
+                const A x = o[i][g][e] * inv;
+                const T y = store_as<T>(x);
+                dst[d] = y;
+                if (p.residue) static_cast<T*>(p.residue)[at + d] = store_as<T>(x - to_acc(y));
             }
-        if (p.lse && tx == 0)
-            static_cast<A*>(p.lse)[static_cast<int64_t>(bh) * p.Lq + row] =
-                l[i] == A(0) ? ninf<A>() : m[i] + static_cast<A>(log(static_cast<double>(l[i])));
+        if (tx == 0)
+            row_stats<A>(p, static_cast<int64_t>(bh) * p.Lq + row, m[i], log2_(l[i]),
+                         l[i] == A(0));
     }
 }
 

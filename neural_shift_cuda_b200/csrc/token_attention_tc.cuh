@@ -1,0 +1,157 @@
+// token_attention_tc.cuh -- what the tensor-core kernels of token attention
+// share: tensor maps of (B, L, H, D) operands, the guard against values that
+// are not finite, score arithmetic, and bounded waits.
+#pragma once
+
+#include <climits>
+
+#include "nsc_tcgen05.cuh"
+#include "token_attention.h"
+
+namespace nsc {
+namespace tok {
+
+constexpr int kRows = 128;            // rows of a tile: lanes of tensor memory
+constexpr int kPanel = kRows * 128;   // bytes of a panel: 128 rows of 64 16-bit elements
+constexpr int kBiasPad = 160;         // distances past the reach that a tile's rows meet
+
+struct Bounded {                      // wait accounting of a launch
+    unsigned* timeouts;
+    int skip;                         // test hook: a copy left unissued
+    unsigned budget;
+};
+
+// As mbar_wait32_ab, all in line: a call would have to keep to the caller's
+// registers, which the warps of a kernel that shares them out do not have alike.
+__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, unsigned* timeouts,
+                                             volatile int* abort_flag) {
+    const uint32_t a = smem_u32(bar);
+    if (mbar_try_wait32(a, parity)) return true;
+    const uint32_t budget = static_cast<uint32_t>(abort_flag[1]);
+    for (uint32_t i = 0; i < budget; ++i) {
+        if (mbar_try_wait_sleep32(a, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    atomicAdd(timeouts, 1u);
+    *abort_flag = 1;
+    return false;
+}
+
+// Coordinates of a (B, L, H, D) tensor map: {D, H, L, B}, boxes of 64 x 128 rows.
+bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, int B, int L, int H,
+                  int D, bool bf16, const char** err);
+
+// Prepares a kernel's shared memory, and refuses one whose launch would hold fewer
+// registers than its warps ask for when they share them out (they would wait
+// for good).
+nsc_status tc_ready(const void* kern, int smem, int threads, int registers);
+
+template <typename T, int DP> nsc_status tc_fwd_run(const Params& p, cudaStream_t st);
+
+// A tile: 128 rows from `row` of head `h`, DP / 64 panels.
+template <int DP>
+__device__ __forceinline__ void load_rows(unsigned char* dst, const CUtensorMap* map, uint64_t* bar,
+                                          int h, int row, int b) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * kPanel, map, bar, 64 * c, h, row, b);
+}
+
+// Sees to it that rows of a landed tile that hold an infinity or NaN do not
+// reach products as anything but zero: a weight of zero does not hide them.
+// `lanes` threads, thread t has rows t, t + lanes, ...; returns a bit for each of
+// its rows (in that order) that held such a value.  x 0 is 0 or NaN, so one
+// multiply-add per two values finds them.
+template <typename T, int DP>
+__device__ __forceinline__ uint32_t scrub_rows(unsigned char* tile, int t, int lanes) {
+    uint32_t bad = 0;
+    int bit = 0;
+    for (int r = t; r < kRows; r += lanes, ++bit) {
+        using T2 = typename std::conditional<sizeof(T) == 2 && std::is_same<T, __half>::value,
+                                             __half2, __nv_bfloat162>::type;
+        T2 acc;
+        reinterpret_cast<uint32_t&>(acc) = 0;
+        T2 zero = acc;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+            const uint4* row = reinterpret_cast<const uint4*>(tile + c * kPanel + r * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint4 v = row[(i + r) & 7];
+                acc = __hfma2(reinterpret_cast<const T2&>(v.x), zero, acc);
+                acc = __hfma2(reinterpret_cast<const T2&>(v.y), zero, acc);
+                acc = __hfma2(reinterpret_cast<const T2&>(v.z), zero, acc);
+                acc = __hfma2(reinterpret_cast<const T2&>(v.w), zero, acc);
+            }
+        }
+        const uint32_t w = reinterpret_cast<const uint32_t&>(acc);
+        if ((w & 0x7FFF7FFFu) == 0) continue;
+        bad |= 1u << bit;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+            uint4* row = reinterpret_cast<uint4*>(tile + c * kPanel + r * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    return bad;
+}
+// Fills row r of a tile with NaN.
+template <int DP>
+__device__ __forceinline__ void poison_row(unsigned char* tile, int r) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+        uint4* row = reinterpret_cast<uint4*>(tile + c * kPanel + r * 128);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+    }
+}
+__device__ __forceinline__ void fence_async_shared() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// tanh of the 32 products of a chunk times y1, in place.  Up to |y| = 1 an odd
+// polynomial: y P(y^2), P of least maximum error of y P(y^2) against tanh y by
+// exchange (2.4e-7), on pairs in the packed FMA pipe and off the exponential unit
+// that bounds these kernels.  A warp with a larger value in the chunk takes
+// tanh |y| = 1 - 2 / (1 + e^(2|y|)) for all of it.
+__device__ __forceinline__ void tanh32(float2* s, float y1) {
+    const float2 k = make_float2(y1, y1);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        s[i] = __fmul2_rn(s[i], k);
+        top = fmaxf(top, fmaxf(fabsf(s[i].x), fabsf(s[i].y)));
+    }
+    if (!__any_sync(0xffffffffu, top > 1.f)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 u = __fmul2_rn(s[i], s[i]);
+            float2 p = make_float2(-0.002839466166f, -0.002839466166f);
+            p = __ffma2_rn(p, u, make_float2(0.01611418278f, 0.01611418278f));
+            p = __ffma2_rn(p, u, make_float2(-0.05097286522f, -0.05097286522f));
+            p = __ffma2_rn(p, u, make_float2(0.1325352535f, 0.1325352535f));
+            p = __ffma2_rn(p, u, make_float2(-0.3332400381f, -0.3332400381f));
+            p = __ffma2_rn(p, u, make_float2(0.9999968539f, 0.9999968539f));
+            s[i] = __fmul2_rn(s[i], p);
+        }
+        return;
+    }
+    float* f = reinterpret_cast<float*>(s);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float e = tc::ex2(fabsf(f[i]) * static_cast<float>(2 * kLog2e));
+        f[i] = copysignf(1.f - __fdividef(2.f, 1.f + e), f[i]);
+    }
+}
+
+// Bias of head h by clamped distance, with kBiasPad more of the end values at
+// each end: E[distance + reach + kBiasPad].
+__device__ __forceinline__ void load_padded_bias(const Params& p, int h, float* E, int t, int n) {
+    for (int i = t; i <= 2 * p.reach + 2 * kBiasPad; i += n) {
+        const int d = min(max(i - kBiasPad, 0), 2 * p.reach);
+        E[i] = bias2_at<float>(p, __ldg(p.lut + d), h);
+    }
+}
+
+}  // namespace tok
+}  // namespace nsc

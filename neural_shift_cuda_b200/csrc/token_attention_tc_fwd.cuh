@@ -1,0 +1,421 @@
+// token_attention_tc_fwd.cuh -- forward of token attention on the tensor
+// cores, fp16 / bf16, head widths up to 128.
+//
+// A block owns two tiles of 128 queries: two heads that share a key head at the
+// same queries (one load of K and V serves both), or 256 queries of one head.
+// Roles by warp: 0-3 and 4-7 the softmax of a tile each, a thread a row; 8 loads K
+// and V blocks of 128 keys through a ring by TMA; 9 issues the products; 10 and
+// 11 guard (below).  Tensor memory holds S of both tiles (P takes the place of
+// its S as 16-bit pairs) and both O.  The products are issued in the order
+// PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1), so one tile's products run beside the
+// other's softmax; they complete in order, so S(j+1) full also says that
+// PV(j) is done and O may be rescaled.
+//
+// Softmax with a running reference m: p = 2^(s2 - m); m moves, and O is
+// rescaled, only when a row's maximum passes m + 8 (p <= 256 keeps 16-bit
+// weights in range), which after the first blocks is rare.  P is rounded to the
+// operand type; the sum of a row is of the fp32 values.
+//
+// Guard: in blocks that some row of a tile does not see whole, a value row
+// that is not finite would reach every row as 0 x NaN.  There the guard warps
+// look each landed V block over; such a row becomes zero in V and NaN in K,
+// so that the rows that see it still give NaN, by their scores.
+//
+// Work per score: one exponential (16 a clock and SM) against D / 32
+// tensor-core clocks, so D = 64 is bounded by the exponentials and the FMA pipe
+// and D = 128 balances.
+#pragma once
+
+#include "token_attention_tc.cuh"
+
+namespace nsc {
+namespace tok {
+namespace {
+
+constexpr int kFwdThreads = 384;
+constexpr float kLazy = 8.f;
+
+template <int DP> struct FwdShape {
+    static constexpr int tile = DP / 64 * kPanel;             // bytes of a tile
+    static constexpr int stages = DP == 64 ? 4 : 2;           // K and V blocks in flight
+    static constexpr int smem = 2 * tile + stages * 2 * tile; // + bias + 1024 of alignment
+};
+
+struct FwdBars {
+    uint64_t q, k_full[4], v_full[4], empty[4], ok[4], s_full[2], p_full[2], o_full[2], drain;
+};
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
+    const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+    const __grid_constant__ CUtensorMap mv, const Params p, const int pair, const Bounded bnd) {
+    using S = FwdShape<DP>;
+    constexpr int NS = S::stages;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ FwdBars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag[2];
+    __shared__ int span[2][4];   // of a tile: least lo, most hi, most lo, least hi
+    unsigned char* smem = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* Qs = smem;                       // two tiles
+    unsigned char* KV = smem + 2 * S::tile;         // stages of K, V
+    float* E = reinterpret_cast<float*>(smem + S::smem);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // pair: tiles are heads h, h + 1 of one row block; else 256 rows of a head
+    const int HH = pair ? p.Hq / 2 : p.Hq;
+    const int64_t BH = static_cast<int64_t>(p.B) * HH;
+    const int nt = gridDim.x / BH;
+    const int t = nt - 1 - static_cast<int>(blockIdx.x / BH);
+    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / HH, h0 = (bh % HH) * (pair ? 2 : 1);
+    const int hk = h0 / p.G, n = keys_of(p, b);
+    const int q0 = t * (pair ? kRows : 2 * kRows);
+
+    if (threadIdx.x < 8) span[threadIdx.x >> 2][threadIdx.x & 3] =
+        (threadIdx.x & 3) == 0 || (threadIdx.x & 3) == 3 ? INT_MAX : 0;
+    if (threadIdx.x == 0) {
+        mbar_init(&bars.q, 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&bars.k_full[i], 1);
+            mbar_init(&bars.v_full[i], 1);
+            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.ok[i], 64);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_full[i], kRows);
+            mbar_init(&bars.o_full[i], 1);
+        }
+        mbar_init(&bars.drain, 1);
+        fence_mbar_init();
+        abort_flag[0] = 0;
+        abort_flag[1] = static_cast<int>(bnd.budget);
+    }
+    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    __syncthreads();
+
+    // the rows' spans, and those of the tiles
+    const int a = warp >> 2;   // tile of a softmax warp
+    const int row = q0 + (pair ? 0 : a * kRows) + static_cast<int>(threadIdx.x & 127);
+    int lo = 0, hi = 0;
+    if (warp < 8) {
+        if (row < p.Lq) key_span(p, b, row, n, lo, hi);
+        int v0 = hi > lo ? lo : INT_MAX, v1 = hi > lo ? hi : 0;
+        int v2 = hi > lo ? lo : 0, v3 = hi > lo ? hi : INT_MAX;
+        v0 = __reduce_min_sync(0xffffffffu, v0);
+        v1 = __reduce_max_sync(0xffffffffu, v1);
+        v2 = __reduce_max_sync(0xffffffffu, v2);
+        v3 = __reduce_min_sync(0xffffffffu, v3);
+        if (lane == 0) {
+            atomicMin(&span[a][0], v0);
+            atomicMax(&span[a][1], v1);
+            atomicMax(&span[a][2], v2);
+            atomicMin(&span[a][3], v3);
+        }
+    }
+    if (BIAS) load_padded_bias(p, h0, E, threadIdx.x, kFwdThreads);
+    if (BIAS && pair)
+        load_padded_bias(p, h0 + 1, E + 2 * p.reach + 2 * kBiasPad + 1, threadIdx.x, kFwdThreads);
+    __syncthreads();
+    const uint32_t tmem = tmem_slot;
+    int fb[2], lb[2];          // key blocks [fb, lb) of a tile
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool any = span[i][1] > span[i][0];
+        fb[i] = any ? span[i][0] / kRows : INT_MAX;
+        lb[i] = any ? (span[i][1] + kRows - 1) / kRows : 0;
+    }
+    const int j0 = min(fb[0], fb[1]), j1 = max(lb[0], lb[1]);
+    auto on = [&](int i, int j) { return j >= fb[i] && j < lb[i]; };
+    auto guarded = [&](int j) {
+        bool g = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            g |= on(i, j) && !(j * kRows >= span[i][2] && min((j + 1) * kRows, n) <= span[i][3]);
+        return g;
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
+    };
+    auto K_at = [&](int s) { return KV + s * 2 * S::tile; };
+    auto V_at = [&](int s) { return KV + s * 2 * S::tile + S::tile; };
+    const int steps = (p.D + 15) / 16;   // of 16 channels
+    const int cols = steps * 16;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + a * 128 + lane_base, to = tmem + 256 + a * DP + lane_base;
+        const int h = h0 + (pair ? a : 0);
+        const int pos = row + n - p.Lq;
+        const float* Eh = E + (pair && a ? 2 * p.reach + 2 * kBiasPad + 1 : 0);
+        const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
+        const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
+        float m = -INFINITY, l = 0.f;
+        bool alive = true;
+        int it = 0;
+        for (int j = fb[a]; j < lb[a]; ++j, ++it) {
+            alive = __all_sync(0xffffffffu, wait(&bars.s_full[a], it & 1));
+            if (!alive) break;
+            tc::fence_after();
+            float2 s[64];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc::load32(ts + 32 * c, reinterpret_cast<float*>(s + 16 * c));
+            tc::wait_ld();
+            const int k0 = j * kRows;
+            if (CAP) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tanh32(s + 16 * c, y1);
+            }
+            float mul = unit;
+            if (BIAS) {
+                mul = 1.f;
+                const int w0 = __shfl_sync(0xffffffffu, pos, 0);   // lanes at w0 .. w0 + 31
+                const float2 u2 = make_float2(unit, unit);
+                if (k0 + 127 - w0 <= -p.reach || k0 - w0 - 31 >= p.reach) {
+                    const float e = Eh[k0 > w0 ? 2 * p.reach + kBiasPad : kBiasPad];
+                    const float2 e2 = make_float2(e, e);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) s[i] = __ffma2_rn(s[i], u2, e2);
+                } else {
+                    const float* er = Eh + (k0 - pos + p.reach + kBiasPad);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        s[i] = __ffma2_rn(s[i], u2, make_float2(er[2 * i], er[2 * i + 1]));
+                }
+            }
+            if (!__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + kRows)) {
+                const uint32_t from = static_cast<uint32_t>(lo - k0);
+                const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    if (2 * i - from >= len) s[i].x = -INFINITY;
+                    if (2 * i + 1 - from >= len) s[i].y = -INFINITY;
+                }
+            }
+            float top = s[0].x;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaxf(s[i].x, s[i].y));
+            top *= mul;
+            // (a row may see nothing of its first blocks: m is then -inf still)
+            float keep = 1.f;
+            if (top > m + kLazy || m == -INFINITY) {
+                keep = m == -INFINITY ? 0.f : tc::ex2(m - top);
+                m = fmaxf(top, m);
+            }
+            if (it > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+                l *= keep;
+                const float2 k2 = make_float2(keep, keep);
+#pragma unroll 1
+                for (int c = 0; c < cols; c += 16) {
+                    float2 o[8];
+                    tc::load16(to + c, reinterpret_cast<float*>(o));
+                    tc::wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = __fmul2_rn(o[i], k2);
+                    tc::store16(to + c, reinterpret_cast<uint32_t*>(o));
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : -m;
+            const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(ref, ref);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x = __ffma2_rn(s[16 * c + i], mul2, ref2);
+                    const float2 e = make_float2(tc::ex2(x.x), tc::ex2(x.y));
+                    sum = __fadd2_rn(sum, e);
+                    w[i] = tc::pack2<T>(e.x, e.y);
+                }
+                tc::store16(ts + 16 * c, w);
+            }
+            l += sum.x + sum.y;
+            tc::wait_st();
+            tc::fence_before();
+            mbar_arrive(&bars.p_full[a]);
+        }
+        // the row's output
+        const bool worked = lb[a] > fb[a];
+        if (alive && worked) alive = __all_sync(0xffffffffu, wait(&bars.o_full[a], 0));
+        if (alive) {
+            tc::fence_after();
+            const bool none = l == 0.f;
+            const float inv = none ? 0.f : 1.f / l;
+            const int64_t at = ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 32) {
+                float o[32];
+                if (worked) {
+                    tc::load32(to + c, o);
+                    tc::wait_ld();
+                }
+                if (row >= p.Lq) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (c + i >= p.D) break;
+                    uint32_t w[4], r[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = none ? 0.f : o[i + 2 * e] * inv;
+                        const float y = none ? 0.f : o[i + 2 * e + 1] * inv;
+                        w[e] = tc::pack2<T>(x, y);
+                        const T* back = reinterpret_cast<const T*>(&w[e]);
+                        r[e] = tc::pack2<T>(x - to_acc(back[0]), y - to_acc(back[1]));
+                    }
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at + c + i) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                    if (p.residue)
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.residue) + at + c + i) =
+                            make_uint4(r[0], r[1], r[2], r[3]);
+                }
+            }
+            if (row < p.Lq)
+                row_stats<float>(p, (static_cast<int64_t>(b) * p.Hq + h) * p.Lq + row, m, log2f(l),
+                                 none);
+            tc::fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 8 && lane == 0 && j0 < j1) {
+            bool alive = true;
+            int copies = 0;
+            mbar_arrive_expect_tx(&bars.q, 2 * S::tile);
+            load_rows<DP>(Qs, &mq, &bars.q, h0, q0, b);
+            load_rows<DP>(Qs + S::tile, &mq, &bars.q, pair ? h0 + 1 : h0, pair ? q0 : q0 + kRows, b);
+            int issued = 0;
+            for (int j = j0; j < j1; ++j, ++issued) {
+                const int s = issued % NS;
+                if (issued >= NS) alive = wait(&bars.empty[s], (issued / NS - 1) & 1);
+                if (!alive) break;
+                mbar_arrive_expect_tx(&bars.k_full[s], S::tile);
+                if (copies++ == bnd.skip) { ++issued; break; }
+                load_rows<DP>(K_at(s), &mk, &bars.k_full[s], hk, j * kRows, b);
+                mbar_arrive_expect_tx(&bars.v_full[s], S::tile);
+                load_rows<DP>(V_at(s), &mv, &bars.v_full[s], hk, j * kRows, b);
+            }
+            // every copy has landed before the block may end
+            mbar_wait32(smem_u32(&bars.q), 0, bnd.timeouts);
+            for (int i = max(0, issued - NS); i < issued; ++i)
+                if (bnd.skip < 0 || i != bnd.skip) {
+                    mbar_wait32(smem_u32(&bars.k_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+                    mbar_wait32(smem_u32(&bars.v_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+                }
+        } else if (warp == 9 && lane == 0 && j0 < j1) {
+            const uint32_t iqk = tc::product(kBf16, 128, 128, false, false);
+            const uint32_t ipv = tc::product(kBf16, 128, cols, false, true);
+            bool alive = wait(&bars.q, 0);
+            int pn[2] = {0, 0};   // P tiles taken
+            uint32_t okp = 0;     // a bit a stage: the phase of its next guarded block
+            for (int j = j0 - 1; alive && j < j1; ++j) {
+                const int i = j - j0, s = (i + NS) % NS, sn = (i + 1) % NS;
+                const uint32_t parity = ((i + 1) / NS) & 1;
+                if (j + 1 < j1) {
+                    alive = wait(&bars.k_full[sn], parity);
+                    if (alive && guarded(j + 1)) {
+                        alive = wait(&bars.ok[sn], okp >> sn & 1);
+                        okp ^= 1u << sn;
+                    }
+                    if (!alive) break;
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (j >= j0 && on(x, j)) {
+                        alive = wait(&bars.v_full[s], (i / NS) & 1) && wait(&bars.p_full[x], pn[x] & 1);
+                        if (!alive) break;
+                        tc::fence_after();
+                        const uint32_t v = smem_u32(V_at(s));
+#pragma unroll 1
+                        for (int k = 0; k < 8; ++k)
+                            tc::mma_ts(tmem + 256 + x * DP, tmem + x * 128 + 8 * k,
+                                       tc::operand(v + k * 2048, kPanel), ipv, pn[x] > 0 || k > 0);
+                        ++pn[x];
+                        if (j + 1 == lb[x]) tc::commit(smem_u32(&bars.o_full[x]));
+                    }
+                    if (on(x, j + 1)) {
+                        const uint32_t q = smem_u32(Qs + x * S::tile), k = smem_u32(K_at(sn));
+#pragma unroll 1
+                        for (int c = 0; c < steps; ++c) {
+                            const uint32_t off = (c >> 2) * kPanel + (c & 3) * 32;
+                            tc::mma_ss(tmem + x * 128, tc::operand(q + off, 16),
+                                       tc::operand(k + off, 16), iqk, c > 0);
+                        }
+                        tc::commit(smem_u32(&bars.s_full[x]));
+                    }
+                }
+                if (alive && j >= j0) tc::commit(smem_u32(&bars.empty[s]));
+            }
+            if (!alive) {   // the products in flight read this block's memory
+                tc::commit(smem_u32(&bars.drain));
+                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
+            }
+        } else if (warp >= 10 && j0 < j1) {
+            const int g = threadIdx.x - 320;
+            int i = 0;
+            for (int j = j0; j < j1; ++j, ++i) {
+                if (!guarded(j)) continue;
+                const int s = i % NS;
+                const uint32_t parity = (i / NS) & 1;
+                if (!wait(&bars.k_full[s], parity) || !wait(&bars.v_full[s], parity)) break;
+                const uint32_t bad = scrub_rows<T, DP>(V_at(s), g, 64);
+                if (bad) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        if (bad >> r & 1) poison_row<DP>(K_at(s), g + 64 * r);
+                }
+                fence_async_shared();
+                mbar_arrive(&bars.ok[s]);
+            }
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc::fence_after();
+        tc::tmem_free(tmem, 512);
+    }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    auto kern = tc_fwd_kernel<T, DP, CAP, BIAS>;
+    const int pair = p.G % 2 == 0;
+    const int smem = FwdShape<DP>::smem + 1024 +
+                     (BIAS ? (pair ? 2 : 1) * 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0);
+    nsc_status ready = tc_ready(reinterpret_cast<const void*>(kern), smem, kFwdThreads,
+                                256 * 208 + 128 * 80);
+    if (ready != NSC_OK) return ready;
+    CUtensorMap mq, mk, mv;
+    const char* err = nullptr;
+    if (!encode_heads(&mq, p.q, p.qs, p.B, p.Lq, p.Hq, p.D, kBf16, &err) ||
+        !encode_heads(&mk, p.k, p.ks, p.B, p.Lk, p.Hkv, p.D, kBf16, &err) ||
+        !encode_heads(&mv, p.v, p.vs, p.B, p.Lk, p.Hkv, p.D, kBf16, &err))
+        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: %s", err);
+    Bounded bnd{wait_timeout_counter(), -1, 0};
+    if (!bnd.timeouts)
+        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: no wait counter");
+    wait_fault_settings(&bnd.skip, &bnd.budget);
+    const int rows = pair ? kRows : 2 * kRows;
+    const int64_t blocks =
+        static_cast<int64_t>((p.Lq + rows - 1) / rows) * p.B * (pair ? p.Hq / 2 : p.Hq);
+    kern<<<static_cast<unsigned>(blocks), kFwdThreads, smem, st>>>(mq, mk, mv, p, pair, bnd);
+    return check_launch("token_attention");
+}
+
+}  // namespace
+
+template <typename T, int DP>
+nsc_status tc_fwd_run(const Params& p, cudaStream_t st) {
+    if (p.cap > 0)
+        return p.table ? tc_fwd_launch<T, DP, true, true>(p, st)
+                       : tc_fwd_launch<T, DP, true, false>(p, st);
+    return p.table ? tc_fwd_launch<T, DP, false, true>(p, st)
+                   : tc_fwd_launch<T, DP, false, false>(p, st);
+}
+
+}  // namespace tok
+}  // namespace nsc

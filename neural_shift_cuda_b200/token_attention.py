@@ -70,6 +70,20 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _tiled(t: torch.Tensor) -> torch.Tensor:
+    """t in a layout the tensor-core kernels can load: unit stride in D, and for
+    16-bit types a 16-byte aligned start and strides (a copy where it is not;
+    the FMA kernels that read any layout would cost far more)."""
+    t = _unit(t)
+    if t.element_size() != 2 or t.shape[3] % 8 or t.shape[3] > 128:
+        return t
+    if t.data_ptr() % 16 == 0 and all(
+            n == 1 or (s > 0 and s % 8 == 0)
+            for n, s in zip(t.shape[:3], t.stride()[:3])):
+        return t
+    return t.contiguous()
+
+
 def _int32(op: str, name: str, t: torch.Tensor, device) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{op}: {name} must be an int32 or int64 tensor")
@@ -258,25 +272,37 @@ def _attention_args(q, k, v, documents, prefix, lengths, table, buckets, scale,
 
 
 def _attention_fwd(q, k, v, documents, prefix, table, buckets, scale, cap, causal,
-                   want_lse):
+                   want_lse, train=False):
+    """(out, lse or None, stats or None, residue or None)"""
     B, Lq, Hq, D = q.shape
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    lse = (torch.empty((B, Hq, Lq), dtype=_acc(q.dtype), device=q.device)
-           if want_lse else None)
+    dev = q.device
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=dev)
+    lse = stats = residue = None
+    if want_lse:
+        lse = torch.empty((B, Hq, Lq), dtype=_acc(q.dtype), device=dev)
+    if train:
+        stats = torch.empty((2, B, Hq, Lq), dtype=_acc(q.dtype), device=dev)
+        if table is not None and q.element_size() == 2:
+            # a bucket sums the score gradients of many rows, each less its
+            # row's sum of grad_out * out: that of the rounded out would show
+            residue = torch.empty_like(out)
     a = _attention_args(q, k, v, documents, prefix, None, table, buckets, scale,
                         cap, causal)
-    with torch.cuda.device(q.device):
-        _lib.call("nsc_token_attention_fwd", _byref(a), _lib.ptr(out),
-                  _lib.ptr(lse), _lib.stream_of(q))
-    return out, lse
+    with torch.cuda.device(dev):
+        _lib.call("nsc_token_attention_fwd", _byref(a), _lib.ptr(out), _lib.ptr(lse),
+                  _lib.ptr(stats), _lib.ptr(residue), _lib.stream_of(q))
+    return out, lse, stats, residue
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, documents, prefix, table, buckets, scale, cap, causal):
-        out, lse = _attention_fwd(q, k, v, documents, prefix, table, buckets,
-                                  scale, cap, causal, True)
-        ctx.save_for_backward(q, k, v, out, lse, documents, prefix, table, buckets)
+    def forward(ctx, q, k, v, documents, prefix, table, buckets, scale, cap, causal,
+                want_lse):
+        out, lse, stats, residue = _attention_fwd(
+            q, k, v, documents, prefix, table, buckets, scale, cap, causal, want_lse,
+            True)
+        ctx.save_for_backward(q, k, v, out, stats, residue, documents, prefix, table,
+                              buckets)
         ctx.scale, ctx.cap, ctx.causal = scale, cap, causal
         ctx.set_materialize_grads(False)
         return out, lse
@@ -284,10 +310,11 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_lse):
-        q, k, v, out, lse, documents, prefix, table, buckets = ctx.saved_tensors
+        (q, k, v, out, stats, residue, documents, prefix, table,
+         buckets) = ctx.saved_tensors
         a = _attention_args(q, k, v, documents, prefix, None, table, buckets,
                             ctx.scale, ctx.cap, ctx.causal)
-        grad_out = torch.zeros_like(out) if grad_out is None else _unit(grad_out)
+        grad_out = torch.zeros_like(out) if grad_out is None else _tiled(grad_out)
         if grad_lse is not None:
             grad_lse = grad_lse.contiguous()
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -299,12 +326,12 @@ class _AttentionFn(torch.autograd.Function):
         g.grad_out_stride[:] = grad_out.stride()[:3]
         with torch.cuda.device(q.device):
             ws = _lib.workspace("nsc_token_attention_bwd_workspace", q.device, _byref(a))
-            g.out, g.lse, g.grad_out, g.grad_lse = (
-                _addr(out), _addr(lse), _addr(grad_out), _addr(grad_lse))
+            g.out, g.stats, g.residue = _addr(out), _addr(stats), _addr(residue)
+            g.grad_out, g.grad_lse = _addr(grad_out), _addr(grad_lse)
             g.grad_q, g.grad_k, g.grad_v = _addr(dq), _addr(dk), _addr(dv)
             g.grad_table, g.workspace = _addr(dt), _addr(ws)
             _lib.call("nsc_token_attention_bwd", _byref(a), _byref(g), _lib.stream_of(q))
-        return dq, dk, dv, None, None, dt, None, None, None, None
+        return dq, dk, dv, None, None, dt, None, None, None, None, None
 
 
 def _check_qkv(op, q, k, v, kname="k", vname="v"):
@@ -395,13 +422,13 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
             raise RuntimeError(f"{op}: prefix must be ({B},) or ({B}, {n}); got "
                                f"{tuple(prefix.shape)}")
     scale, cap = _numbers(q, scale, softcap)
-    args = (_unit(q), _unit(k), _unit(v), documents, prefix, table, buckets, scale,
-            cap, bool(causal))
+    args = (_tiled(q), _tiled(k), _tiled(v), documents, prefix, table, buckets, scale,
+            cap, bool(causal), return_lse)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (table is not None and table.requires_grad)):
         out, lse = _AttentionFn.apply(*args)
     else:
-        out, lse = _attention_fwd(*args, return_lse)
+        out, lse = _attention_fwd(*args)[:2]
     return (out, lse) if return_lse else out
 
 

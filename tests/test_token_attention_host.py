@@ -100,17 +100,17 @@ def test_entry_point_refusals(change, status, match):
     """Before any device is touched: the addresses here are not real."""
     lib = _lib.load()
     a = _att(**change)
-    assert lib.nsc_token_attention_fwd(ctypes.byref(a), None, None, None) == status
+    assert lib.nsc_token_attention_fwd(ctypes.byref(a), *[None] * 5) == status
     assert match in lib.nsc_last_error_string().decode()
     g = _lib.AttentionGrad()
     assert lib.nsc_token_attention_bwd(ctypes.byref(a), ctypes.byref(g), None) == status
-    assert lib.nsc_token_attention_fwd(None, None, None, None) == 1
+    assert lib.nsc_token_attention_fwd(*[None] * 6) == 1
 
 
 def test_empty_calls_are_noops():
     lib = _lib.load()
     a = _att(B=0)
-    assert lib.nsc_token_attention_fwd(ctypes.byref(a), None, None, None) == 0
+    assert lib.nsc_token_attention_fwd(ctypes.byref(a), *[None] * 5) == 0
     a = _att(B=0, causal=1)
     assert lib.nsc_token_attention_decode(ctypes.byref(a), None, None, None, None) == 0
     n = _lib.NormRotate()
