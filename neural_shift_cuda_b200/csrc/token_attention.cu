@@ -120,7 +120,9 @@ extern "C" NSC_API int64_t nsc_token_attention_bwd_workspace(const nsc_attention
     if (check("token_attention", a, false) != NSC_OK) return -1;
     int64_t n = align256(a->B * a->Hq * a->Lq * acc_size(a->dtype));
     if (a->table) n += align256(a->Hq * query_parts(a) * a->n_buckets * acc_size(a->dtype));
-    return n;
+    // whichever kernels the call will take
+    const int64_t tc = tc_bwd_workspace(a->B, a->Hq, a->Lq, a->table ? a->n_buckets : 0);
+    return n > tc ? n : tc;
 }
 
 extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
@@ -147,6 +149,8 @@ extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
     gr.dq = g->grad_q;
     gr.dk = g->grad_k;
     gr.dv = g->grad_v;
+    if (tc_bwd_fits(p, gr, a->dtype))
+        return tc_bwd(p, gr, g->workspace, g->grad_table, a->dtype, s);
     gr.delta = g->workspace;
     if (g->grad_table) {
         gr.n_part = rows ? query_parts(a) : 0;

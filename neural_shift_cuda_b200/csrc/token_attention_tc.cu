@@ -24,6 +24,58 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
+// The row records, 16 lanes a row, 16 bytes a lane.  Bound by memory: out,
+// residue and grad_out read once.
+template <typename T>
+__global__ __launch_bounds__(256) void record_kernel(Params p, Grads g, RowRec* recs, float* norms,
+                                                     int blocks_h) {
+    __shared__ float top[16];
+    const int bh = blockIdx.x / blocks_h, blk = blockIdx.x % blocks_h;
+    const int b = bh / p.Hq, h = bh % p.Hq, sub = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Lq;
+    float most = 0.f;
+#pragma unroll
+    for (int u = 0; u < kRecRows / 16; ++u) {
+        const int l = blk * kRecRows + 16 * u + sub;
+        float sum = 0.f, sq = 0.f;
+        if (l < p.Lq && 8 * c < p.D) {
+            const int64_t at = ((static_cast<int64_t>(b) * p.Lq + l) * p.Hq + h) * p.D + 8 * c;
+            const uint4 o = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + at));
+            const uint4 d = __ldg(reinterpret_cast<const uint4*>(
+                static_cast<const T*>(g.dout) + b * g.dos[0] + l * g.dos[1] + h * g.dos[2] + 8 * c));
+            uint4 r = make_uint4(0, 0, 0, 0);
+            if (p.residue)
+                r = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.residue) + at));
+            const T *op = reinterpret_cast<const T*>(&o), *dp = reinterpret_cast<const T*>(&d),
+                    *rp = reinterpret_cast<const T*>(&r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = to_acc(dp[i]);
+                sum += (to_acc(op[i]) + to_acc(rp[i])) * x;
+                sq += x * x;
+            }
+        }
+#pragma unroll
+        for (int i = 8; i; i >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, i);
+            sq += __shfl_xor_sync(0xffffffffu, sq, i);
+        }
+        if (c == 0 && l < p.Lq) {
+            const int64_t at = static_cast<int64_t>(bh) * p.Lq + l;
+            if (g.dlse) sum -= static_cast<const float*>(g.dlse)[at];
+            const float* stats = static_cast<const float*>(p.stats);
+            recs[at] = RowRec{stats[at] + (sum - sum), stats[rows + at], sum, sqrtf(sq)};
+            most = fmaxf(most, sqrtf(sq));
+        }
+    }
+    if (c == 0) top[sub] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
+        norms[blockIdx.x] = most;
+    }
+}
+
 bool aligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
 
 bool boxable(const int64_t* s, int B, int L, int H) {
@@ -97,6 +149,50 @@ nsc_status tc_fwd(const Params& p, int dtype, cudaStream_t st) {
         return p.D <= 64 ? tc_fwd_run<__nv_bfloat16, 64>(p, st)
                          : tc_fwd_run<__nv_bfloat16, 128>(p, st);
     return p.D <= 64 ? tc_fwd_run<__half, 64>(p, st) : tc_fwd_run<__half, 128>(p, st);
+}
+
+namespace {
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t rec_bytes(int64_t B, int64_t Hq, int64_t Lq) { return round256(B * Hq * Lq * sizeof(RowRec)); }
+int64_t norm_bytes(int64_t B, int64_t Hq, int64_t Lq) {
+    return round256(B * Hq * ((Lq + kRecRows - 1) / kRecRows) * sizeof(float));
+}
+}  // namespace
+
+int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t nb) {
+    return rec_bytes(B, Hq, Lq) + norm_bytes(B, Hq, Lq) +
+           (nb ? round256(Hq * B * ((Lq + kRows - 1) / kRows) * nb * sizeof(float)) : 0);
+}
+
+bool tc_bwd_fits(const Params& p, const Grads& g, int dtype) {
+    return tc_fits(p, dtype) && p.Lq > 0 && aligned(g.dout) && aligned(p.out) &&
+           aligned(p.residue) && aligned(g.dq) && aligned(g.dk) && aligned(g.dv) &&
+           boxable(g.dos, p.B, p.Lq, p.Hq);
+}
+
+nsc_status tc_bwd(const Params& p, Grads g, void* workspace, void* grad_table, int dtype,
+                  cudaStream_t st) {
+    char* w = static_cast<char*>(workspace);
+    RowRec* recs = reinterpret_cast<RowRec*>(w);
+    float* norms = reinterpret_cast<float*>(w + rec_bytes(p.B, p.Hq, p.Lq));
+    if (grad_table) {
+        g.tab = w + rec_bytes(p.B, p.Hq, p.Lq) + norm_bytes(p.B, p.Hq, p.Lq);
+        g.n_part = p.B * ((p.Lq + kRows - 1) / kRows);
+    }
+    const int n = (p.Lq + kRecRows - 1) / kRecRows;
+    const unsigned blocks = static_cast<unsigned>(p.B) * p.Hq * n;
+    if (dtype == NSC_BF16) record_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(p, g, recs, norms, n);
+    else record_kernel<__half><<<blocks, 256, 0, st>>>(p, g, recs, norms, n);
+    nsc_status r = check_launch("token_attention backward");
+    if (r != NSC_OK) return r;
+    if (dtype == NSC_BF16)
+        r = p.D <= 64 ? tc_bwd_run<__nv_bfloat16, 64>(p, g, recs, norms, n, st)
+                      : tc_bwd_run<__nv_bfloat16, 128>(p, g, recs, norms, n, st);
+    else
+        r = p.D <= 64 ? tc_bwd_run<__half, 64>(p, g, recs, norms, n, st)
+                      : tc_bwd_run<__half, 128>(p, g, recs, norms, n, st);
+    if (r == NSC_OK && grad_table) r = launch_table_join(p, g, grad_table, st);
+    return r;
 }
 
 }  // namespace tok

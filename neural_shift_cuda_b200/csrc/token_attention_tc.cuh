@@ -47,6 +47,14 @@ bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, in
 nsc_status tc_ready(const void* kern, int smem, int threads, int registers);
 
 template <typename T, int DP> nsc_status tc_fwd_run(const Params& p, cudaStream_t st);
+template <typename T, int DP>
+nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, const float* norms,
+                      int n_norm, cudaStream_t st);
+
+// A query row as the backward kernels read it: the forward's statistics (m NaN
+// where delta is not finite), delta, and the norm of its output gradient.
+struct RowRec { float m, ll, delta, norm; };
+constexpr int kRecRows = 32;   // rows of a record block, and of one entry of `norms`
 
 // A tile: 128 rows from `row` of head `h`, DP / 64 panels.
 template <int DP>

@@ -1,0 +1,839 @@
+// token_attention_tc_bwd.cuh -- backward of token attention on the tensor
+// cores, fp16 / bf16, head widths up to 128.  The formulas are those of
+// token_attention_general_bwd.cu; two kernels, no atomics.
+//
+// tc_dkv_kernel keeps 128 keys in place and passes the query tiles of every head
+// that shares the key head.  It works transposed (S^T = K Q^T, dP^T = V dO^T: a
+// thread's lane is a key), so that P^T and dS^T are left in tensor memory as the
+// A operands of dV = P^T dO and dK = dS^T Q, and Q and dO serve each as both
+// kinds of operand from one landed tile.  256 threads take half a row each, in
+// two phases: P from S, then dS from dP.  The products of one phase run beside
+// the other: dV(i), S(i+1) beside phase two of i, dK(i), dP(i+1) beside phase one of
+// i+1.  Four products a tile, 16 D clocks of the tensor pipe; tensor memory is
+// full at D = 128 (S, dP, dK, dV).
+//
+// tc_dq_kernel keeps 128 queries in place: S, dP, then dQ += dS K with dS in the
+// place of its S.  S has two buffers and dP is free once it is in registers, so
+// S(j+1) and dP(j+1) run beside the arithmetic of block j.  Recomputing the
+// scores here costs two of seven products and buys sums in one order without
+// an fp32 gradient in memory.
+//
+// fp16: weights and score gradients of long rows lie below its normal range.
+// P is held times 2^6 and the gradient of a row divided by a power of two near
+// the norm of its dO (dq) or the largest such norm of the key's queries (dkv);
+// both are undone in fp32 at the end.
+#pragma once
+
+#include "token_attention_tc.cuh"
+
+namespace nsc {
+namespace tok {
+namespace {
+
+constexpr int kBwdThreads = 384;
+constexpr float kPShift = 6.f;   // fp16: log2 of the factor of P
+
+template <int DP> struct BwdShape {
+    static constexpr int tile = DP / 64 * kPanel;
+    static constexpr int stages = DP == 64 ? 4 : 2;
+    static constexpr int smem = 2 * tile + stages * 2 * tile;
+};
+
+struct BwdBars {
+    uint64_t fixed, x_full[4], y_full[4], empty[4], ok[4];
+    uint64_t s_full, dp_full, p_ready, ds_ready, dp_free, done, drain;
+};
+
+__device__ __forceinline__ float pow2_near(float v) {   // a power of two at or above v, or 1
+    if (!(v > 0.f) || !(v < 3e38f)) return 1.f;
+    const int e = static_cast<int>((__float_as_uint(v) >> 23) & 0xFF) + 1;
+    return __uint_as_float(static_cast<uint32_t>(min(max(e, 20), 230)) << 23);
+}
+
+// x2 of 64 products of a thread: the score, less the row reference, in units of
+// log 2; `s` is left as the product (or its tanh).  Bias e[i] by `at(i)`.
+template <bool CAP>
+__device__ __forceinline__ void scores64(float2* s, float y1) {
+    if (CAP) {
+        tanh32(s, y1);
+        tanh32(s + 16, y1);
+    }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
+    const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mo,
+    const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p,
+    const Grads gr, const RowRec* __restrict__ recs, const float* __restrict__ norms, const int n_norm,
+    const Bounded bnd) {
+    using S = BwdShape<DP>;
+    constexpr int NS = S::stages;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ BwdBars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag[2];
+    __shared__ int span[4];
+    __shared__ unsigned top_norm;
+    // per stage: -m (or -(m + ll) without bias), -ll, delta g
+    __shared__ __align__(16) float rows[NS][3][kRows];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* Ks = smem;
+    unsigned char* Vs = smem + S::tile;
+    unsigned char* ring = smem + 2 * S::tile;   // stages of Q, dO
+    float* E = reinterpret_cast<float*>(smem + S::smem);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t BH = static_cast<int64_t>(p.B) * p.Hkv;
+    const int t = static_cast<int>(blockIdx.x / BH);
+    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hkv, hk = bh % p.Hkv;
+    const int k0 = t * kRows, off = p.Lk - p.Lq;
+
+    if (threadIdx.x < 4) span[threadIdx.x] = threadIdx.x == 0 || threadIdx.x == 3 ? INT_MAX : 0;
+    if (threadIdx.x == 0) {
+        mbar_init(&bars.fixed, 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&bars.x_full[i], 1);
+            mbar_init(&bars.y_full[i], 1);
+            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.ok[i], 64);
+        }
+        mbar_init(&bars.s_full, 1);
+        mbar_init(&bars.dp_full, 1);
+        mbar_init(&bars.p_ready, 256);
+        mbar_init(&bars.ds_ready, 256);
+        mbar_init(&bars.done, 1);
+        mbar_init(&bars.drain, 1);
+        fence_mbar_init();
+        abort_flag[0] = 0;
+        abort_flag[1] = static_cast<int>(bnd.budget);
+        top_norm = 0;
+    }
+    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    __syncthreads();
+    const int key = k0 + static_cast<int>(threadIdx.x & 127);
+    int lo = 0, hi = 0;
+    if (warp < 8) {
+        query_span(p, b, key, lo, hi);
+        const int v0 = __reduce_min_sync(0xffffffffu, hi > lo ? lo : INT_MAX);
+        const int v1 = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
+        const int v2 = __reduce_max_sync(0xffffffffu, hi > lo ? lo : 0);
+        const int v3 = __reduce_min_sync(0xffffffffu, hi > lo ? hi : INT_MAX);
+        if (lane == 0 && warp < 4) {
+            atomicMin(&span[0], v0);
+            atomicMax(&span[1], v1);
+            atomicMax(&span[2], v2);
+            atomicMin(&span[3], v3);
+        }
+    }
+    if (!kBf16) {   // the largest norm of dO among the heads of the group
+        float top = 0.f;
+        const float* src = norms + (static_cast<int64_t>(b) * p.Hq + hk * p.G) * n_norm;
+        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.G) * n_norm; i += kBwdThreads)
+            top = fmaxf(top, src[i]);
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        if (lane == 0) atomicMax(&top_norm, __float_as_uint(top));
+    }
+    __syncthreads();
+    const uint32_t tmem = tmem_slot;
+    const bool any = span[1] > span[0];
+    const int fb = any ? span[0] / kRows : 0, lb = any ? (span[1] + kRows - 1) / kRows : 0;
+    const int nq = lb - fb, total = nq * p.G;
+    const float g = kBf16 ? 1.f : pow2_near(__uint_as_float(top_norm));
+    // a key tail past Lk has zero rows of K and V, and sees nothing
+    auto guarded = [&](int j) {
+        return !(j * kRows >= span[2] && min((j + 1) * kRows, p.Lq) <= span[3]);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
+    };
+    auto Q_at = [&](int s) { return ring + s * 2 * S::tile; };
+    auto O_at = [&](int s) { return ring + s * 2 * S::tile + S::tile; };
+    const int steps = (p.D + 15) / 16, cols = steps * 16;
+    const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int half = warp >> 2;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t at_s = t_s + lane_base + 64 * half, at_dp = t_dp + lane_base + 64 * half;
+        const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
+        const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
+        const float2 u2 = make_float2(unit, unit), g2 = make_float2(1.f / g, 1.f / g);
+        bool alive = true;
+        int it = 0;
+        for (int u = 0; u < p.G && nq > 0; ++u) {
+            if (BIAS) {   // E of this head, once all are done with the last (a warp
+                          // that gave up comes here too)
+                named_sync(1, 256);
+                load_padded_bias(p, hk * p.G + u, E, threadIdx.x, 256);
+                named_sync(1, 256);
+            }
+            for (int j = fb; alive && j < lb; ++j, ++it) {
+                const int st = it % NS;
+                alive = __all_sync(0xffffffffu, wait(&bars.ok[st], (it / NS) & 1) &&
+                                                    wait(&bars.s_full, it & 1));
+                if (!alive) break;
+                tc::fence_after();
+                float2 s[32];
+                tc::load32(at_s, reinterpret_cast<float*>(s));
+                tc::load32(at_s + 32, reinterpret_cast<float*>(s + 16));
+                tc::wait_ld();
+                scores64<CAP>(s, y1);
+                const int q0 = j * kRows + 64 * half;
+                const float4* m4 = reinterpret_cast<const float4*>(rows[st][0] + 64 * half);
+                const float4* l4 = reinterpret_cast<const float4*>(rows[st][1] + 64 * half);
+                const bool whole = __all_sync(0xffffffffu, lo <= q0 && hi >= q0 + 64);
+                const uint32_t from = static_cast<uint32_t>(lo - q0);
+                const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
+                const int rel0 = key - (q0 + off);   // distance at column 0, one less a column
+                const int w0 = __shfl_sync(0xffffffffu, rel0, 0);
+                bool far = false;
+                float e_far = 0.f;
+                if (BIAS) {
+                    far = w0 + 31 <= -p.reach || w0 - 63 >= p.reach;
+                    if (far) e_far = E[w0 > 0 ? 2 * p.reach + kBiasPad : kBiasPad];
+                }
+                const float* er = E + rel0 + p.reach + kBiasPad;
+                uint32_t w[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float4 m = m4[i];
+                    float2 x0, x1;
+                    if (BIAS) {
+                        const float4 l = l4[i];
+                        float2 b0 = make_float2(e_far, e_far), b1 = b0;
+                        if (!far) {
+                            b0 = make_float2(er[-4 * i], er[-4 * i - 1]);
+                            b1 = make_float2(er[-4 * i - 2], er[-4 * i - 3]);
+                        }
+                        x0 = __fadd2_rn(__fadd2_rn(__ffma2_rn(s[2 * i], u2, b0), make_float2(m.x, m.y)),
+                                        make_float2(l.x, l.y));
+                        x1 = __fadd2_rn(__fadd2_rn(__ffma2_rn(s[2 * i + 1], u2, b1), make_float2(m.z, m.w)),
+                                        make_float2(l.z, l.w));
+                    } else {
+                        x0 = __ffma2_rn(s[2 * i], u2, make_float2(m.x, m.y));
+                        x1 = __ffma2_rn(s[2 * i + 1], u2, make_float2(m.z, m.w));
+                    }
+                    float2 p0 = make_float2(tc::ex2(x0.x), tc::ex2(x0.y));
+                    float2 p1 = make_float2(tc::ex2(x1.x), tc::ex2(x1.y));
+                    if (!whole) {
+                        if (4 * i - from >= len) p0.x = 0.f;
+                        if (4 * i + 1 - from >= len) p0.y = 0.f;
+                        if (4 * i + 2 - from >= len) p1.x = 0.f;
+                        if (4 * i + 3 - from >= len) p1.y = 0.f;
+                    }
+                    w[2 * i] = tc::pack2<T>(p0.x, p0.y);
+                    w[2 * i + 1] = tc::pack2<T>(p1.x, p1.y);
+                    if (CAP) {   // keep p (1 - tanh^2)
+                        const float2 n0 = __fmul2_rn(s[2 * i], make_float2(-s[2 * i].x, -s[2 * i].y));
+                        const float2 n1 = __fmul2_rn(s[2 * i + 1],
+                                                     make_float2(-s[2 * i + 1].x, -s[2 * i + 1].y));
+                        s[2 * i] = __ffma2_rn(p0, n0, p0);
+                        s[2 * i + 1] = __ffma2_rn(p1, n1, p1);
+                    } else {
+                        s[2 * i] = p0;
+                        s[2 * i + 1] = p1;
+                    }
+                }
+                tc::store32(at_s, w);
+                tc::wait_st();
+                tc::fence_before();
+                mbar_arrive(&bars.p_ready);
+
+                alive = __all_sync(0xffffffffu, wait(&bars.dp_full, it & 1));
+                if (!alive) break;
+                tc::fence_after();
+                float2 d[32];
+                tc::load32(at_dp, reinterpret_cast<float*>(d));
+                tc::load32(at_dp + 32, reinterpret_cast<float*>(d + 16));
+                tc::wait_ld();
+                const float4* d4 = reinterpret_cast<const float4*>(rows[st][2] + 64 * half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float4 dl = d4[i];
+                    float2 a0, a1;
+                    if (kBf16) {
+                        a0 = __fadd2_rn(d[2 * i], make_float2(dl.x, dl.y));
+                        a1 = __fadd2_rn(d[2 * i + 1], make_float2(dl.z, dl.w));
+                    } else {
+                        a0 = __ffma2_rn(d[2 * i], g2, make_float2(dl.x, dl.y));
+                        a1 = __ffma2_rn(d[2 * i + 1], g2, make_float2(dl.z, dl.w));
+                    }
+                    a0 = __fmul2_rn(a0, s[2 * i]);
+                    a1 = __fmul2_rn(a1, s[2 * i + 1]);
+                    if (!whole) {   // (a hidden pair's dP need not be finite)
+                        if (4 * i - from >= len) a0.x = 0.f;
+                        if (4 * i + 1 - from >= len) a0.y = 0.f;
+                        if (4 * i + 2 - from >= len) a1.x = 0.f;
+                        if (4 * i + 3 - from >= len) a1.y = 0.f;
+                    }
+                    w[2 * i] = tc::pack2<T>(a0.x, a0.y);
+                    w[2 * i + 1] = tc::pack2<T>(a1.x, a1.y);
+                }
+                tc::store32(at_dp, w);
+                tc::wait_st();
+                tc::fence_before();
+                mbar_arrive(&bars.ds_ready);
+            }
+        }
+        if (alive && total > 0) alive = __all_sync(0xffffffffu, wait(&bars.done, 0));
+        if (alive) {
+            tc::fence_after();
+            // first half of the warps: dV, second: dK
+            const uint32_t src = (half ? t_dk : t_dv) + lane_base;
+            const float back = kBf16 ? 1.f : 1.f / 64.f;
+            const float mul = half ? static_cast<float>(p.scale) * back * g : back;
+            T* dst = static_cast<T*>(half ? gr.dk : gr.dv) +
+                     ((static_cast<int64_t>(b) * p.Lk + key) * p.Hkv + hk) * p.D;
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 32) {
+                float o[32];
+                if (total > 0) {
+                    tc::load32(src + c, o);
+                    tc::wait_ld();
+                }
+                if (key >= p.Lk) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (c + i >= p.D) break;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = total > 0 && hi > lo
+                                   ? tc::pack2<T>(o[i + 2 * e] * mul, o[i + 2 * e + 1] * mul)
+                                   : 0u;
+                    *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            tc::fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 8 && lane == 0 && total > 0) {
+            bool alive = true;
+            mbar_arrive_expect_tx(&bars.fixed, 2 * S::tile);
+            load_rows<DP>(Ks, &mk, &bars.fixed, hk, k0, b);
+            load_rows<DP>(Vs, &mv, &bars.fixed, hk, k0, b);
+            int it = 0;
+            for (; it < total; ++it) {
+                const int s = it % NS, h = hk * p.G + it / nq, j = fb + it % nq;
+                if (it >= NS) alive = wait(&bars.empty[s], (it / NS - 1) & 1);
+                if (!alive) break;
+                mbar_arrive_expect_tx(&bars.x_full[s], S::tile);
+                if (it == bnd.skip) { ++it; break; }
+                load_rows<DP>(Q_at(s), &mq, &bars.x_full[s], h, j * kRows, b);
+                mbar_arrive_expect_tx(&bars.y_full[s], S::tile);
+                load_rows<DP>(O_at(s), &mo, &bars.y_full[s], h, j * kRows, b);
+            }
+            mbar_wait32(smem_u32(&bars.fixed), 0, bnd.timeouts);
+            for (int i = max(0, it - NS); i < it; ++i)
+                if (i != bnd.skip) {
+                    mbar_wait32(smem_u32(&bars.x_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+                    mbar_wait32(smem_u32(&bars.y_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+                }
+        } else if (warp == 9 && lane == 0 && total > 0) {
+            const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
+            const uint32_t its = tc::product(kBf16, 128, cols, false, true);
+            // [keys x queries] = A (keys) B (queries)^T over the channels
+            auto scores = [&](uint32_t d, unsigned char* A, unsigned char* B) {
+                const uint32_t a = smem_u32(A), q = smem_u32(B);
+#pragma unroll 1
+                for (int c = 0; c < steps; ++c) {
+                    const uint32_t o = (c >> 2) * kPanel + (c & 3) * 32;
+                    tc::mma_ss(d, tc::operand(a + o, 16), tc::operand(q + o, 16), iss, c > 0);
+                }
+            };
+            // [keys x channels] += W (keys x queries, tensor memory) B (queries x channels)
+            auto mix = [&](uint32_t d, uint32_t w, unsigned char* B, bool add) {
+                const uint32_t q = smem_u32(B);
+#pragma unroll 1
+                for (int k = 0; k < 8; ++k)
+                    tc::mma_ts(d, w + (k >> 2) * 64 + (k & 3) * 8, tc::operand(q + k * 2048, kPanel),
+                               its, add || k > 0);
+            };
+            bool alive = wait(&bars.fixed, 0);
+            for (int it = -1; alive && it < total; ++it) {
+                const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
+                const uint32_t pn = (next / NS) & 1;
+                if (it >= 0) {
+                    alive = wait(&bars.p_ready, it & 1);
+                    if (!alive) break;
+                    tc::fence_after();
+                    mix(t_dv, t_s, O_at(s), it > 0);
+                }
+                if (next < total) {
+                    alive = wait(&bars.x_full[sn], pn) &&
+                            (!guarded(fb + next % nq) || wait(&bars.ok[sn], pn));
+                    if (!alive) break;
+                    scores(t_s, Ks, Q_at(sn));
+                    tc::commit(smem_u32(&bars.s_full));
+                }
+                if (it >= 0) {
+                    alive = wait(&bars.ds_ready, it & 1);
+                    if (!alive) break;
+                    tc::fence_after();
+                    mix(t_dk, t_dp, Q_at(s), it > 0);
+                    tc::commit(smem_u32(&bars.empty[s]));
+                }
+                if (next < total) {
+                    alive = wait(&bars.y_full[sn], pn);
+                    if (!alive) break;
+                    scores(t_dp, Vs, O_at(sn));
+                    tc::commit(smem_u32(&bars.dp_full));
+                }
+            }
+            if (alive) tc::commit(smem_u32(&bars.done));
+            else {
+                tc::commit(smem_u32(&bars.drain));
+                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
+            }
+        } else if (warp >= 10 && total > 0) {
+            const int gt = threadIdx.x - 320;
+            for (int it = 0; it < total; ++it) {
+                const int s = it % NS, h = hk * p.G + it / nq, j = fb + it % nq;
+                const uint32_t parity = (it / NS) & 1;
+                const RowRec* src = recs + (static_cast<int64_t>(b) * p.Hq + h) * p.Lq;
+                float4 rec[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = j * kRows + gt + 64 * r;
+                    rec[r] = row < p.Lq ? __ldg(reinterpret_cast<const float4*>(src + row))
+                                        : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+                }
+                if (it >= NS && !wait(&bars.empty[s], (it / NS - 1) & 1)) break;
+                uint32_t bad = 0;
+                if (guarded(j)) {
+                    if (!wait(&bars.x_full[s], parity) || !wait(&bars.y_full[s], parity)) break;
+                    bad = scrub_rows<T, DP>(Q_at(s), gt, 64) | scrub_rows<T, DP>(O_at(s), gt, 64);
+                    fence_async_shared();
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int at = gt + 64 * r;
+                    float m = -rec[r].x, ll = -rec[r].y + (kBf16 ? 0.f : kPShift);
+                    if (rec[r].x == -INFINITY) m = -INFINITY;   // sees nothing: weight zero
+                    if (bad >> r & 1) m = NAN;
+                    rows[s][0][at] = BIAS ? m : m + ll;
+                    rows[s][1][at] = ll;
+                    rows[s][2][at] = -rec[r].z / g;
+                }
+                mbar_arrive(&bars.ok[s]);
+            }
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc::fence_after();
+        tc::tmem_free(tmem, 512);
+    }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
+    const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mo,
+    const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p,
+    const Grads gr, const RowRec* __restrict__ recs, const Bounded bnd) {
+    using S = BwdShape<DP>;
+    constexpr int NS = S::stages;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ BwdBars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag[2];
+    __shared__ int span[4];
+    __shared__ float diag[8][2][64], far_sum[8][2];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* Qs = smem;
+    unsigned char* Os = smem + S::tile;
+    unsigned char* ring = smem + 2 * S::tile;   // stages of K, V
+    float* E = reinterpret_cast<float*>(smem + S::smem);
+    float* acc = E + 2 * p.reach + 2 * kBiasPad + 1;   // table sums, 8 warps by buckets
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t BH = static_cast<int64_t>(p.B) * p.Hq;
+    const int nt = (p.Lq + kRows - 1) / kRows;
+    const int t = nt - 1 - static_cast<int>(blockIdx.x / BH);
+    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hq, h = bh % p.Hq;
+    const int hk = h / p.G, q0 = t * kRows, off = p.Lk - p.Lq;
+
+    if (threadIdx.x < 4) span[threadIdx.x] = threadIdx.x == 0 || threadIdx.x == 3 ? INT_MAX : 0;
+    if (threadIdx.x == 0) {
+        mbar_init(&bars.fixed, 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&bars.x_full[i], 1);
+            mbar_init(&bars.y_full[i], 1);
+            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.ok[i], 64);
+        }
+        mbar_init(&bars.s_full, 1);
+        mbar_init(&bars.dp_full, 1);
+        mbar_init(&bars.ds_ready, 256);
+        mbar_init(&bars.dp_free, 256);
+        mbar_init(&bars.done, 1);
+        mbar_init(&bars.drain, 1);
+        fence_mbar_init();
+        abort_flag[0] = 0;
+        abort_flag[1] = static_cast<int>(bnd.budget);
+    }
+    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    if (BIAS) {
+        load_padded_bias(p, h, E, threadIdx.x, kBwdThreads);
+        if (gr.tab)
+            for (int i = threadIdx.x; i < 8 * p.nb; i += kBwdThreads) acc[i] = 0.f;
+    }
+    __syncthreads();
+    const int row = q0 + static_cast<int>(threadIdx.x & 127);
+    int lo = 0, hi = 0;
+    if (warp < 8) {
+        if (row < p.Lq) key_span(p, b, row, p.Lk, lo, hi);
+        const int v0 = __reduce_min_sync(0xffffffffu, hi > lo ? lo : INT_MAX);
+        const int v1 = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
+        const int v2 = __reduce_max_sync(0xffffffffu, hi > lo ? lo : 0);
+        const int v3 = __reduce_min_sync(0xffffffffu, hi > lo ? hi : INT_MAX);
+        if (lane == 0 && warp < 4) {
+            atomicMin(&span[0], v0);
+            atomicMax(&span[1], v1);
+            atomicMax(&span[2], v2);
+            atomicMin(&span[3], v3);
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem = tmem_slot;
+    const bool any = span[1] > span[0];
+    const int fb = any ? span[0] / kRows : 0, lb = any ? (span[1] + kRows - 1) / kRows : 0;
+    const int total = lb - fb;
+    auto guarded = [&](int j) {
+        return !(j * kRows >= span[2] && min((j + 1) * kRows, p.Lk) <= span[3]);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
+    };
+    auto K_at = [&](int s) { return ring + s * 2 * S::tile; };
+    auto V_at = [&](int s) { return ring + s * 2 * S::tile + S::tile; };
+    const int steps = (p.D + 15) / 16, cols = steps * 16;
+    const uint32_t t_s = tmem, t_dp = tmem + 256, t_dq = tmem + 384;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int half = warp >> 2;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t at_s = t_s + lane_base + 64 * half, at_dp = t_dp + lane_base + 64 * half;
+        const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
+        const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
+        float m = -INFINITY, ll = 0.f, delta = 0.f, g = 1.f;
+        if (row < p.Lq) {
+            const float4 r = __ldg(reinterpret_cast<const float4*>(
+                recs + (static_cast<int64_t>(b) * p.Hq + h) * p.Lq + row));
+            if (!kBf16) g = pow2_near(r.w);
+            m = r.x == -INFINITY ? r.x : -r.x;
+            ll = -r.y + (kBf16 ? 0.f : kPShift);
+            delta = -r.z / g;
+        }
+        if (!BIAS) m += ll;
+        const float2 u2 = make_float2(unit, unit), g2 = make_float2(1.f / g, 1.f / g);
+        const float2 m2 = make_float2(m, m), l2 = make_float2(ll, ll), d2 = make_float2(delta, delta);
+        float far_lo = 0.f, far_hi = 0.f;
+        const float undo = kBf16 ? 1.f : g / 64.f;
+        bool alive = true;
+        int it = 0;
+        for (int j = fb; j < lb; ++j, ++it) {
+            alive = __all_sync(0xffffffffu, wait(&bars.dp_full, it & 1));
+            if (!alive) break;
+            tc::fence_after();
+            float2 s[32], d[32];
+            const uint32_t as = at_s + 128 * (it & 1);
+            tc::load32(at_dp, reinterpret_cast<float*>(d));
+            tc::load32(at_dp + 32, reinterpret_cast<float*>(d + 16));
+            tc::load32(as, reinterpret_cast<float*>(s));
+            tc::load32(as + 32, reinterpret_cast<float*>(s + 16));
+            tc::wait_ld();
+            tc::fence_before();
+            mbar_arrive(&bars.dp_free);
+            scores64<CAP>(s, y1);
+            const int k0 = j * kRows + 64 * half;
+            const bool whole = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 64);
+            const uint32_t from = static_cast<uint32_t>(lo - k0);
+            const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
+            const int rel0 = k0 - (row + off);   // distance at column 0, one more a column
+            const int w0 = __shfl_sync(0xffffffffu, rel0, 0);   // lane r: w0 - r
+            bool far = false;
+            float e_far = 0.f;
+            if (BIAS) {
+                far = w0 + 63 <= -p.reach || w0 - 31 >= p.reach;
+                if (far) e_far = E[w0 > 0 ? 2 * p.reach + kBiasPad : kBiasPad];
+            }
+            const float* er = E + rel0 + p.reach + kBiasPad;
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                float2 x;
+                if (BIAS) {
+                    float2 e = make_float2(e_far, e_far);
+                    if (!far) e = make_float2(er[2 * i], er[2 * i + 1]);
+                    x = __fadd2_rn(__fadd2_rn(__ffma2_rn(s[i], u2, e), m2), l2);
+                } else {
+                    x = __ffma2_rn(s[i], u2, m2);
+                }
+                const float2 pr = make_float2(tc::ex2(x.x), tc::ex2(x.y));
+                float2 z = kBf16 ? __fadd2_rn(d[i], d2) : __ffma2_rn(d[i], g2, d2);
+                z = __fmul2_rn(z, pr);
+                if (!whole) {
+                    if (2 * i - from >= len) z.x = 0.f;
+                    if (2 * i + 1 - from >= len) z.y = 0.f;
+                }
+                if (BIAS) d[i] = z;
+                if (CAP) {
+                    const float2 n = __fmul2_rn(s[i], make_float2(-s[i].x, -s[i].y));
+                    z = __ffma2_rn(z, n, z);
+                }
+                w[i] = tc::pack2<T>(z.x, z.y);
+            }
+            tc::store32(as, w);
+            tc::wait_st();
+            tc::fence_before();
+            mbar_arrive(&bars.ds_ready);
+            if (BIAS && gr.tab) {
+                if (far) {
+                    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum = __fadd2_rn(sum, d[i]);
+                    const float v = (sum.x + sum.y) * undo;
+                    if (w0 > 0) far_hi += v; else far_lo += v;
+                } else {
+                    // sums along the diagonals of the warp's 32 x 64 part, as two
+                    // squares side by side: a sum moves one lane up a column, and
+                    // is whole in lane 31, or where it is at the end.  Entry
+                    // 31 + c - r of a square.
+                    float a = 0.f, c = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float za = (i & 1) ? d[i >> 1].y : d[i >> 1].x;
+                        const float zc = (i & 1) ? d[16 + (i >> 1)].y : d[16 + (i >> 1)].x;
+                        a = __shfl_up_sync(0xffffffffu, a, 1);
+                        c = __shfl_up_sync(0xffffffffu, c, 1);
+                        a = fmaf(za, undo, lane == 0 ? 0.f : a);
+                        c = fmaf(zc, undo, lane == 0 ? 0.f : c);
+                        if (lane == 31) {
+                            diag[warp][0][i] = a;
+                            diag[warp][1][i] = c;
+                        }
+                    }
+                    if (lane < 31) {
+                        diag[warp][0][62 - lane] = a;
+                        diag[warp][1][62 - lane] = c;
+                    }
+                    __syncwarp();
+                    for (int u = lane; u < p.nb; u += 32) {
+                        float sum = 0.f;
+                        for (int i = 0; i < 95; ++i) {
+                            const int at = min(max(w0 + i - 31, -p.reach), p.reach) + p.reach;
+                            const int bu = min(max(__ldg(p.lut + at), 0), p.nb - 1);
+                            if (bu == u)
+                                sum += (i < 63 ? diag[warp][0][i] : 0.f) +
+                                       (i >= 32 ? diag[warp][1][i - 32] : 0.f);
+                        }
+                        acc[warp * p.nb + u] += sum;
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (BIAS && gr.tab) {
+#pragma unroll
+            for (int i = 16; i; i >>= 1) {
+                far_lo += __shfl_xor_sync(0xffffffffu, far_lo, i);
+                far_hi += __shfl_xor_sync(0xffffffffu, far_hi, i);
+            }
+            if (lane == 0) {
+                far_sum[warp][0] = far_lo;
+                far_sum[warp][1] = far_hi;
+            }
+        }
+        if (alive && total > 0) alive = __all_sync(0xffffffffu, wait(&bars.done, 0));
+        if (alive) {
+            tc::fence_after();
+            const float mul = static_cast<float>(p.scale) * undo;
+            T* dst = static_cast<T*>(gr.dq) +
+                     ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
+#pragma unroll 1
+            for (int c = 32 * half; c < cols; c += 64) {
+                float o[32];
+                if (total > 0) {
+                    tc::load32(t_dq + lane_base + c, o);
+                    tc::wait_ld();
+                }
+                if (row >= p.Lq) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (c + i >= p.D) break;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = total > 0 && hi > lo
+                                   ? tc::pack2<T>(o[i + 2 * e] * mul, o[i + 2 * e + 1] * mul)
+                                   : 0u;
+                    *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            tc::fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 8 && lane == 0 && total > 0) {
+            bool alive = true;
+            mbar_arrive_expect_tx(&bars.fixed, 2 * S::tile);
+            load_rows<DP>(Qs, &mq, &bars.fixed, h, q0, b);
+            load_rows<DP>(Os, &mo, &bars.fixed, h, q0, b);
+            int it = 0;
+            for (; it < total; ++it) {
+                const int s = it % NS, j = fb + it;
+                if (it >= NS) alive = wait(&bars.empty[s], (it / NS - 1) & 1);
+                if (!alive) break;
+                mbar_arrive_expect_tx(&bars.x_full[s], S::tile);
+                if (it == bnd.skip) { ++it; break; }
+                load_rows<DP>(K_at(s), &mk, &bars.x_full[s], hk, j * kRows, b);
+                mbar_arrive_expect_tx(&bars.y_full[s], S::tile);
+                load_rows<DP>(V_at(s), &mv, &bars.y_full[s], hk, j * kRows, b);
+            }
+            mbar_wait32(smem_u32(&bars.fixed), 0, bnd.timeouts);
+            for (int i = max(0, it - NS); i < it; ++i)
+                if (i != bnd.skip) {
+                    mbar_wait32(smem_u32(&bars.x_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+                    mbar_wait32(smem_u32(&bars.y_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+                }
+        } else if (warp == 9 && lane == 0 && total > 0) {
+            const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
+            const uint32_t its = tc::product(kBf16, 128, cols, false, true);
+            auto scores = [&](uint32_t d, unsigned char* A, unsigned char* B) {
+                const uint32_t a = smem_u32(A), q = smem_u32(B);
+#pragma unroll 1
+                for (int c = 0; c < steps; ++c) {
+                    const uint32_t o = (c >> 2) * kPanel + (c & 3) * 32;
+                    tc::mma_ss(d, tc::operand(a + o, 16), tc::operand(q + o, 16), iss, c > 0);
+                }
+            };
+            bool alive = wait(&bars.fixed, 0);
+            uint32_t okp = 0;
+            for (int it = -1; alive && it < total; ++it) {
+                const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
+                const uint32_t pn = (next / NS) & 1;
+                if (next < total) {
+                    alive = wait(&bars.x_full[sn], pn);
+                    if (alive && guarded(fb + next)) {
+                        alive = wait(&bars.ok[sn], okp >> sn & 1);
+                        okp ^= 1u << sn;
+                    }
+                    if (!alive) break;
+                    scores(t_s + 128 * (next & 1), Qs, K_at(sn));
+                    alive = wait(&bars.y_full[sn], pn) && (it < 0 || wait(&bars.dp_free, it & 1));
+                    if (!alive) break;
+                    tc::fence_after();
+                    scores(t_dp, Os, V_at(sn));
+                    tc::commit(smem_u32(&bars.dp_full));
+                }
+                if (it >= 0) {
+                    alive = wait(&bars.ds_ready, it & 1);
+                    if (!alive) break;
+                    tc::fence_after();
+                    const uint32_t k = smem_u32(K_at(s)), w = t_s + 128 * (it & 1);
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c)
+                        tc::mma_ts(t_dq, w + (c >> 2) * 64 + (c & 3) * 8,
+                                   tc::operand(k + c * 2048, kPanel), its, it > 0 || c > 0);
+                    tc::commit(smem_u32(&bars.empty[s]));
+                }
+            }
+            if (alive) tc::commit(smem_u32(&bars.done));
+            else {
+                tc::commit(smem_u32(&bars.drain));
+                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
+            }
+        } else if (warp >= 10 && total > 0) {
+            const int gt = threadIdx.x - 320;
+            for (int it = 0; it < total; ++it) {
+                if (!guarded(fb + it)) continue;
+                const int s = it % NS;
+                const uint32_t parity = (it / NS) & 1;
+                if (!wait(&bars.x_full[s], parity) || !wait(&bars.y_full[s], parity)) break;
+                const uint32_t bad = scrub_rows<T, DP>(K_at(s), gt, 64);
+                if (bad) {   // the rows that see it get NaN by dP
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        if (bad >> r & 1) poison_row<DP>(V_at(s), gt + 64 * r);
+                }
+                fence_async_shared();
+                mbar_arrive(&bars.ok[s]);
+            }
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    if (BIAS && gr.tab && static_cast<int>(threadIdx.x) < p.nb) {
+        const int u = threadIdx.x;
+        const int b_lo = min(max(__ldg(p.lut), 0), p.nb - 1);
+        const int b_hi = min(max(__ldg(p.lut + 2 * p.reach), 0), p.nb - 1);
+        float sum = 0.f;
+        for (int i = 0; i < 8; ++i) {
+            sum += acc[i * p.nb + u];
+            if (u == b_lo) sum += far_sum[i][0];
+            if (u == b_hi) sum += far_sum[i][1];
+        }
+        static_cast<float*>(gr.tab)[(static_cast<int64_t>(h) * gr.n_part + b * nt + t) * p.nb + u] = sum;
+    }
+    if (warp == 9) {
+        tc::fence_after();
+        tc::tmem_free(tmem, 512);
+    }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, const float* norms,
+                         int n_norm, cudaStream_t st) {
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    auto kk = tc_dkv_kernel<T, DP, CAP, BIAS>;
+    auto kq = tc_dq_kernel<T, DP, CAP, BIAS>;
+    const int e = BIAS ? 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0;
+    const int smk = BwdShape<DP>::smem + 1024 + e;
+    const int smq = smk + (BIAS && g.tab ? 4 * 8 * p.nb : 0);
+    const int regs = 256 * 208 + 128 * 80;
+    nsc_status ready = tc_ready(reinterpret_cast<const void*>(kk), smk, kBwdThreads, regs);
+    if (ready == NSC_OK) ready = tc_ready(reinterpret_cast<const void*>(kq), smq, kBwdThreads, regs);
+    if (ready != NSC_OK) return ready;
+    CUtensorMap mq, mo, mk, mv;
+    const char* err = nullptr;
+    if (!encode_heads(&mq, p.q, p.qs, p.B, p.Lq, p.Hq, p.D, kBf16, &err) ||
+        !encode_heads(&mo, g.dout, g.dos, p.B, p.Lq, p.Hq, p.D, kBf16, &err) ||
+        !encode_heads(&mk, p.k, p.ks, p.B, p.Lk, p.Hkv, p.D, kBf16, &err) ||
+        !encode_heads(&mv, p.v, p.vs, p.B, p.Lk, p.Hkv, p.D, kBf16, &err))
+        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention backward: %s", err);
+    Bounded bnd{wait_timeout_counter(), -1, 0};
+    if (!bnd.timeouts)
+        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention backward: no wait counter");
+    wait_fault_settings(&bnd.skip, &bnd.budget);
+    const int64_t nk = static_cast<int64_t>((p.Lk + kRows - 1) / kRows) * p.B * p.Hkv;
+    const int64_t nq = static_cast<int64_t>((p.Lq + kRows - 1) / kRows) * p.B * p.Hq;
+    kk<<<static_cast<unsigned>(nk), kBwdThreads, smk, st>>>(mq, mo, mk, mv, p, g, recs, norms, n_norm,
+                                                           bnd);
+    kq<<<static_cast<unsigned>(nq), kBwdThreads, smq, st>>>(mq, mo, mk, mv, p, g, recs, bnd);
+    return check_launch("token_attention backward");
+}
+
+}  // namespace
+
+template <typename T, int DP>
+nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, const float* norms,
+                      int n_norm, cudaStream_t st) {
+    const RowRec* r = static_cast<const RowRec*>(recs);
+    if (p.cap > 0)
+        return p.table ? tc_bwd_launch<T, DP, true, true>(p, g, r, norms, n_norm, st)
+                       : tc_bwd_launch<T, DP, true, false>(p, g, r, norms, n_norm, st);
+    return p.table ? tc_bwd_launch<T, DP, false, true>(p, g, r, norms, n_norm, st)
+                   : tc_bwd_launch<T, DP, false, false>(p, g, r, norms, n_norm, st);
+}
+
+}  // namespace tok
+}  // namespace nsc

@@ -1,0 +1,9 @@
+// Tensor-core token attention backward, f16, head widths up to 64.
+#include "token_attention_tc_bwd.cuh"
+
+namespace nsc {
+namespace tok {
+template nsc_status tc_bwd_run<__half, 64>(const Params&, const Grads&, const void*, const float*, int,
+                                         cudaStream_t);
+}  // namespace tok
+}  // namespace nsc

@@ -241,6 +241,25 @@ def test_what_is_not_seen_has_no_influence(cuda, dt, D, bad):
         assert (a[:, 290:] == 0).all()
 
 
+@pytest.mark.parametrize("dt,D", [(F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("mul", [2.0 ** -12, 1.0, 2.0 ** 8])
+def test_scale_of_the_output_gradient(cuda, dt, D, mul):
+    """Long uniform rows and small (or large) output gradients: weights and
+    score gradients far below the normal range of fp16, or near its end.
+    Powers of two scale the gradients and nothing else; what fp16 cannot
+    hold of them (below 2^-24) bounds the rest."""
+    q, k, v, go = (randn(i, 1, 1200, 2, D, dtype=dt, mul=m).to(cuda)
+                   for i, m in ((0, 0.3), (1, 0.3), (2, 1.0), (3, 1.0)))
+    go = go * mul
+    leaves = [leaf(t) for t in (q, k, v)]
+    got = torch.autograd.grad(nsc.token_attention(*leaves), leaves, go)
+    want = reference(q, k, v, T.visible(1, 1200, 1200), go, D ** -0.5)[2:5]
+    floor = 2.0 ** -24 if dt == F16 else 0.0
+    for g, w in zip(got, want):
+        d = (g.double() - w).norm()
+        assert d <= 3 * U[dt] * w.norm() + floor * w.numel() ** 0.5
+
+
 def test_rows_that_see_nothing(cuda):
     for dt in (BF16, F32):
         q, k, v = (randn(i, 2, 200, 2, 64, dtype=dt).to(cuda) for i in range(3))
