@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 import weakref
 from typing import Optional
@@ -67,9 +68,13 @@ class AttentionGrad(ctypes.Structure):
                              "grad_q", "grad_k", "grad_v", "grad_table", "workspace")]
 
 
-_NR = ctypes.POINTER(NormRotate)
-_AT = ctypes.POINTER(Attention)
-_AG = ctypes.POINTER(AttentionGrad)
+# The same structures packed at once, in the native layout: filling the fields
+# one by one costs more than a small launch.  Passed as a pointer to the bytes.
+pack_norm_rotate = struct.Struct("@13q7P3id").pack
+pack_attention = struct.Struct("@20q8P2d3i").pack
+pack_attention_grad = struct.Struct("@3q10P").pack
+
+_NR = _AT = _AG = _P
 
 # argument lists, in header order
 _SIGS = {
@@ -220,6 +225,21 @@ def dtype_code(dt: torch.dtype) -> int:
         return _DTYPES[dt]
     except KeyError:
         raise TypeError(f"unsupported dtype {dt}") from None
+
+
+def launch(device, name: str, *args) -> None:
+    """`call` on the tensors' device, with its current stream as last argument."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        call(name, *args, _raw_stream(i))
+        return
+    with torch.cuda.device(i):
+        call(name, *args, _raw_stream(i))
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream's handle, without the object around it."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: Optional[torch.Tensor]):

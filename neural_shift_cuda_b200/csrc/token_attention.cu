@@ -165,7 +165,7 @@ extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
 
 extern "C" NSC_API int64_t nsc_token_attention_decode_workspace(const nsc_attention* a) {
     if (check("token_attention_decode", a, false) != NSC_OK) return -1;
-    return 0;
+    return decode_workspace(params(a), a->dtype);
 }
 
 extern "C" NSC_API nsc_status nsc_token_attention_decode(const nsc_attention* a, void* out,
@@ -178,9 +178,8 @@ extern "C" NSC_API nsc_status nsc_token_attention_decode(const nsc_attention* a,
     if (!a->lengths || !out) return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
     if (a->documents || a->prefix || !a->causal)
         return fail(NSC_ERR_INVALID_ARG, "%s: causal, without documents or prefix", op);
-    (void)workspace;
     Params p = params(a);
     p.out = out;
     p.lse = lse;
-    return general_fwd(p, a->dtype, as_stream(stream));
+    return decode(p, workspace, a->dtype, as_stream(stream));
 }

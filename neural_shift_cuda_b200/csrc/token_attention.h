@@ -136,6 +136,10 @@ int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t n_buckets);
 nsc_status tc_bwd(const Params& p, Grads g, void* workspace, void* grad_table, int dtype,
                   cudaStream_t st);
 
+// token_decode.cu
+int64_t decode_workspace(const Params& p, int dtype);
+nsc_status decode(const Params& p, void* workspace, int dtype, cudaStream_t st);
+
 // delta (and its layout (B, Hq, Lq)) for a backward pass; joining of the
 // table-gradient partials.
 nsc_status launch_delta(const Params& p, const Grads& g, int dtype, cudaStream_t st);

@@ -19,7 +19,6 @@ has a counterpart in the reference.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -27,17 +26,23 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _require_cuda
 
 __all__ = ["qk_norm_rotate", "token_attention", "token_attention_decode",
            "relative_buckets"]
-
-_byref = ctypes.byref
 
 
 # ---------------------------------------------------------------------------
 # argument handling
 # ---------------------------------------------------------------------------
+
+def _require_cuda(op: str, q: torch.Tensor) -> None:
+    """(The other tensors are known to share q's device.)"""
+    if not q.is_cuda:
+        raise RuntimeError(
+            f"neural_shift_cuda_b200.{op}: expects CUDA tensors (got a "
+            f"{q.device} tensor); this package has no CPU path")
+    _lib.load()
+
 
 def _check_heads(op: str, name: str, t: torch.Tensor) -> None:
     if t.dim() != 4:
@@ -85,6 +90,9 @@ def _tiled(t: torch.Tensor) -> torch.Tensor:
 
 
 def _int32(op: str, name: str, t: torch.Tensor, device) -> torch.Tensor:
+    if (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device
+            and t.is_contiguous()):
+        return t
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{op}: {name} must be an int32 or int64 tensor")
     if t.device != device:
@@ -96,8 +104,8 @@ def _acc(dt: torch.dtype) -> torch.dtype:
     return torch.float64 if dt == torch.float64 else torch.float32
 
 
-def _addr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 # ---------------------------------------------------------------------------
@@ -106,27 +114,22 @@ def _addr(t: Optional[torch.Tensor]):
 
 def _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps):
     B, L, Hq, D = q.shape
-    a = _lib.NormRotate()
-    a.B, a.L, a.Hq, a.Hkv, a.D = B, L, Hq, k.shape[2], D
-    a.rot_dim, a.rows = 2 * cos.shape[1], cos.shape[0]
-    a.q_stride[:] = q.stride()[:3]
-    a.k_stride[:] = k.stride()[:3]
-    a.q, a.k, a.q_weight, a.k_weight = _addr(q), _addr(k), _addr(wq), _addr(wk)
-    a.cos, a.sin, a.positions = _addr(cos), _addr(sin), _addr(positions)
-    a.dtype = _lib.dtype_code(q.dtype)
+    rows, half = cos.shape
     w = wq if wq is not None else wk
-    a.weight_dtype = _lib.dtype_code(q.dtype if w is None else w.dtype)
-    a.adjacent, a.eps = int(adjacent), eps
-    return a
+    code = _lib.dtype_code(q.dtype)
+    return _lib.pack_norm_rotate(
+        B, L, Hq, k.shape[2], D, 2 * half, rows, *q.stride()[:3], *k.stride()[:3],
+        q.data_ptr(), k.data_ptr(), _addr(wq), _addr(wk), cos.data_ptr(),
+        sin.data_ptr(), _addr(positions), code,
+        code if w is None else _lib.dtype_code(w.dtype), adjacent, eps)
 
 
 def _rotate_fwd(q, k, wq, wk, cos, sin, positions, adjacent, eps):
     qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    a = _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps)
-    with torch.cuda.device(q.device):
-        _lib.call("nsc_qk_norm_rotate_fwd", _byref(a), _lib.ptr(qo),
-                  _lib.ptr(ko), _lib.stream_of(q))
+    _lib.launch(q.device, "nsc_qk_norm_rotate_fwd",
+                _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps),
+                qo.data_ptr(), ko.data_ptr())
     return qo, ko
 
 
@@ -147,13 +150,11 @@ class _RotateFn(torch.autograd.Function):
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
-        with torch.cuda.device(q.device):
-            ws = None
-            if dwq is not None or dwk is not None:
-                ws = _lib.workspace("nsc_qk_norm_rotate_workspace", q.device, _byref(a))
-            _lib.call("nsc_qk_norm_rotate_bwd", _byref(a), _lib.ptr(gq),
-                      _lib.ptr(gk), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dwq),
-                      _lib.ptr(dwk), _lib.ptr(ws), _lib.stream_of(q))
+        ws = None
+        if dwq is not None or dwk is not None:
+            ws = _lib.workspace("nsc_qk_norm_rotate_workspace", q.device, a)
+        _lib.launch(q.device, "nsc_qk_norm_rotate_bwd", a, gq.data_ptr(), gk.data_ptr(),
+                    dq.data_ptr(), dk.data_ptr(), _addr(dwq), _addr(dwk), _addr(ws))
         return dq, dk, dwq, dwk, None, None, None, None, None
 
 
@@ -194,7 +195,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
                            f"{tuple(cos.shape)}, {tuple(sin.shape)}")
     if cos.device != q.device or sin.device != q.device:
         raise ValueError(f"{op}: cos and sin must be on {q.device}")
-    _require_cuda(op, q, k)
+    _require_cuda(op, q)
     if positions is not None:
         positions = _int32(op, "positions", positions, q.device)
         if positions.shape == (L,):
@@ -209,7 +210,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
     cos, sin = cos.detach().to(acc).contiguous(), sin.detach().to(acc).contiguous()
     wq = None if q_weight is None else q_weight.contiguous()
     wk = None if k_weight is None else k_weight.contiguous()
-    args = (_unit(q), _unit(k), wq, wk, cos, sin, positions, bool(adjacent), float(eps))
+    args = (_unit(q), _unit(k), wq, wk, cos, sin, positions, int(adjacent), float(eps))
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _RotateFn.apply(*args)
@@ -249,26 +250,20 @@ def relative_buckets(num_buckets: int, max_distance: int,
 def _attention_args(q, k, v, documents, prefix, lengths, table, buckets, scale,
                     cap, causal):
     B, Lq, Hq, D = q.shape
-    a = _lib.Attention()
-    a.B, a.Lq, a.Lk, a.Hq, a.Hkv, a.D = B, Lq, k.shape[1], Hq, k.shape[2], D
-    a.q_stride[:] = q.stride()[:3]
-    a.k_stride[:] = k.stride()[:3]
-    a.v_stride[:] = v.stride()[:3]
-    a.q, a.k, a.v = _addr(q), _addr(k), _addr(v)
-    a.dtype = _lib.dtype_code(q.dtype)
+    code = _lib.dtype_code(q.dtype)
+    docs = docs_stride = n_buckets = reach = 0
+    table_code = code
     if documents is not None:
-        a.documents, a.docs = _addr(documents), documents.shape[1] - 1
-        a.docs_stride = documents.stride(0)
-    if prefix is not None:
-        a.prefix, a.prefix_stride = _addr(prefix), prefix.stride(0)
-    if lengths is not None:
-        a.lengths = _addr(lengths)
+        docs, docs_stride = documents.shape[1] - 1, documents.stride(0)
     if table is not None:
-        a.table, a.buckets = _addr(table), _addr(buckets)
-        a.table_dtype = _lib.dtype_code(table.dtype)
-        a.n_buckets, a.reach = table.shape[0], buckets.shape[0] // 2
-    a.scale, a.softcap, a.causal = scale, cap, int(causal)
-    return a
+        n_buckets, reach = table.shape[0], buckets.shape[0] // 2
+        table_code = _lib.dtype_code(table.dtype)
+    return _lib.pack_attention(
+        B, Lq, k.shape[1], Hq, k.shape[2], D, *q.stride()[:3], *k.stride()[:3],
+        *v.stride()[:3], docs, docs_stride, 0 if prefix is None else prefix.stride(0),
+        n_buckets, reach, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(documents),
+        _addr(prefix), _addr(lengths), _addr(buckets), _addr(table), scale, cap, code,
+        table_code, causal)
 
 
 def _attention_fwd(q, k, v, documents, prefix, table, buckets, scale, cap, causal,
@@ -288,9 +283,8 @@ def _attention_fwd(q, k, v, documents, prefix, table, buckets, scale, cap, causa
             residue = torch.empty_like(out)
     a = _attention_args(q, k, v, documents, prefix, None, table, buckets, scale,
                         cap, causal)
-    with torch.cuda.device(dev):
-        _lib.call("nsc_token_attention_fwd", _byref(a), _lib.ptr(out), _lib.ptr(lse),
-                  _lib.ptr(stats), _lib.ptr(residue), _lib.stream_of(q))
+    _lib.launch(dev, "nsc_token_attention_fwd", a, out.data_ptr(), _addr(lse),
+                _addr(stats), _addr(residue))
     return out, lse, stats, residue
 
 
@@ -322,15 +316,12 @@ class _AttentionFn(torch.autograd.Function):
         dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         dt = (torch.empty_like(table) if table is not None and ctx.needs_input_grad[5]
               else None)
-        g = _lib.AttentionGrad()
-        g.grad_out_stride[:] = grad_out.stride()[:3]
-        with torch.cuda.device(q.device):
-            ws = _lib.workspace("nsc_token_attention_bwd_workspace", q.device, _byref(a))
-            g.out, g.stats, g.residue = _addr(out), _addr(stats), _addr(residue)
-            g.grad_out, g.grad_lse = _addr(grad_out), _addr(grad_lse)
-            g.grad_q, g.grad_k, g.grad_v = _addr(dq), _addr(dk), _addr(dv)
-            g.grad_table, g.workspace = _addr(dt), _addr(ws)
-            _lib.call("nsc_token_attention_bwd", _byref(a), _byref(g), _lib.stream_of(q))
+        ws = _lib.workspace("nsc_token_attention_bwd_workspace", q.device, a)
+        g = _lib.pack_attention_grad(
+            *grad_out.stride()[:3], out.data_ptr(), stats.data_ptr(), _addr(residue),
+            grad_out.data_ptr(), _addr(grad_lse), dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), _addr(dt), _addr(ws))
+        _lib.launch(q.device, "nsc_token_attention_bwd", a, g)
         return dq, dk, dv, None, None, dt, None, None, None, None, None
 
 
@@ -398,7 +389,7 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     table, buckets = _check_bias(op, q, bias_table, bias_buckets)
     if prefix is not None and not causal:
         raise ValueError(f"{op}: a prefix needs causal=True")
-    _require_cuda(op, q, k, v)
+    _require_cuda(op, q)
     if documents is not None:
         documents = _int32(op, "documents", documents, dev)
         if documents.dim() == 1:
@@ -423,7 +414,7 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                                f"{tuple(prefix.shape)}")
     scale, cap = _numbers(q, scale, softcap)
     args = (_tiled(q), _tiled(k), _tiled(v), documents, prefix, table, buckets, scale,
-            cap, bool(causal), return_lse)
+            cap, int(causal), return_lse)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (table is not None and table.requires_grad)):
         out, lse = _AttentionFn.apply(*args)
@@ -453,7 +444,7 @@ def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
             t is not None and t.requires_grad for t in (q, k_cache, v_cache, table)):
         raise RuntimeError(f"{op} has no backward; use token_attention, or "
                            f"torch.no_grad()")
-    _require_cuda(op, q, k_cache, v_cache)
+    _require_cuda(op, q)
     lengths = _int32(op, "lengths", lengths, q.device)
     B, T, Hq, D = q.shape
     if lengths.shape != (B,):
@@ -464,9 +455,8 @@ def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
     lse = (torch.empty((B, Hq, T), dtype=_acc(q.dtype), device=q.device)
            if return_lse else None)
     a = _attention_args(q, k_cache, v_cache, None, None, lengths, table, buckets,
-                        scale, cap, True)
-    with torch.cuda.device(q.device):
-        ws = _lib.workspace("nsc_token_attention_decode_workspace", q.device, _byref(a))
-        _lib.call("nsc_token_attention_decode", _byref(a), _lib.ptr(out),
-                  _lib.ptr(lse), _lib.ptr(ws), _lib.stream_of(q))
+                        scale, cap, 1)
+    ws = _lib.workspace("nsc_token_attention_decode_workspace", q.device, a)
+    _lib.launch(q.device, "nsc_token_attention_decode", a, out.data_ptr(), _addr(lse),
+                _addr(ws))
     return (out, lse) if return_lse else out
