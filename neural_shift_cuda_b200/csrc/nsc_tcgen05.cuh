@@ -46,19 +46,15 @@ __device__ __forceinline__ void commit(uint32_t bar) {
         : "memory");
 }
 
-// Descriptor of a swizzled operand at shared address `addr` (its panel is
-// 1024-byte aligned).  K-major: `group` = 1024 bytes between groups of eight
-// rows.  MN-major: `panel` bytes between panels of 64 along M or N, 1024
-// between groups of eight reduced rows.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t panel_bytes) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>((panel_bytes >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
-    d |= 1ull << 46;
-    d |= 2ull << 61;   // 128-byte swizzle
-    return d;
+// Descriptor of a swizzled operand whose panel is 1024-byte aligned: the low word
+// for shared address `addr`, to which an offset in 16-byte units may be added,
+// and the constant high word.  K-major: 1024 bytes between groups of eight rows.
+// MN-major: `panel` bytes between panels of 64 along M or N, 1024 between groups
+// of eight reduced rows.
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t panel_bytes) {
+    return ((addr & 0x3FFFFu) >> 4) | ((panel_bytes >> 4) << 16);
 }
+constexpr uint32_t kOperandHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // 128-byte swizzle
 
 // Instruction descriptor of a 16-bit product with fp32 accumulators.
 __host__ __device__ constexpr uint32_t product(bool bf16, int M, int N, bool a_mn, bool b_mn) {
@@ -67,22 +63,25 @@ __host__ __device__ constexpr uint32_t product(bool bf16, int M, int N, bool a_m
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// D (tensor memory) = A (shared) B (shared) [+ D]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+// D (tensor memory) = A (shared) B (shared) [+ D].  Issued by one thread, whose few
+// instructions a product are in series: what a loop computes per product shows.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "n"(kOperandHi)
         : "memory");
 }
 // D = A (tensor memory, 16-bit pairs, a row a lane) B (shared) [+ D]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 y, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "n"(kOperandHi)
         : "memory");
 }
 

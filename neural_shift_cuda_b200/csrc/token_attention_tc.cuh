@@ -124,13 +124,13 @@ __device__ __forceinline__ void fence_async_shared() {
 // tanh |y| = 1 - 2 / (1 + e^(2|y|)) for all of it.
 __device__ __forceinline__ void tanh32(float2* s, float y1) {
     const float2 k = make_float2(y1, y1);
-    float top = 0.f;
+    float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         s[i] = __fmul2_rn(s[i], k);
-        top = fmaxf(top, fmaxf(fabsf(s[i].x), fabsf(s[i].y)));
+        top[i & 3] = fmaxf(top[i & 3], fmaxf(fabsf(s[i].x), fabsf(s[i].y)));
     }
-    if (!__any_sync(0xffffffffu, top > 1.f)) {
+    if (!__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 1.f)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float2 u = __fmul2_rn(s[i], s[i]);
@@ -159,6 +159,29 @@ __device__ __forceinline__ void load_padded_bias(const Params& p, int h, float* 
         const int d = min(max(i - kBiasPad, 0), 2 * p.reach);
         E[i] = bias2_at<float>(p, __ldg(p.lut + d), h);
     }
+}
+
+// The products of two tiles, issued by one thread.  scores_mma: [128 x 128] = A B^T over
+// the channels, both tiles K-major; `steps` of 16 channels.  mix_mma: [128 x channels]
+// += W B with the 128 x 128 weights W in tensor memory, their k-steps 4 to 7 at
+// column `w + gap`, and the 128 rows of B as the reduced dimension.
+template <int DP>
+__device__ __forceinline__ void scores_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                           int steps) {
+    const uint32_t x = tc::operand(a, 16), y = tc::operand(b, 16);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+        if (c < steps) {
+            const uint32_t o = ((c >> 2) * kPanel + (c & 3) * 32) >> 4;
+            tc::mma_ss(d, x + o, y + o, idesc, c > 0);
+        }
+}
+template <int GAP>
+__device__ __forceinline__ void mix_mma(uint32_t d, uint32_t w, uint32_t b, uint32_t idesc, bool add) {
+    const uint32_t y = tc::operand(b, kPanel);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        tc::mma_ts(d, w + (k >> 2) * GAP + (k & 3) * 8, y + ((k * 2048) >> 4), idesc, add || k > 0);
 }
 
 }  // namespace tok

@@ -336,23 +336,6 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         } else if (warp == 9 && lane == 0 && total > 0) {
             const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
             const uint32_t its = tc::product(kBf16, 128, cols, false, true);
-            // [keys x queries] = A (keys) B (queries)^T over the channels
-            auto scores = [&](uint32_t d, unsigned char* A, unsigned char* B) {
-                const uint32_t a = smem_u32(A), q = smem_u32(B);
-#pragma unroll 1
-                for (int c = 0; c < steps; ++c) {
-                    const uint32_t o = (c >> 2) * kPanel + (c & 3) * 32;
-                    tc::mma_ss(d, tc::operand(a + o, 16), tc::operand(q + o, 16), iss, c > 0);
-                }
-            };
-            // [keys x channels] += W (keys x queries, tensor memory) B (queries x channels)
-            auto mix = [&](uint32_t d, uint32_t w, unsigned char* B, bool add) {
-                const uint32_t q = smem_u32(B);
-#pragma unroll 1
-                for (int k = 0; k < 8; ++k)
-                    tc::mma_ts(d, w + (k >> 2) * 64 + (k & 3) * 8, tc::operand(q + k * 2048, kPanel),
-                               its, add || k > 0);
-            };
             bool alive = wait(&bars.fixed, 0);
             for (int it = -1; alive && it < total; ++it) {
                 const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
@@ -361,26 +344,26 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     alive = wait(&bars.p_ready, it & 1);
                     if (!alive) break;
                     tc::fence_after();
-                    mix(t_dv, t_s, O_at(s), it > 0);
+                    mix_mma<64>(t_dv, t_s, smem_u32(O_at(s)), its, it > 0);
                 }
                 if (next < total) {
                     alive = wait(&bars.x_full[sn], pn) &&
                             (!guarded(fb + next % nq) || wait(&bars.ok[sn], pn));
                     if (!alive) break;
-                    scores(t_s, Ks, Q_at(sn));
+                    scores_mma<DP>(t_s, smem_u32(Ks), smem_u32(Q_at(sn)), iss, steps);
                     tc::commit(smem_u32(&bars.s_full));
                 }
                 if (it >= 0) {
                     alive = wait(&bars.ds_ready, it & 1);
                     if (!alive) break;
                     tc::fence_after();
-                    mix(t_dk, t_dp, Q_at(s), it > 0);
+                    mix_mma<64>(t_dk, t_dp, smem_u32(Q_at(s)), its, it > 0);
                     tc::commit(smem_u32(&bars.empty[s]));
                 }
                 if (next < total) {
                     alive = wait(&bars.y_full[sn], pn);
                     if (!alive) break;
-                    scores(t_dp, Vs, O_at(sn));
+                    scores_mma<DP>(t_dp, smem_u32(Vs), smem_u32(O_at(sn)), iss, steps);
                     tc::commit(smem_u32(&bars.dp_full));
                 }
             }
@@ -708,14 +691,6 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
         } else if (warp == 9 && lane == 0 && total > 0) {
             const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
             const uint32_t its = tc::product(kBf16, 128, cols, false, true);
-            auto scores = [&](uint32_t d, unsigned char* A, unsigned char* B) {
-                const uint32_t a = smem_u32(A), q = smem_u32(B);
-#pragma unroll 1
-                for (int c = 0; c < steps; ++c) {
-                    const uint32_t o = (c >> 2) * kPanel + (c & 3) * 32;
-                    tc::mma_ss(d, tc::operand(a + o, 16), tc::operand(q + o, 16), iss, c > 0);
-                }
-            };
             bool alive = wait(&bars.fixed, 0);
             uint32_t okp = 0;
             for (int it = -1; alive && it < total; ++it) {
@@ -728,22 +703,18 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                         okp ^= 1u << sn;
                     }
                     if (!alive) break;
-                    scores(t_s + 128 * (next & 1), Qs, K_at(sn));
+                    scores_mma<DP>(t_s + 128 * (next & 1), smem_u32(Qs), smem_u32(K_at(sn)), iss, steps);
                     alive = wait(&bars.y_full[sn], pn) && (it < 0 || wait(&bars.dp_free, it & 1));
                     if (!alive) break;
                     tc::fence_after();
-                    scores(t_dp, Os, V_at(sn));
+                    scores_mma<DP>(t_dp, smem_u32(Os), smem_u32(V_at(sn)), iss, steps);
                     tc::commit(smem_u32(&bars.dp_full));
                 }
                 if (it >= 0) {
                     alive = wait(&bars.ds_ready, it & 1);
                     if (!alive) break;
                     tc::fence_after();
-                    const uint32_t k = smem_u32(K_at(s)), w = t_s + 128 * (it & 1);
-#pragma unroll 1
-                    for (int c = 0; c < 8; ++c)
-                        tc::mma_ts(t_dq, w + (c >> 2) * 64 + (c & 3) * 8,
-                                   tc::operand(k + c * 2048, kPanel), its, it > 0 || c > 0);
+                    mix_mma<64>(t_dq, t_s + 128 * (it & 1), smem_u32(K_at(s)), its, it > 0);
                     tc::commit(smem_u32(&bars.empty[s]));
                 }
             }

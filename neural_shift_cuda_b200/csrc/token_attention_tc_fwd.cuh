@@ -195,10 +195,12 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     if (2 * i + 1 - from >= len) s[i].y = -INFINITY;
                 }
             }
-            float top = s[0].x;
+            // (four maxima, and four sums below, side by side: one chain would wait
+            // out the latency of each of its 64 steps)
+            float tops[4] = {s[0].x, s[1].x, s[2].x, s[3].x};
 #pragma unroll
-            for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaxf(s[i].x, s[i].y));
-            top *= mul;
+            for (int i = 0; i < 64; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
             // (a row may see nothing of its first blocks: m is then -inf still)
             float keep = 1.f;
             if (top > m + kLazy || m == -INFINITY) {
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             }
             const float ref = m == -INFINITY ? 0.f : -m;
             const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(ref, ref);
-            float2 sum = make_float2(0.f, 0.f);
+            float2 sums[4] = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t w[16];
@@ -228,11 +230,12 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 for (int i = 0; i < 16; ++i) {
                     const float2 x = __ffma2_rn(s[16 * c + i], mul2, ref2);
                     const float2 e = make_float2(tc::ex2(x.x), tc::ex2(x.y));
-                    sum = __fadd2_rn(sum, e);
+                    sums[i & 3] = __fadd2_rn(sums[i & 3], e);
                     w[i] = tc::pack2<T>(e.x, e.y);
                 }
                 tc::store16(ts + 16 * c, w);
             }
+            const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
             l += sum.x + sum.y;
             tc::wait_st();
             tc::fence_before();
@@ -327,22 +330,14 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                         alive = wait(&bars.v_full[s], (i / NS) & 1) && wait(&bars.p_full[x], pn[x] & 1);
                         if (!alive) break;
                         tc::fence_after();
-                        const uint32_t v = smem_u32(V_at(s));
-#pragma unroll 1
-                        for (int k = 0; k < 8; ++k)
-                            tc::mma_ts(tmem + 256 + x * DP, tmem + x * 128 + 8 * k,
-                                       tc::operand(v + k * 2048, kPanel), ipv, pn[x] > 0 || k > 0);
+                        mix_mma<32>(tmem + 256 + x * DP, tmem + x * 128, smem_u32(V_at(s)), ipv,
+                                    pn[x] > 0);
                         ++pn[x];
                         if (j + 1 == lb[x]) tc::commit(smem_u32(&bars.o_full[x]));
                     }
                     if (on(x, j + 1)) {
-                        const uint32_t q = smem_u32(Qs + x * S::tile), k = smem_u32(K_at(sn));
-#pragma unroll 1
-                        for (int c = 0; c < steps; ++c) {
-                            const uint32_t off = (c >> 2) * kPanel + (c & 3) * 32;
-                            tc::mma_ss(tmem + x * 128, tc::operand(q + off, 16),
-                                       tc::operand(k + off, 16), iqk, c > 0);
-                        }
+                        scores_mma<DP>(tmem + x * 128, smem_u32(Qs + x * S::tile),
+                                       smem_u32(K_at(sn)), iqk, steps);
                         tc::commit(smem_u32(&bars.s_full[x]));
                     }
                 }

@@ -19,7 +19,7 @@ namespace rot {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxPart = 1184;   // blocks that hold weight-gradient partials (8 a SM)
+constexpr int kMaxPart = 592;    // blocks that hold weight-gradient partials: 4 an SM
 
 struct Args {
     const void *q, *k, *wq, *wk, *cos, *sin;
@@ -180,49 +180,58 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Args a, Out o, int nq, in
     }
 }
 
+// Blocks [0, q_blocks) pass over q, the others over k, so that a thread holds the
+// weight sums of one of them.
 template <typename T, typename A, int LANES, bool ADJ>
-__global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grad g, int nq, int nk) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void bwd_kernel(Args a, Grad g,
+                                                                              int q_blocks) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     constexpr int GROUPS = kThreads / LANES;
     constexpr int U = 2;
     const int c = threadIdx.x % LANES, half = a.D / 2;
-    A dw[2][16];
+    const bool is_k = static_cast<int>(blockIdx.x) >= q_blocks, lane_in = 8 * c < half;
+    const int H = is_k ? a.Hkv : a.Hq, chunks = (H + a.per - 1) / a.per;
+    const int64_t s0 = is_k ? a.ks[0] : a.qs[0], s1 = is_k ? a.ks[1] : a.qs[1];
+    const int64_t s2 = is_k ? a.ks[2] : a.qs[2];
+    const T* src = static_cast<const T*>(is_k ? a.k : a.q) + 8 * c;
+    const T* gsrc = static_cast<const T*>(is_k ? g.gk : g.gq) + 8 * c;
+    T* dst = static_cast<T*>(is_k ? g.dk : g.dq) + 8 * c;
+    A dw[16], w[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0;
-    const int64_t jobs = a.tokens * (nq + nk);
-    const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+    for (int i = 0; i < 16; ++i) {
+        dw[i] = 0;
+        w[i] = lane_in ? weight_at<A>(is_k ? a.wk : a.wq, a.w_dtype, (i < 8 ? 0 : half - 8) + 8 * c + i)
+                       : A(0);
+    }
+    const int first = is_k ? static_cast<int>(blockIdx.x) - q_blocks : static_cast<int>(blockIdx.x);
+    const int blocks = is_k ? static_cast<int>(gridDim.x) - q_blocks : q_blocks;
+    const int64_t jobs = a.tokens * chunks, step = static_cast<int64_t>(blocks) * GROUPS;
+    const A inv_d = A(1) / a.D;
     // all lanes of the block make the same number of rounds
-    for (int64_t j0 = static_cast<int64_t>(blockIdx.x) * GROUPS; j0 < jobs; j0 += step) {
+    for (int64_t j0 = static_cast<int64_t>(first) * GROUPS; j0 < jobs; j0 += step) {
         const int64_t j = j0 + threadIdx.x / LANES;
-        const bool work = j < jobs, lane_on = work && 8 * c < half;
-        Job jb = job_at(a, work ? j : 0, nq, nk);
-        const int64_t b = jb.token / a.L, l = jb.token - b * a.L;
-        const int H = jb.is_k ? a.Hkv : a.Hq;
-        const int64_t* st = jb.is_k ? a.ks : a.qs;
-        const T* src = static_cast<const T*>(jb.is_k ? a.k : a.q) + b * st[0] + l * st[1] + 8 * c;
-        const T* gsrc = static_cast<const T*>(jb.is_k ? g.gk : g.gq) + jb.token * H * a.D + 8 * c;
-        T* dst = static_cast<T*>(jb.is_k ? g.dk : g.dq) + jb.token * H * a.D + 8 * c;
-        A cs[8], sn[8], w[16];
-        if (lane_on) {
-            turn_at<A>(a, a.pos ? __ldg(a.pos + jb.token) : l, c, ADJ, cs, sn);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                w[i] = weight_at<A>(jb.is_k ? a.wk : a.wq, a.w_dtype,
-                                    (i < 8 ? 0 : half - 8) + 8 * c + i);
-        }
-        for (int h0 = jb.h0; h0 < jb.h0 + a.per; h0 += U) {
+        const bool lane_on = j < jobs && lane_in;
+        const int64_t token = j < jobs ? j / chunks : 0;
+        const int h_first = j < jobs ? static_cast<int>(j - token * chunks) * a.per : 0;
+        const int h_end = min(h_first + a.per, H);
+        const int64_t b = token / a.L, l = token - b * a.L;
+        const T* x_at = src + b * s0 + l * s1;
+        const int64_t row0 = token * H;
+        A cs[8], sn[8];
+        if (lane_on) turn_at<A>(a, a.pos ? __ldg(a.pos + token) : l, c, ADJ, cs, sn);
+        for (int h0 = h_first; h0 < h_first + a.per; h0 += U) {
             Raw<T> rx[U], ry[U], rg[U], ri[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (lane_on && h0 + u < jb.h1) {
-                    rx[u] = load8<T>(src + (h0 + u) * st[2]);
-                    ry[u] = load8<T>(src + (h0 + u) * st[2] + half);
-                    rg[u] = load8<T>(gsrc + static_cast<int64_t>(h0 + u) * a.D);
-                    ri[u] = load8<T>(gsrc + static_cast<int64_t>(h0 + u) * a.D + half);
+                if (lane_on && h0 + u < h_end) {
+                    rx[u] = load8<T>(x_at + (h0 + u) * s2);
+                    ry[u] = load8<T>(x_at + (h0 + u) * s2 + half);
+                    rg[u] = load8<T>(gsrc + (row0 + h0 + u) * a.D);
+                    ri[u] = load8<T>(gsrc + (row0 + h0 + u) * a.D + half);
                 }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const bool on = lane_on && h0 + u < jb.h1;
+                const bool on = lane_on && h0 + u < h_end;
                 A x[8], y[8], p[8], q[8], sq = 0, dot = 0;
                 if (on) {
                     unpack<T>(rx[u], x);
@@ -239,19 +248,18 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grad g, int nq, i
                 sq = group_sum<A, LANES>(sq);
                 dot = group_sum<A, LANES>(dot);
                 if (!on) continue;
-                const A r = rsqrt_<A>(sq / a.D + static_cast<A>(a.eps));
-                const A f = r * r * r * dot / a.D;
+                const A r = rsqrt_<A>(sq * inv_d + static_cast<A>(a.eps));
+                const A f = r * r * r * dot * inv_d;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const A dx = p[i] * x[i] * r, dy = q[i] * y[i] * r;
-                    dw[0][i] += jb.is_k ? A(0) : dx;
-                    dw[0][8 + i] += jb.is_k ? A(0) : dy;
-                    dw[1][i] += jb.is_k ? dx : A(0);
-                    dw[1][8 + i] += jb.is_k ? dy : A(0);
-                    x[i] = r * p[i] * w[i] - x[i] * f;
-                    y[i] = r * q[i] * w[8 + i] - y[i] * f;
+                    p[i] *= r;
+                    q[i] *= r;
+                    dw[i] += p[i] * x[i];
+                    dw[8 + i] += q[i] * y[i];
+                    x[i] = p[i] * w[i] - x[i] * f;
+                    y[i] = q[i] * w[8 + i] - y[i] * f;
                 }
-                T* d = dst + static_cast<int64_t>(h0 + u) * a.D;
+                T* d = dst + (row0 + h0 + u) * a.D;
                 store8<T>(d, x);
                 store8<T>(d + half, y);
             }
@@ -259,25 +267,21 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grad g, int nq, i
     }
     if (!g.want_w) return;
     // groups of a warp, then the warps, in a fixed order
-    A* sh = reinterpret_cast<A*>(smem_raw);   // [warps][2][16 * LANES]
+    A* sh = reinterpret_cast<A*>(smem_raw);   // [warps][16 * LANES]
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int i = 0; i < 16; ++i) {
+        A v = dw[i];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            A v = dw[s][i];
-#pragma unroll
-            for (int m = LANES; m < 32; m <<= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-            if (lane < LANES)
-                sh[(warp * 2 + s) * 16 * LANES + (i < 8 ? 0 : 8 * LANES) + 8 * c + (i & 7)] = v;
-        }
+        for (int m = LANES; m < 32; m <<= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+        if (lane < LANES) sh[warp * 16 * LANES + (i < 8 ? 0 : 8 * LANES) + 8 * c + (i & 7)] = v;
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * a.D; i += kThreads) {
-        const int s = i / a.D, d = i % a.D;
+    for (int d = threadIdx.x; d < a.D; d += kThreads) {
         const int at = d < half ? d : 8 * LANES + d - half;
         A v = 0;
-        for (int k = 0; k < kThreads / 32; ++k) v += sh[(k * 2 + s) * 16 * LANES + at];
-        static_cast<A*>(g.part)[static_cast<int64_t>(blockIdx.x) * 2 * a.D + i] = v;
+        for (int k = 0; k < kThreads / 32; ++k) v += sh[k * 16 * LANES + at];
+        static_cast<A*>(g.part)[static_cast<int64_t>(blockIdx.x) * a.D + d] = v;
     }
 }
 
@@ -351,36 +355,45 @@ __global__ __launch_bounds__(kThreads) void any_kernel(Args a, Out o, Grad g, in
     if (!back || !g.want_w) return;
     __syncthreads();
     const A* all = reinterpret_cast<A*>(smem_raw) + warps * a.D;
+    // (a block has a row of sums of q, and further on one of k)
     for (int i = threadIdx.x; i < 2 * a.D; i += kThreads) {
         A v = 0;
         for (int k = 0; k < warps; ++k) v += all[k * 2 * a.D + i];
-        static_cast<A*>(g.part)[static_cast<int64_t>(blockIdx.x) * 2 * a.D + i] = v;
+        const int64_t row = blockIdx.x + (i < a.D ? 0 : gridDim.x);
+        static_cast<A*>(g.part)[row * a.D + (i < a.D ? i : i - a.D)] = v;
     }
 }
 
-// Sums of the blocks' partials: 32 columns a block, 8 rows at a time.
+// Sums of the blocks' partials, rows [0, nq) of q and [nq, n) of k: a block 32 columns
+// of one of them, its 32 warps side by side over the rows.
 template <typename A>
-__global__ __launch_bounds__(256) void join_kernel(const A* part, int n, int D, void* wq, void* wk,
-                                                   int dt) {
-    __shared__ A sh[8][32];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, i = blockIdx.x * 32 + x;
+__global__ __launch_bounds__(1024) void join_kernel(const A* part, int nq, int n, int D, void* wq,
+                                                    void* wk, int dt) {
+    __shared__ A sh[32][33];
+    const bool is_k = blockIdx.y == 1;
+    void* w = is_k ? wk : wq;
+    if (!w) return;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, d = blockIdx.x * 32 + x;
+    const int r0 = is_k ? nq : 0, r1 = is_k ? n : nq;
     A v = 0;
-    if (i < 2 * D)
-        for (int r = y; r < n; r += 8) v += part[static_cast<int64_t>(r) * 2 * D + i];
+    if (d < D)
+#pragma unroll 8
+        for (int r = r0 + y; r < r1; r += 32) v += part[static_cast<int64_t>(r) * D + d];
     sh[y][x] = v;
     __syncthreads();
-    if (y || i >= 2 * D) return;
-    for (int k = 1; k < 8; ++k) v += sh[k][x];
-    void* w = i < D ? wq : wk;
-    const int d = i < D ? i : i - D;
-    if (!w) return;
+    // warp y sums column y
+    v = sh[x][y];
+#pragma unroll
+    for (int i = 16; i; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
+    const int o = blockIdx.x * 32 + y;
+    if (x || o >= D) return;
     switch (dt) {
-        case NSC_F16: static_cast<__half*>(w)[d] = __float2half_rn(static_cast<float>(v)); break;
+        case NSC_F16: static_cast<__half*>(w)[o] = __float2half_rn(static_cast<float>(v)); break;
         case NSC_BF16:
-            static_cast<__nv_bfloat16*>(w)[d] = __float2bfloat16_rn(static_cast<float>(v));
+            static_cast<__nv_bfloat16*>(w)[o] = __float2bfloat16_rn(static_cast<float>(v));
             break;
-        case NSC_F32: static_cast<float*>(w)[d] = static_cast<float>(v); break;
-        default: static_cast<double*>(w)[d] = v;
+        case NSC_F32: static_cast<float*>(w)[o] = static_cast<float>(v); break;
+        default: static_cast<double*>(w)[o] = v;
     }
 }
 
@@ -462,8 +475,7 @@ int heads_per_job(const Args& a, int lanes) {
 }
 
 template <typename T, typename A, int LANES>
-nsc_status run_wide(Args a, const Out* o, const Grad* g, int blocks_max, int* n_part,
-                    cudaStream_t st) {
+nsc_status run_wide(Args a, const Out* o, const Grad* g, int* n_part, cudaStream_t st) {
     a.per = heads_per_job(a, LANES);
     const int nq = (a.Hq + a.per - 1) / a.per, nk = (a.Hkv + a.per - 1) / a.per;
     const int64_t jobs = a.tokens * (nq + nk);
@@ -475,13 +487,20 @@ nsc_status run_wide(Args a, const Out* o, const Grad* g, int blocks_max, int* n_
         else fwd_kernel<T, A, LANES, false><<<n, kThreads, 0, st>>>(a, *o, nq, nk);
         return check_launch("qk_norm_rotate");
     }
-    *n_part = static_cast<int>(blocks < blocks_max ? blocks : blocks_max);
-    const size_t smem = sizeof(A) * (kThreads / 32) * 2 * 16 * LANES;
+    // blocks of q and of k in the ratio of their work, two rounds an SM at most
+    constexpr int groups = kThreads / LANES;
+    int64_t bq = (a.tokens * nq + groups - 1) / groups, bk = (a.tokens * nk + groups - 1) / groups;
+    if (bq + bk > kMaxPart) {
+        const int64_t all = static_cast<int64_t>(a.Hq) + a.Hkv;
+        bk = a.Hkv ? (kMaxPart * static_cast<int64_t>(a.Hkv) + all - 1) / all : 0;
+        bq = kMaxPart - bk;
+        if (a.Hq && bq < 1) { bq = 1; bk = kMaxPart - 1; }
+    }
+    n_part[0] = static_cast<int>(bq);
+    n_part[1] = static_cast<int>(bq + bk);
+    const size_t smem = sizeof(A) * (kThreads / 32) * 16 * LANES;
     auto kern = a.adjacent ? bwd_kernel<T, A, LANES, true> : bwd_kernel<T, A, LANES, false>;
-    if (smem > 48 * 1024)
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-    kern<<<*n_part, kThreads, smem, st>>>(a, *g, nq, nk);
+    kern<<<n_part[1], kThreads, smem, st>>>(a, *g, n_part[0]);
     return check_launch("qk_norm_rotate backward");
 }
 
@@ -491,18 +510,21 @@ nsc_status run(const nsc_norm_rotate* n, const Out* o, const Grad* g, int* n_par
     Args a = args(n);
     if constexpr (sizeof(T) < 8) if (wide(n)) {
         switch (lanes_for(a.D)) {
-            case 1: return run_wide<T, A, 1>(a, o, g, kMaxPart, n_part, st);
-            case 2: return run_wide<T, A, 2>(a, o, g, kMaxPart, n_part, st);
-            case 4: return run_wide<T, A, 4>(a, o, g, kMaxPart, n_part, st);
-            case 8: return run_wide<T, A, 8>(a, o, g, kMaxPart, n_part, st);
-            case 16: return run_wide<T, A, 16>(a, o, g, kMaxPart, n_part, st);
-            default: return run_wide<T, A, 32>(a, o, g, kMaxPart, n_part, st);
+            case 1: return run_wide<T, A, 1>(a, o, g, n_part, st);
+            case 2: return run_wide<T, A, 2>(a, o, g, n_part, st);
+            case 4: return run_wide<T, A, 4>(a, o, g, n_part, st);
+            case 8: return run_wide<T, A, 8>(a, o, g, n_part, st);
+            case 16: return run_wide<T, A, 16>(a, o, g, n_part, st);
+            default: return run_wide<T, A, 32>(a, o, g, n_part, st);
         }
     }
     const int warps = kThreads / 32;
     int64_t blocks = (a.tokens * (a.Hq + a.Hkv) + warps - 1) / warps;
     if (blocks > kMaxPart) blocks = kMaxPart;
-    if (n_part) *n_part = static_cast<int>(blocks);
+    if (n_part) {
+        n_part[0] = static_cast<int>(blocks);
+        n_part[1] = static_cast<int>(2 * blocks);
+    }
     const size_t smem = g ? sizeof(A) * warps * 3 * a.D : 0;
     if (smem > 48 * 1024)
         cudaFuncSetAttribute(any_kernel<T, A>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -560,21 +582,21 @@ extern "C" NSC_API nsc_status nsc_qk_norm_rotate_bwd(const nsc_norm_rotate* a,
         (want && !workspace) || (grad_q_weight && !a->q_weight) || (grad_k_weight && !a->k_weight))
         return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
     cudaStream_t s = as_stream(stream);
-    int n_part = 0;
+    int n_part[2] = {0, 0};
     if (any && a->Hq + a->Hkv) {
         const Grad g{grad_q_out, grad_k_out, grad_q, grad_k, workspace, want};
-        st = dispatch(a, nullptr, &g, &n_part, s);
+        st = dispatch(a, nullptr, &g, n_part, s);
         if (st != NSC_OK) return st;
     }
     if (!want) return ok();
-    const unsigned blocks = static_cast<unsigned>((2 * a->D + 31) / 32);
+    const dim3 blocks(static_cast<unsigned>((a->D + 31) / 32), 2);
     if (a->dtype == NSC_F64)
-        join_kernel<double><<<blocks, 256, 0, s>>>(static_cast<const double*>(workspace), n_part,
-                                                   static_cast<int>(a->D), grad_q_weight,
-                                                   grad_k_weight, a->weight_dtype);
+        join_kernel<double><<<blocks, 1024, 0, s>>>(static_cast<const double*>(workspace), n_part[0],
+                                                    n_part[1], static_cast<int>(a->D),
+                                                    grad_q_weight, grad_k_weight, a->weight_dtype);
     else
-        join_kernel<float><<<blocks, 256, 0, s>>>(static_cast<const float*>(workspace), n_part,
-                                                  static_cast<int>(a->D), grad_q_weight,
-                                                  grad_k_weight, a->weight_dtype);
+        join_kernel<float><<<blocks, 1024, 0, s>>>(static_cast<const float*>(workspace), n_part[0],
+                                                   n_part[1], static_cast<int>(a->D),
+                                                   grad_q_weight, grad_k_weight, a->weight_dtype);
     return check_launch(op);
 }
