@@ -17,6 +17,21 @@
 namespace nsc {
 namespace tc {
 
+// A value that is the same in every lane, as one the compiler knows to be: what the
+// products take from uniform registers then stays there.  (From a thread on its
+// own every operand of a product is moved across first, 60 to 100 clocks each time.)
+template <typename T> __device__ __forceinline__ T uniform(T x) {
+    return __shfl_sync(0xffffffffu, x, 0);
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(slot)),
@@ -63,8 +78,7 @@ __host__ __device__ constexpr uint32_t product(bool bf16, int M, int N, bool a_m
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// D (tensor memory) = A (shared) B (shared) [+ D].  Issued by one thread, whose few
-// instructions a product are in series: what a loop computes per product shows.
+// D (tensor memory) = A (shared) B (shared) [+ D].  Issued by one lane.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        bool add) {
     asm volatile(

@@ -161,10 +161,11 @@ __device__ __forceinline__ void load_padded_bias(const Params& p, int h, float* 
     }
 }
 
-// The products of two tiles, issued by one thread.  scores_mma: [128 x 128] = A B^T over
+// The products of two tiles, issued by one lane of a converged warp.  scores_mma: [128 x 128] = A B^T over
 // the channels, both tiles K-major; `steps` of 16 channels.  mix_mma: [128 x channels]
-// += W B with the 128 x 128 weights W in tensor memory, their k-steps 4 to 7 at
-// column `w + gap`, and the 128 rows of B as the reduced dimension.
+// += W B with the 128 x 128 weights W in tensor memory, STEPS k-steps side by side and
+// GAP columns from one such run to the next, and the 128 rows of B as the reduced
+// dimension.
 template <int DP>
 __device__ __forceinline__ void scores_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            int steps) {
@@ -176,12 +177,12 @@ __device__ __forceinline__ void scores_mma(uint32_t d, uint32_t a, uint32_t b, u
             tc::mma_ss(d, x + o, y + o, idesc, c > 0);
         }
 }
-template <int GAP>
+template <int STEPS, int GAP>
 __device__ __forceinline__ void mix_mma(uint32_t d, uint32_t w, uint32_t b, uint32_t idesc, bool add) {
     const uint32_t y = tc::operand(b, kPanel);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-        tc::mma_ts(d, w + (k >> 2) * GAP + (k & 3) * 8, y + ((k * 2048) >> 4), idesc, add || k > 0);
+        tc::mma_ts(d, w + k / STEPS * GAP + k % STEPS * 8, y + ((k * 2048) >> 4), idesc, add || k > 0);
 }
 
 }  // namespace tok

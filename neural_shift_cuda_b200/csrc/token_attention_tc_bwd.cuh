@@ -30,7 +30,9 @@ namespace nsc {
 namespace tok {
 namespace {
 
-constexpr int kBwdThreads = 384;
+constexpr int kBwdMath = 512;      // 16 warps of arithmetic, a quarter of a row a thread
+constexpr int kBwdThreads = kBwdMath + 128;
+constexpr int kMathRegs = 104, kOtherRegs = 64;
 constexpr float kPShift = 6.f;   // fp16: log2 of the factor of P
 
 template <int DP> struct BwdShape {
@@ -41,23 +43,15 @@ template <int DP> struct BwdShape {
 
 struct BwdBars {
     uint64_t fixed, x_full[4], y_full[4], empty[4], ok[4];
-    uint64_t s_full, dp_full, p_ready, ds_ready, dp_free, done, drain;
+    // (two each where a warp, or the products, may be a step ahead of a slower warp,
+    // whose wait or arrival would else be taken for that of the other step)
+    uint64_t s_full[2], p_ready[2], ds_ready[2], dp_full, dp_free, used_p, used_ds, done, drain;
 };
 
 __device__ __forceinline__ float pow2_near(float v) {   // a power of two at or above v, or 1
     if (!(v > 0.f) || !(v < 3e38f)) return 1.f;
     const int e = static_cast<int>((__float_as_uint(v) >> 23) & 0xFF) + 1;
     return __uint_as_float(static_cast<uint32_t>(min(max(e, 20), 230)) << 23);
-}
-
-// x2 of 64 products of a thread: the score, less the row reference, in units of
-// log 2; `s` is left as the product (or its tanh).  Bias e[i] by `at(i)`.
-template <bool CAP>
-__device__ __forceinline__ void scores64(float2* s, float y1) {
-    if (CAP) {
-        tanh32(s, y1);
-        tanh32(s + 16, y1);
-    }
 }
 
 template <typename T, int DP, bool CAP, bool BIAS>
@@ -84,7 +78,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     unsigned char* ring = smem + 2 * S::tile;   // stages of Q, dO
     float* E = reinterpret_cast<float*>(smem + S::smem);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = tc::uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const int64_t BH = static_cast<int64_t>(p.B) * p.Hkv;
     const int t = static_cast<int>(blockIdx.x / BH);
     const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hkv, hk = bh % p.Hkv;
@@ -99,10 +93,14 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             mbar_init(&bars.empty[i], 1);
             mbar_init(&bars.ok[i], 64);
         }
-        mbar_init(&bars.s_full, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_ready[i], kBwdMath);
+            mbar_init(&bars.ds_ready[i], kBwdMath);
+        }
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.p_ready, 256);
-        mbar_init(&bars.ds_ready, 256);
+        mbar_init(&bars.used_p, 1);
+        mbar_init(&bars.used_ds, 1);
         mbar_init(&bars.done, 1);
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
@@ -110,11 +108,11 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         abort_flag[1] = static_cast<int>(bnd.budget);
         top_norm = 0;
     }
-    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    if (warp == 17) tc::tmem_alloc(&tmem_slot, 512);
     __syncthreads();
     const int key = k0 + static_cast<int>(threadIdx.x & 127);
     int lo = 0, hi = 0;
-    if (warp < 8) {
+    if (warp < 16) {
         query_span(p, b, key, lo, hi);
         const int v0 = __reduce_min_sync(0xffffffffu, hi > lo ? lo : INT_MAX);
         const int v1 = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
@@ -136,14 +134,16 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         if (lane == 0) atomicMax(&top_norm, __float_as_uint(top));
     }
     __syncthreads();
-    const uint32_t tmem = tmem_slot;
-    const bool any = span[1] > span[0];
-    const int fb = any ? span[0] / kRows : 0, lb = any ? (span[1] + kRows - 1) / kRows : 0;
+    const uint32_t tmem = tc::uniform(tmem_slot);
+    const int s_lo = tc::uniform(span[0]), s_hi = tc::uniform(span[1]);
+    const int all_lo = tc::uniform(span[2]), all_hi = tc::uniform(span[3]);
+    const int fb = s_hi > s_lo ? s_lo / kRows : 0;
+    const int lb = s_hi > s_lo ? (s_hi + kRows - 1) / kRows : 0;
     const int nq = lb - fb, total = nq * p.G;
     const float g = kBf16 ? 1.f : pow2_near(__uint_as_float(top_norm));
     // a key tail past Lk has zero rows of K and V, and sees nothing
     auto guarded = [&](int j) {
-        return !(j * kRows >= span[2] && min((j + 1) * kRows, p.Lq) <= span[3]);
+        return !(j * kRows >= all_lo && min((j + 1) * kRows, p.Lq) <= all_hi);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
@@ -151,13 +151,16 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     auto Q_at = [&](int s) { return ring + s * 2 * S::tile; };
     auto O_at = [&](int s) { return ring + s * 2 * S::tile + S::tile; };
     const int steps = (p.D + 15) / 16, cols = steps * 16;
-    const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+    // at D <= 64 there is room for two S: S(i+1) need not wait for dV(i) to read P(i)
+    constexpr bool kTwoS = DP == 64;
+    const uint32_t t_s = tmem, t_dp = tmem + (kTwoS ? 256 : 128);
+    const uint32_t t_dv = t_dp + 128, t_dk = t_dv + DP;
 
-    if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int half = warp >> 2;
+    if (warp < 16) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMathRegs));
+        const int part = warp >> 2;   // columns 32 part and on
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t at_s = t_s + lane_base + 64 * half, at_dp = t_dp + lane_base + 64 * half;
+        const uint32_t at_s0 = t_s + lane_base + 32 * part, at_dp = t_dp + lane_base + 32 * part;
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
         const float2 u2 = make_float2(unit, unit), g2 = make_float2(1.f / g, 1.f / g);
@@ -166,25 +169,25 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         for (int u = 0; u < p.G && nq > 0; ++u) {
             if (BIAS) {   // E of this head, once all are done with the last (a warp
                           // that gave up comes here too)
-                named_sync(1, 256);
-                load_padded_bias(p, hk * p.G + u, E, threadIdx.x, 256);
-                named_sync(1, 256);
+                named_sync(1, kBwdMath);
+                load_padded_bias(p, hk * p.G + u, E, threadIdx.x, kBwdMath);
+                named_sync(1, kBwdMath);
             }
             for (int j = fb; alive && j < lb; ++j, ++it) {
                 const int st = it % NS;
+                const uint32_t at_s = at_s0 + (kTwoS ? 128 * (it & 1) : 0);
                 alive = __all_sync(0xffffffffu, wait(&bars.ok[st], (it / NS) & 1) &&
-                                                    wait(&bars.s_full, it & 1));
+                                                    wait(&bars.s_full[it & 1], (it >> 1) & 1));
                 if (!alive) break;
                 tc::fence_after();
-                float2 s[32];
+                float2 s[16];
                 tc::load32(at_s, reinterpret_cast<float*>(s));
-                tc::load32(at_s + 32, reinterpret_cast<float*>(s + 16));
                 tc::wait_ld();
-                scores64<CAP>(s, y1);
-                const int q0 = j * kRows + 64 * half;
-                const float4* m4 = reinterpret_cast<const float4*>(rows[st][0] + 64 * half);
-                const float4* l4 = reinterpret_cast<const float4*>(rows[st][1] + 64 * half);
-                const bool whole = __all_sync(0xffffffffu, lo <= q0 && hi >= q0 + 64);
+                if (CAP) tanh32(s, y1);
+                const int q0 = j * kRows + 32 * part;
+                const float4* m4 = reinterpret_cast<const float4*>(rows[st][0] + 32 * part);
+                const float4* l4 = reinterpret_cast<const float4*>(rows[st][1] + 32 * part);
+                const bool whole = __all_sync(0xffffffffu, lo <= q0 && hi >= q0 + 32);
                 const uint32_t from = static_cast<uint32_t>(lo - q0);
                 const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
                 const int rel0 = key - (q0 + off);   // distance at column 0, one less a column
@@ -192,13 +195,13 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                 bool far = false;
                 float e_far = 0.f;
                 if (BIAS) {
-                    far = w0 + 31 <= -p.reach || w0 - 63 >= p.reach;
+                    far = w0 + 31 <= -p.reach || w0 - 31 >= p.reach;
                     if (far) e_far = E[w0 > 0 ? 2 * p.reach + kBiasPad : kBiasPad];
                 }
                 const float* er = E + rel0 + p.reach + kBiasPad;
-                uint32_t w[32];
+                uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     const float4 m = m4[i];
                     float2 x0, x1;
                     if (BIAS) {
@@ -237,21 +240,20 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                         s[2 * i + 1] = p1;
                     }
                 }
-                tc::store32(at_s, w);
+                tc::store16(at_s, w);
                 tc::wait_st();
                 tc::fence_before();
-                mbar_arrive(&bars.p_ready);
+                mbar_arrive(&bars.p_ready[it & 1]);
 
                 alive = __all_sync(0xffffffffu, wait(&bars.dp_full, it & 1));
                 if (!alive) break;
                 tc::fence_after();
-                float2 d[32];
+                float2 d[16];
                 tc::load32(at_dp, reinterpret_cast<float*>(d));
-                tc::load32(at_dp + 32, reinterpret_cast<float*>(d + 16));
                 tc::wait_ld();
-                const float4* d4 = reinterpret_cast<const float4*>(rows[st][2] + 64 * half);
+                const float4* d4 = reinterpret_cast<const float4*>(rows[st][2] + 32 * part);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     const float4 dl = d4[i];
                     float2 a0, a1;
                     if (kBf16) {
@@ -272,23 +274,24 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     w[2 * i] = tc::pack2<T>(a0.x, a0.y);
                     w[2 * i + 1] = tc::pack2<T>(a1.x, a1.y);
                 }
-                tc::store32(at_dp, w);
+                tc::store16(at_dp, w);
                 tc::wait_st();
                 tc::fence_before();
-                mbar_arrive(&bars.ds_ready);
+                mbar_arrive(&bars.ds_ready[it & 1]);
             }
         }
         if (alive && total > 0) alive = __all_sync(0xffffffffu, wait(&bars.done, 0));
         if (alive) {
             tc::fence_after();
-            // first half of the warps: dV, second: dK
+            // even parts: dV, odd: dK, each every other 32 columns
+            const bool half = part & 1;
             const uint32_t src = (half ? t_dk : t_dv) + lane_base;
             const float back = kBf16 ? 1.f : 1.f / 64.f;
             const float mul = half ? static_cast<float>(p.scale) * back * g : back;
             T* dst = static_cast<T*>(half ? gr.dk : gr.dv) +
                      ((static_cast<int64_t>(b) * p.Lk + key) * p.Hkv + hk) * p.D;
 #pragma unroll 1
-            for (int c = 0; c < cols; c += 32) {
+            for (int c = 32 * (part >> 1); c < cols; c += 64) {
                 float o[32];
                 if (total > 0) {
                     tc::load32(src + c, o);
@@ -310,15 +313,16 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             tc::fence_before();
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 8 && lane == 0 && total > 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 16 && lane == 0 && total > 0) {
             bool alive = true;
             mbar_arrive_expect_tx(&bars.fixed, 2 * S::tile);
             load_rows<DP>(Ks, &mk, &bars.fixed, hk, k0, b);
             load_rows<DP>(Vs, &mv, &bars.fixed, hk, k0, b);
-            int it = 0;
-            for (; it < total; ++it) {
-                const int s = it % NS, h = hk * p.G + it / nq, j = fb + it % nq;
+            int it = 0, h = hk * p.G, j = fb;
+            for (; it < total; ++it, ++j) {
+                const int s = it % NS;
+                if (j == lb) { j = fb; ++h; }
                 if (it >= NS) alive = wait(&bars.empty[s], (it / NS - 1) & 1);
                 if (!alive) break;
                 mbar_arrive_expect_tx(&bars.x_full[s], S::tile);
@@ -333,49 +337,77 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     mbar_wait32(smem_u32(&bars.x_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                     mbar_wait32(smem_u32(&bars.y_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                 }
-        } else if (warp == 9 && lane == 0 && total > 0) {
+        } else if (warp == 17 && total > 0) {
             const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
             const uint32_t its = tc::product(kBf16, 128, cols, false, true);
-            bool alive = wait(&bars.fixed, 0);
+            const bool lead = tc::elect();
+            auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+            bool alive = all(wait(&bars.fixed, 0));
+            auto S_at = [&](int i) { return t_s + (kTwoS ? 128 * (i & 1) : 0); };
+            // S(i) into its place, once the product that read P there is done
+            auto scores = [&](int i) {
+                const int s = i % NS, last = kTwoS ? i - 2 : i - 1;
+                alive = all(wait(&bars.x_full[s], (i / NS) & 1) && wait(&bars.ok[s], (i / NS) & 1) &&
+                            (last < 0 || wait(&bars.used_p, last & 1)));
+                if (!alive) return;
+                tc::fence_after();
+                if (lead) {
+                    scores_mma<DP>(S_at(i), smem_u32(Ks), smem_u32(Q_at(s)), iss, steps);
+                    tc::commit(smem_u32(&bars.s_full[i & 1]));
+                }
+            };
             for (int it = -1; alive && it < total; ++it) {
                 const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
-                const uint32_t pn = (next / NS) & 1;
-                if (it >= 0) {
-                    alive = wait(&bars.p_ready, it & 1);
+                if (kTwoS && next < total) {
+                    scores(next);
                     if (!alive) break;
-                    tc::fence_after();
-                    mix_mma<64>(t_dv, t_s, smem_u32(O_at(s)), its, it > 0);
-                }
-                if (next < total) {
-                    alive = wait(&bars.x_full[sn], pn) &&
-                            (!guarded(fb + next % nq) || wait(&bars.ok[sn], pn));
-                    if (!alive) break;
-                    scores_mma<DP>(t_s, smem_u32(Ks), smem_u32(Q_at(sn)), iss, steps);
-                    tc::commit(smem_u32(&bars.s_full));
                 }
                 if (it >= 0) {
-                    alive = wait(&bars.ds_ready, it & 1);
+                    alive = all(wait(&bars.p_ready[it & 1], (it >> 1) & 1));
                     if (!alive) break;
                     tc::fence_after();
-                    mix_mma<64>(t_dk, t_dp, smem_u32(Q_at(s)), its, it > 0);
-                    tc::commit(smem_u32(&bars.empty[s]));
+                    if (lead) {
+                        mix_mma<2, 32>(t_dv, S_at(it), smem_u32(O_at(s)), its, it > 0);
+                        tc::commit(smem_u32(&bars.used_p));
+                    }
+                }
+                if (!kTwoS && next < total) {
+                    scores(next);
+                    if (!alive) break;
+                }
+                if (it >= 0) {
+                    alive = all(wait(&bars.ds_ready[it & 1], (it >> 1) & 1));
+                    if (!alive) break;
+                    tc::fence_after();
+                    if (lead) {
+                        mix_mma<2, 32>(t_dk, t_dp, smem_u32(Q_at(s)), its, it > 0);
+                        tc::commit(smem_u32(&bars.used_ds));
+                        tc::commit(smem_u32(&bars.empty[s]));
+                    }
                 }
                 if (next < total) {
-                    alive = wait(&bars.y_full[sn], pn);
+                    alive = all(wait(&bars.y_full[sn], (next / NS) & 1) &&
+                                (it < 0 || wait(&bars.used_ds, it & 1)));
                     if (!alive) break;
-                    scores_mma<DP>(t_dp, smem_u32(Vs), smem_u32(O_at(sn)), iss, steps);
-                    tc::commit(smem_u32(&bars.dp_full));
+                    tc::fence_after();
+                    if (lead) {
+                        scores_mma<DP>(t_dp, smem_u32(Vs), smem_u32(O_at(sn)), iss, steps);
+                        tc::commit(smem_u32(&bars.dp_full));
+                    }
                 }
             }
-            if (alive) tc::commit(smem_u32(&bars.done));
-            else {
-                tc::commit(smem_u32(&bars.drain));
+            if (alive) {
+                if (lead) tc::commit(smem_u32(&bars.done));
+            } else {
+                if (lead) tc::commit(smem_u32(&bars.drain));
                 mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
             }
-        } else if (warp >= 10 && total > 0) {
-            const int gt = threadIdx.x - 320;
-            for (int it = 0; it < total; ++it) {
-                const int s = it % NS, h = hk * p.G + it / nq, j = fb + it % nq;
+        } else if (warp >= 18 && total > 0) {
+            const int gt = threadIdx.x - (kBwdMath + 64);
+            int h = hk * p.G, j = fb;
+            for (int it = 0; it < total; ++it, ++j) {
+                const int s = it % NS;
+                if (j == lb) { j = fb; ++h; }
                 const uint32_t parity = (it / NS) & 1;
                 const RowRec* src = recs + (static_cast<int64_t>(b) * p.Hq + h) * p.Lq;
                 float4 rec[2];
@@ -408,7 +440,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         __syncwarp();
     }
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         tc::fence_after();
         tc::tmem_free(tmem, 512);
     }
@@ -427,16 +459,16 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag[2];
     __shared__ int span[4];
-    __shared__ float diag[8][2][64], far_sum[8][2];
+    __shared__ float diag[16][64], far_sum[16][2];
     unsigned char* smem = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* Qs = smem;
     unsigned char* Os = smem + S::tile;
     unsigned char* ring = smem + 2 * S::tile;   // stages of K, V
     float* E = reinterpret_cast<float*>(smem + S::smem);
-    float* acc = E + 2 * p.reach + 2 * kBiasPad + 1;   // table sums, 8 warps by buckets
+    float* acc = E + 2 * p.reach + 2 * kBiasPad + 1;   // table sums, 16 warps by buckets
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = tc::uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const int64_t BH = static_cast<int64_t>(p.B) * p.Hq;
     const int nt = (p.Lq + kRows - 1) / kRows;
     const int t = nt - 1 - static_cast<int>(blockIdx.x / BH);
@@ -452,26 +484,28 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             mbar_init(&bars.empty[i], 1);
             mbar_init(&bars.ok[i], 64);
         }
-        mbar_init(&bars.s_full, 1);
+        mbar_init(&bars.ds_ready[0], kBwdMath);
+        mbar_init(&bars.ds_ready[1], kBwdMath);
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.ds_ready, 256);
-        mbar_init(&bars.dp_free, 256);
+        mbar_init(&bars.dp_free, kBwdMath);
+        mbar_init(&bars.used_p, 1);
+        mbar_init(&bars.used_ds, 1);
         mbar_init(&bars.done, 1);
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
         abort_flag[0] = 0;
         abort_flag[1] = static_cast<int>(bnd.budget);
     }
-    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    if (warp == 17) tc::tmem_alloc(&tmem_slot, 512);
     if (BIAS) {
         load_padded_bias(p, h, E, threadIdx.x, kBwdThreads);
         if (gr.tab)
-            for (int i = threadIdx.x; i < 8 * p.nb; i += kBwdThreads) acc[i] = 0.f;
+            for (int i = threadIdx.x; i < 16 * p.nb; i += kBwdThreads) acc[i] = 0.f;
     }
     __syncthreads();
     const int row = q0 + static_cast<int>(threadIdx.x & 127);
     int lo = 0, hi = 0;
-    if (warp < 8) {
+    if (warp < 16) {
         if (row < p.Lq) key_span(p, b, row, p.Lk, lo, hi);
         const int v0 = __reduce_min_sync(0xffffffffu, hi > lo ? lo : INT_MAX);
         const int v1 = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
@@ -485,12 +519,14 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
         }
     }
     __syncthreads();
-    const uint32_t tmem = tmem_slot;
-    const bool any = span[1] > span[0];
-    const int fb = any ? span[0] / kRows : 0, lb = any ? (span[1] + kRows - 1) / kRows : 0;
+    const uint32_t tmem = tc::uniform(tmem_slot);
+    const int s_lo = tc::uniform(span[0]), s_hi = tc::uniform(span[1]);
+    const int all_lo = tc::uniform(span[2]), all_hi = tc::uniform(span[3]);
+    const int fb = s_hi > s_lo ? s_lo / kRows : 0;
+    const int lb = s_hi > s_lo ? (s_hi + kRows - 1) / kRows : 0;
     const int total = lb - fb;
     auto guarded = [&](int j) {
-        return !(j * kRows >= span[2] && min((j + 1) * kRows, p.Lk) <= span[3]);
+        return !(j * kRows >= all_lo && min((j + 1) * kRows, p.Lk) <= all_hi);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
@@ -500,11 +536,11 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
     const int steps = (p.D + 15) / 16, cols = steps * 16;
     const uint32_t t_s = tmem, t_dp = tmem + 256, t_dq = tmem + 384;
 
-    if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int half = warp >> 2;
+    if (warp < 16) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMathRegs));
+        const int part = warp >> 2;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t at_s = t_s + lane_base + 64 * half, at_dp = t_dp + lane_base + 64 * half;
+        const uint32_t at_s = t_s + lane_base + 32 * part, at_dp = t_dp + lane_base + 32 * part;
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
         float m = -INFINITY, ll = 0.f, delta = 0.f, g = 1.f;
@@ -527,18 +563,16 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             alive = __all_sync(0xffffffffu, wait(&bars.dp_full, it & 1));
             if (!alive) break;
             tc::fence_after();
-            float2 s[32], d[32];
+            float2 s[16], d[16];
             const uint32_t as = at_s + 128 * (it & 1);
             tc::load32(at_dp, reinterpret_cast<float*>(d));
-            tc::load32(at_dp + 32, reinterpret_cast<float*>(d + 16));
             tc::load32(as, reinterpret_cast<float*>(s));
-            tc::load32(as + 32, reinterpret_cast<float*>(s + 16));
             tc::wait_ld();
             tc::fence_before();
             mbar_arrive(&bars.dp_free);
-            scores64<CAP>(s, y1);
-            const int k0 = j * kRows + 64 * half;
-            const bool whole = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 64);
+            if (CAP) tanh32(s, y1);
+            const int k0 = j * kRows + 32 * part;
+            const bool whole = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 32);
             const uint32_t from = static_cast<uint32_t>(lo - k0);
             const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
             const int rel0 = k0 - (row + off);   // distance at column 0, one more a column
@@ -546,13 +580,13 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             bool far = false;
             float e_far = 0.f;
             if (BIAS) {
-                far = w0 + 63 <= -p.reach || w0 - 31 >= p.reach;
+                far = w0 + 31 <= -p.reach || w0 - 31 >= p.reach;
                 if (far) e_far = E[w0 > 0 ? 2 * p.reach + kBiasPad : kBiasPad];
             }
             const float* er = E + rel0 + p.reach + kBiasPad;
-            uint32_t w[32];
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
+            for (int i = 0; i < 16; ++i) {
                 float2 x;
                 if (BIAS) {
                     float2 e = make_float2(e_far, e_far);
@@ -575,49 +609,37 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                 }
                 w[i] = tc::pack2<T>(z.x, z.y);
             }
-            tc::store32(as, w);
+            tc::store16(as, w);
             tc::wait_st();
             tc::fence_before();
-            mbar_arrive(&bars.ds_ready);
+            mbar_arrive(&bars.ds_ready[it & 1]);
             if (BIAS && gr.tab) {
                 if (far) {
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum = __fadd2_rn(sum, d[i]);
+                    for (int i = 0; i < 16; ++i) sum = __fadd2_rn(sum, d[i]);
                     const float v = (sum.x + sum.y) * undo;
                     if (w0 > 0) far_hi += v; else far_lo += v;
                 } else {
-                    // sums along the diagonals of the warp's 32 x 64 part, as two
-                    // squares side by side: a sum moves one lane up a column, and
-                    // is whole in lane 31, or where it is at the end.  Entry
-                    // 31 + c - r of a square.
-                    float a = 0.f, c = 0.f;
+                    // sums along the diagonals of the warp's 32 x 32 part: a sum moves
+                    // one lane up a column, and is whole in lane 31, or where it is at
+                    // the end.  Entry 31 + c - r.
+                    float a = 0.f;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float za = (i & 1) ? d[i >> 1].y : d[i >> 1].x;
-                        const float zc = (i & 1) ? d[16 + (i >> 1)].y : d[16 + (i >> 1)].x;
+                        const float z = (i & 1) ? d[i >> 1].y : d[i >> 1].x;
                         a = __shfl_up_sync(0xffffffffu, a, 1);
-                        c = __shfl_up_sync(0xffffffffu, c, 1);
-                        a = fmaf(za, undo, lane == 0 ? 0.f : a);
-                        c = fmaf(zc, undo, lane == 0 ? 0.f : c);
-                        if (lane == 31) {
-                            diag[warp][0][i] = a;
-                            diag[warp][1][i] = c;
-                        }
+                        a = fmaf(z, undo, lane == 0 ? 0.f : a);
+                        if (lane == 31) diag[warp][i] = a;
                     }
-                    if (lane < 31) {
-                        diag[warp][0][62 - lane] = a;
-                        diag[warp][1][62 - lane] = c;
-                    }
+                    if (lane < 31) diag[warp][62 - lane] = a;
                     __syncwarp();
                     for (int u = lane; u < p.nb; u += 32) {
                         float sum = 0.f;
-                        for (int i = 0; i < 95; ++i) {
+                        for (int i = 0; i < 63; ++i) {
                             const int at = min(max(w0 + i - 31, -p.reach), p.reach) + p.reach;
                             const int bu = min(max(__ldg(p.lut + at), 0), p.nb - 1);
-                            if (bu == u)
-                                sum += (i < 63 ? diag[warp][0][i] : 0.f) +
-                                       (i >= 32 ? diag[warp][1][i - 32] : 0.f);
+                            if (bu == u) sum += diag[warp][i];
                         }
                         acc[warp * p.nb + u] += sum;
                     }
@@ -643,7 +665,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             T* dst = static_cast<T*>(gr.dq) +
                      ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
 #pragma unroll 1
-            for (int c = 32 * half; c < cols; c += 64) {
+            for (int c = 32 * part; c < cols; c += 128) {
                 float o[32];
                 if (total > 0) {
                     tc::load32(t_dq + lane_base + c, o);
@@ -665,8 +687,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             tc::fence_before();
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 8 && lane == 0 && total > 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 16 && lane == 0 && total > 0) {
             bool alive = true;
             mbar_arrive_expect_tx(&bars.fixed, 2 * S::tile);
             load_rows<DP>(Qs, &mq, &bars.fixed, h, q0, b);
@@ -688,47 +710,54 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                     mbar_wait32(smem_u32(&bars.x_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                     mbar_wait32(smem_u32(&bars.y_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                 }
-        } else if (warp == 9 && lane == 0 && total > 0) {
+        } else if (warp == 17 && total > 0) {
             const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
             const uint32_t its = tc::product(kBf16, 128, cols, false, true);
-            bool alive = wait(&bars.fixed, 0);
-            uint32_t okp = 0;
+            const bool lead = tc::elect();
+            auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+            bool alive = all(wait(&bars.fixed, 0));
             for (int it = -1; alive && it < total; ++it) {
                 const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
                 const uint32_t pn = (next / NS) & 1;
                 if (next < total) {
-                    alive = wait(&bars.x_full[sn], pn);
-                    if (alive && guarded(fb + next)) {
-                        alive = wait(&bars.ok[sn], okp >> sn & 1);
-                        okp ^= 1u << sn;
-                    }
-                    if (!alive) break;
-                    scores_mma<DP>(t_s + 128 * (next & 1), smem_u32(Qs), smem_u32(K_at(sn)), iss, steps);
-                    alive = wait(&bars.y_full[sn], pn) && (it < 0 || wait(&bars.dp_free, it & 1));
+                    alive = all(wait(&bars.x_full[sn], pn));
+                    // (its place holds dS of the block before last until dQ has read it)
+                    alive = alive && all(wait(&bars.ok[sn], pn) &&
+                                         (it < 1 || wait(&bars.used_ds, (it - 1) & 1)));
                     if (!alive) break;
                     tc::fence_after();
-                    scores_mma<DP>(t_dp, smem_u32(Os), smem_u32(V_at(sn)), iss, steps);
-                    tc::commit(smem_u32(&bars.dp_full));
+                    if (lead) scores_mma<DP>(t_s + 128 * (next & 1), smem_u32(Qs), smem_u32(K_at(sn)), iss, steps);
+                    alive = all(wait(&bars.y_full[sn], pn) && (it < 0 || wait(&bars.dp_free, it & 1)));
+                    if (!alive) break;
+                    tc::fence_after();
+                    if (lead) scores_mma<DP>(t_dp, smem_u32(Os), smem_u32(V_at(sn)), iss, steps);
+                    if (lead) tc::commit(smem_u32(&bars.dp_full));
                 }
                 if (it >= 0) {
-                    alive = wait(&bars.ds_ready, it & 1);
+                    alive = all(wait(&bars.ds_ready[it & 1], (it >> 1) & 1));
                     if (!alive) break;
                     tc::fence_after();
-                    mix_mma<64>(t_dq, t_s + 128 * (it & 1), smem_u32(K_at(s)), its, it > 0);
-                    tc::commit(smem_u32(&bars.empty[s]));
+                    if (lead) mix_mma<2, 32>(t_dq, t_s + 128 * (it & 1), smem_u32(K_at(s)), its, it > 0);
+                    if (lead) tc::commit(smem_u32(&bars.used_ds));
+                    if (lead) tc::commit(smem_u32(&bars.empty[s]));
                 }
             }
-            if (alive) tc::commit(smem_u32(&bars.done));
-            else {
-                tc::commit(smem_u32(&bars.drain));
+            if (alive) {
+                if (lead) tc::commit(smem_u32(&bars.done));
+            } else {
+                if (lead) tc::commit(smem_u32(&bars.drain));
                 mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
             }
-        } else if (warp >= 10 && total > 0) {
-            const int gt = threadIdx.x - 320;
+        } else if (warp >= 18 && total > 0) {
+            const int gt = threadIdx.x - (kBwdMath + 64);
             for (int it = 0; it < total; ++it) {
-                if (!guarded(fb + it)) continue;
                 const int s = it % NS;
                 const uint32_t parity = (it / NS) & 1;
+                if (it >= NS && !wait(&bars.empty[s], parity ^ 1)) break;
+                if (!guarded(fb + it)) {
+                    mbar_arrive(&bars.ok[s]);
+                    continue;
+                }
                 if (!wait(&bars.x_full[s], parity) || !wait(&bars.y_full[s], parity)) break;
                 const uint32_t bad = scrub_rows<T, DP>(K_at(s), gt, 64);
                 if (bad) {   // the rows that see it get NaN by dP
@@ -748,14 +777,14 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
         const int b_lo = min(max(__ldg(p.lut), 0), p.nb - 1);
         const int b_hi = min(max(__ldg(p.lut + 2 * p.reach), 0), p.nb - 1);
         float sum = 0.f;
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
             sum += acc[i * p.nb + u];
             if (u == b_lo) sum += far_sum[i][0];
             if (u == b_hi) sum += far_sum[i][1];
         }
         static_cast<float*>(gr.tab)[(static_cast<int64_t>(h) * gr.n_part + b * nt + t) * p.nb + u] = sum;
     }
-    if (warp == 9) {
+    if (warp == 17) {
         tc::fence_after();
         tc::tmem_free(tmem, 512);
     }
@@ -769,8 +798,8 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, co
     auto kq = tc_dq_kernel<T, DP, CAP, BIAS>;
     const int e = BIAS ? 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0;
     const int smk = BwdShape<DP>::smem + 1024 + e;
-    const int smq = smk + (BIAS && g.tab ? 4 * 8 * p.nb : 0);
-    const int regs = 256 * 208 + 128 * 80;
+    const int smq = smk + (BIAS && g.tab ? 4 * 16 * p.nb : 0);
+    const int regs = kBwdMath * kMathRegs + 128 * kOtherRegs;
     nsc_status ready = tc_ready(reinterpret_cast<const void*>(kk), smk, kBwdThreads, regs);
     if (ready == NSC_OK) ready = tc_ready(reinterpret_cast<const void*>(kq), smq, kBwdThreads, regs);
     if (ready != NSC_OK) return ready;

@@ -5,11 +5,14 @@
 // same queries (one load of K and V serves both), or 256 queries of one head.
 // Roles by warp: 0-3 and 4-7 the softmax of a tile each, a thread a row; 8 loads K
 // and V blocks of 128 keys through a ring by TMA; 9 issues the products; 10 and
-// 11 guard (below).  Tensor memory holds S of both tiles (P takes the place of
-// its S as 16-bit pairs) and both O.  The products are issued in the order
-// PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1), so one tile's products run beside the
-// other's softmax; they complete in order, so S(j+1) full also says that
-// PV(j) is done and O may be rescaled.
+// 11 guard (below).
+//
+// Tensor memory holds S and O of both tiles.  At D <= 64 there is room for P, as
+// 16-bit pairs, beside S: QK(j+1) starts as soon as S(j) is in registers and runs
+// beside the softmax of block j.  At D = 128 P takes the place of its S, so QK(j+1)
+// waits until PV(j) is done, and one tile's products run beside the other's softmax.
+// (Products of different shapes or accumulators need not complete in the order
+// of their issue; whatever overwrites an operand waits for its reader's commit.)
 //
 // Softmax with a running reference m: p = 2^(s2 - m); m moves, and O is
 // rescaled, only when a row's maximum passes m + 8 (p <= 256 keeps 16-bit
@@ -36,13 +39,16 @@ constexpr int kFwdThreads = 384;
 constexpr float kLazy = 8.f;
 
 template <int DP> struct FwdShape {
+    static constexpr bool apart = DP == 64;                   // P beside S
+    static constexpr int p_col = apart ? 256 : 0, p_step = apart ? 64 : 128;
+    static constexpr int o_col = apart ? 384 : 256;
     static constexpr int tile = DP / 64 * kPanel;             // bytes of a tile
     static constexpr int stages = DP == 64 ? 4 : 2;           // K and V blocks in flight
     static constexpr int smem = 2 * tile + stages * 2 * tile; // + bias + 1024 of alignment
 };
 
 struct FwdBars {
-    uint64_t q, k_full[4], v_full[4], empty[4], ok[4], s_full[2], p_full[2], o_full[2], drain;
+    uint64_t q, k_full[4], v_full[4], empty[4], ok[4], s_full[2], s_free[2], p_full[2], pv[2], o_full[2], drain;
 };
 
 template <typename T, int DP, bool CAP, bool BIAS>
@@ -63,7 +69,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     unsigned char* KV = smem + 2 * S::tile;         // stages of K, V
     float* E = reinterpret_cast<float*>(smem + S::smem);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = tc::uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     // pair: tiles are heads h, h + 1 of one row block; else 256 rows of a head
     const int HH = pair ? p.Hq / 2 : p.Hq;
     const int64_t BH = static_cast<int64_t>(p.B) * HH;
@@ -85,7 +91,9 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.s_free[i], kRows);
             mbar_init(&bars.p_full[i], kRows);
+            mbar_init(&bars.pv[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
         mbar_init(&bars.drain, 1);
@@ -119,13 +127,16 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     if (BIAS && pair)
         load_padded_bias(p, h0 + 1, E + 2 * p.reach + 2 * kBiasPad + 1, threadIdx.x, kFwdThreads);
     __syncthreads();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = tc::uniform(tmem_slot);
     int fb[2], lb[2];          // key blocks [fb, lb) of a tile
+    int all_lo[2], all_hi[2];  // keys that all its rows see
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const bool any = span[i][1] > span[i][0];
-        fb[i] = any ? span[i][0] / kRows : INT_MAX;
-        lb[i] = any ? (span[i][1] + kRows - 1) / kRows : 0;
+        const int s0 = tc::uniform(span[i][0]), s1 = tc::uniform(span[i][1]);
+        all_lo[i] = tc::uniform(span[i][2]);
+        all_hi[i] = tc::uniform(span[i][3]);
+        fb[i] = s1 > s0 ? s0 / kRows : INT_MAX;
+        lb[i] = s1 > s0 ? (s1 + kRows - 1) / kRows : 0;
     }
     const int j0 = min(fb[0], fb[1]), j1 = max(lb[0], lb[1]);
     auto on = [&](int i, int j) { return j >= fb[i] && j < lb[i]; };
@@ -133,7 +144,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         bool g = false;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            g |= on(i, j) && !(j * kRows >= span[i][2] && min((j + 1) * kRows, n) <= span[i][3]);
+            g |= on(i, j) && !(j * kRows >= all_lo[i] && min((j + 1) * kRows, n) <= all_hi[i]);
         return g;
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -147,7 +158,8 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + a * 128 + lane_base, to = tmem + 256 + a * DP + lane_base;
+        const uint32_t ts = tmem + a * 128 + lane_base, to = tmem + S::o_col + a * DP + lane_base;
+        const uint32_t tp = tmem + S::p_col + a * S::p_step + lane_base;
         const int h = h0 + (pair ? a : 0);
         const int pos = row + n - p.Lq;
         const float* Eh = E + (pair && a ? 2 * p.reach + 2 * kBiasPad + 1 : 0);
@@ -164,6 +176,10 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
 #pragma unroll
             for (int c = 0; c < 4; ++c) tc::load32(ts + 32 * c, reinterpret_cast<float*>(s + 16 * c));
             tc::wait_ld();
+            if (S::apart) {
+                tc::fence_before();
+                mbar_arrive(&bars.s_free[a]);
+            }
             const int k0 = j * kRows;
             if (CAP) {
 #pragma unroll
@@ -207,6 +223,11 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 keep = m == -INFINITY ? 0.f : tc::ex2(m - top);
                 m = fmaxf(top, m);
             }
+            if (S::apart && it > 0) {   // PV of the last block: P and O are free
+                alive = __all_sync(0xffffffffu, wait(&bars.pv[a], (it - 1) & 1));
+                if (!alive) break;
+                tc::fence_after();
+            }
             if (it > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
                 l *= keep;
                 const float2 k2 = make_float2(keep, keep);
@@ -233,7 +254,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     sums[i & 3] = __fadd2_rn(sums[i & 3], e);
                     w[i] = tc::pack2<T>(e.x, e.y);
                 }
-                tc::store16(ts + 16 * c, w);
+                tc::store16(tp + 16 * c, w);
             }
             const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
             l += sum.x + sum.y;
@@ -307,53 +328,80 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     mbar_wait32(smem_u32(&bars.k_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                     mbar_wait32(smem_u32(&bars.v_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                 }
-        } else if (warp == 9 && lane == 0 && j0 < j1) {
+        } else if (warp == 9 && j0 < j1) {
             const uint32_t iqk = tc::product(kBf16, 128, 128, false, false);
             const uint32_t ipv = tc::product(kBf16, 128, cols, false, true);
-            bool alive = wait(&bars.q, 0);
-            int pn[2] = {0, 0};   // P tiles taken
-            uint32_t okp = 0;     // a bit a stage: the phase of its next guarded block
+            const bool lead = tc::elect();
+            auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+            bool alive = all(wait(&bars.q, 0));
+            int pn[2] = {0, 0};   // blocks of a tile multiplied with V
+            auto scores = [&](int x, int sn) {
+                if (!lead) return;
+                scores_mma<DP>(tmem + x * 128, smem_u32(Qs + x * S::tile), smem_u32(K_at(sn)), iqk,
+                               steps);
+                tc::commit(smem_u32(&bars.s_full[x]));
+            };
+            auto mix = [&](int x, int s, bool last) {
+                if (!lead) return;
+                mix_mma<8, 64>(tmem + S::o_col + x * DP, tmem + S::p_col + x * S::p_step,
+                               smem_u32(V_at(s)), ipv, pn[x] > 0);
+                tc::commit(smem_u32(&bars.pv[x]));
+                if (last) tc::commit(smem_u32(&bars.o_full[x]));
+            };
             for (int j = j0 - 1; alive && j < j1; ++j) {
                 const int i = j - j0, s = (i + NS) % NS, sn = (i + 1) % NS;
                 const uint32_t parity = ((i + 1) / NS) & 1;
                 if (j + 1 < j1) {
-                    alive = wait(&bars.k_full[sn], parity);
-                    if (alive && guarded(j + 1)) {
-                        alive = wait(&bars.ok[sn], okp >> sn & 1);
-                        okp ^= 1u << sn;
-                    }
+                    alive = all(wait(&bars.k_full[sn], parity) && wait(&bars.ok[sn], parity));
+                    if (!alive) break;
+                }
+                if (S::apart) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        if (on(x, j + 1)) {
+                            if (on(x, j)) alive = alive && all(wait(&bars.s_free[x], pn[x] & 1));
+                            if (!alive) break;
+                            tc::fence_after();
+                            scores(x, sn);
+                        }
                     if (!alive) break;
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if (j >= j0 && on(x, j)) {
-                        alive = wait(&bars.v_full[s], (i / NS) & 1) && wait(&bars.p_full[x], pn[x] & 1);
+                        alive = all(wait(&bars.v_full[s], (i / NS) & 1) &&
+                                    wait(&bars.p_full[x], pn[x] & 1));
                         if (!alive) break;
                         tc::fence_after();
-                        mix_mma<32>(tmem + 256 + x * DP, tmem + x * 128, smem_u32(V_at(s)), ipv,
-                                    pn[x] > 0);
+                        mix(x, s, j + 1 == lb[x]);
                         ++pn[x];
-                        if (j + 1 == lb[x]) tc::commit(smem_u32(&bars.o_full[x]));
                     }
-                    if (on(x, j + 1)) {
-                        scores_mma<DP>(tmem + x * 128, smem_u32(Qs + x * S::tile),
-                                       smem_u32(K_at(sn)), iqk, steps);
-                        tc::commit(smem_u32(&bars.s_full[x]));
+                    if (!S::apart && on(x, j + 1)) {
+                        if (pn[x] > 0) alive = all(wait(&bars.pv[x], (pn[x] - 1) & 1));
+                        if (!alive) break;
+                        tc::fence_after();
+                        scores(x, sn);
                     }
                 }
-                if (alive && j >= j0) tc::commit(smem_u32(&bars.empty[s]));
+                if (alive && j >= j0 && lead) tc::commit(smem_u32(&bars.empty[s]));
             }
             if (!alive) {   // the products in flight read this block's memory
-                tc::commit(smem_u32(&bars.drain));
+                if (lead) tc::commit(smem_u32(&bars.drain));
                 mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
             }
         } else if (warp >= 10 && j0 < j1) {
             const int g = threadIdx.x - 320;
+            // in step with the ring: every block is passed on, after the one before it in
+            // the stage was used up, so no phase of a barrier is taken for another
             int i = 0;
             for (int j = j0; j < j1; ++j, ++i) {
-                if (!guarded(j)) continue;
                 const int s = i % NS;
                 const uint32_t parity = (i / NS) & 1;
+                if (i >= NS && !wait(&bars.empty[s], parity ^ 1)) break;
+                if (!guarded(j)) {
+                    mbar_arrive(&bars.ok[s]);
+                    continue;
+                }
                 if (!wait(&bars.k_full[s], parity) || !wait(&bars.v_full[s], parity)) break;
                 const uint32_t bad = scrub_rows<T, DP>(V_at(s), g, 64);
                 if (bad) {
