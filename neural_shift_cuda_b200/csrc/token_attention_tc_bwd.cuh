@@ -48,6 +48,19 @@ struct BwdBars {
     uint64_t s_full[2], p_ready[2], ds_ready[2], dp_full, dp_free, used_p, used_ds, done, drain;
 };
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+}
+// A float at this block's shared address `at`, in block `rank` of the cluster.
+__device__ __forceinline__ float cluster_load(uint32_t at, int rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float pow2_near(float v) {   // a power of two at or above v, or 1
     if (!(v > 0.f) || !(v < 3e38f)) return 1.f;
     const int e = static_cast<int>((__float_as_uint(v) >> 23) & 0xFF) + 1;
@@ -59,6 +72,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mo,
     const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p,
     const Grads gr, const RowRec* __restrict__ recs, const float* __restrict__ norms, const int n_norm,
+    const int split,
     const Bounded bnd) {
     using S = BwdShape<DP>;
     constexpr int NS = S::stages;
@@ -79,9 +93,12 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     float* E = reinterpret_cast<float*>(smem + S::smem);
 
     const int warp = tc::uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    // a cluster of `split` blocks shares the query heads of a key head
     const int64_t BH = static_cast<int64_t>(p.B) * p.Hkv;
-    const int t = static_cast<int>(blockIdx.x / BH);
-    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hkv, hk = bh % p.Hkv;
+    const int64_t unit_id = blockIdx.x / split;
+    const int t = static_cast<int>(unit_id / BH), rank = static_cast<int>(blockIdx.x % split);
+    const int bh = static_cast<int>(unit_id % BH), b = bh / p.Hkv, hk = bh % p.Hkv;
+    const int heads = p.G / split, head0 = hk * p.G + rank * heads;
     const int k0 = t * kRows, off = p.Lk - p.Lq;
 
     if (threadIdx.x < 4) span[threadIdx.x] = threadIdx.x == 0 || threadIdx.x == 3 ? INT_MAX : 0;
@@ -139,7 +156,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     const int all_lo = tc::uniform(span[2]), all_hi = tc::uniform(span[3]);
     const int fb = s_hi > s_lo ? s_lo / kRows : 0;
     const int lb = s_hi > s_lo ? (s_hi + kRows - 1) / kRows : 0;
-    const int nq = lb - fb, total = nq * p.G;
+    const int nq = lb - fb, total = nq * heads;
     const float g = kBf16 ? 1.f : pow2_near(__uint_as_float(top_norm));
     // a key tail past Lk has zero rows of K and V, and sees nothing
     auto guarded = [&](int j) {
@@ -166,11 +183,11 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         const float2 u2 = make_float2(unit, unit), g2 = make_float2(1.f / g, 1.f / g);
         bool alive = true;
         int it = 0;
-        for (int u = 0; u < p.G && nq > 0; ++u) {
+        for (int u = 0; u < heads && nq > 0; ++u) {
             if (BIAS) {   // E of this head, once all are done with the last (a warp
                           // that gave up comes here too)
                 named_sync(1, kBwdMath);
-                load_padded_bias(p, hk * p.G + u, E, threadIdx.x, kBwdMath);
+                load_padded_bias(p, head0 + u, E, threadIdx.x, kBwdMath);
                 named_sync(1, kBwdMath);
             }
             for (int j = fb; alive && j < lb; ++j, ++it) {
@@ -281,19 +298,18 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             }
         }
         if (alive && total > 0) alive = __all_sync(0xffffffffu, wait(&bars.done, 0));
-        if (alive) {
-            tc::fence_after();
-            // even parts: dV, odd: dK, each every other 32 columns
-            const bool half = part & 1;
-            const uint32_t src = (half ? t_dk : t_dv) + lane_base;
-            const float back = kBf16 ? 1.f : 1.f / 64.f;
-            const float mul = half ? static_cast<float>(p.scale) * back * g : back;
-            T* dst = static_cast<T*>(half ? gr.dk : gr.dv) +
-                     ((static_cast<int64_t>(b) * p.Lk + key) * p.Hkv + hk) * p.D;
+        const bool half = part & 1;   // even parts: dV, odd: dK, each every other 32 columns
+        const uint32_t src = (half ? t_dk : t_dv) + lane_base;
+        const float back = kBf16 ? 1.f : 1.f / 64.f;
+        const float mul = half ? static_cast<float>(p.scale) * back * g : back;
+        T* dst = static_cast<T*>(half ? gr.dk : gr.dv) +
+                 ((static_cast<int64_t>(b) * p.Lk + key) * p.Hkv + hk) * p.D;
+        tc::fence_after();
+        if (split == 1) {
 #pragma unroll 1
             for (int c = 32 * (part >> 1); c < cols; c += 64) {
                 float o[32];
-                if (total > 0) {
+                if (total > 0 && alive) {
                     tc::load32(src + c, o);
                     tc::wait_ld();
                 }
@@ -310,8 +326,22 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
-            tc::fence_before();
+        } else {
+            // this block's sums to its own shared memory, [dV, dK][column][row]
+            float* own = reinterpret_cast<float*>(smem) + (half ? DP * kRows : 0);
+#pragma unroll 1
+            for (int c = 32 * (part >> 1); c < cols; c += 64) {
+                float o[32];
+                if (total > 0 && alive) {
+                    tc::load32(src + c, o);
+                    tc::wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    own[(c + i) * kRows + (threadIdx.x & 127)] = total > 0 && hi > lo ? o[i] * mul : 0.f;
+            }
         }
+        tc::fence_before();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == 16 && lane == 0 && total > 0) {
@@ -319,7 +349,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             mbar_arrive_expect_tx(&bars.fixed, 2 * S::tile);
             load_rows<DP>(Ks, &mk, &bars.fixed, hk, k0, b);
             load_rows<DP>(Vs, &mv, &bars.fixed, hk, k0, b);
-            int it = 0, h = hk * p.G, j = fb;
+            int it = 0, h = head0, j = fb;
             for (; it < total; ++it, ++j) {
                 const int s = it % NS;
                 if (j == lb) { j = fb; ++h; }
@@ -404,7 +434,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             }
         } else if (warp >= 18 && total > 0) {
             const int gt = threadIdx.x - (kBwdMath + 64);
-            int h = hk * p.G, j = fb;
+            int h = head0, j = fb;
             for (int it = 0; it < total; ++it, ++j) {
                 const int s = it % NS;
                 if (j == lb) { j = fb; ++h; }
@@ -438,6 +468,31 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             }
         }
         __syncwarp();
+    }
+    if (split > 1) {
+        // Joined over the cluster in the order of its ranks: block `rank` sums its share of
+        // the columns, four at a time, from every block's shared memory.
+        cluster_sync();
+        if (warp < 16 && k0 + static_cast<int>(threadIdx.x & 127) < p.Lk) {
+            const int row = threadIdx.x & 127, groups = cols / 4;
+            for (int x = static_cast<int>(threadIdx.x >> 7) * split + rank; x < 2 * groups;
+                 x += 4 * split) {
+                const bool half = x >= groups;
+                const int c = (half ? x - groups : x) * 4;
+                if (c >= p.D) continue;
+                const uint32_t at = smem_u32(reinterpret_cast<float*>(smem) +
+                                             ((half ? DP : 0) + c) * kRows + row);
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int r = 0; r < split; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] += cluster_load(at + e * kRows * 4, r);
+                T* dst = static_cast<T*>(half ? gr.dk : gr.dv) +
+                         ((static_cast<int64_t>(b) * p.Lk + k0 + row) * p.Hkv + hk) * p.D + c;
+                *reinterpret_cast<uint2*>(dst) =
+                    make_uint2(tc::pack2<T>(sum[0], sum[1]), tc::pack2<T>(sum[2], sum[3]));
+            }
+        }
+        cluster_sync();   // no block leaves while another reads its memory
     }
     __syncthreads();
     if (warp == 17) {
@@ -814,10 +869,31 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, co
     if (!bnd.timeouts)
         return fail(NSC_ERR_LAUNCH_FAILED, "token_attention backward: no wait counter");
     wait_fault_settings(&bnd.skip, &bnd.budget);
-    const int64_t nk = static_cast<int64_t>((p.Lk + kRows - 1) / kRows) * p.B * p.Hkv;
+    // Blocks of a cluster share the query heads of a key head where there would be fewer
+    // than three blocks an SM: the few long blocks of a causal or packed batch end last.
+    // No more of them than that takes, since a cluster's blocks have to find SMs side by
+    // side.  (16 heads on 4, four documents in 8192 tokens, 256 key tiles of 4 heads: 500 us
+    // alone, 341 in twos, 402 in fours.)
+    const int64_t tiles = static_cast<int64_t>((p.Lk + kRows - 1) / kRows) * p.B * p.Hkv;
+    int split = 1;
+    for (int i = 2; i <= 8 && tiles * split < 3 * 148; ++i)
+        if (p.G % i == 0) split = i;
+    const int64_t nk = tiles * split;
     const int64_t nq = static_cast<int64_t>((p.Lq + kRows - 1) / kRows) * p.B * p.Hq;
-    kk<<<static_cast<unsigned>(nk), kBwdThreads, smk, st>>>(mq, mo, mk, mv, p, g, recs, norms, n_norm,
-                                                           bnd);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(nk));
+    cfg.blockDim = dim3(kBwdThreads);
+    cfg.dynamicSmemBytes = smk;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = split;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kk, mq, mo, mk, mv, p, g, recs, norms, n_norm, split, bnd) !=
+        cudaSuccess)
+        return check_launch("token_attention backward");
     kq<<<static_cast<unsigned>(nq), kBwdThreads, smq, st>>>(mq, mo, mk, mv, p, g, recs, bnd);
     return check_launch("token_attention backward");
 }

@@ -356,3 +356,22 @@ def test_no_queries_or_no_keys(cuda):
         assert (g == 0).all()
     e = torch.zeros(0, 5, 2, 64, dtype=BF16, device=cuda)
     assert nsc.token_attention(e, e, e).shape == (0, 5, 2, 64)
+
+
+def test_slow_and_fast_warps_keep_in_step(cuda):
+    """Warps whose scores pass the cap's polynomial take far longer than others; no
+    block of products may start before the slowest has written its part."""
+    for dt, D in ((BF16, 64), (F16, 64), (BF16, 128)):
+        q = randn(0, 1, 140, 2, D, dtype=dt, mul=6.0).to(cuda)
+        k = randn(1, 1, 700, 1, D, dtype=dt, mul=6.0).to(cuda)
+        k[:, ::3] *= 0.01
+        v = randn(2, 1, 700, 1, D, dtype=dt).to(cuda)
+        go = randn(3, 1, 140, 2, D, dtype=dt).to(cuda)
+        first = None
+        for _ in range(12):
+            leaves = [leaf(t) for t in (q, k, v)]
+            out = nsc.token_attention(*leaves, causal=True, softcap=10.0)
+            now = [out, *torch.autograd.grad(out, leaves, go)]
+            first = first or now
+            for a, b in zip(first, now):
+                assert torch.equal(a, b)
