@@ -112,6 +112,7 @@ extern "C" NSC_API nsc_status nsc_token_attention_fwd(const nsc_attention* a, vo
     p.lse = lse;
     p.stats = stats;
     p.residue = residue;
+    if (short_fits(p, a->dtype)) return short_fwd(p, a->dtype, as_stream(stream));
     if (tc_fits(p, a->dtype)) return tc_fwd(p, a->dtype, as_stream(stream));
     return general_fwd(p, a->dtype, as_stream(stream));
 }

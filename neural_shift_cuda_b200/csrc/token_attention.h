@@ -131,6 +131,9 @@ int general_tile(int dtype, int D);
 // call's layout is one that their TMA boxes describe.
 bool tc_fits(const Params& p, int dtype);
 nsc_status tc_fwd(const Params& p, int dtype, cudaStream_t st);
+// token_attention_short.cu
+bool short_fits(const Params& p, int dtype);
+nsc_status short_fwd(const Params& p, int dtype, cudaStream_t st);
 bool tc_bwd_fits(const Params& p, const Grads& g, int dtype);
 int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t n_buckets);
 nsc_status tc_bwd(const Params& p, Grads g, void* workspace, void* grad_table, int dtype,
