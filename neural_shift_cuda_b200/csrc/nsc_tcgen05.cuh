@@ -161,5 +161,19 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return r;
 }
 
+// What rounding a and b to the 16-bit pair `w` dropped, rounded itself: w + rest has
+// twice the digits.
+template <typename T> __device__ __forceinline__ uint32_t rest2(float2 v, uint32_t w);
+template <> __device__ __forceinline__ uint32_t rest2<__nv_bfloat16>(float2 v, uint32_t w) {
+    const float2 h = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    const float2 r = __ffma2_rn(h, make_float2(-1.f, -1.f), v);
+    return pack2<__nv_bfloat16>(r.x, r.y);
+}
+template <> __device__ __forceinline__ uint32_t rest2<__half>(float2 v, uint32_t w) {
+    const float2 h = __half22float2(reinterpret_cast<const __half2&>(w));
+    const float2 r = __ffma2_rn(h, make_float2(-1.f, -1.f), v);
+    return pack2<__half>(r.x, r.y);
+}
+
 }  // namespace tc
 }  // namespace nsc

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {   // 16 keys
-            uint32_t pa[4];
+            uint32_t pa[4], rest[4];
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
@@ -185,6 +185,7 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
                     const float e1 = tc::ex2(s[2 * i + y][2 * x + 1] - ref);
                     l[x] += e0 + e1;
                     pa[2 * y + x] = tc::pack2<T>(e0, e1);
+                    rest[2 * y + x] = tc::rest2<T>(make_float2(e0, e1), pa[2 * y + x]);
                 }
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
@@ -192,6 +193,10 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
                 ldm4t(va + i * 16 * LD + 32 * c, f);
                 mma16816<T>(o[2 * c], pa, f[0], f[1]);
                 mma16816<T>(o[2 * c + 1], pa, f[2], f[3]);
+                if (BIAS && p.residue) {   // see the tensor-core forward
+                    mma16816<T>(o[2 * c], rest, f[0], f[1]);
+                    mma16816<T>(o[2 * c + 1], rest, f[2], f[3]);
+                }
             }
         }
     }

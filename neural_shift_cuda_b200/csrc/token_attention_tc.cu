@@ -64,8 +64,10 @@ __global__ __launch_bounds__(256) void record_kernel(Params p, Grads g, RowRec* 
             const int64_t at = static_cast<int64_t>(bh) * p.Lq + l;
             if (g.dlse) sum -= static_cast<const float*>(g.dlse)[at];
             const float* stats = static_cast<const float*>(p.stats);
-            recs[at] = RowRec{stats[at] + (sum - sum), stats[rows + at], sum, sqrtf(sq)};
-            most = fmaxf(most, sqrtf(sq));
+            // (a row that is not finite gives NaN, and does not set the others' scale)
+            const float norm = sq < INFINITY ? sqrtf(sq) : 0.f;
+            recs[at] = RowRec{stats[at] + (sum - sum), stats[rows + at], sum, norm};
+            most = fmaxf(most, norm);
         }
     }
     if (c == 0) top[sub] = most;

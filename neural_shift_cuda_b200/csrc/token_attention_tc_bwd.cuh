@@ -142,11 +142,14 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             atomicMin(&span[3], v3);
         }
     }
-    if (!kBf16) {   // the largest norm of dO among the heads of the group
+    __syncthreads();
+    if (!kBf16 && span[1] > span[0]) {   // the largest norm of dO among the queries of this tile
+        const int n0 = span[0] / kRows * (kRows / kRecRows);
+        const int n = min((span[1] + kRows - 1) / kRows * (kRows / kRecRows), n_norm) - n0;
+        const float* src = norms + (static_cast<int64_t>(b) * p.Hq + hk * p.G) * n_norm + n0;
         float top = 0.f;
-        const float* src = norms + (static_cast<int64_t>(b) * p.Hq + hk * p.G) * n_norm;
-        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.G) * n_norm; i += kBwdThreads)
-            top = fmaxf(top, src[i]);
+        for (int i = threadIdx.x; i < p.G * n; i += kBwdThreads)
+            top = fmaxf(top, src[static_cast<int64_t>(i / n) * n_norm + i % n]);
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         if (lane == 0) atomicMax(&top_norm, __float_as_uint(top));
     }
@@ -268,6 +271,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                 float2 d[16];
                 tc::load32(at_dp, reinterpret_cast<float*>(d));
                 tc::wait_ld();
+                uint32_t rest[16];
                 const float4* d4 = reinterpret_cast<const float4*>(rows[st][2] + 32 * part);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -290,8 +294,11 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     }
                     w[2 * i] = tc::pack2<T>(a0.x, a0.y);
                     w[2 * i + 1] = tc::pack2<T>(a1.x, a1.y);
+                    rest[2 * i] = tc::rest2<T>(a0, w[2 * i]);
+                    rest[2 * i + 1] = tc::rest2<T>(a1, w[2 * i + 1]);
                 }
                 tc::store16(at_dp, w);
+                tc::store16(at_dp + 16, rest);
                 tc::wait_st();
                 tc::fence_before();
                 mbar_arrive(&bars.ds_ready[it & 1]);
@@ -411,6 +418,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     tc::fence_after();
                     if (lead) {
                         mix_mma<2, 32>(t_dk, t_dp, smem_u32(Q_at(s)), its, it > 0);
+                        mix_mma<2, 32>(t_dk, t_dp + 16, smem_u32(Q_at(s)), its, true);
                         tc::commit(smem_u32(&bars.used_ds));
                         tc::commit(smem_u32(&bars.empty[s]));
                     }
@@ -639,7 +647,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                 if (far) e_far = E[w0 > 0 ? 2 * p.reach + kBiasPad : kBiasPad];
             }
             const float* er = E + rel0 + p.reach + kBiasPad;
-            uint32_t w[16];
+            uint32_t w[16], rest[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float2 x;
@@ -663,8 +671,10 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                     z = __ffma2_rn(z, n, z);
                 }
                 w[i] = tc::pack2<T>(z.x, z.y);
+                rest[i] = tc::rest2<T>(z, w[i]);
             }
             tc::store16(as, w);
+            tc::store16(as + 16, rest);
             tc::wait_st();
             tc::fence_before();
             mbar_arrive(&bars.ds_ready[it & 1]);
@@ -792,7 +802,11 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                     alive = all(wait(&bars.ds_ready[it & 1], (it >> 1) & 1));
                     if (!alive) break;
                     tc::fence_after();
-                    if (lead) mix_mma<2, 32>(t_dq, t_s + 128 * (it & 1), smem_u32(K_at(s)), its, it > 0);
+                    if (lead) {
+                        const uint32_t w = t_s + 128 * (it & 1);
+                        mix_mma<2, 32>(t_dq, w, smem_u32(K_at(s)), its, it > 0);
+                        mix_mma<2, 32>(t_dq, w + 16, smem_u32(K_at(s)), its, true);
+                    }
                     if (lead) tc::commit(smem_u32(&bars.used_ds));
                     if (lead) tc::commit(smem_u32(&bars.empty[s]));
                 }

@@ -17,7 +17,11 @@
 // Softmax with a running reference m: p = 2^(s2 - m); m moves, and O is
 // rescaled, only when a row's maximum passes m + 8 (p <= 256 keeps 16-bit
 // weights in range), which after the first blocks is rare.  P is rounded to the
-// operand type; the sum of a row is of the fp32 values.
+// operand type; the sum of a row is of the fp32 values.  REST, for training with a
+// bias table: what that rounding drops is multiplied too, as a second operand.  The
+// backward's row sums of grad_out * out are then those of the weights it recomputes, and
+// a bucket's gradient, a sum of many rows' nearly cancelling terms, keeps its digits
+// (bf16, 8192 rows: 1.7e-3 of it off, its own rounding, where 3.1e-3 were).
 //
 // Guard: in blocks that some row of a tile does not see whole, a value row
 // that is not finite would reach every row as 0 x NaN.  There the guard warps
@@ -38,8 +42,8 @@ namespace {
 constexpr int kFwdThreads = 384;
 constexpr float kLazy = 8.f;
 
-template <int DP> struct FwdShape {
-    static constexpr bool apart = DP == 64;                   // P beside S
+template <int DP, bool REST> struct FwdShape {
+    static constexpr bool apart = DP == 64 && !REST;          // P beside S
     static constexpr int p_col = apart ? 256 : 0, p_step = apart ? 64 : 128;
     static constexpr int o_col = apart ? 384 : 256;
     static constexpr int tile = DP / 64 * kPanel;             // bytes of a tile
@@ -51,11 +55,11 @@ struct FwdBars {
     uint64_t q, k_full[4], v_full[4], empty[4], ok[4], s_full[2], s_free[2], p_full[2], pv[2], o_full[2], drain;
 };
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool REST>
 __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
     const __grid_constant__ CUtensorMap mv, const Params p, const int pair, const Bounded bnd) {
-    using S = FwdShape<DP>;
+    using S = FwdShape<DP, REST>;
     constexpr int NS = S::stages;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char smem_raw[];
@@ -246,15 +250,17 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             float2 sums[4] = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                uint32_t w[16];
+                uint32_t w[16], rest[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float2 x = __ffma2_rn(s[16 * c + i], mul2, ref2);
                     const float2 e = make_float2(tc::ex2(x.x), tc::ex2(x.y));
                     sums[i & 3] = __fadd2_rn(sums[i & 3], e);
                     w[i] = tc::pack2<T>(e.x, e.y);
+                    if (REST) rest[i] = tc::rest2<T>(e, w[i]);
                 }
                 tc::store16(tp + 16 * c, w);
+                if (REST) tc::store16(tp + 64 + 16 * c, rest);
             }
             const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
             l += sum.x + sum.y;
@@ -345,6 +351,9 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 if (!lead) return;
                 mix_mma<8, 64>(tmem + S::o_col + x * DP, tmem + S::p_col + x * S::p_step,
                                smem_u32(V_at(s)), ipv, pn[x] > 0);
+                if (REST)
+                    mix_mma<8, 64>(tmem + S::o_col + x * DP, tmem + S::p_col + x * S::p_step + 64,
+                                   smem_u32(V_at(s)), ipv, true);
                 tc::commit(smem_u32(&bars.pv[x]));
                 if (last) tc::commit(smem_u32(&bars.o_full[x]));
             };
@@ -422,12 +431,12 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     }
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool REST = false>
 nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-    auto kern = tc_fwd_kernel<T, DP, CAP, BIAS>;
+    auto kern = tc_fwd_kernel<T, DP, CAP, BIAS, REST>;
     const int pair = p.G % 2 == 0;
-    const int smem = FwdShape<DP>::smem + 1024 +
+    const int smem = FwdShape<DP, REST>::smem + 1024 +
                      (BIAS ? (pair ? 2 : 1) * 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0);
     nsc_status ready = tc_ready(reinterpret_cast<const void*>(kern), smem, kFwdThreads,
                                 256 * 208 + 128 * 80);
@@ -453,6 +462,9 @@ nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
 
 template <typename T, int DP>
 nsc_status tc_fwd_run(const Params& p, cudaStream_t st) {
+    if (p.table && p.residue)
+        return p.cap > 0 ? tc_fwd_launch<T, DP, true, true, true>(p, st)
+                         : tc_fwd_launch<T, DP, false, true, true>(p, st);
     if (p.cap > 0)
         return p.table ? tc_fwd_launch<T, DP, true, true>(p, st)
                        : tc_fwd_launch<T, DP, true, false>(p, st);
