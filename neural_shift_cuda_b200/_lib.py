@@ -212,10 +212,12 @@ def call(name: str, *args) -> None:
 
 def workspace(name: str, device, *args) -> Optional[torch.Tensor]:
     """A buffer of the size that workspace query `name` gives (None for 0)."""
-    lib = load()
-    n = int(getattr(lib, name)(*args))
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    n = fn(*args)
     if n < 0:
-        raise RuntimeError(f"{lib.nsc_last_error_string().decode()} "
+        raise RuntimeError(f"{load().nsc_last_error_string().decode()} "
                            f"[{_STATUS[1]}]")
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
@@ -227,19 +229,26 @@ def dtype_code(dt: torch.dtype) -> int:
         raise TypeError(f"unsupported dtype {dt}") from None
 
 
+_fns: dict = {}   # bound entry points by name
+
+
 def launch(device, name: str, *args) -> None:
-    """`call` on the tensors' device, with its current stream as last argument."""
+    """`call` on the tensors' device, with its current stream as last argument.
+
+    For the operators whose kernels take a few microseconds: what `call` and a
+    device context would cost around each launch shows in theirs."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
     i = device.index
-    if i == torch.cuda.current_device():
-        call(name, *args, _raw_stream(i))
-        return
-    with torch.cuda.device(i):
-        call(name, *args, _raw_stream(i))
-
-
-def _raw_stream(index: int) -> int:
-    """The current stream's handle, without the object around it."""
-    return torch._C._cuda_getCurrentRawStream(index)
+    if i == torch._C._cuda_getDevice():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if st != 0:
+        msg = load().nsc_last_error_string().decode()
+        raise RuntimeError(f"{msg} [{_STATUS.get(st, st)}]")
 
 
 def ptr(t: Optional[torch.Tensor]):

@@ -87,7 +87,7 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t acc_size(int dtype) { return dtype == NSC_F64 ? 8 : 4; }
 
 int query_parts(const nsc_attention* a) {
-    const int tl = general_tile(a->dtype, static_cast<int>(a->D));
+    const int tl = general_tile(a->dtype, a->B, a->Hkv, a->Lq, a->Lk, a->D);
     return static_cast<int>(a->B * ((a->Lq + tl - 1) / tl));
 }
 

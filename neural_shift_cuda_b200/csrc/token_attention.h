@@ -125,7 +125,7 @@ __device__ __forceinline__ void row_stats(const Params& p, int64_t row, A m, A l
 // Kernels for any type, strides and head width (token_attention_general.cu).
 nsc_status general_fwd(const Params& p, int dtype, cudaStream_t st);
 nsc_status general_bwd(const Params& p, const Grads& g, int dtype, cudaStream_t st);
-int general_tile(int dtype, int D);
+int general_tile(int dtype, int64_t B, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t D);
 
 // Tensor-core kernels for fp16 / bf16 (token_attention_tc_*.cu); tc_fits: whether a
 // call's layout is one that their TMA boxes describe.

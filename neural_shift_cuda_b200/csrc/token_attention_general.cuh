@@ -161,13 +161,17 @@ size_t gen_smem(int tiles, int weights, int reach_entries) {
                         static_cast<size_t>(weights) * TL * G::LP + reach_entries);
 }
 
-// f<T, A, DP, TL>() for a dtype and a head width.
+// f<T, A, DP, TL>() for a dtype, a head width and a tile of 64 or 32 (general_tile).
 #define NSC_GEN_WIDTHS(F, T, A)                                       \
-    (p.D <= 32 ? F<T, A, 32, 64>(NSC_GEN_ARGS)                        \
+    (p.D > 128 ? F<T, A, 256, 32>(NSC_GEN_ARGS)                       \
+     : tile == 32 ? (p.D <= 32 ? F<T, A, 32, 32>(NSC_GEN_ARGS)        \
+                     : p.D <= 64 ? F<T, A, 64, 32>(NSC_GEN_ARGS)      \
+                                 : F<T, A, 128, 32>(NSC_GEN_ARGS))    \
+     : p.D <= 32 ? F<T, A, 32, 64>(NSC_GEN_ARGS)                      \
      : p.D <= 64 ? F<T, A, 64, 64>(NSC_GEN_ARGS)                      \
-     : p.D <= 128 ? F<T, A, 128, 64>(NSC_GEN_ARGS)                    \
-                  : F<T, A, 256, 32>(NSC_GEN_ARGS))
+                 : F<T, A, 128, 64>(NSC_GEN_ARGS))
 #define NSC_GEN_DISPATCH(F)                                           \
+    const int tile = general_tile(dtype, p.B, p.Hkv, p.Lq, p.Lk, p.D); \
     switch (dtype) {                                                  \
         case NSC_F16: return NSC_GEN_WIDTHS(F, __half, float);        \
         case NSC_BF16: return NSC_GEN_WIDTHS(F, __nv_bfloat16, float);\

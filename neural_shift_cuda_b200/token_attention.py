@@ -45,7 +45,7 @@ def _require_cuda(op: str, q: torch.Tensor) -> None:
 
 
 def _check_heads(op: str, name: str, t: torch.Tensor) -> None:
-    if t.dim() != 4:
+    if t.ndim != 4:
         raise RuntimeError(f"{op}: {name} must be (B, L, H, D); got "
                            f"{tuple(t.shape)}")
 
@@ -75,16 +75,28 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _table(t: torch.Tensor, acc: torch.dtype) -> torch.Tensor:
+    """Cosines or sines as the kernels read them (no gradient)."""
+    if t.dtype == acc and not t.requires_grad and t.is_contiguous():
+        return t
+    return t.detach().to(acc).contiguous()
+
+
 def _tiled(t: torch.Tensor) -> torch.Tensor:
     """t in a layout the tensor-core kernels can load: unit stride in D, and for
     16-bit types a 16-byte aligned start and strides (a copy where it is not;
     the FMA kernels that read any layout would cost far more)."""
-    t = _unit(t)
-    if t.element_size() != 2 or t.shape[3] % 8 or t.shape[3] > 128:
+    n, s = t.shape, t.stride()
+    if s[3] != 1 and n[3] != 1:
+        return t.contiguous()
+    if t.element_size() != 2 or n[3] % 8 or n[3] > 128:
         return t
     if t.data_ptr() % 16 == 0 and all(
-            n == 1 or (s > 0 and s % 8 == 0)
-            for n, s in zip(t.shape[:3], t.stride()[:3])):
+            n[i] == 1 or (s[i] > 0 and s[i] % 8 == 0) for i in (0, 1, 2)):
         return t
     return t.contiguous()
 
@@ -125,8 +137,7 @@ def _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps):
 
 
 def _rotate_fwd(q, k, wq, wk, cos, sin, positions, adjacent, eps):
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
     _lib.launch(q.device, "nsc_qk_norm_rotate_fwd",
                 _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps),
                 qo.data_ptr(), ko.data_ptr())
@@ -146,8 +157,7 @@ class _RotateFn(torch.autograd.Function):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         a = _rotate_args(q, k, wq, wk, cos, sin, positions, ctx.adjacent, ctx.eps)
         gq, gk = gq.contiguous(), gk.contiguous()
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
         ws = None
@@ -207,12 +217,12 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
         raise RuntimeError(f"{op}: cos and sin have {cos.shape[0]} rows for "
                            f"{L} positions")
     acc = _acc(q.dtype)
-    cos, sin = cos.detach().to(acc).contiguous(), sin.detach().to(acc).contiguous()
-    wq = None if q_weight is None else q_weight.contiguous()
-    wk = None if k_weight is None else k_weight.contiguous()
-    args = (_unit(q), _unit(k), wq, wk, cos, sin, positions, int(adjacent), float(eps))
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    args = (_unit(q), _unit(k), _dense(q_weight), _dense(k_weight), _table(cos, acc),
+            _table(sin, acc), positions, int(adjacent), float(eps))
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad
+            or (q_weight is not None and q_weight.requires_grad)
+            or (k_weight is not None and k_weight.requires_grad)):
         return _RotateFn.apply(*args)
     return _rotate_fwd(*args)
 
@@ -271,7 +281,7 @@ def _attention_fwd(q, k, v, documents, prefix, table, buckets, scale, cap, causa
     """(out, lse or None, stats or None, residue or None)"""
     B, Lq, Hq, D = q.shape
     dev = q.device
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=dev)
+    out = q.new_empty((B, Lq, Hq, D))
     lse = stats = residue = None
     if want_lse:
         lse = torch.empty((B, Hq, Lq), dtype=_acc(q.dtype), device=dev)
@@ -311,9 +321,8 @@ class _AttentionFn(torch.autograd.Function):
         grad_out = torch.zeros_like(out) if grad_out is None else _tiled(grad_out)
         if grad_lse is not None:
             grad_lse = grad_lse.contiguous()
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+        dv = v.new_empty(v.shape)
         dt = (torch.empty_like(table) if table is not None and ctx.needs_input_grad[5]
               else None)
         ws = _lib.workspace("nsc_token_attention_bwd_workspace", q.device, a)
@@ -351,7 +360,7 @@ def _check_bias(op, q, table, buckets):
     if buckets.dim() != 1 or buckets.shape[0] % 2 == 0:
         raise RuntimeError(f"{op}: bias_buckets must have 2 reach + 1 entries; got "
                            f"{tuple(buckets.shape)}")
-    return table.contiguous(), buckets
+    return _dense(table), buckets
 
 
 def _numbers(q, scale, softcap):
@@ -440,8 +449,9 @@ def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
     op = "token_attention_decode"
     _check_qkv(op, q, k_cache, v_cache, "k_cache", "v_cache")
     table, buckets = _check_bias(op, q, bias_table, bias_buckets)
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (q, k_cache, v_cache, table)):
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+            or (table is not None and table.requires_grad)):
         raise RuntimeError(f"{op} has no backward; use token_attention, or "
                            f"torch.no_grad()")
     _require_cuda(op, q)
@@ -451,7 +461,7 @@ def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
         raise RuntimeError(f"{op}: lengths must be ({B},); got {tuple(lengths.shape)}")
     scale, cap = _numbers(q, scale, softcap)
     q, k_cache, v_cache = _unit(q), _unit(k_cache), _unit(v_cache)
-    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, T, Hq, D))
     lse = (torch.empty((B, Hq, T), dtype=_acc(q.dtype), device=q.device)
            if return_lse else None)
     a = _attention_args(q, k_cache, v_cache, None, None, lengths, table, buckets,
