@@ -93,6 +93,42 @@ __device__ __forceinline__ A table_at(const Params& p, int b, int h) {
     return static_cast<A>(static_cast<const double*>(p.table)[at]);
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+}
+// The value at this block's shared address `at`, in block `rank` of the cluster.
+template <typename A> __device__ __forceinline__ A cluster_load(uint32_t at, int rank) {
+    uint32_t a;
+    A v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    if constexpr (sizeof(A) == 4)
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    else
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
+    return v;
+}
+// A launch of `blocks` blocks in clusters of `cluster`.
+template <typename K, typename... Args>
+inline nsc_status launch_cluster(const char* op, K kern, int64_t blocks, int threads, size_t smem,
+                                 int cluster, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = static_cast<unsigned>(cluster);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess)
+        return fail(NSC_ERR_LAUNCH_FAILED, "%s: kernel launch failed: %s", op, cudaGetErrorString(e));
+    return ok();
+}
+
 constexpr double kLog2e = 1.4426950408889634;
 constexpr double kLn2 = 0.6931471805599453;
 

@@ -150,8 +150,8 @@ __device__ __forceinline__ void join_spans(int lo, int hi, int* box, int& first,
         atomicMax(box + 1, hi);
     }
     __syncthreads();
-    first = box[0];
     last = box[1];
+    first = last ? box[0] : 0;   // (no row sees anything: 0, 0)
 }
 
 template <typename A, int DP, int TL>

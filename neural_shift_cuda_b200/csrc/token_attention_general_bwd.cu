@@ -9,8 +9,9 @@
 //     dQ = ds K,   dK = ds^T Q,   dV = P^T dO
 // Two kernels, one with a query tile in place (dQ, table) and one with a key
 // tile in place (dK, dV, summed over the query heads that share the key
-// head).  Each recomputes the scores; no sum is split over blocks, so no
-// atomics and one order of every sum.
+// head).  Each recomputes the scores.  Where there are few tiles a cluster of blocks
+// shares one: each takes every `share`-th step, and the sums are joined over the
+// cluster's shared memory in the order of its ranks; no atomics, one order of every sum.
 #include <climits>
 
 #include "token_attention_general.cuh"
@@ -39,13 +40,43 @@ __device__ __forceinline__ Pair<A> pair_grad(A dot, A dp, A bias, A m, A ll, A d
     return r;
 }
 
+__device__ __forceinline__ uint32_t shared_at(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// A thread's sums into a tile of shared memory, and those of every block of the
+// cluster, row by row, out of it: block `rank` takes every `share`-th element.
+template <typename A, int DP, int TL>
+__device__ __forceinline__ void spill_tile(A* tile, const A (&v)[TL / 16][GenTile<DP, TL>::NG]
+                                                             [GenTile<DP, TL>::VEC],
+                                           int tx, int ty) {
+    using G = GenTile<DP, TL>;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+        for (int g = 0; g < G::NG; ++g)
+#pragma unroll
+            for (int e = 0; e < G::VEC; ++e)
+                tile[(ty + 16 * i) * G::LD + (g * 16 + tx) * G::VEC + e] = v[i][g][e];
+}
+template <typename A, int DP, int TL, typename F>
+__device__ __forceinline__ void join_tile(const A* tile, int rank, int share, int D, F put) {
+    using G = GenTile<DP, TL>;
+    for (int i = threadIdx.x * share + rank; i < TL * DP; i += kGenThreads * share) {
+        const int r = i / DP, d = i % DP;
+        if (d >= D) continue;
+        A v = 0;
+        for (int x = 0; x < share; ++x) v += cluster_load<A>(shared_at(tile + r * G::LD + d), x);
+        put(r, d, v);
+    }
+}
+
 template <typename T, typename A, int DP, int TL>
-__global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads gr) {
+__global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads gr, int share) {
     using G = GenTile<DP, TL>;
     constexpr int MI = G::MI;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int box[2];
-    __shared__ A diag[2 * TL];
+    __shared__ A diag[2 * TL], mines[kGenThreads];
     A* Qs = reinterpret_cast<A*>(smem_raw);
     A* Os = Qs + TL * G::LD;
     A* Ks = Os + TL * G::LD;
@@ -55,8 +86,10 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
 
     const int nt = (p.Lq + TL - 1) / TL;
     const int64_t BH = static_cast<int64_t>(p.B) * p.Hq;
-    const int t = nt - 1 - static_cast<int>(blockIdx.x / BH);
-    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hq, h = bh % p.Hq;
+    const int64_t id = blockIdx.x / share;
+    const int rank = static_cast<int>(blockIdx.x % share);
+    const int t = nt - 1 - static_cast<int>(id / BH);
+    const int bh = static_cast<int>(id % BH), b = bh / p.Hq, h = bh % p.Hq;
     const int hk = h / p.G, q0 = t * TL, off = p.Lk - p.Lq;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2];
@@ -96,7 +129,7 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
     A mine = 0;  // bucket threadIdx.x of the table gradient
     const A scale = p.scale, unit = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
     const A y1 = p.cap > 0 ? p.scale / p.cap : 0;
-    for (int k0 = first / TL * TL; k0 < last; k0 += TL) {
+    for (int k0 = (first / TL + rank) * TL; k0 < last; k0 += TL * share) {
         __syncthreads();
         const bool odd = load_tile<T, A, DP, TL>(Ks, k, p.ks[1], k0, first, last, p.D);
         load_tile<T, A, DP, TL>(Vs, v, p.vs[1], k0, first, last, p.D);
@@ -144,19 +177,35 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
         }
         mix_tile<A, DP, TL>(Ps, Ks, tx, ty, strict, dq);
     }
+    if (share > 1) {
+        __syncthreads();
+        spill_tile<A, DP, TL>(Qs, dq, tx, ty);
+        mines[threadIdx.x] = mine;
+        cluster_sync();
+        join_tile<A, DP, TL>(Qs, rank, share, p.D, [&](int r, int d, A v) {
+            if (q0 + r < p.Lq)
+                static_cast<T*>(gr.dq)[((static_cast<int64_t>(b) * p.Lq + q0 + r) * p.Hq + h) * p.D + d] =
+                    store_as<T>(v);
+        });
+        if (rank == 0 && gr.tab)
+            for (int r = 1; r < share; ++r) mine += cluster_load<A>(shared_at(mines + threadIdx.x), r);
+        cluster_sync();   // no block leaves while another reads its memory
+        if (rank) return;
+    } else {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int row = q0 + ty + 16 * i;
-        if (row >= p.Lq) continue;
-        T* dst = static_cast<T*>(gr.dq) +
-                 ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
+        for (int i = 0; i < MI; ++i) {
+            const int row = q0 + ty + 16 * i;
+            if (row >= p.Lq) continue;
+            T* dst = static_cast<T*>(gr.dq) +
+                     ((static_cast<int64_t>(b) * p.Lq + row) * p.Hq + h) * p.D;
 #pragma unroll
-        for (int g = 0; g < G::NG; ++g)
+            for (int g = 0; g < G::NG; ++g)
 #pragma unroll
-            for (int e = 0; e < G::VEC; ++e) {
-                const int d = (g * 16 + tx) * G::VEC + e;
-                if (d < p.D) dst[d] = store_as<T>(dq[i][g][e]);
-            }
+                for (int e = 0; e < G::VEC; ++e) {
+                    const int d = (g * 16 + tx) * G::VEC + e;
+                    if (d < p.D) dst[d] = store_as<T>(dq[i][g][e]);
+                }
+        }
     }
     if (gr.tab && threadIdx.x < p.nb)
         static_cast<A*>(gr.tab)[(static_cast<int64_t>(h) * gr.n_part + b * nt + t) * p.nb +
@@ -164,7 +213,7 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
 }
 
 template <typename T, typename A, int DP, int TL>
-__global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grads gr) {
+__global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grads gr, int share) {
     using G = GenTile<DP, TL>;
     constexpr int MI = G::MI;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -179,8 +228,10 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
     A* bias = Ss + TL * G::LP;
 
     const int64_t BH = static_cast<int64_t>(p.B) * p.Hkv;
-    const int t = static_cast<int>(blockIdx.x / BH);
-    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hkv, hk = bh % p.Hkv;
+    const int64_t id = blockIdx.x / share;
+    const int rank = static_cast<int>(blockIdx.x % share);
+    const int t = static_cast<int>(id / BH);
+    const int bh = static_cast<int>(id % BH), b = bh / p.Hkv, hk = bh % p.Hkv;
     const int k0 = t * TL, off = p.Lk - p.Lq;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
@@ -206,6 +257,7 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
             for (int e = 0; e < G::VEC; ++e) dk[i][g][e] = dv[i][g][e] = 0;
     const A scale = p.scale, unit = (p.cap > 0 ? p.cap : p.scale) * kLog2e;
     const A y1 = p.cap > 0 ? p.scale / p.cap : 0;
+    int step = 0;
     for (int u = 0; u < p.G; ++u) {
         const int h = hk * p.G + u;
         const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2];
@@ -213,7 +265,8 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
         const int64_t row0 = (static_cast<int64_t>(b) * p.Hq + h) * p.Lq;
         __syncthreads();
         if (p.table) load_bias<A>(p, h, bias);
-        for (int q0 = first / TL * TL; q0 < last; q0 += TL) {
+        for (int q0 = first / TL * TL; q0 < last; q0 += TL, ++step) {
+            if (step % share != rank) continue;
             __syncthreads();
             bool odd = load_tile<T, A, DP, TL>(Qs, q, p.qs[1], q0, first, last, p.D);
             odd |= load_tile<T, A, DP, TL>(Os, go, gr.dos[1], q0, first, last, p.D);
@@ -245,6 +298,23 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
             mix_tile<A, DP, TL>(Ps, Os, tx, ty, strict, dv);
             mix_tile<A, DP, TL>(Ss, Qs, tx, ty, strict, dk);
         }
+    }
+    if (share > 1) {
+        __syncthreads();
+        spill_tile<A, DP, TL>(Qs, dk, tx, ty);
+        spill_tile<A, DP, TL>(Os, dv, tx, ty);
+        cluster_sync();
+        auto put = [&](void* out) {
+            return [&, out](int r, int d, A v) {
+                if (k0 + r < p.Lk)
+                    static_cast<T*>(out)[((static_cast<int64_t>(b) * p.Lk + k0 + r) * p.Hkv + hk) * p.D +
+                                         d] = store_as<T>(v);
+            };
+        };
+        join_tile<A, DP, TL>(Qs, rank, share, p.D, put(gr.dk));
+        join_tile<A, DP, TL>(Os, rank, share, p.D, put(gr.dv));
+        cluster_sync();   // no block leaves while another reads its memory
+        return;
     }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -319,8 +389,19 @@ nsc_status launch(const Params& p, const Grads& g, cudaStream_t st) {
     cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smk));
     const int64_t nq = static_cast<int64_t>((p.Lq + TL - 1) / TL) * p.B * p.Hq;
     const int64_t nk = static_cast<int64_t>((p.Lk + TL - 1) / TL) * p.B * p.Hkv;
-    if (nk) kk<<<static_cast<unsigned>(nk), kGenThreads, smk, st>>>(p, g);
-    if (nq) kq<<<static_cast<unsigned>(nq), kGenThreads, smq, st>>>(p, g);
+    // blocks of a tile: up to about four an SM in all, none without a step
+    auto share_of = [](int64_t tiles, int64_t steps) {
+        int n = 1;
+        while (n < 8 && tiles * n * 2 <= 4 * 148 && n * 2 <= steps) n *= 2;
+        return n;
+    };
+    const char* op = "token_attention backward";
+    const int nqt = (p.Lq + TL - 1) / TL, nkt = (p.Lk + TL - 1) / TL;
+    const int sk = share_of(nk, static_cast<int64_t>(p.G) * nqt), sq = share_of(nq, nkt);
+    nsc_status r = NSC_OK;
+    if (nk) r = launch_cluster(op, kk, nk * sk, kGenThreads, smk, sk, st, p, g, sk);
+    if (r == NSC_OK && nq) r = launch_cluster(op, kq, nq * sq, kGenThreads, smq, sq, st, p, g, sq);
+    if (r != NSC_OK) return r;
     return check_launch("token_attention backward");
 }
 

@@ -48,19 +48,6 @@ struct BwdBars {
     uint64_t s_full[2], p_ready[2], ds_ready[2], dp_full, dp_free, used_p, used_ds, done, drain;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                     : "memory");
-}
-// A float at this block's shared address `at`, in block `rank` of the cluster.
-__device__ __forceinline__ float cluster_load(uint32_t at, int rank) {
-    uint32_t a;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
-
 __device__ __forceinline__ float pow2_near(float v) {   // a power of two at or above v, or 1
     if (!(v > 0.f) || !(v < 3e38f)) return 1.f;
     const int e = static_cast<int>((__float_as_uint(v) >> 23) & 0xFF) + 1;
@@ -493,7 +480,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 for (int r = 0; r < split; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[e] += cluster_load(at + e * kRows * 4, r);
+                    for (int e = 0; e < 4; ++e) sum[e] += cluster_load<float>(at + e * kRows * 4, r);
                 T* dst = static_cast<T*>(half ? gr.dk : gr.dv) +
                          ((static_cast<int64_t>(b) * p.Lk + k0 + row) * p.Hkv + hk) * p.D + c;
                 *reinterpret_cast<uint2*>(dst) =
@@ -894,20 +881,9 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, co
         if (p.G % i == 0) split = i;
     const int64_t nk = tiles * split;
     const int64_t nq = static_cast<int64_t>((p.Lq + kRows - 1) / kRows) * p.B * p.Hq;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(nk));
-    cfg.blockDim = dim3(kBwdThreads);
-    cfg.dynamicSmemBytes = smk;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = split;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kk, mq, mo, mk, mv, p, g, recs, norms, n_norm, split, bnd) !=
-        cudaSuccess)
-        return check_launch("token_attention backward");
+    ready = launch_cluster("token_attention backward", kk, nk, kBwdThreads, smk, split, st, mq, mo, mk,
+                           mv, p, g, recs, norms, n_norm, split, bnd);
+    if (ready != NSC_OK) return ready;
     kq<<<static_cast<unsigned>(nq), kBwdThreads, smq, st>>>(mq, mo, mk, mv, p, g, recs, bnd);
     return check_launch("token_attention backward");
 }
