@@ -90,7 +90,7 @@ bool boxable(const int64_t* s, int B, int L, int H) {
 }  // namespace
 
 bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, int B, int L, int H,
-                  int D, bool bf16, const char** err) {
+                  int D, bool bf16, const char** err, int rows) {
     auto fn = encoder();
     if (!fn) {
         *err = "cuTensorMapEncodeTiled is unavailable";
@@ -102,7 +102,7 @@ bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, in
     const cuuint64_t row = 2ull * D;
     const cuuint64_t st[3] = {H > 1 ? 2ull * strides[2] : row, L > 1 ? 2ull * strides[1] : row,
                               B > 1 ? 2ull * strides[0] : row};
-    const cuuint32_t box[4] = {64, 1, kRows, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1}, one[4] = {1, 1, 1, 1};
     const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                           4, const_cast<void*>(base), dims, st, box, one,

@@ -37,9 +37,9 @@ __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, uns
     return false;
 }
 
-// Coordinates of a (B, L, H, D) tensor map: {D, H, L, B}, boxes of 64 x 128 rows.
+// Coordinates of a (B, L, H, D) tensor map: {D, H, L, B}, boxes of 64 channels of `rows` rows.
 bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, int B, int L, int H,
-                  int D, bool bf16, const char** err);
+                  int D, bool bf16, const char** err, int rows = kRows);
 
 // Prepares a kernel's shared memory, and refuses one whose launch would hold fewer
 // registers than its warps ask for when they share them out (they would wait
@@ -56,12 +56,12 @@ nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, const f
 struct RowRec { float m, ll, delta, norm; };
 constexpr int kRecRows = 32;   // rows of a record block, and of one entry of `norms`
 
-// A tile: 128 rows from `row` of head `h`, DP / 64 panels.
-template <int DP>
+// A tile: ROWS rows from `row` of head `h`, DP / 64 panels.
+template <int DP, int ROWS = kRows>
 __device__ __forceinline__ void load_rows(unsigned char* dst, const CUtensorMap* map, uint64_t* bar,
                                           int h, int row, int b) {
 #pragma unroll
-    for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * kPanel, map, bar, 64 * c, h, row, b);
+    for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * ROWS * 128, map, bar, 64 * c, h, row, b);
 }
 
 // Sees to it that rows of a landed tile that hold an infinity or NaN do not
@@ -69,11 +69,11 @@ __device__ __forceinline__ void load_rows(unsigned char* dst, const CUtensorMap*
 // `lanes` threads, thread t has rows t, t + lanes, ...; returns a bit for each of
 // its rows (in that order) that held such a value.  x 0 is 0 or NaN, so one
 // multiply-add per two values finds them.
-template <typename T, int DP>
+template <typename T, int DP, int ROWS = kRows>
 __device__ __forceinline__ uint32_t scrub_rows(unsigned char* tile, int t, int lanes) {
     uint32_t bad = 0;
     int bit = 0;
-    for (int r = t; r < kRows; r += lanes, ++bit) {
+    for (int r = t; r < ROWS; r += lanes, ++bit) {
         using T2 = typename std::conditional<sizeof(T) == 2 && std::is_same<T, __half>::value,
                                              __half2, __nv_bfloat162>::type;
         T2 acc;
@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t scrub_rows(unsigned char* tile, int t, int l
         T2 zero = acc;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-            const uint4* row = reinterpret_cast<const uint4*>(tile + c * kPanel + r * 128);
+            const uint4* row = reinterpret_cast<const uint4*>(tile + c * ROWS * 128 + r * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint4 v = row[(i + r) & 7];
@@ -96,7 +96,7 @@ __device__ __forceinline__ uint32_t scrub_rows(unsigned char* tile, int t, int l
         bad |= 1u << bit;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(tile + c * kPanel + r * 128);
+            uint4* row = reinterpret_cast<uint4*>(tile + c * ROWS * 128 + r * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
         }
@@ -104,11 +104,11 @@ __device__ __forceinline__ uint32_t scrub_rows(unsigned char* tile, int t, int l
     return bad;
 }
 // Fills row r of a tile with NaN.
-template <int DP>
+template <int DP, int ROWS = kRows>
 __device__ __forceinline__ void poison_row(unsigned char* tile, int r) {
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c) {
-        uint4* row = reinterpret_cast<uint4*>(tile + c * kPanel + r * 128);
+        uint4* row = reinterpret_cast<uint4*>(tile + c * ROWS * 128 + r * 128);
 #pragma unroll
         for (int i = 0; i < 8; ++i) row[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
     }
@@ -161,28 +161,28 @@ __device__ __forceinline__ void load_padded_bias(const Params& p, int h, float* 
     }
 }
 
-// The products of two tiles, issued by one lane of a converged warp.  scores_mma: [128 x 128] = A B^T over
-// the channels, both tiles K-major; `steps` of 16 channels.  mix_mma: [128 x channels]
-// += W B with the 128 x 128 weights W in tensor memory, STEPS k-steps side by side and
-// GAP columns from one such run to the next, and the 128 rows of B as the reduced
-// dimension.
-template <int DP>
+// The products of two tiles, issued by one lane of a converged warp.  scores_mma:
+// [128 x N] = A B^T over the channels, A of 128 rows and B of N, both K-major; `steps` of
+// 16 channels.  mix_mma: [128 x channels] += W B with the weights W (128 x 16 K) in tensor
+// memory, RUN k-steps side by side and GAP columns from one such run to the next, and the
+// 16 K rows of B, in panels of `panel` bytes, as the reduced dimension.
+template <int DP, int N = kRows>
 __device__ __forceinline__ void scores_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            int steps) {
     const uint32_t x = tc::operand(a, 16), y = tc::operand(b, 16);
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c)
-        if (c < steps) {
-            const uint32_t o = ((c >> 2) * kPanel + (c & 3) * 32) >> 4;
-            tc::mma_ss(d, x + o, y + o, idesc, c > 0);
-        }
+        if (c < steps)
+            tc::mma_ss(d, x + (((c >> 2) * kPanel + (c & 3) * 32) >> 4),
+                       y + (((c >> 2) * N * 128 + (c & 3) * 32) >> 4), idesc, c > 0);
 }
-template <int STEPS, int GAP>
-__device__ __forceinline__ void mix_mma(uint32_t d, uint32_t w, uint32_t b, uint32_t idesc, bool add) {
-    const uint32_t y = tc::operand(b, kPanel);
+template <int K, int RUN, int GAP>
+__device__ __forceinline__ void mix_mma(uint32_t d, uint32_t w, uint32_t b, uint32_t panel,
+                                        uint32_t idesc, bool add) {
+    const uint32_t y = tc::operand(b, panel);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        tc::mma_ts(d, w + k / STEPS * GAP + k % STEPS * 8, y + ((k * 2048) >> 4), idesc, add || k > 0);
+    for (int k = 0; k < K; ++k)
+        tc::mma_ts(d, w + k / RUN * GAP + k % RUN * 8, y + ((k * 2048) >> 4), idesc, add || k > 0);
 }
 
 }  // namespace tok

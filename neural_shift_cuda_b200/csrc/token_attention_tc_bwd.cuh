@@ -391,7 +391,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     if (!alive) break;
                     tc::fence_after();
                     if (lead) {
-                        mix_mma<2, 32>(t_dv, S_at(it), smem_u32(O_at(s)), its, it > 0);
+                        mix_mma<8, 2, 32>(t_dv, S_at(it), smem_u32(O_at(s)), kPanel, its, it > 0);
                         tc::commit(smem_u32(&bars.used_p));
                     }
                 }
@@ -404,8 +404,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     if (!alive) break;
                     tc::fence_after();
                     if (lead) {
-                        mix_mma<2, 32>(t_dk, t_dp, smem_u32(Q_at(s)), its, it > 0);
-                        mix_mma<2, 32>(t_dk, t_dp + 16, smem_u32(Q_at(s)), its, true);
+                        mix_mma<8, 2, 32>(t_dk, t_dp, smem_u32(Q_at(s)), kPanel, its, it > 0);
+                        mix_mma<8, 2, 32>(t_dk, t_dp + 16, smem_u32(Q_at(s)), kPanel, its, true);
                         tc::commit(smem_u32(&bars.used_ds));
                         tc::commit(smem_u32(&bars.empty[s]));
                     }
@@ -791,8 +791,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                     tc::fence_after();
                     if (lead) {
                         const uint32_t w = t_s + 128 * (it & 1);
-                        mix_mma<2, 32>(t_dq, w, smem_u32(K_at(s)), its, it > 0);
-                        mix_mma<2, 32>(t_dq, w + 16, smem_u32(K_at(s)), its, true);
+                        mix_mma<8, 2, 32>(t_dq, w, smem_u32(K_at(s)), kPanel, its, it > 0);
+                        mix_mma<8, 2, 32>(t_dq, w + 16, smem_u32(K_at(s)), kPanel, its, true);
                     }
                     if (lead) tc::commit(smem_u32(&bars.used_ds));
                     if (lead) tc::commit(smem_u32(&bars.empty[s]));

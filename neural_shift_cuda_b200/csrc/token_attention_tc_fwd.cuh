@@ -4,15 +4,16 @@
 // A block owns two tiles of 128 queries: two heads that share a key head at the
 // same queries (one load of K and V serves both), or 256 queries of one head.
 // Roles by warp: 0-3 and 4-7 the softmax of a tile each, a thread a row; 8 loads K
-// and V blocks of 128 keys through a ring by TMA; 9 issues the products; 10 and
-// 11 guard (below).
+// and V blocks of 64 keys through a ring by TMA; 9 and 10 issue the products of a tile
+// each (one warp for both was late for either: its waits and issue took as long as a
+// block's softmax); 11 guards (below).
 //
-// Tensor memory holds S and O of both tiles.  At D <= 64 there is room for P, as
-// 16-bit pairs, beside S: QK(j+1) starts as soon as S(j) is in registers and runs
-// beside the softmax of block j.  At D = 128 P takes the place of its S, so QK(j+1)
-// waits until PV(j) is done, and one tile's products run beside the other's softmax.
-// (Products of different shapes or accumulators need not complete in the order
-// of their issue; whatever overwrites an operand waits for its reader's commit.)
+// Tensor memory holds O of both tiles and two S of each: blocks are of 64 keys, so that
+// S(j+1) is computed beside the softmax of block j.  P takes the place of its S as 16-bit
+// pairs.  (Products of different shapes or accumulators need not complete in the order
+// of their issue: whatever overwrites an operand waits for its reader's commit.)  With
+// blocks of 128 keys and one S, a tile's warps waited a third of the time for their
+// scores: 212 against NEW us for 32 heads of 128, 4096 causal tokens, capped.
 //
 // Softmax with a running reference m: p = 2^(s2 - m); m moves, and O is
 // rescaled, only when a row's maximum passes m + 8 (p <= 256 keeps 16-bit
@@ -24,8 +25,8 @@
 // (bf16, 8192 rows: 1.7e-3 of it off, its own rounding, where 3.1e-3 were).
 //
 // Guard: in blocks that some row of a tile does not see whole, a value row
-// that is not finite would reach every row as 0 x NaN.  There the guard warps
-// look each landed V block over; such a row becomes zero in V and NaN in K,
+// that is not finite would reach every row as 0 x NaN.  There the guard warp
+// looks each landed V block over; such a row becomes zero in V and NaN in K,
 // so that the rows that see it still give NaN, by their scores.
 //
 // Work per score: one exponential (16 a clock and SM) against D / 32
@@ -42,24 +43,27 @@ namespace {
 constexpr int kFwdThreads = 384;
 constexpr float kLazy = 8.f;
 
-template <int DP, bool REST> struct FwdShape {
-    static constexpr bool apart = DP == 64 && !REST;          // P beside S
-    static constexpr int p_col = apart ? 256 : 0, p_step = apart ? 64 : 128;
-    static constexpr int o_col = apart ? 384 : 256;
-    static constexpr int tile = DP / 64 * kPanel;             // bytes of a tile
-    static constexpr int stages = DP == 64 ? 4 : 2;           // K and V blocks in flight
-    static constexpr int smem = 2 * tile + stages * 2 * tile; // + bias + 1024 of alignment
+constexpr int kKeys = 64;   // keys of a block
+
+template <int DP> struct FwdShape {
+    static constexpr int tile = DP / 64 * kPanel;                  // bytes of a query tile
+    static constexpr int panel = kKeys * 128, block = DP / 64 * panel;   // of a K or V block
+    static constexpr int stages = DP == 64 ? 6 : 4;                // K and V blocks in flight
+    static constexpr int smem = 2 * tile + stages * 2 * block;     // + bias + 1024 of alignment
 };
 
 struct FwdBars {
-    uint64_t q, k_full[4], v_full[4], empty[4], ok[4], s_full[2], s_free[2], p_full[2], pv[2], o_full[2], drain;
+    // (two of s_full and p_full of a tile, for even and odd blocks: the products, and a
+    // fast warp, may be a block ahead of a slow warp)
+    uint64_t q, k_full[6], v_full[6], empty[6], ok[6], s_full[2][2], p_full[2][2], pv[2], o_full[2];
+    uint64_t drain[2];
 };
 
 template <typename T, int DP, bool CAP, bool BIAS, bool REST>
 __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
     const __grid_constant__ CUtensorMap mv, const Params p, const int pair, const Bounded bnd) {
-    using S = FwdShape<DP, REST>;
+    using S = FwdShape<DP>;
     constexpr int NS = S::stages;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char smem_raw[];
@@ -90,17 +94,19 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         for (int i = 0; i < NS; ++i) {
             mbar_init(&bars.k_full[i], 1);
             mbar_init(&bars.v_full[i], 1);
-            mbar_init(&bars.empty[i], 1);
-            mbar_init(&bars.ok[i], 64);
+            mbar_init(&bars.empty[i], 2);
+            mbar_init(&bars.ok[i], 32);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.s_free[i], kRows);
-            mbar_init(&bars.p_full[i], kRows);
+            for (int y = 0; y < 2; ++y) {
+                mbar_init(&bars.s_full[i][y], 1);
+                mbar_init(&bars.p_full[i][y], kRows);
+            }
             mbar_init(&bars.pv[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
-        mbar_init(&bars.drain, 1);
+        mbar_init(&bars.drain[0], 1);
+        mbar_init(&bars.drain[1], 1);
         fence_mbar_init();
         abort_flag[0] = 0;
         abort_flag[1] = static_cast<int>(bnd.budget);
@@ -139,8 +145,8 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         const int s0 = tc::uniform(span[i][0]), s1 = tc::uniform(span[i][1]);
         all_lo[i] = tc::uniform(span[i][2]);
         all_hi[i] = tc::uniform(span[i][3]);
-        fb[i] = s1 > s0 ? s0 / kRows : INT_MAX;
-        lb[i] = s1 > s0 ? (s1 + kRows - 1) / kRows : 0;
+        fb[i] = s1 > s0 ? s0 / kKeys : INT_MAX;
+        lb[i] = s1 > s0 ? (s1 + kKeys - 1) / kKeys : 0;
     }
     const int j0 = min(fb[0], fb[1]), j1 = max(lb[0], lb[1]);
     auto on = [&](int i, int j) { return j >= fb[i] && j < lb[i]; };
@@ -148,22 +154,21 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         bool g = false;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            g |= on(i, j) && !(j * kRows >= all_lo[i] && min((j + 1) * kRows, n) <= all_hi[i]);
+            g |= on(i, j) && !(j * kKeys >= all_lo[i] && min((j + 1) * kKeys, n) <= all_hi[i]);
         return g;
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
     };
-    auto K_at = [&](int s) { return KV + s * 2 * S::tile; };
-    auto V_at = [&](int s) { return KV + s * 2 * S::tile + S::tile; };
+    auto K_at = [&](int s) { return KV + s * 2 * S::block; };
+    auto V_at = [&](int s) { return KV + s * 2 * S::block + S::block; };
     const int steps = (p.D + 15) / 16;   // of 16 channels
     const int cols = steps * 16;
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + a * 128 + lane_base, to = tmem + S::o_col + a * DP + lane_base;
-        const uint32_t tp = tmem + S::p_col + a * S::p_step + lane_base;
+        const uint32_t to = tmem + 256 + a * DP + lane_base;
         const int h = h0 + (pair ? a : 0);
         const int pos = row + n - p.Lq;
         const float* Eh = E + (pair && a ? 2 * p.reach + 2 * kBiasPad + 1 : 0);
@@ -173,44 +178,41 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         bool alive = true;
         int it = 0;
         for (int j = fb[a]; j < lb[a]; ++j, ++it) {
-            alive = __all_sync(0xffffffffu, wait(&bars.s_full[a], it & 1));
+            alive = __all_sync(0xffffffffu, wait(&bars.s_full[a][it & 1], (it >> 1) & 1));
             if (!alive) break;
             tc::fence_after();
-            float2 s[64];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc::load32(ts + 32 * c, reinterpret_cast<float*>(s + 16 * c));
+            const uint32_t ts = tmem + lane_base + a * 128 + (it & 1) * kKeys;
+            float2 s[32];
+            tc::load32(ts, reinterpret_cast<float*>(s));
+            tc::load32(ts + 32, reinterpret_cast<float*>(s + 16));
             tc::wait_ld();
-            if (S::apart) {
-                tc::fence_before();
-                mbar_arrive(&bars.s_free[a]);
-            }
-            const int k0 = j * kRows;
+            const int k0 = j * kKeys;
             if (CAP) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tanh32(s + 16 * c, y1);
+                tanh32(s, y1);
+                tanh32(s + 16, y1);
             }
             float mul = unit;
             if (BIAS) {
                 mul = 1.f;
                 const int w0 = __shfl_sync(0xffffffffu, pos, 0);   // lanes at w0 .. w0 + 31
                 const float2 u2 = make_float2(unit, unit);
-                if (k0 + 127 - w0 <= -p.reach || k0 - w0 - 31 >= p.reach) {
+                if (k0 + kKeys - 1 - w0 <= -p.reach || k0 - w0 - 31 >= p.reach) {
                     const float e = Eh[k0 > w0 ? 2 * p.reach + kBiasPad : kBiasPad];
                     const float2 e2 = make_float2(e, e);
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) s[i] = __ffma2_rn(s[i], u2, e2);
+                    for (int i = 0; i < 32; ++i) s[i] = __ffma2_rn(s[i], u2, e2);
                 } else {
                     const float* er = Eh + (k0 - pos + p.reach + kBiasPad);
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
+                    for (int i = 0; i < 32; ++i)
                         s[i] = __ffma2_rn(s[i], u2, make_float2(er[2 * i], er[2 * i + 1]));
                 }
             }
-            if (!__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + kRows)) {
+            if (!__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + kKeys)) {
                 const uint32_t from = static_cast<uint32_t>(lo - k0);
                 const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
+                for (int i = 0; i < 32; ++i) {
                     if (2 * i - from >= len) s[i].x = -INFINITY;
                     if (2 * i + 1 - from >= len) s[i].y = -INFINITY;
                 }
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             // out the latency of each of its 64 steps)
             float tops[4] = {s[0].x, s[1].x, s[2].x, s[3].x};
 #pragma unroll
-            for (int i = 0; i < 64; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
+            for (int i = 0; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
             // (a row may see nothing of its first blocks: m is then -inf still)
             float keep = 1.f;
@@ -227,12 +229,11 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 keep = m == -INFINITY ? 0.f : tc::ex2(m - top);
                 m = fmaxf(top, m);
             }
-            if (S::apart && it > 0) {   // PV of the last block: P and O are free
+            if (it > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+                // (PV of the last block is done, and this one's has not begun)
                 alive = __all_sync(0xffffffffu, wait(&bars.pv[a], (it - 1) & 1));
                 if (!alive) break;
                 tc::fence_after();
-            }
-            if (it > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
                 l *= keep;
                 const float2 k2 = make_float2(keep, keep);
 #pragma unroll 1
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(ref, ref);
             float2 sums[4] = {};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 uint32_t w[16], rest[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -259,14 +260,14 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     w[i] = tc::pack2<T>(e.x, e.y);
                     if (REST) rest[i] = tc::rest2<T>(e, w[i]);
                 }
-                tc::store16(tp + 16 * c, w);
-                if (REST) tc::store16(tp + 64 + 16 * c, rest);
+                tc::store16(ts + 16 * c, w);
+                if (REST) tc::store16(ts + 32 + 16 * c, rest);
             }
             const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
             l += sum.x + sum.y;
             tc::wait_st();
             tc::fence_before();
-            mbar_arrive(&bars.p_full[a]);
+            mbar_arrive(&bars.p_full[a][it & 1]);
         }
         // the row's output
         const bool worked = lb[a] > fb[a];
@@ -321,11 +322,11 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 const int s = issued % NS;
                 if (issued >= NS) alive = wait(&bars.empty[s], (issued / NS - 1) & 1);
                 if (!alive) break;
-                mbar_arrive_expect_tx(&bars.k_full[s], S::tile);
+                mbar_arrive_expect_tx(&bars.k_full[s], S::block);
                 if (copies++ == bnd.skip) { ++issued; break; }
-                load_rows<DP>(K_at(s), &mk, &bars.k_full[s], hk, j * kRows, b);
-                mbar_arrive_expect_tx(&bars.v_full[s], S::tile);
-                load_rows<DP>(V_at(s), &mv, &bars.v_full[s], hk, j * kRows, b);
+                load_rows<DP, kKeys>(K_at(s), &mk, &bars.k_full[s], hk, j * kKeys, b);
+                mbar_arrive_expect_tx(&bars.v_full[s], S::block);
+                load_rows<DP, kKeys>(V_at(s), &mv, &bars.v_full[s], hk, j * kKeys, b);
             }
             // every copy has landed before the block may end
             mbar_wait32(smem_u32(&bars.q), 0, bnd.timeouts);
@@ -334,72 +335,54 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     mbar_wait32(smem_u32(&bars.k_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                     mbar_wait32(smem_u32(&bars.v_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                 }
-        } else if (warp == 9 && j0 < j1) {
-            const uint32_t iqk = tc::product(kBf16, 128, 128, false, false);
+        } else if ((warp == 9 || warp == 10) && j0 < j1) {
+            const int x = warp - 9;
+            const uint32_t iqk = tc::product(kBf16, 128, kKeys, false, false);
             const uint32_t ipv = tc::product(kBf16, 128, cols, false, true);
+            const uint32_t t_s = tmem + x * 128, t_o = tmem + 256 + x * DP;
+            const uint32_t q = smem_u32(Qs + x * S::tile);
+            const int f = tc::uniform(x ? fb[1] : fb[0]), e = tc::uniform(x ? lb[1] : lb[0]);
             const bool lead = tc::elect();
-            auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-            bool alive = all(wait(&bars.q, 0));
-            int pn[2] = {0, 0};   // blocks of a tile multiplied with V
-            auto scores = [&](int x, int sn) {
-                if (!lead) return;
-                scores_mma<DP>(tmem + x * 128, smem_u32(Qs + x * S::tile), smem_u32(K_at(sn)), iqk,
-                               steps);
-                tc::commit(smem_u32(&bars.s_full[x]));
-            };
-            auto mix = [&](int x, int s, bool last) {
-                if (!lead) return;
-                mix_mma<8, 64>(tmem + S::o_col + x * DP, tmem + S::p_col + x * S::p_step,
-                               smem_u32(V_at(s)), ipv, pn[x] > 0);
-                if (REST)
-                    mix_mma<8, 64>(tmem + S::o_col + x * DP, tmem + S::p_col + x * S::p_step + 64,
-                                   smem_u32(V_at(s)), ipv, true);
-                tc::commit(smem_u32(&bars.pv[x]));
-                if (last) tc::commit(smem_u32(&bars.o_full[x]));
-            };
-            for (int j = j0 - 1; alive && j < j1; ++j) {
-                const int i = j - j0, s = (i + NS) % NS, sn = (i + 1) % NS;
-                const uint32_t parity = ((i + 1) / NS) & 1;
-                if (j + 1 < j1) {
-                    alive = all(wait(&bars.k_full[sn], parity) && wait(&bars.ok[sn], parity));
-                    if (!alive) break;
+            bool fine = wait(&bars.q, 0);
+            int st = 0, phase = 0, last = 0;   // ring stage of block j + 1 and its phase; of block j
+            for (int j = j0 - 1; j < j1; ++j) {
+                const int n = j + 1 - f, c = j - f;   // blocks of this tile so far
+                if (j + 1 < j1) fine &= wait(&bars.ok[st], phase);
+                if (j + 1 >= f && j + 1 < e) {
+                    // S(n) in the place of S and P of the block before last, once PV has read that
+                    if (n > 1) fine &= wait(&bars.pv[x], n & 1);
+                    tc::fence_after();
+                    if (lead) {
+                        scores_mma<DP, kKeys>(t_s + (n & 1) * kKeys, q, smem_u32(K_at(st)), iqk, steps);
+                        tc::commit(smem_u32(&bars.s_full[x][n & 1]));
+                    }
                 }
-                if (S::apart) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        if (on(x, j + 1)) {
-                            if (on(x, j)) alive = alive && all(wait(&bars.s_free[x], pn[x] & 1));
-                            if (!alive) break;
-                            tc::fence_after();
-                            scores(x, sn);
+                if (j >= j0) {
+                    if (j >= f && j < e) {
+                        fine &= wait(&bars.p_full[x][c & 1], (c >> 1) & 1);
+                        tc::fence_after();
+                        if (lead) {
+                            const uint32_t w = t_s + (c & 1) * kKeys, v = smem_u32(V_at(last));
+                            mix_mma<4, 4, 0>(t_o, w, v, S::panel, ipv, c > 0);
+                            if (REST) mix_mma<4, 4, 0>(t_o, w + 32, v, S::panel, ipv, true);
+                            tc::commit(smem_u32(&bars.pv[x]));
+                            if (j + 1 == e) tc::commit(smem_u32(&bars.o_full[x]));
                         }
-                    if (!alive) break;
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (j >= j0 && on(x, j)) {
-                        alive = all(wait(&bars.v_full[s], (i / NS) & 1) &&
-                                    wait(&bars.p_full[x], pn[x] & 1));
-                        if (!alive) break;
-                        tc::fence_after();
-                        mix(x, s, j + 1 == lb[x]);
-                        ++pn[x];
                     }
-                    if (!S::apart && on(x, j + 1)) {
-                        if (pn[x] > 0) alive = all(wait(&bars.pv[x], (pn[x] - 1) & 1));
-                        if (!alive) break;
-                        tc::fence_after();
-                        scores(x, sn);
-                    }
+                    if (lead) tc::commit(smem_u32(&bars.empty[last]));
                 }
-                if (alive && j >= j0 && lead) tc::commit(smem_u32(&bars.empty[s]));
+                last = st;
+                if (++st == NS) {
+                    st = 0;
+                    phase ^= 1;
+                }
+                if (!__all_sync(0xffffffffu, fine)) break;
             }
-            if (!alive) {   // the products in flight read this block's memory
-                if (lead) tc::commit(smem_u32(&bars.drain));
-                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
+            if (!__all_sync(0xffffffffu, fine)) {   // the products in flight read this block's memory
+                if (lead) tc::commit(smem_u32(&bars.drain[x]));
+                mbar_wait32(smem_u32(&bars.drain[x]), 0, bnd.timeouts);
             }
-        } else if (warp >= 10 && j0 < j1) {
-            const int g = threadIdx.x - 320;
+        } else if (warp == 11 && j0 < j1) {
             // in step with the ring: every block is passed on, after the one before it in
             // the stage was used up, so no phase of a barrier is taken for another
             int i = 0;
@@ -407,18 +390,14 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 const int s = i % NS;
                 const uint32_t parity = (i / NS) & 1;
                 if (i >= NS && !wait(&bars.empty[s], parity ^ 1)) break;
-                if (!guarded(j)) {
-                    mbar_arrive(&bars.ok[s]);
-                    continue;
-                }
                 if (!wait(&bars.k_full[s], parity) || !wait(&bars.v_full[s], parity)) break;
-                const uint32_t bad = scrub_rows<T, DP>(V_at(s), g, 64);
-                if (bad) {
+                if (guarded(j)) {
+                    const uint32_t bad = scrub_rows<T, DP, kKeys>(V_at(s), lane, 32);
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        if (bad >> r & 1) poison_row<DP>(K_at(s), g + 64 * r);
+                        if (bad >> r & 1) poison_row<DP, kKeys>(K_at(s), lane + 32 * r);
+                    fence_async_shared();
                 }
-                fence_async_shared();
                 mbar_arrive(&bars.ok[s]);
             }
         }
@@ -436,7 +415,7 @@ nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     auto kern = tc_fwd_kernel<T, DP, CAP, BIAS, REST>;
     const int pair = p.G % 2 == 0;
-    const int smem = FwdShape<DP, REST>::smem + 1024 +
+    const int smem = FwdShape<DP>::smem + 1024 +
                      (BIAS ? (pair ? 2 : 1) * 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0);
     nsc_status ready = tc_ready(reinterpret_cast<const void*>(kern), smem, kFwdThreads,
                                 256 * 208 + 128 * 80);
@@ -444,8 +423,8 @@ nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     CUtensorMap mq, mk, mv;
     const char* err = nullptr;
     if (!encode_heads(&mq, p.q, p.qs, p.B, p.Lq, p.Hq, p.D, kBf16, &err) ||
-        !encode_heads(&mk, p.k, p.ks, p.B, p.Lk, p.Hkv, p.D, kBf16, &err) ||
-        !encode_heads(&mv, p.v, p.vs, p.B, p.Lk, p.Hkv, p.D, kBf16, &err))
+        !encode_heads(&mk, p.k, p.ks, p.B, p.Lk, p.Hkv, p.D, kBf16, &err, kKeys) ||
+        !encode_heads(&mv, p.v, p.vs, p.B, p.Lk, p.Hkv, p.D, kBf16, &err, kKeys))
         return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: %s", err);
     Bounded bnd{wait_timeout_counter(), -1, 0};
     if (!bnd.timeouts)
