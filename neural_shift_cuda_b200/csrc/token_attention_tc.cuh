@@ -117,40 +117,51 @@ __device__ __forceinline__ void fence_async_shared() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// tanh of the 32 products of a chunk times y1, in place.  Up to |y| = 1 an odd
-// polynomial: y P(y^2), P of least maximum error of y P(y^2) against tanh y by
-// exchange (2.4e-7), on pairs in the packed FMA pipe and off the exponential unit
-// that bounds these kernels.  A warp with a larger value in the chunk takes
-// tanh |y| = 1 - 2 / (1 + e^(2|y|)) for all of it.
-__device__ __forceinline__ void tanh32(float2* s, float y1) {
-    const float2 k = make_float2(y1, y1);
-    float top[4] = {0.f, 0.f, 0.f, 0.f};
+// The cap, f tanh(y1 s) of 32 products s, in place.  Up to |y| = 1, tanh y is an odd
+// polynomial y P(y^2), P of least maximum error of y P(y^2) against tanh y by
+// exchange: 2.4e-7 with six terms (fp16), 2.8e-6 with five (bf16: at a cap of 50,
+// 1.4e-4 of a softmax weight that is rounded to 4e-3).  It runs on the FMA pipe,
+// beside the exponentials that bound these kernels, in pairs, with y1 and f in the
+// coefficients; the hardware's tanh would be one more exponential's time, with 5e-4 of
+// error.  A warp with a larger |y| in the chunk takes tanh |y| = 1 - 2 / (1 + e^(2|y|)).
+template <typename T> struct Cap {
+    static constexpr int N = std::is_same<T, __half>::value ? 6 : 5;
+    float c[N], y1, f, limit;   // |s| up to `limit`
+    __device__ __forceinline__ Cap(float y1_, float f_) : y1(y1_), f(f_) {
+        constexpr float k6[6] = {0.9999968539f, -0.3332400381f, 0.1325352535f,
+                                 -0.05097286522f, 0.01611418278f, -0.002839466166f};
+        constexpr float k5[6] = {0.9999684695f, -0.3326582321f, 0.1292206686f,
+                                 -0.04329986371f, 0.008365886550f, 0.f};
+        float y = y1 * f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        s[i] = __fmul2_rn(s[i], k);
-        top[i & 3] = fmaxf(top[i & 3], fmaxf(fabsf(s[i].x), fabsf(s[i].y)));
+        for (int i = 0; i < N; ++i, y *= y1 * y1) c[i] = (N == 6 ? k6[i] : k5[i]) * y;
+        limit = y1 != 0.f ? 1.f / fabsf(y1) : INFINITY;
     }
-    if (!__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 1.f)) {
+    __device__ __forceinline__ void operator()(float2* s) const {
+        float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float2 u = __fmul2_rn(s[i], s[i]);
-            float2 p = make_float2(-0.002839466166f, -0.002839466166f);
-            p = __ffma2_rn(p, u, make_float2(0.01611418278f, 0.01611418278f));
-            p = __ffma2_rn(p, u, make_float2(-0.05097286522f, -0.05097286522f));
-            p = __ffma2_rn(p, u, make_float2(0.1325352535f, 0.1325352535f));
-            p = __ffma2_rn(p, u, make_float2(-0.3332400381f, -0.3332400381f));
-            p = __ffma2_rn(p, u, make_float2(0.9999968539f, 0.9999968539f));
-            s[i] = __fmul2_rn(s[i], p);
+        for (int i = 0; i < 16; ++i)
+            top[i & 3] = fmaxf(top[i & 3], fmaxf(fabsf(s[i].x), fabsf(s[i].y)));
+        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > limit)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 u = __fmul2_rn(s[i], s[i]);
+                float2 p = make_float2(c[N - 1], c[N - 1]);
+#pragma unroll
+                for (int k = N - 2; k >= 0; --k) p = __ffma2_rn(p, u, make_float2(c[k], c[k]));
+                s[i] = __fmul2_rn(s[i], p);
+            }
+            return;
         }
-        return;
-    }
-    float* f = reinterpret_cast<float*>(s);
+        float* v = reinterpret_cast<float*>(s);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const float e = tc::ex2(fabsf(f[i]) * static_cast<float>(2 * kLog2e));
-        f[i] = copysignf(1.f - __fdividef(2.f, 1.f + e), f[i]);
+        for (int i = 0; i < 32; ++i) {
+            const float y = v[i] * y1;
+            const float e = tc::ex2(fabsf(y) * static_cast<float>(2 * kLog2e));
+            v[i] = copysignf(f - __fdividef(2.f * f, 1.f + e), y);
+        }
     }
-}
+};
 
 // Bias of head h by clamped distance, with kBiasPad more of the end values at
 // each end: E[distance + reach + kBiasPad].

@@ -170,7 +170,10 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         const uint32_t at_s0 = t_s + lane_base + 32 * part, at_dp = t_dp + lane_base + 32 * part;
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
-        const float2 u2 = make_float2(unit, unit), g2 = make_float2(1.f / g, 1.f / g);
+        const Cap<T> cap(y1, unit);
+        const float2 u2 = CAP ? make_float2(1.f, 1.f) : make_float2(unit, unit);
+        const float2 g2 = make_float2(1.f / g, 1.f / g);
+        const float2 slope2 = make_float2(-1.f / (unit * unit), -1.f / (unit * unit));   // 1 - tanh^2 = 1 + s^2 slope
         bool alive = true;
         int it = 0;
         for (int u = 0; u < heads && nq > 0; ++u) {
@@ -190,7 +193,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                 float2 s[16];
                 tc::load32(at_s, reinterpret_cast<float*>(s));
                 tc::wait_ld();
-                if (CAP) tanh32(s, y1);
+                if (CAP) cap(s);
                 const int q0 = j * kRows + 32 * part;
                 const float4* m4 = reinterpret_cast<const float4*>(rows[st][0] + 32 * part);
                 const float4* l4 = reinterpret_cast<const float4*>(rows[st][1] + 32 * part);
@@ -237,9 +240,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     w[2 * i] = tc::pack2<T>(p0.x, p0.y);
                     w[2 * i + 1] = tc::pack2<T>(p1.x, p1.y);
                     if (CAP) {   // keep p (1 - tanh^2)
-                        const float2 n0 = __fmul2_rn(s[2 * i], make_float2(-s[2 * i].x, -s[2 * i].y));
-                        const float2 n1 = __fmul2_rn(s[2 * i + 1],
-                                                     make_float2(-s[2 * i + 1].x, -s[2 * i + 1].y));
+                        const float2 n0 = __fmul2_rn(__fmul2_rn(s[2 * i], s[2 * i]), slope2);
+                        const float2 n1 = __fmul2_rn(__fmul2_rn(s[2 * i + 1], s[2 * i + 1]), slope2);
                         s[2 * i] = __ffma2_rn(p0, n0, p0);
                         s[2 * i + 1] = __ffma2_rn(p1, n1, p1);
                     } else {
@@ -603,7 +605,10 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             delta = -r.z / g;
         }
         if (!BIAS) m += ll;
-        const float2 u2 = make_float2(unit, unit), g2 = make_float2(1.f / g, 1.f / g);
+        const Cap<T> cap(y1, unit);
+        const float2 u2 = CAP ? make_float2(1.f, 1.f) : make_float2(unit, unit);
+        const float2 g2 = make_float2(1.f / g, 1.f / g);
+        const float2 slope2 = make_float2(-1.f / (unit * unit), -1.f / (unit * unit));   // 1 - tanh^2 = 1 + s^2 slope
         const float2 m2 = make_float2(m, m), l2 = make_float2(ll, ll), d2 = make_float2(delta, delta);
         float far_lo = 0.f, far_hi = 0.f;
         const float undo = kBf16 ? 1.f : g / 64.f;
@@ -620,7 +625,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             tc::wait_ld();
             tc::fence_before();
             mbar_arrive(&bars.dp_free);
-            if (CAP) tanh32(s, y1);
+            if (CAP) cap(s);
             const int k0 = j * kRows + 32 * part;
             const bool whole = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 32);
             const uint32_t from = static_cast<uint32_t>(lo - k0);
@@ -654,7 +659,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                 }
                 if (BIAS) d[i] = z;
                 if (CAP) {
-                    const float2 n = __fmul2_rn(s[i], make_float2(-s[i].x, -s[i].y));
+                    const float2 n = __fmul2_rn(__fmul2_rn(s[i], s[i]), slope2);
                     z = __ffma2_rn(z, n, z);
                 }
                 w[i] = tc::pack2<T>(z.x, z.y);

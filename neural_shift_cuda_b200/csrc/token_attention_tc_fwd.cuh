@@ -57,6 +57,7 @@ struct FwdBars {
     // fast warp, may be a block ahead of a slow warp)
     uint64_t q, k_full[6], v_full[6], empty[6], ok[6], s_full[2][2], p_full[2][2], pv[2], o_full[2];
     uint64_t drain[2];
+    uint64_t turn[4][2];   // of a scheduler: its warp of a tile may use the exponential unit
 };
 
 template <typename T, int DP, bool CAP, bool BIAS, bool REST>
@@ -105,6 +106,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             mbar_init(&bars.pv[i], 1);
             mbar_init(&bars.o_full[i], 1);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(&bars.turn[i >> 1][i & 1], 1);
         mbar_init(&bars.drain[0], 1);
         mbar_init(&bars.drain[1], 1);
         fence_mbar_init();
@@ -174,6 +176,8 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         const float* Eh = E + (pair && a ? 2 * p.reach + 2 * kBiasPad + 1 : 0);
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
+        const int turns = max(0, min(lb[0] - fb[0], lb[1] - fb[1]));   // (fb may be INT_MAX)
+        const Cap<T> cap(y1, unit);
         float m = -INFINITY, l = 0.f;
         bool alive = true;
         int it = 0;
@@ -188,14 +192,13 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             tc::wait_ld();
             const int k0 = j * kKeys;
             if (CAP) {
-                tanh32(s, y1);
-                tanh32(s + 16, y1);
+                cap(s);
+                cap(s + 16);
             }
-            float mul = unit;
+            const float mul = CAP || BIAS ? 1.f : unit;   // of what `s` holds then
             if (BIAS) {
-                mul = 1.f;
                 const int w0 = __shfl_sync(0xffffffffu, pos, 0);   // lanes at w0 .. w0 + 31
-                const float2 u2 = make_float2(unit, unit);
+                const float2 u2 = CAP ? make_float2(1.f, 1.f) : make_float2(unit, unit);
                 if (k0 + kKeys - 1 - w0 <= -p.reach || k0 - w0 - 31 >= p.reach) {
                     const float e = Eh[k0 > w0 ? 2 * p.reach + kBiasPad : kBiasPad];
                     const float2 e2 = make_float2(e, e);
@@ -246,6 +249,12 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     tc::store16(to + c, reinterpret_cast<uint32_t*>(o));
                 }
             }
+            // The two warps of a scheduler take turns at the exponentials: side by side both
+            // would be slow here, and then both elsewhere with the unit idle.
+            if (it < turns && (a == 1 || it > 0)) {
+                alive = __all_sync(0xffffffffu, wait(&bars.turn[warp & 3][a], (it - 1 + a) & 1));
+                if (!alive) break;
+            }
             const float ref = m == -INFINITY ? 0.f : -m;
             const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(ref, ref);
             float2 sums[4] = {};
@@ -264,6 +273,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 if (REST) tc::store16(ts + 32 + 16 * c, rest);
             }
             const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
+            if (it < turns && lane == 0) mbar_arrive(&bars.turn[warp & 3][1 - a]);
             l += sum.x + sum.y;
             tc::wait_st();
             tc::fence_before();
