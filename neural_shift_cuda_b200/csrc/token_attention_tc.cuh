@@ -76,22 +76,25 @@ __device__ __forceinline__ uint32_t scrub_rows(unsigned char* tile, int t, int l
     for (int r = t; r < ROWS; r += lanes, ++bit) {
         using T2 = typename std::conditional<sizeof(T) == 2 && std::is_same<T, __half>::value,
                                              __half2, __nv_bfloat162>::type;
-        T2 acc;
-        reinterpret_cast<uint32_t&>(acc) = 0;
-        T2 zero = acc;
+        T2 zero, acc[4];   // (four: one chain would wait out each step)
+        reinterpret_cast<uint32_t&>(zero) = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = zero;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const uint4* row = reinterpret_cast<const uint4*>(tile + c * ROWS * 128 + r * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint4 v = row[(i + r) & 7];
-                acc = __hfma2(reinterpret_cast<const T2&>(v.x), zero, acc);
-                acc = __hfma2(reinterpret_cast<const T2&>(v.y), zero, acc);
-                acc = __hfma2(reinterpret_cast<const T2&>(v.z), zero, acc);
-                acc = __hfma2(reinterpret_cast<const T2&>(v.w), zero, acc);
+                acc[0] = __hfma2(reinterpret_cast<const T2&>(v.x), zero, acc[0]);
+                acc[1] = __hfma2(reinterpret_cast<const T2&>(v.y), zero, acc[1]);
+                acc[2] = __hfma2(reinterpret_cast<const T2&>(v.z), zero, acc[2]);
+                acc[3] = __hfma2(reinterpret_cast<const T2&>(v.w), zero, acc[3]);
             }
         }
-        const uint32_t w = reinterpret_cast<const uint32_t&>(acc);
+        uint32_t w = 0;   // zeros (of either sign), or NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= reinterpret_cast<const uint32_t&>(acc[i]);
         if ((w & 0x7FFF7FFFu) == 0) continue;
         bad |= 1u << bit;
 #pragma unroll

@@ -45,7 +45,8 @@ struct BwdBars {
     uint64_t fixed, x_full[4], y_full[4], empty[4], ok[4];
     // (two each where a warp, or the products, may be a step ahead of a slower warp,
     // whose wait or arrival would else be taken for that of the other step)
-    uint64_t s_full[2], p_ready[2], ds_ready[2], dp_full, dp_free, used_p, used_ds, done, drain;
+    uint64_t s_full[2], p_ready[2], ds_ready[2], used_p[2], used_ds[2], dp_full, dp_free, done;
+    uint64_t drain[2];
 };
 
 __device__ __forceinline__ float pow2_near(float v) {   // a power of two at or above v, or 1
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             mbar_init(&bars.x_full[i], 1);
             mbar_init(&bars.y_full[i], 1);
             mbar_init(&bars.empty[i], 1);
-            mbar_init(&bars.ok[i], 64);
+            mbar_init(&bars.ok[i], 32);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.s_full[i], 1);
@@ -103,10 +104,13 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             mbar_init(&bars.ds_ready[i], kBwdMath);
         }
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.used_p, 1);
-        mbar_init(&bars.used_ds, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.used_p[i], 1);
+            mbar_init(&bars.used_ds[i], 1);
+        }
         mbar_init(&bars.done, 1);
-        mbar_init(&bars.drain, 1);
+        mbar_init(&bars.drain[0], 1);
+        mbar_init(&bars.drain[1], 1);
         fence_mbar_init();
         abort_flag[0] = 0;
         abort_flag[1] = static_cast<int>(bnd.budget);
@@ -363,97 +367,86 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     mbar_wait32(smem_u32(&bars.x_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                     mbar_wait32(smem_u32(&bars.y_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                 }
-        } else if (warp == 17 && total > 0) {
+        } else if (warp == 17 && total > 0) {   // S and dP
             const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
-            const uint32_t its = tc::product(kBf16, 128, cols, false, true);
             const bool lead = tc::elect();
-            auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-            bool alive = all(wait(&bars.fixed, 0));
-            auto S_at = [&](int i) { return t_s + (kTwoS ? 128 * (i & 1) : 0); };
-            // S(i) into its place, once the product that read P there is done
-            auto scores = [&](int i) {
+            bool fine = wait(&bars.fixed, 0);
+            for (int i = 0; i < total; ++i) {
                 const int s = i % NS, last = kTwoS ? i - 2 : i - 1;
-                alive = all(wait(&bars.x_full[s], (i / NS) & 1) && wait(&bars.ok[s], (i / NS) & 1) &&
-                            (last < 0 || wait(&bars.used_p, last & 1)));
-                if (!alive) return;
+                // S(i) into its place, once the product that read P there is done
+                fine &= wait(&bars.x_full[s], (i / NS) & 1) && wait(&bars.ok[s], (i / NS) & 1);
+                if (last >= 0) fine &= wait(&bars.used_p[last & 1], (last >> 1) & 1);
                 tc::fence_after();
                 if (lead) {
-                    scores_mma<DP>(S_at(i), smem_u32(Ks), smem_u32(Q_at(s)), iss, steps);
+                    scores_mma<DP>(t_s + (kTwoS ? 128 * (i & 1) : 0), smem_u32(Ks), smem_u32(Q_at(s)),
+                                   iss, steps);
                     tc::commit(smem_u32(&bars.s_full[i & 1]));
                 }
-            };
-            for (int it = -1; alive && it < total; ++it) {
-                const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
-                if (kTwoS && next < total) {
-                    scores(next);
-                    if (!alive) break;
+                fine &= wait(&bars.y_full[s], (i / NS) & 1);
+                if (i > 0) fine &= wait(&bars.used_ds[(i - 1) & 1], ((i - 1) >> 1) & 1);
+                tc::fence_after();
+                if (lead) {
+                    scores_mma<DP>(t_dp, smem_u32(Vs), smem_u32(O_at(s)), iss, steps);
+                    tc::commit(smem_u32(&bars.dp_full));
                 }
-                if (it >= 0) {
-                    alive = all(wait(&bars.p_ready[it & 1], (it >> 1) & 1));
-                    if (!alive) break;
-                    tc::fence_after();
-                    if (lead) {
-                        mix_mma<8, 2, 32>(t_dv, S_at(it), smem_u32(O_at(s)), kPanel, its, it > 0);
-                        tc::commit(smem_u32(&bars.used_p));
-                    }
-                }
-                if (!kTwoS && next < total) {
-                    scores(next);
-                    if (!alive) break;
-                }
-                if (it >= 0) {
-                    alive = all(wait(&bars.ds_ready[it & 1], (it >> 1) & 1));
-                    if (!alive) break;
-                    tc::fence_after();
-                    if (lead) {
-                        mix_mma<8, 2, 32>(t_dk, t_dp, smem_u32(Q_at(s)), kPanel, its, it > 0);
-                        mix_mma<8, 2, 32>(t_dk, t_dp + 16, smem_u32(Q_at(s)), kPanel, its, true);
-                        tc::commit(smem_u32(&bars.used_ds));
-                        tc::commit(smem_u32(&bars.empty[s]));
-                    }
-                }
-                if (next < total) {
-                    alive = all(wait(&bars.y_full[sn], (next / NS) & 1) &&
-                                (it < 0 || wait(&bars.used_ds, it & 1)));
-                    if (!alive) break;
-                    tc::fence_after();
-                    if (lead) {
-                        scores_mma<DP>(t_dp, smem_u32(Vs), smem_u32(O_at(sn)), iss, steps);
-                        tc::commit(smem_u32(&bars.dp_full));
-                    }
-                }
+                if (!__all_sync(0xffffffffu, fine)) break;
             }
-            if (alive) {
-                if (lead) tc::commit(smem_u32(&bars.done));
-            } else {
-                if (lead) tc::commit(smem_u32(&bars.drain));
-                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
+            if (!__all_sync(0xffffffffu, fine)) {   // the products in flight read this block's memory
+                if (lead) tc::commit(smem_u32(&bars.drain[0]));
+                mbar_wait32(smem_u32(&bars.drain[0]), 0, bnd.timeouts);
             }
-        } else if (warp >= 18 && total > 0) {
-            const int gt = threadIdx.x - (kBwdMath + 64);
+        } else if (warp == 18 && total > 0) {   // dV and dK
+            const uint32_t its = tc::product(kBf16, 128, cols, false, true);
+            const bool lead = tc::elect();
+            bool fine = true;
+            for (int i = 0; i < total; ++i) {
+                const int s = i % NS;
+                fine &= wait(&bars.p_ready[i & 1], (i >> 1) & 1);
+                tc::fence_after();
+                if (lead) {
+                    mix_mma<8, 2, 32>(t_dv, t_s + (kTwoS ? 128 * (i & 1) : 0), smem_u32(O_at(s)), kPanel,
+                                      its, i > 0);
+                    tc::commit(smem_u32(&bars.used_p[i & 1]));
+                }
+                fine &= wait(&bars.ds_ready[i & 1], (i >> 1) & 1);
+                tc::fence_after();
+                if (lead) {
+                    mix_mma<8, 2, 32>(t_dk, t_dp, smem_u32(Q_at(s)), kPanel, its, i > 0);
+                    mix_mma<8, 2, 32>(t_dk, t_dp + 16, smem_u32(Q_at(s)), kPanel, its, true);
+                    tc::commit(smem_u32(&bars.used_ds[i & 1]));
+                    tc::commit(smem_u32(&bars.empty[s]));
+                }
+                if (!__all_sync(0xffffffffu, fine)) break;
+            }
+            if (lead) tc::commit(smem_u32(&bars.done));
+            if (!__all_sync(0xffffffffu, fine)) {   // the products in flight read this block's memory
+                if (lead) tc::commit(smem_u32(&bars.drain[1]));
+                mbar_wait32(smem_u32(&bars.drain[1]), 0, bnd.timeouts);
+            }
+        } else if (warp == 19 && total > 0) {
             int h = head0, j = fb;
             for (int it = 0; it < total; ++it, ++j) {
                 const int s = it % NS;
                 if (j == lb) { j = fb; ++h; }
                 const uint32_t parity = (it / NS) & 1;
                 const RowRec* src = recs + (static_cast<int64_t>(b) * p.Hq + h) * p.Lq;
-                float4 rec[2];
+                float4 rec[4];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int row = j * kRows + gt + 64 * r;
+                for (int r = 0; r < 4; ++r) {
+                    const int row = j * kRows + lane + 32 * r;
                     rec[r] = row < p.Lq ? __ldg(reinterpret_cast<const float4*>(src + row))
                                         : make_float4(-INFINITY, 0.f, 0.f, 0.f);
                 }
-                if (it >= NS && !wait(&bars.empty[s], (it / NS - 1) & 1)) break;
+                if (it >= NS && !wait(&bars.empty[s], parity ^ 1)) break;
                 uint32_t bad = 0;
                 if (guarded(j)) {
                     if (!wait(&bars.x_full[s], parity) || !wait(&bars.y_full[s], parity)) break;
-                    bad = scrub_rows<T, DP>(Q_at(s), gt, 64) | scrub_rows<T, DP>(O_at(s), gt, 64);
+                    bad = scrub_rows<T, DP>(Q_at(s), lane, 32) | scrub_rows<T, DP>(O_at(s), lane, 32);
                     fence_async_shared();
                 }
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int at = gt + 64 * r;
+                for (int r = 0; r < 4; ++r) {
+                    const int at = lane + 32 * r;
                     float m = -rec[r].x, ll = -rec[r].y + (kBf16 ? 0.f : kPShift);
                     if (rec[r].x == -INFINITY) m = -INFINITY;   // sees nothing: weight zero
                     if (bad >> r & 1) m = NAN;
@@ -534,16 +527,19 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             mbar_init(&bars.x_full[i], 1);
             mbar_init(&bars.y_full[i], 1);
             mbar_init(&bars.empty[i], 1);
-            mbar_init(&bars.ok[i], 64);
+            mbar_init(&bars.ok[i], 32);
         }
         mbar_init(&bars.ds_ready[0], kBwdMath);
         mbar_init(&bars.ds_ready[1], kBwdMath);
         mbar_init(&bars.dp_full, 1);
         mbar_init(&bars.dp_free, kBwdMath);
-        mbar_init(&bars.used_p, 1);
-        mbar_init(&bars.used_ds, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.used_p[i], 1);
+            mbar_init(&bars.used_ds[i], 1);
+        }
         mbar_init(&bars.done, 1);
-        mbar_init(&bars.drain, 1);
+        mbar_init(&bars.drain[0], 1);
+        mbar_init(&bars.drain[1], 1);
         fence_mbar_init();
         abort_flag[0] = 0;
         abort_flag[1] = static_cast<int>(bnd.budget);
@@ -767,66 +763,66 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                     mbar_wait32(smem_u32(&bars.x_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                     mbar_wait32(smem_u32(&bars.y_full[i % NS]), (i / NS) & 1, bnd.timeouts);
                 }
-        } else if (warp == 17 && total > 0) {
+        } else if (warp == 17 && total > 0) {   // S and dP
             const uint32_t iss = tc::product(kBf16, 128, 128, false, false);
+            const bool lead = tc::elect();
+            bool fine = wait(&bars.fixed, 0);
+            for (int i = 0; i < total; ++i) {
+                const int s = i % NS;
+                fine &= wait(&bars.x_full[s], (i / NS) & 1) && wait(&bars.ok[s], (i / NS) & 1);
+                // (the place of S(i) holds dS of the block before last until dQ has read it)
+                if (i > 1) fine &= wait(&bars.used_ds[i & 1], ((i - 2) >> 1) & 1);
+                tc::fence_after();
+                if (lead)
+                    scores_mma<DP>(t_s + 128 * (i & 1), smem_u32(Qs), smem_u32(K_at(s)), iss, steps);
+                fine &= wait(&bars.y_full[s], (i / NS) & 1);
+                if (i > 0) fine &= wait(&bars.dp_free, (i - 1) & 1);
+                tc::fence_after();
+                if (lead) {
+                    scores_mma<DP>(t_dp, smem_u32(Os), smem_u32(V_at(s)), iss, steps);
+                    tc::commit(smem_u32(&bars.dp_full));
+                }
+                if (!__all_sync(0xffffffffu, fine)) break;
+            }
+            if (!__all_sync(0xffffffffu, fine)) {   // the products in flight read this block's memory
+                if (lead) tc::commit(smem_u32(&bars.drain[0]));
+                mbar_wait32(smem_u32(&bars.drain[0]), 0, bnd.timeouts);
+            }
+        } else if (warp == 18 && total > 0) {   // dQ
             const uint32_t its = tc::product(kBf16, 128, cols, false, true);
             const bool lead = tc::elect();
-            auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-            bool alive = all(wait(&bars.fixed, 0));
-            for (int it = -1; alive && it < total; ++it) {
-                const int s = (it + NS) % NS, sn = (it + 1) % NS, next = it + 1;
-                const uint32_t pn = (next / NS) & 1;
-                if (next < total) {
-                    alive = all(wait(&bars.x_full[sn], pn));
-                    // (its place holds dS of the block before last until dQ has read it)
-                    alive = alive && all(wait(&bars.ok[sn], pn) &&
-                                         (it < 1 || wait(&bars.used_ds, (it - 1) & 1)));
-                    if (!alive) break;
-                    tc::fence_after();
-                    if (lead) scores_mma<DP>(t_s + 128 * (next & 1), smem_u32(Qs), smem_u32(K_at(sn)), iss, steps);
-                    alive = all(wait(&bars.y_full[sn], pn) && (it < 0 || wait(&bars.dp_free, it & 1)));
-                    if (!alive) break;
-                    tc::fence_after();
-                    if (lead) scores_mma<DP>(t_dp, smem_u32(Os), smem_u32(V_at(sn)), iss, steps);
-                    if (lead) tc::commit(smem_u32(&bars.dp_full));
+            bool fine = true;
+            for (int i = 0; i < total; ++i) {
+                const int s = i % NS;
+                fine &= wait(&bars.ds_ready[i & 1], (i >> 1) & 1);
+                tc::fence_after();
+                if (lead) {
+                    const uint32_t w = t_s + 128 * (i & 1);
+                    mix_mma<8, 2, 32>(t_dq, w, smem_u32(K_at(s)), kPanel, its, i > 0);
+                    mix_mma<8, 2, 32>(t_dq, w + 16, smem_u32(K_at(s)), kPanel, its, true);
+                    tc::commit(smem_u32(&bars.used_ds[i & 1]));
+                    tc::commit(smem_u32(&bars.empty[s]));
                 }
-                if (it >= 0) {
-                    alive = all(wait(&bars.ds_ready[it & 1], (it >> 1) & 1));
-                    if (!alive) break;
-                    tc::fence_after();
-                    if (lead) {
-                        const uint32_t w = t_s + 128 * (it & 1);
-                        mix_mma<8, 2, 32>(t_dq, w, smem_u32(K_at(s)), kPanel, its, it > 0);
-                        mix_mma<8, 2, 32>(t_dq, w + 16, smem_u32(K_at(s)), kPanel, its, true);
-                    }
-                    if (lead) tc::commit(smem_u32(&bars.used_ds));
-                    if (lead) tc::commit(smem_u32(&bars.empty[s]));
-                }
+                if (!__all_sync(0xffffffffu, fine)) break;
             }
-            if (alive) {
-                if (lead) tc::commit(smem_u32(&bars.done));
-            } else {
-                if (lead) tc::commit(smem_u32(&bars.drain));
-                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
+            if (lead) tc::commit(smem_u32(&bars.done));
+            if (!__all_sync(0xffffffffu, fine)) {   // the products in flight read this block's memory
+                if (lead) tc::commit(smem_u32(&bars.drain[1]));
+                mbar_wait32(smem_u32(&bars.drain[1]), 0, bnd.timeouts);
             }
-        } else if (warp >= 18 && total > 0) {
-            const int gt = threadIdx.x - (kBwdMath + 64);
+        } else if (warp == 19 && total > 0) {
             for (int it = 0; it < total; ++it) {
                 const int s = it % NS;
                 const uint32_t parity = (it / NS) & 1;
                 if (it >= NS && !wait(&bars.empty[s], parity ^ 1)) break;
-                if (!guarded(fb + it)) {
-                    mbar_arrive(&bars.ok[s]);
-                    continue;
-                }
-                if (!wait(&bars.x_full[s], parity) || !wait(&bars.y_full[s], parity)) break;
-                const uint32_t bad = scrub_rows<T, DP>(K_at(s), gt, 64);
-                if (bad) {   // the rows that see it get NaN by dP
+                if (guarded(fb + it)) {
+                    if (!wait(&bars.x_full[s], parity) || !wait(&bars.y_full[s], parity)) break;
+                    const uint32_t bad = scrub_rows<T, DP>(K_at(s), lane, 32);
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        if (bad >> r & 1) poison_row<DP>(V_at(s), gt + 64 * r);
+                    for (int r = 0; r < 4; ++r)   // the rows that see it get NaN by dP
+                        if (bad >> r & 1) poison_row<DP>(V_at(s), lane + 32 * r);
+                    fence_async_shared();
                 }
-                fence_async_shared();
                 mbar_arrive(&bars.ok[s]);
             }
         }
