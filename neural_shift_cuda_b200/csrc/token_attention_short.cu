@@ -20,7 +20,7 @@ namespace {
 constexpr int kShortThreads = 128;
 constexpr int kKeys = 64;
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool REST>
 __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) void short_fwd_kernel(const Params p) {
     constexpr int LD = 2 * DP + 16, KS = DP / 16, CH = DP / 8;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
                     const float e1 = tc::ex2(s[2 * i + y][2 * x + 1] - ref);
                     l[x] += e0 + e1;
                     pa[2 * y + x] = tc::pack2<T>(e0, e1);
-                    rest[2 * y + x] = tc::rest2<T>(make_float2(e0, e1), pa[2 * y + x]);
+                    if (REST) rest[2 * y + x] = tc::rest2<T>(make_float2(e0, e1), pa[2 * y + x]);
                 }
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
                 ldm4t(va + i * 16 * LD + 32 * c, f);
                 mma16816<T>(o[2 * c], pa, f[0], f[1]);
                 mma16816<T>(o[2 * c + 1], pa, f[2], f[3]);
-                if (BIAS && p.residue) {   // see the tensor-core forward
+                if (REST) {   // see the tensor-core forward
                     mma16816<T>(o[2 * c], rest, f[0], f[1]);
                     mma16816<T>(o[2 * c + 1], rest, f[2], f[3]);
                 }
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
             const float u = none ? 0.f : o[c][2 * x] * inv, v = none ? 0.f : o[c][2 * x + 1] * inv;
             const uint32_t w = tc::pack2<T>(u, v);
             *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at + d) = w;
-            if (p.residue) {
+            if (REST) {
                 const T* back = reinterpret_cast<const T*>(&w);
                 *reinterpret_cast<uint32_t*>(static_cast<T*>(p.residue) + at + d) =
                     tc::pack2<T>(u - to_acc(back[0]), v - to_acc(back[1]));
@@ -226,24 +226,28 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
     }
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool REST>
 nsc_status launch(const Params& p, cudaStream_t st) {
-    auto kern = short_fwd_kernel<T, DP, CAP, BIAS>;
+    auto kern = short_fwd_kernel<T, DP, CAP, BIAS, REST>;
     // at most 35 KB of tiles and 8 KB of bias: no opt-in is needed
     const int smem = 2 * kKeys * (2 * DP + 16) + (BIAS ? 4 * (2 * p.reach + 1) : 0);
     const int64_t blocks = static_cast<int64_t>(p.B) * p.Hq * ((p.Lq + 63) / 64);
     kern<<<static_cast<unsigned>(blocks), kShortThreads, smem, st>>>(p);
     return check_launch("token_attention");
 }
-template <typename T, int DP>
+template <typename T, int DP, bool REST>
 nsc_status run(const Params& p, cudaStream_t st) {
     if (p.cap > 0)
-        return p.table ? launch<T, DP, true, true>(p, st) : launch<T, DP, true, false>(p, st);
-    return p.table ? launch<T, DP, false, true>(p, st) : launch<T, DP, false, false>(p, st);
+        return p.table ? launch<T, DP, true, true, REST>(p, st)
+                       : launch<T, DP, true, false, REST>(p, st);
+    return p.table ? launch<T, DP, false, true, REST>(p, st)
+                   : launch<T, DP, false, false, REST>(p, st);
 }
-template <typename T>
+template <typename T, bool REST>
 nsc_status run(const Params& p, cudaStream_t st) {
-    return p.D <= 32 ? run<T, 32>(p, st) : p.D <= 64 ? run<T, 64>(p, st) : run<T, 128>(p, st);
+    return p.D <= 32   ? run<T, 32, REST>(p, st)
+           : p.D <= 64 ? run<T, 64, REST>(p, st)
+                       : run<T, 128, REST>(p, st);
 }
 
 }  // namespace
@@ -252,7 +256,9 @@ nsc_status run(const Params& p, cudaStream_t st) {
 bool short_fits(const Params& p, int dtype) { return tc_fits(p, dtype) && p.Lk <= 128 && p.Lq <= 128; }
 
 nsc_status short_fwd(const Params& p, int dtype, cudaStream_t st) {
-    return dtype == NSC_BF16 ? run<__nv_bfloat16>(p, st) : run<__half>(p, st);
+    if (p.residue)
+        return dtype == NSC_BF16 ? run<__nv_bfloat16, true>(p, st) : run<__half, true>(p, st);
+    return dtype == NSC_BF16 ? run<__nv_bfloat16, false>(p, st) : run<__half, false>(p, st);
 }
 
 }  // namespace tok

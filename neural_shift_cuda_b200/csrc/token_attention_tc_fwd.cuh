@@ -18,11 +18,14 @@
 // Softmax with a running reference m: p = 2^(s2 - m); m moves, and O is
 // rescaled, only when a row's maximum passes m + 8 (p <= 256 keeps 16-bit
 // weights in range), which after the first blocks is rare.  P is rounded to the
-// operand type; the sum of a row is of the fp32 values.  REST, for training with a
-// bias table: what that rounding drops is multiplied too, as a second operand.  The
-// backward's row sums of grad_out * out are then those of the weights it recomputes, and
-// a bucket's gradient, a sum of many rows' nearly cancelling terms, keeps its digits
-// (bf16, 8192 rows: 1.7e-3 of it off, its own rounding, where 3.1e-3 were).
+// operand type; the sum of a row is of the fp32 values.  REST, for training
+// (a residue is wanted): what that rounding drops is multiplied too, as a second operand.
+// The backward's row sums of grad_out * out are then those of the weights it recomputes;
+// without it the score gradients of rows with few keys, and the sums of many such terms in
+// a bucket, lose digits (documents of some keys, bf16: grad_q and grad_k 2.8e-3 off
+// instead of 1.7e-3, which is their own rounding; a bucket of 8192 rows 3.1e-3 instead of
+// 1.7e-3).  It costs 15 % of a capped forward with heads of 128 (200 -> 230 us, 16 heads,
+// 8192 tokens in 4 documents).
 //
 // Guard: in blocks that some row of a tile does not see whole, a value row
 // that is not finite would reach every row as 0 x NaN.  There the guard warp
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     }
 }
 
-template <typename T, int DP, bool CAP, bool BIAS, bool REST = false>
+template <typename T, int DP, bool CAP, bool BIAS, bool REST>
 nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     auto kern = tc_fwd_kernel<T, DP, CAP, BIAS, REST>;
@@ -449,16 +452,18 @@ nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
 
 }  // namespace
 
+template <typename T, int DP, bool REST>
+nsc_status tc_fwd_scores(const Params& p, cudaStream_t st) {
+    if (p.cap > 0)
+        return p.table ? tc_fwd_launch<T, DP, true, true, REST>(p, st)
+                       : tc_fwd_launch<T, DP, true, false, REST>(p, st);
+    return p.table ? tc_fwd_launch<T, DP, false, true, REST>(p, st)
+                   : tc_fwd_launch<T, DP, false, false, REST>(p, st);
+}
+
 template <typename T, int DP>
 nsc_status tc_fwd_run(const Params& p, cudaStream_t st) {
-    if (p.table && p.residue)
-        return p.cap > 0 ? tc_fwd_launch<T, DP, true, true, true>(p, st)
-                         : tc_fwd_launch<T, DP, false, true, true>(p, st);
-    if (p.cap > 0)
-        return p.table ? tc_fwd_launch<T, DP, true, true>(p, st)
-                       : tc_fwd_launch<T, DP, true, false>(p, st);
-    return p.table ? tc_fwd_launch<T, DP, false, true>(p, st)
-                   : tc_fwd_launch<T, DP, false, false>(p, st);
+    return p.residue ? tc_fwd_scores<T, DP, true>(p, st) : tc_fwd_scores<T, DP, false>(p, st);
 }
 
 }  // namespace tok

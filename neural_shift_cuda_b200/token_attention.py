@@ -287,9 +287,9 @@ def _attention_fwd(q, k, v, documents, prefix, table, buckets, scale, cap, causa
         lse = torch.empty((B, Hq, Lq), dtype=_acc(q.dtype), device=dev)
     if train:
         stats = torch.empty((2, B, Hq, Lq), dtype=_acc(q.dtype), device=dev)
-        if table is not None and q.element_size() == 2:
-            # a bucket sums the score gradients of many rows, each less its
-            # row's sum of grad_out * out: that of the rounded out would show
+        if q.element_size() == 2:
+            # a score's gradient is less its row's sum of grad_out * out: with few
+            # keys, or summed up in a bias bucket, what rounding out drops would show
             residue = torch.empty_like(out)
     a = _attention_args(q, k, v, documents, prefix, None, table, buckets, scale,
                         cap, causal)

@@ -76,9 +76,9 @@ def _run(dt, B, Lq, Lk, Hq, Hkv, D, kind, cap=0.0, buckets=None, mul=1.0, seed=0
         check(got[3], want[5], dt, "grad_table")
     with torch.no_grad():
         again = nsc.token_attention(q, k, v, softcap=cap, bias_table=table, bias_buckets=m, **kw)
-    if table is None or dt in (F32, F64):
+    if dt in (F32, F64):
         assert torch.equal(again, out.detach())
-    else:   # training with a bias table keeps more digits of the weights
+    else:   # training keeps more digits of the weights
         check(again, want[0], dt, "out without gradients")
     return out, got
 
@@ -378,3 +378,23 @@ def test_slow_and_fast_warps_keep_in_step(cuda):
             first = first or now
             for a, b in zip(first, now):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("L", [96, 387])
+@pytest.mark.parametrize("dt,D", [(F16, 64), (BF16, 64), (BF16, 128)])
+def test_score_gradients_of_rows_with_few_keys(cuda, dt, D, L):
+    """Documents of three tokens: a score's gradient is a small difference, of the
+    weights' gradients and the row's sum of grad_out * out.  What reaches grad_q and
+    grad_k is their own rounding; a quarter more is left for all else."""
+    q, k, v, go = (randn(71 + i, 2, L, 4, D, dtype=dt, mul=1.5 if i < 2 else 1.0).to(cuda)
+                   for i in range(4))
+    rows = [list(range(0, L + 1, 3))] * 2
+    want = reference(q, k, v, T.visible(2, L, L, False, None, rows), go, D ** -0.5)
+    ql, kl, vl = leaf(q), leaf(k), leaf(v)
+    out = nsc.token_attention(ql, kl, vl, documents=torch.tensor(rows, device=cuda))
+    got = torch.autograd.grad(out, [ql, kl, vl], go)
+    for name, g, w in zip(("grad_q", "grad_k"), got, want[2:4]):
+        own = float((w.to(dt).double() - w).norm() / w.norm())
+        off = float((g.double() - w).norm() / w.norm())
+        print(name, own, off)
+        assert off <= 1.25 * own, f"{name}: {off:.3g}, its own rounding is {own:.3g}"
