@@ -6,12 +6,20 @@
 //     dx = r h w - x r^3 mean(h w x)
 //
 // Bound by memory: a head is read once and written once (backward: x and
-// grad_out read, dx written).  A group of `LANES` lanes holds one head, 16
-// channels a lane as two chunks of 8 half a head apart: both ends of a rotated
-// pair are then in the same lane for either pairing, the only exchange is
-// that of the sums, and every access is 16 bytes.  A group walks several
-// heads of one token with its cosines and sines in registers, the loads of
-// up to four heads in flight.
+// grad_out read, dx written).  A group of `LANES` lanes holds one head, 8
+// channels a lane as two chunks of 4 half a head apart (past 256 channels, two of 8):
+// both ends of a rotated pair are then in the same lane for either pairing, and the
+// only exchange is that of the sums.  A group walks the heads of a token with its
+// cosines and sines in registers; as soon as a head is unpacked, the load of the one
+// four further on takes its place, across tokens too.  Arithmetic is two pairs an
+// instruction: at one each it took as long as the memory.
+//
+// 4 x 4096 tokens, 16 + 16 heads of 128, bf16 (slices of a projection): forward 49 us for
+// 268 MB (5.4 TB/s of the 6.5 that a copy reaches), backward 79 us for 403 MB (5.1
+// TB/s).  Before: blocks of one round each, 16 channels a lane, one pair an instruction:
+// 62 and 104 us.
+#include <type_traits>
+
 #include "nsc_host.h"
 
 namespace nsc {
@@ -19,7 +27,11 @@ namespace rot {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxPart = 592;    // blocks that hold weight-gradient partials: 4 an SM
+constexpr int kMaxPart = 592;   // most rows of weight-gradient partials of a tensor
+// Resident blocks an SM, by registers (forward: with 4 of 64 registers 52 us, with 2 55 us;
+// backward: with 3 of 80 it spills, 134 us).
+constexpr int kFwdPerSm = 3, kBwdPerSm = 2;
+constexpr int kAhead = 4;   // heads in flight a group (16-bit types)
 
 struct Args {
     const void *q, *k, *wq, *wk, *cos, *sin;
@@ -48,64 +60,109 @@ __device__ __forceinline__ A weight_at(const void* w, int dt, int d) {
     return static_cast<A>(static_cast<const double*>(w)[d]);
 }
 
-// 8 values, 16-byte aligned, as raw words
-template <typename T> struct Raw { uint4 u[sizeof(T) / 2]; };
-template <typename T>
-__device__ __forceinline__ Raw<T> load8(const T* p) {
-    Raw<T> r;
+// V values as raw words, read in accesses of up to 16 bytes
+template <typename T, int V> struct Raw {
+    static constexpr int kBytes = V * sizeof(T), kWord = kBytes < 16 ? kBytes : 16;
+    using Word = typename std::conditional<kWord == 16, uint4, uint2>::type;
+    Word u[kBytes / kWord];
+};
+template <int V, typename T>
+__device__ __forceinline__ Raw<T, V> load(const T* p) {
+    using R = Raw<T, V>;
+    R r;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-        r.u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < R::kBytes / R::kWord; ++i)
+        r.u[i] = __ldg(reinterpret_cast<const typename R::Word*>(p) + i);
     return r;
-}
-template <typename T, typename A>
-__device__ __forceinline__ void unpack(const Raw<T>& r, A (&v)[8]) {
-    const T* t = reinterpret_cast<const T*>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_acc(t[i]);
 }
 template <typename T> __device__ __forceinline__ T cast_to(float v) { return from_float<T>(v); }
 template <typename T> __device__ __forceinline__ T cast_to(double v) { return v; }
-template <typename T, typename A>
-__device__ __forceinline__ void store8(T* p, const A (&v)[8]) {
-    Raw<T> r;
-    T* t = reinterpret_cast<T*>(&r);
+
+// A lane's V pairs (u, v), two by two: channels x of the first half of the head and y of
+// the second are u and v (ADJ: neighbours in x, then neighbours in y).
+template <int V> struct Pairs { float2 u[V / 2], v[V / 2]; };
+template <int V, bool ADJ>
+__device__ __forceinline__ Pairs<V> pairs_of(const float (&x)[V], const float (&y)[V]) {
+    Pairs<V> p;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = cast_to<T>(v[i]);
+    for (int i = 0; i < V / 2; ++i)
+        if (ADJ) {
+            const float(&t)[V] = i < V / 4 ? x : y;
+            const int e = 4 * (i % (V / 4));
+            p.u[i] = make_float2(t[e], t[e + 2]);
+            p.v[i] = make_float2(t[e + 1], t[e + 3]);
+        } else {
+            p.u[i] = make_float2(x[2 * i], x[2 * i + 1]);
+            p.v[i] = make_float2(y[2 * i], y[2 * i + 1]);
+        }
+    return p;
+}
+template <bool ADJ, typename T, int V>
+__device__ __forceinline__ Pairs<V> unpack(const Raw<T, V>& rx, const Raw<T, V>& ry) {
+    float x[V], y[V];
+    const T *tx = reinterpret_cast<const T*>(&rx), *ty = reinterpret_cast<const T*>(&ry);
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-        reinterpret_cast<uint4*>(p)[i] = r.u[i];
+    for (int i = 0; i < V; ++i) {
+        x[i] = to_acc(tx[i]);
+        y[i] = to_acc(ty[i]);
+    }
+    return pairs_of<V, ADJ>(x, y);
+}
+template <bool ADJ, typename T, int V>
+__device__ __forceinline__ void store(T* d, int half, const Pairs<V>& p) {
+    using R = Raw<T, V>;
+    R rx, ry;
+    T *tx = reinterpret_cast<T*>(&rx), *ty = reinterpret_cast<T*>(&ry);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+        if (ADJ) {
+            T* t = i < V / 4 ? tx : ty;
+            const int e = 4 * (i % (V / 4));
+            t[e] = cast_to<T>(p.u[i].x);
+            t[e + 1] = cast_to<T>(p.v[i].x);
+            t[e + 2] = cast_to<T>(p.u[i].y);
+            t[e + 3] = cast_to<T>(p.v[i].y);
+        } else {
+            tx[2 * i] = cast_to<T>(p.u[i].x);
+            tx[2 * i + 1] = cast_to<T>(p.u[i].y);
+            ty[2 * i] = cast_to<T>(p.v[i].x);
+            ty[2 * i + 1] = cast_to<T>(p.v[i].y);
+        }
+#pragma unroll
+    for (int i = 0; i < R::kBytes / R::kWord; ++i) {
+        reinterpret_cast<typename R::Word*>(d)[i] = rx.u[i];
+        reinterpret_cast<typename R::Word*>(d + half)[i] = ry.u[i];
+    }
 }
 
-// Cosines and sines of a lane's 8 pairs at a position; outside the table NaN.
-template <typename A>
-__device__ __forceinline__ void turn_at(const Args& a, int64_t pos, int c, int adjacent, A (&cs)[8],
-                                        A (&sn)[8]) {
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
+
+// Cosines and sines of a lane's pairs at a position; outside the table NaN.
+template <int V> struct Angles { float2 c[V / 2], s[V / 2]; };
+template <int V, bool ADJ>
+__device__ __forceinline__ Angles<V> angles_at(const Args& a, int64_t pos, int c) {
     const bool in = pos >= 0 && pos < a.rows;
-    const A* cp = static_cast<const A*>(a.cos) + (in ? pos : 0) * (a.D / 2);
-    const A* sp = static_cast<const A*>(a.sin) + (in ? pos : 0) * (a.D / 2);
+    const int64_t row = (in ? pos : 0) * (a.D / 2);
+    const float *cp = static_cast<const float*>(a.cos) + row, *sp = static_cast<const float*>(a.sin) + row;
+    Angles<V> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int at = adjacent ? (i < 4 ? 4 * c + i : a.D / 4 + 4 * c + i - 4) : 8 * c + i;
-        cs[i] = in ? __ldg(cp + at) : static_cast<A>(NAN);
-        sn[i] = in ? __ldg(sp + at) : static_cast<A>(NAN);
+    for (int i = 0; i < V / 2; ++i) {
+        const int at = ADJ ? (i < V / 4 ? 0 : a.D / 4 - V / 2) + V / 2 * c + 2 * i : V * c + 2 * i;
+        r.c[i] = in ? make_float2(__ldg(cp + at), __ldg(cp + at + 1)) : twice(NAN);
+        r.s[i] = in ? make_float2(__ldg(sp + at), __ldg(sp + at + 1)) : twice(NAN);
     }
+    return r;
 }
 
-// Turns the lane's pairs in place; back: by the opposite angle.
-template <typename A, bool ADJ, bool BACK>
-__device__ __forceinline__ void turn(A (&x)[8], A (&y)[8], const A (&cs)[8], const A (&sn)[8]) {
+// Sums over a head's lanes, of N values side by side.
+template <int LANES, int N>
+__device__ __forceinline__ void group_sums(float (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        A& u = ADJ ? (i < 4 ? x[2 * (i & 3)] : y[2 * (i & 3)]) : x[i];
-        A& v = ADJ ? (i < 4 ? x[2 * (i & 3) + 1] : y[2 * (i & 3) + 1]) : y[i];
-        const A s = BACK ? -sn[i] : sn[i];
-        const A a = u * cs[i] - v * s, b = v * cs[i] + u * s;
-        u = a;
-        v = b;
-    }
+    for (int i = 1; i < LANES; i <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], i);
 }
-
 template <typename A, int LANES>
 __device__ __forceinline__ A group_sum(A v) {
 #pragma unroll
@@ -113,175 +170,265 @@ __device__ __forceinline__ A group_sum(A v) {
     return v;
 }
 
-// A job is `per` heads of q, or of k, of one token.
-struct Job { int64_t token; bool is_k; int h0, h1; };
-__device__ __forceinline__ Job job_at(const Args& a, int64_t j, int nq, int nk) {
-    Job r;
-    r.token = j / (nq + nk);
-    const int c = static_cast<int>(j - r.token * (nq + nk));
-    r.is_k = c >= nq;
-    r.h0 = (r.is_k ? c - nq : c) * a.per;
-    r.h1 = min(r.h0 + a.per, r.is_k ? a.Hkv : a.Hq);
-    return r;
-}
+// A block's share of the work: blocks [0, q_blocks) pass over q, the others over k, so
+// that a thread has one tensor's weights (and weight sums).  A job is `per` heads of one
+// token; a group takes every `step`-th job.
+template <typename T> struct Share {
+    bool is_k;
+    int H, chunks, per, L;
+    int64_t s0, s1, s2, jobs, first, step;
+    const T* src;
 
-template <typename T, typename A, int LANES, bool ADJ>
-__global__ __launch_bounds__(kThreads) void fwd_kernel(Args a, Out o, int nq, int nk) {
-    constexpr int U = sizeof(T) == 2 ? 4 : 2;   // heads in flight
-    const int c = threadIdx.x % LANES, half = a.D / 2;
-    const int64_t j = static_cast<int64_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
-    const bool work = j < a.tokens * (nq + nk), lane_on = work && 8 * c < half;
-    Job jb = job_at(a, work ? j : 0, nq, nk);
-    const int64_t b = jb.token / a.L, l = jb.token - b * a.L;
-    const int H = jb.is_k ? a.Hkv : a.Hq;
-    const int64_t* st = jb.is_k ? a.ks : a.qs;
-    const T* src = static_cast<const T*>(jb.is_k ? a.k : a.q) + b * st[0] + l * st[1] + 8 * c;
-    T* dst = static_cast<T*>(jb.is_k ? o.k : o.q) + jb.token * H * a.D + 8 * c;
-    A cs[8], sn[8], w[16];
-    if (lane_on) {
-        turn_at<A>(a, a.pos ? __ldg(a.pos + jb.token) : l, c, ADJ, cs, sn);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            w[i] = weight_at<A>(jb.is_k ? a.wk : a.wq, a.w_dtype,
-                                (i < 8 ? 0 : half - 8) + 8 * c + i);
+    __device__ __forceinline__ Share(const Args& a, int q_blocks, int groups) {
+        const int block = static_cast<int>(blockIdx.x);
+        is_k = block >= q_blocks;
+        H = is_k ? a.Hkv : a.Hq;
+        per = a.per;
+        L = a.L;
+        chunks = (H + per - 1) / per;
+        s0 = is_k ? a.ks[0] : a.qs[0];
+        s1 = is_k ? a.ks[1] : a.qs[1];
+        s2 = is_k ? a.ks[2] : a.qs[2];
+        jobs = a.tokens * chunks;
+        first = static_cast<int64_t>(is_k ? block - q_blocks : block) * groups;
+        step = static_cast<int64_t>(is_k ? static_cast<int>(gridDim.x) - q_blocks : q_blocks) * groups;
+        src = static_cast<const T*>(is_k ? a.k : a.q);
     }
-    // all lanes of a warp take part in the exchanges: the trip count is `per`
-    for (int h0 = jb.h0; h0 < jb.h0 + a.per; h0 += U) {
-        Raw<T> rx[U], ry[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (lane_on && h0 + u < jb.h1) {
-                rx[u] = load8<T>(src + (h0 + u) * st[2]);
-                ry[u] = load8<T>(src + (h0 + u) * st[2] + half);
-            }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool on = lane_on && h0 + u < jb.h1;
-            A x[8], y[8], sq = 0;
-            if (on) {
-                unpack<T>(rx[u], x);
-                unpack<T>(ry[u], y);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sq += x[i] * x[i] + y[i] * y[i];
-            }
-            sq = group_sum<A, LANES>(sq);
-            if (!on) continue;
-            const A r = rsqrt_<A>(sq / a.D + static_cast<A>(a.eps));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] *= r * w[i];
-                y[i] *= r * w[8 + i];
-            }
-            turn<A, ADJ, false>(x, y, cs, sn);
-            T* d = dst + static_cast<int64_t>(h0 + u) * a.D;
-            store8<T>(d, x);
-            store8<T>(d + half, y);
+};
+// Heads [h, end) of a token: x in place, the contiguous tensors at row token H + h.
+// Where there is no such head (past a job, past the jobs) reads take the job's first one
+// or that of token 0, so that no load waits for a branch; nothing is written then.
+template <typename T> struct Spot {
+    const T* x;
+    int64_t row, token;
+    int left;   // heads from here on
+
+    __device__ __forceinline__ Spot(const Share<T>& s, int64_t j) {
+        const bool on = j < s.jobs;
+        token = on ? static_cast<int64_t>(static_cast<uint64_t>(j) / static_cast<unsigned>(s.chunks)) : 0;
+        const int h = on ? static_cast<int>(j - token * s.chunks) * s.per : 0;
+        left = on ? min(s.per, s.H - h) : 0;
+        const int64_t b = token / s.L;
+        x = s.src + b * s.s0 + (token - b * s.L) * s.s1 + h * s.s2;
+        row = token * s.H + h;
+    }
+    __device__ __forceinline__ Spot after(const Share<T>& s, int n) const {
+        Spot r = *this;
+        r.left = left - n;
+        if (r.left > 0) {
+            r.x += n * s.s2;
+            r.row += n;
         }
+        return r;
     }
+};
+__device__ __forceinline__ int64_t position(const Args& a, int64_t token) {
+    return a.pos ? __ldg(a.pos + token) : token % a.L;
 }
 
-// Blocks [0, q_blocks) pass over q, the others over k, so that a thread holds the
-// weight sums of one of them.
-template <typename T, typename A, int LANES, bool ADJ>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void bwd_kernel(Args a, Grad g,
-                                                                              int q_blocks) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    constexpr int GROUPS = kThreads / LANES;
-    constexpr int U = 2;
-    const int c = threadIdx.x % LANES, half = a.D / 2;
-    const bool is_k = static_cast<int>(blockIdx.x) >= q_blocks, lane_in = 8 * c < half;
-    const int H = is_k ? a.Hkv : a.Hq, chunks = (H + a.per - 1) / a.per;
-    const int64_t s0 = is_k ? a.ks[0] : a.qs[0], s1 = is_k ? a.ks[1] : a.qs[1];
-    const int64_t s2 = is_k ? a.ks[2] : a.qs[2];
-    const T* src = static_cast<const T*>(is_k ? a.k : a.q) + 8 * c;
-    const T* gsrc = static_cast<const T*>(is_k ? g.gk : g.gq) + 8 * c;
-    T* dst = static_cast<T*>(is_k ? g.dk : g.dq) + 8 * c;
-    A dw[16], w[16];
+// Weights of a lane's pairs, kept as fp32 in shared memory.
+template <int V, bool ADJ>
+__device__ __forceinline__ Pairs<V> weights_at(const float* w, int c, int half) {
+    float x[V], y[V];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        dw[i] = 0;
-        w[i] = lane_in ? weight_at<A>(is_k ? a.wk : a.wq, a.w_dtype, (i < 8 ? 0 : half - 8) + 8 * c + i)
-                       : A(0);
+    for (int i = 0; i < V; ++i) {
+        x[i] = w[V * c + i];
+        y[i] = w[half + V * c + i];
     }
-    const int first = is_k ? static_cast<int>(blockIdx.x) - q_blocks : static_cast<int>(blockIdx.x);
-    const int blocks = is_k ? static_cast<int>(gridDim.x) - q_blocks : q_blocks;
-    const int64_t jobs = a.tokens * chunks, step = static_cast<int64_t>(blocks) * GROUPS;
-    const A inv_d = A(1) / a.D;
+    return pairs_of<V, ADJ>(x, y);
+}
+
+constexpr int kWidest = 512;
+
+template <typename T, int LANES, int V, bool ADJ>
+__global__ __launch_bounds__(kThreads, V == 8 ? 1 : kFwdPerSm) void fwd_kernel(Args a, Out o, int q_blocks) {
+    // U heads in flight, two of them worked on at a time
+    constexpr int GROUPS = kThreads / LANES, U = sizeof(T) == 2 ? kAhead : 2, P = V / 2;
+    __shared__ __align__(16) float w[kWidest];
+    const int half = a.D / 2;
+    const bool lane_in = V * (threadIdx.x % LANES) < half;
+    const int c = lane_in ? threadIdx.x % LANES : 0;
+    const Share<T> s(a, q_blocks, GROUPS);
+    T* dst = static_cast<T*>(s.is_k ? o.k : o.q) + V * c;
+    int64_t j = s.first + threadIdx.x / LANES;
+    Spot<T> at(s, j);
+    Raw<T, V> rx[U], ry[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const T* x = at.x + (u < at.left ? u : 0) * s.s2 + V * c;
+        rx[u] = load<V>(x);
+        ry[u] = load<V>(x + half);
+    }
+    Angles<V> turn = angles_at<V, ADJ>(a, position(a, at.token), c);
+    for (int d = threadIdx.x; d < a.D; d += kThreads)
+        w[d] = weight_at<float>(s.is_k ? a.wk : a.wq, a.w_dtype, d);
+    __syncthreads();
+    const float inv_d = 1.f / a.D, eps = static_cast<float>(a.eps);
     // all lanes of the block make the same number of rounds
-    for (int64_t j0 = static_cast<int64_t>(first) * GROUPS; j0 < jobs; j0 += step) {
-        const int64_t j = j0 + threadIdx.x / LANES;
-        const bool lane_on = j < jobs && lane_in;
-        const int64_t token = j < jobs ? j / chunks : 0;
-        const int h_first = j < jobs ? static_cast<int>(j - token * chunks) * a.per : 0;
-        const int h_end = min(h_first + a.per, H);
-        const int64_t b = token / a.L, l = token - b * a.L;
-        const T* x_at = src + b * s0 + l * s1;
-        const int64_t row0 = token * H;
-        A cs[8], sn[8];
-        if (lane_on) turn_at<A>(a, a.pos ? __ldg(a.pos + token) : l, c, ADJ, cs, sn);
-        for (int h0 = h_first; h0 < h_first + a.per; h0 += U) {
-            Raw<T> rx[U], ry[U], rg[U], ri[U];
+    for (int64_t j0 = s.first; j0 < s.jobs; j0 += s.step) {
+        // the weights go into the cosines and sines of a token
+        float2 uc[P], us[P], vc[P], vs[P];
+        const Pairs<V> wp = weights_at<V, ADJ>(w, c, half);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (lane_on && h0 + u < h_end) {
-                    rx[u] = load8<T>(x_at + (h0 + u) * s2);
-                    ry[u] = load8<T>(x_at + (h0 + u) * s2 + half);
-                    rg[u] = load8<T>(gsrc + (row0 + h0 + u) * a.D);
-                    ri[u] = load8<T>(gsrc + (row0 + h0 + u) * a.D + half);
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const bool on = lane_on && h0 + u < h_end;
-                A x[8], y[8], p[8], q[8], sq = 0, dot = 0;
-                if (on) {
-                    unpack<T>(rx[u], x);
-                    unpack<T>(ry[u], y);
-                    unpack<T>(rg[u], p);
-                    unpack<T>(ri[u], q);
-                    turn<A, ADJ, true>(p, q, cs, sn);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        sq += x[i] * x[i] + y[i] * y[i];
-                        dot += p[i] * w[i] * x[i] + q[i] * w[8 + i] * y[i];
-                    }
-                }
-                sq = group_sum<A, LANES>(sq);
-                dot = group_sum<A, LANES>(dot);
-                if (!on) continue;
-                const A r = rsqrt_<A>(sq * inv_d + static_cast<A>(a.eps));
-                const A f = r * r * r * dot * inv_d;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] *= r;
-                    q[i] *= r;
-                    dw[i] += p[i] * x[i];
-                    dw[8 + i] += q[i] * y[i];
-                    x[i] = p[i] * w[i] - x[i] * f;
-                    y[i] = q[i] * w[8 + i] - y[i] * f;
-                }
-                T* d = dst + (row0 + h0 + u) * a.D;
-                store8<T>(d, x);
-                store8<T>(d + half, y);
-            }
+        for (int i = 0; i < P; ++i) {
+            uc[i] = __fmul2_rn(wp.u[i], turn.c[i]);
+            us[i] = __fmul2_rn(wp.u[i], turn.s[i]);
+            vc[i] = __fmul2_rn(wp.v[i], turn.c[i]);
+            vs[i] = neg(__fmul2_rn(wp.v[i], turn.s[i]));
         }
+        j += s.step;
+        const Spot<T> next(s, j);
+        turn = angles_at<V, ADJ>(a, position(a, next.token), c);
+        for (int r = 0; r < s.per; r += U) {
+            const Spot<T> then = r + U >= s.per ? next : at.after(s, U);
+#pragma unroll
+            for (int u0 = 0; u0 < U; u0 += 2) {
+                Pairs<V> x[2];
+                float sq[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int u = u0 + k;
+                    x[k] = unpack<ADJ>(rx[u], ry[u]);
+                    const T* from = then.x + (u < then.left ? u : 0) * s.s2 + V * c;
+                    rx[u] = load<V>(from);
+                    ry[u] = load<V>(from + half);
+                    float2 q = __fmul2_rn(x[k].u[0], x[k].u[0]);
+                    q = __ffma2_rn(x[k].v[0], x[k].v[0], q);
+#pragma unroll
+                    for (int i = 1; i < P; ++i) {
+                        q = __ffma2_rn(x[k].u[i], x[k].u[i], q);
+                        q = __ffma2_rn(x[k].v[i], x[k].v[i], q);
+                    }
+                    sq[k] = lane_in ? q.x + q.y : 0.f;
+                }
+                group_sums<LANES>(sq);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float2 rn = twice(rsqrtf(sq[k] * inv_d + eps));
+                    Pairs<V> y;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const float2 p = __fmul2_rn(x[k].u[i], rn), q = __fmul2_rn(x[k].v[i], rn);
+                        y.u[i] = __ffma2_rn(p, uc[i], __fmul2_rn(q, vs[i]));
+                        y.v[i] = __ffma2_rn(p, us[i], __fmul2_rn(q, vc[i]));
+                    }
+                    if (lane_in && u0 + k < at.left)
+                        store<ADJ>(dst + (at.row + u0 + k) * a.D, half, y);
+                }
+            }
+            at = then;
+        }
+    }
+}
+
+template <typename T, int LANES, int V, bool ADJ>
+__global__ __launch_bounds__(kThreads, V == 8 ? 1 : kBwdPerSm) void bwd_kernel(Args a, Grad g, int q_blocks) {
+    constexpr int GROUPS = kThreads / LANES, U = sizeof(T) == 2 ? kAhead : 2, P = V / 2;
+    constexpr int WARPS = kThreads / 32;
+    __shared__ __align__(16) float w[kWidest];
+    __shared__ float sums[WARPS][2 * V * LANES];
+    const int half = a.D / 2;
+    const bool lane_in = V * (threadIdx.x % LANES) < half;
+    const int c = lane_in ? threadIdx.x % LANES : 0;
+    const Share<T> s(a, q_blocks, GROUPS);
+    const T* gsrc = static_cast<const T*>(s.is_k ? g.gk : g.gq) + V * c;
+    T* dst = static_cast<T*>(s.is_k ? g.dk : g.dq) + V * c;
+    int64_t j = s.first + threadIdx.x / LANES;
+    Spot<T> at(s, j);
+    Raw<T, V> rx[U], ry[U], rg[U], ri[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int h = u < at.left ? u : 0;
+        const T *x = at.x + h * s.s2 + V * c, *y = gsrc + (at.row + h) * a.D;
+        rx[u] = load<V>(x);
+        ry[u] = load<V>(x + half);
+        rg[u] = load<V>(y);
+        ri[u] = load<V>(y + half);
+    }
+    Angles<V> turn = angles_at<V, ADJ>(a, position(a, at.token), c);
+    for (int d = threadIdx.x; d < a.D; d += kThreads)
+        w[d] = weight_at<float>(s.is_k ? a.wk : a.wq, a.w_dtype, d);
+    __syncthreads();
+    const Pairs<V> wp = weights_at<V, ADJ>(w, c, half);
+    Pairs<V> dw;
+#pragma unroll
+    for (int i = 0; i < P; ++i) dw.u[i] = dw.v[i] = twice(0.f);
+    const float inv_d = 1.f / a.D, eps = static_cast<float>(a.eps);
+    for (int64_t j0 = s.first; j0 < s.jobs; j0 += s.step) {
+        j += s.step;
+        const Spot<T> next(s, j);
+        const Angles<V> turn_next = angles_at<V, ADJ>(a, position(a, next.token), c);
+        for (int r = 0; r < s.per; r += U) {
+            const Spot<T> then = r + U >= s.per ? next : at.after(s, U);
+#pragma unroll
+            for (int u0 = 0; u0 < U; u0 += 2) {
+                Pairs<V> x[2], h[2];
+                float part[4];   // of both heads: squares, then products
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int u = u0 + k;
+                    x[k] = unpack<ADJ>(rx[u], ry[u]);
+                    const Pairs<V> y = unpack<ADJ>(rg[u], ri[u]);
+                    const int hd = u < then.left ? u : 0;
+                    const T *from = then.x + hd * s.s2 + V * c, *gfrom = gsrc + (then.row + hd) * a.D;
+                    rx[u] = load<V>(from);
+                    ry[u] = load<V>(from + half);
+                    rg[u] = load<V>(gfrom);
+                    ri[u] = load<V>(gfrom + half);
+                    float2 q = twice(0.f), dot = twice(0.f);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        q = __ffma2_rn(x[k].u[i], x[k].u[i], q);
+                        q = __ffma2_rn(x[k].v[i], x[k].v[i], q);
+                        // turned back
+                        h[k].u[i] = __ffma2_rn(y.u[i], turn.c[i], __fmul2_rn(y.v[i], turn.s[i]));
+                        h[k].v[i] = __ffma2_rn(y.v[i], turn.c[i], __fmul2_rn(y.u[i], neg(turn.s[i])));
+                        dot = __ffma2_rn(__fmul2_rn(h[k].u[i], wp.u[i]), x[k].u[i], dot);
+                        dot = __ffma2_rn(__fmul2_rn(h[k].v[i], wp.v[i]), x[k].v[i], dot);
+                    }
+                    part[k] = lane_in ? q.x + q.y : 0.f;
+                    part[2 + k] = lane_in ? dot.x + dot.y : 0.f;
+                }
+                group_sums<LANES>(part);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (!lane_in || u0 + k >= at.left) continue;
+                    const float rn = rsqrtf(part[k] * inv_d + eps);
+                    const float2 r2 = twice(rn), f = twice(-rn * rn * rn * part[2 + k] * inv_d);
+                    Pairs<V> dx;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const float2 p = __fmul2_rn(h[k].u[i], r2), q = __fmul2_rn(h[k].v[i], r2);
+                        dw.u[i] = __ffma2_rn(p, x[k].u[i], dw.u[i]);
+                        dw.v[i] = __ffma2_rn(q, x[k].v[i], dw.v[i]);
+                        dx.u[i] = __ffma2_rn(p, wp.u[i], __fmul2_rn(x[k].u[i], f));
+                        dx.v[i] = __ffma2_rn(q, wp.v[i], __fmul2_rn(x[k].v[i], f));
+                    }
+                    store<ADJ>(dst + (at.row + u0 + k) * a.D, half, dx);
+                }
+            }
+            at = then;
+        }
+        turn = turn_next;
     }
     if (!g.want_w) return;
     // groups of a warp, then the warps, in a fixed order
-    A* sh = reinterpret_cast<A*>(smem_raw);   // [warps][16 * LANES]
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        A v = dw[i];
+    for (int i = 0; i < 2 * V; ++i) {
+        const float2 t = i < V ? dw.u[i / 2] : dw.v[(i - V) / 2];
+        float v = i % 2 ? t.y : t.x;
 #pragma unroll
         for (int m = LANES; m < 32; m <<= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-        if (lane < LANES) sh[warp * 16 * LANES + (i < 8 ? 0 : 8 * LANES) + 8 * c + (i & 7)] = v;
+        if (lane < LANES) sums[warp][i * LANES + lane] = v;
     }
     __syncthreads();
     for (int d = threadIdx.x; d < a.D; d += kThreads) {
-        const int at = d < half ? d : 8 * LANES + d - half;
-        A v = 0;
-        for (int k = 0; k < kThreads / 32; ++k) v += sh[k * 16 * LANES + at];
-        static_cast<A*>(g.part)[static_cast<int64_t>(blockIdx.x) * a.D + d] = v;
+        const int e = d < half ? d : d - half, in = e % V;   // channel of a lane's x or y
+        const int i = ADJ ? (in % 2 ? V : 0) + (d < half ? 0 : V / 2) + in / 2 : (d < half ? 0 : V) + in;
+        float v = 0;
+        for (int k = 0; k < WARPS; ++k) v += sums[k][i * LANES + e / V];
+        static_cast<float*>(g.part)[static_cast<int64_t>(blockIdx.x) * a.D + d] = v;
     }
 }
 
@@ -445,20 +592,21 @@ Args args(const nsc_norm_rotate* a) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Whether 16-byte accesses of whole chunks serve this call.
+// Whether accesses of whole chunks serve this call.
 bool wide(const nsc_norm_rotate* a) {
     const int64_t es = dtype_size(a->dtype);
     // (fp64 would spill its two chunks; it takes the other kernel)
-    bool w = a->dtype != NSC_F64 && a->D % 16 == 0 && a->rot_dim == a->D && a->rows > 0 && aligned16(a->q) &&
+    bool w = a->dtype != NSC_F64 && a->D % 8 == 0 && (a->D <= 256 || a->D % 16 == 0) && a->rot_dim == a->D && a->rows > 0 && aligned16(a->q) &&
              aligned16(a->k);
     for (int i = 0; i < 3; ++i)
         w = w && a->q_stride[i] * es % 16 == 0 && a->k_stride[i] * es % 16 == 0;
     return w;
 }
 
+// (two chunks of four channels a lane, past 256 channels of eight)
 int lanes_for(int D) {
     int n = 1;
-    while (n * 16 < D) n <<= 1;
+    while (n * 8 < D && n < 32) n <<= 1;
     return n;
 }
 
@@ -474,33 +622,30 @@ int heads_per_job(const Args& a, int lanes) {
     return per;
 }
 
-template <typename T, typename A, int LANES>
+template <typename T, int LANES, int V = 4>
 nsc_status run_wide(Args a, const Out* o, const Grad* g, int* n_part, cudaStream_t st) {
     a.per = heads_per_job(a, LANES);
     const int nq = (a.Hq + a.per - 1) / a.per, nk = (a.Hkv + a.per - 1) / a.per;
-    const int64_t jobs = a.tokens * (nq + nk);
-    const int64_t blocks = (jobs + kThreads / LANES - 1) / (kThreads / LANES);
-    if (o) {
-        if (blocks >= (1LL << 31)) return fail(NSC_ERR_INVALID_ARG, "qk_norm_rotate: too many tokens");
-        const unsigned n = static_cast<unsigned>(blocks);
-        if (a.adjacent) fwd_kernel<T, A, LANES, true><<<n, kThreads, 0, st>>>(a, *o, nq, nk);
-        else fwd_kernel<T, A, LANES, false><<<n, kThreads, 0, st>>>(a, *o, nq, nk);
-        return check_launch("qk_norm_rotate");
-    }
-    // blocks of q and of k in the ratio of their work, two rounds an SM at most
+    // blocks of q and of k in the ratio of their work, as many as are resident at most
     constexpr int groups = kThreads / LANES;
+    const int64_t most = 148 * (V == 8 ? 1 : o ? kFwdPerSm : kBwdPerSm);
     int64_t bq = (a.tokens * nq + groups - 1) / groups, bk = (a.tokens * nk + groups - 1) / groups;
-    if (bq + bk > kMaxPart) {
+    if (bq + bk > most) {
         const int64_t all = static_cast<int64_t>(a.Hq) + a.Hkv;
-        bk = a.Hkv ? (kMaxPart * static_cast<int64_t>(a.Hkv) + all - 1) / all : 0;
-        bq = kMaxPart - bk;
-        if (a.Hq && bq < 1) { bq = 1; bk = kMaxPart - 1; }
+        bk = a.Hkv ? (most * static_cast<int64_t>(a.Hkv) + all - 1) / all : 0;
+        bq = most - bk;
+        if (a.Hq && bq < 1) { bq = 1; bk = most - 1; }
+    }
+    const unsigned blocks = static_cast<unsigned>(bq + bk);
+    if (o) {
+        auto kern = a.adjacent ? fwd_kernel<T, LANES, V, true> : fwd_kernel<T, LANES, V, false>;
+        kern<<<blocks, kThreads, 0, st>>>(a, *o, static_cast<int>(bq));
+        return check_launch("qk_norm_rotate");
     }
     n_part[0] = static_cast<int>(bq);
     n_part[1] = static_cast<int>(bq + bk);
-    const size_t smem = sizeof(A) * (kThreads / 32) * 16 * LANES;
-    auto kern = a.adjacent ? bwd_kernel<T, A, LANES, true> : bwd_kernel<T, A, LANES, false>;
-    kern<<<n_part[1], kThreads, smem, st>>>(a, *g, n_part[0]);
+    auto kern = a.adjacent ? bwd_kernel<T, LANES, V, true> : bwd_kernel<T, LANES, V, false>;
+    kern<<<blocks, kThreads, 0, st>>>(a, *g, n_part[0]);
     return check_launch("qk_norm_rotate backward");
 }
 
@@ -510,12 +655,14 @@ nsc_status run(const nsc_norm_rotate* n, const Out* o, const Grad* g, int* n_par
     Args a = args(n);
     if constexpr (sizeof(T) < 8) if (wide(n)) {
         switch (lanes_for(a.D)) {
-            case 1: return run_wide<T, A, 1>(a, o, g, n_part, st);
-            case 2: return run_wide<T, A, 2>(a, o, g, n_part, st);
-            case 4: return run_wide<T, A, 4>(a, o, g, n_part, st);
-            case 8: return run_wide<T, A, 8>(a, o, g, n_part, st);
-            case 16: return run_wide<T, A, 16>(a, o, g, n_part, st);
-            default: return run_wide<T, A, 32>(a, o, g, n_part, st);
+            case 1: return run_wide<T, 1>(a, o, g, n_part, st);
+            case 2: return run_wide<T, 2>(a, o, g, n_part, st);
+            case 4: return run_wide<T, 4>(a, o, g, n_part, st);
+            case 8: return run_wide<T, 8>(a, o, g, n_part, st);
+            case 16: return run_wide<T, 16>(a, o, g, n_part, st);
+            default:
+                return a.D <= 256 ? run_wide<T, 32>(a, o, g, n_part, st)
+                                  : run_wide<T, 32, 8>(a, o, g, n_part, st);
         }
     }
     const int warps = kThreads / 32;
