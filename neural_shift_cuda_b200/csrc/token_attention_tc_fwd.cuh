@@ -43,7 +43,7 @@ namespace nsc {
 namespace tok {
 namespace {
 
-constexpr int kFwdThreads = 384;
+constexpr int kFwdThreads = 256, kFwdMathRegs = 176, kFwdOtherRegs = 80;
 constexpr float kLazy = 8.f;
 
 constexpr int kKeys = 64;   // keys of a block
@@ -51,22 +51,20 @@ constexpr int kKeys = 64;   // keys of a block
 template <int DP> struct FwdShape {
     static constexpr int tile = DP / 64 * kPanel;                  // bytes of a query tile
     static constexpr int panel = kKeys * 128, block = DP / 64 * panel;   // of a K or V block
-    static constexpr int stages = DP == 64 ? 6 : 4;                // K and V blocks in flight
-    static constexpr int smem = 2 * tile + stages * 2 * block;     // + bias + 1024 of alignment
+    static constexpr int stages = DP == 64 ? 5 : 2;                // K and V blocks in flight
+    static constexpr int smem = tile + stages * 2 * block;         // + bias + 1024 of alignment
 };
 
 struct FwdBars {
-    // (two of s_full and p_full of a tile, for even and odd blocks: the products, and a
-    // fast warp, may be a block ahead of a slow warp)
-    uint64_t q, k_full[6], v_full[6], empty[6], ok[6], s_full[2][2], p_full[2][2], pv[2], o_full[2];
-    uint64_t drain[2];
-    uint64_t turn[4][2];   // of a scheduler: its warp of a tile may use the exponential unit
+    // (two of s_full and p_full, for even and odd blocks: the products, and a fast warp,
+    // may be a block ahead of a slow warp)
+    uint64_t q, k_full[5], v_full[5], k_empty[5], v_empty[5], ok[5], s_full[2], p_full[2], pv, o_full, drain;
 };
 
 template <typename T, int DP, bool CAP, bool BIAS, bool REST>
-__global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
+__global__ __launch_bounds__(kFwdThreads, 2) void tc_fwd_kernel(
     const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-    const __grid_constant__ CUtensorMap mv, const Params p, const int pair, const Bounded bnd) {
+    const __grid_constant__ CUtensorMap mv, const Params p, const Bounded bnd) {
     using S = FwdShape<DP>;
     constexpr int NS = S::stages;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -74,56 +72,49 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     __shared__ FwdBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag[2];
-    __shared__ int span[2][4];   // of a tile: least lo, most hi, most lo, least hi
+    __shared__ int span[4];   // of the rows: least lo, most hi, most lo, least hi
     unsigned char* smem = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    unsigned char* Qs = smem;                       // two tiles
-    unsigned char* KV = smem + 2 * S::tile;         // stages of K, V
+    unsigned char* Qs = smem;
+    unsigned char* KV = smem + S::tile;             // stages of K, V
     float* E = reinterpret_cast<float*>(smem + S::smem);
 
     const int warp = tc::uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    // pair: tiles are heads h, h + 1 of one row block; else 256 rows of a head
-    const int HH = pair ? p.Hq / 2 : p.Hq;
-    const int64_t BH = static_cast<int64_t>(p.B) * HH;
+    const int64_t BH = static_cast<int64_t>(p.B) * p.Hq;
     const int nt = gridDim.x / BH;
-    const int t = nt - 1 - static_cast<int>(blockIdx.x / BH);
-    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / HH, h0 = (bh % HH) * (pair ? 2 : 1);
-    const int hk = h0 / p.G, n = keys_of(p, b);
-    const int q0 = t * (pair ? kRows : 2 * kRows);
+    const int t = nt - 1 - static_cast<int>(blockIdx.x / BH);   // (causal: the longest first)
+    const int bh = static_cast<int>(blockIdx.x % BH), b = bh / p.Hq, h = bh % p.Hq;
+    const int hk = h / p.G, n = keys_of(p, b);
+    const int q0 = t * kRows;
 
-    if (threadIdx.x < 8) span[threadIdx.x >> 2][threadIdx.x & 3] =
-        (threadIdx.x & 3) == 0 || (threadIdx.x & 3) == 3 ? INT_MAX : 0;
+    if (threadIdx.x < 4) span[threadIdx.x] = threadIdx.x == 0 || threadIdx.x == 3 ? INT_MAX : 0;
     if (threadIdx.x == 0) {
         mbar_init(&bars.q, 1);
         for (int i = 0; i < NS; ++i) {
             mbar_init(&bars.k_full[i], 1);
             mbar_init(&bars.v_full[i], 1);
-            mbar_init(&bars.empty[i], 2);
+            mbar_init(&bars.k_empty[i], 1);
+            mbar_init(&bars.v_empty[i], 1);
             mbar_init(&bars.ok[i], 32);
         }
         for (int i = 0; i < 2; ++i) {
-            for (int y = 0; y < 2; ++y) {
-                mbar_init(&bars.s_full[i][y], 1);
-                mbar_init(&bars.p_full[i][y], kRows);
-            }
-            mbar_init(&bars.pv[i], 1);
-            mbar_init(&bars.o_full[i], 1);
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_full[i], kRows);
         }
-        for (int i = 0; i < 8; ++i) mbar_init(&bars.turn[i >> 1][i & 1], 1);
-        mbar_init(&bars.drain[0], 1);
-        mbar_init(&bars.drain[1], 1);
+        mbar_init(&bars.pv, 1);
+        mbar_init(&bars.o_full, 1);
+        mbar_init(&bars.drain, 1);
         fence_mbar_init();
         abort_flag[0] = 0;
         abort_flag[1] = static_cast<int>(bnd.budget);
     }
-    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    if (warp == 5) tc::tmem_alloc(&tmem_slot, 256);
     __syncthreads();
 
-    // the rows' spans, and those of the tiles
-    const int a = warp >> 2;   // tile of a softmax warp
-    const int row = q0 + (pair ? 0 : a * kRows) + static_cast<int>(threadIdx.x & 127);
+    // the rows' spans, and the tile's
+    const int row = q0 + static_cast<int>(threadIdx.x & 127);
     int lo = 0, hi = 0;
-    if (warp < 8) {
+    if (warp < 4) {
         if (row < p.Lq) key_span(p, b, row, n, lo, hi);
         int v0 = hi > lo ? lo : INT_MAX, v1 = hi > lo ? hi : 0;
         int v2 = hi > lo ? lo : 0, v3 = hi > lo ? hi : INT_MAX;
@@ -132,35 +123,20 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         v2 = __reduce_max_sync(0xffffffffu, v2);
         v3 = __reduce_min_sync(0xffffffffu, v3);
         if (lane == 0) {
-            atomicMin(&span[a][0], v0);
-            atomicMax(&span[a][1], v1);
-            atomicMax(&span[a][2], v2);
-            atomicMin(&span[a][3], v3);
+            atomicMin(&span[0], v0);
+            atomicMax(&span[1], v1);
+            atomicMax(&span[2], v2);
+            atomicMin(&span[3], v3);
         }
     }
-    if (BIAS) load_padded_bias(p, h0, E, threadIdx.x, kFwdThreads);
-    if (BIAS && pair)
-        load_padded_bias(p, h0 + 1, E + 2 * p.reach + 2 * kBiasPad + 1, threadIdx.x, kFwdThreads);
+    if (BIAS) load_padded_bias(p, h, E, threadIdx.x, kFwdThreads);
     __syncthreads();
     const uint32_t tmem = tc::uniform(tmem_slot);
-    int fb[2], lb[2];          // key blocks [fb, lb) of a tile
-    int all_lo[2], all_hi[2];  // keys that all its rows see
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int s0 = tc::uniform(span[i][0]), s1 = tc::uniform(span[i][1]);
-        all_lo[i] = tc::uniform(span[i][2]);
-        all_hi[i] = tc::uniform(span[i][3]);
-        fb[i] = s1 > s0 ? s0 / kKeys : INT_MAX;
-        lb[i] = s1 > s0 ? (s1 + kKeys - 1) / kKeys : 0;
-    }
-    const int j0 = min(fb[0], fb[1]), j1 = max(lb[0], lb[1]);
-    auto on = [&](int i, int j) { return j >= fb[i] && j < lb[i]; };
+    const int s0 = tc::uniform(span[0]), s1 = tc::uniform(span[1]);
+    const int all_lo = tc::uniform(span[2]), all_hi = tc::uniform(span[3]);   // keys that all rows see
+    const int j0 = s1 > s0 ? s0 / kKeys : 0, j1 = s1 > s0 ? (s1 + kKeys - 1) / kKeys : 0;   // key blocks
     auto guarded = [&](int j) {
-        bool g = false;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            g |= on(i, j) && !(j * kKeys >= all_lo[i] && min((j + 1) * kKeys, n) <= all_hi[i]);
-        return g;
+        return !(j * kKeys >= all_lo && min((j + 1) * kKeys, n) <= all_hi);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         return wait_bounded(bar, parity, bnd.timeouts, abort_flag);
@@ -170,25 +146,22 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
     const int steps = (p.D + 15) / 16;   // of 16 channels
     const int cols = steps * 16;
 
-    if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (warp < 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwdMathRegs));
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t to = tmem + 256 + a * DP + lane_base;
-        const int h = h0 + (pair ? a : 0);
+        const uint32_t to = tmem + 128 + lane_base;
         const int pos = row + n - p.Lq;
-        const float* Eh = E + (pair && a ? 2 * p.reach + 2 * kBiasPad + 1 : 0);
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
-        const int turns = max(0, min(lb[0] - fb[0], lb[1] - fb[1]));   // (fb may be INT_MAX)
         const Cap<T> cap(y1, unit);
         float m = -INFINITY, l = 0.f;
         bool alive = true;
         int it = 0;
-        for (int j = fb[a]; j < lb[a]; ++j, ++it) {
-            alive = __all_sync(0xffffffffu, wait(&bars.s_full[a][it & 1], (it >> 1) & 1));
+        for (int j = j0; j < j1; ++j, ++it) {
+            alive = __all_sync(0xffffffffu, wait(&bars.s_full[it & 1], (it >> 1) & 1));
             if (!alive) break;
             tc::fence_after();
-            const uint32_t ts = tmem + lane_base + a * 128 + (it & 1) * kKeys;
+            const uint32_t ts = tmem + lane_base + (it & 1) * kKeys;
             float2 s[32];
             tc::load32(ts, reinterpret_cast<float*>(s));
             tc::load32(ts + 32, reinterpret_cast<float*>(s + 16));
@@ -203,12 +176,12 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 const int w0 = __shfl_sync(0xffffffffu, pos, 0);   // lanes at w0 .. w0 + 31
                 const float2 u2 = CAP ? make_float2(1.f, 1.f) : make_float2(unit, unit);
                 if (k0 + kKeys - 1 - w0 <= -p.reach || k0 - w0 - 31 >= p.reach) {
-                    const float e = Eh[k0 > w0 ? 2 * p.reach + kBiasPad : kBiasPad];
+                    const float e = E[k0 > w0 ? 2 * p.reach + kBiasPad : kBiasPad];
                     const float2 e2 = make_float2(e, e);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[i] = __ffma2_rn(s[i], u2, e2);
                 } else {
-                    const float* er = Eh + (k0 - pos + p.reach + kBiasPad);
+                    const float* er = E + (k0 - pos + p.reach + kBiasPad);
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         s[i] = __ffma2_rn(s[i], u2, make_float2(er[2 * i], er[2 * i + 1]));
@@ -237,7 +210,7 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             }
             if (it > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
                 // (PV of the last block is done, and this one's has not begun)
-                alive = __all_sync(0xffffffffu, wait(&bars.pv[a], (it - 1) & 1));
+                alive = __all_sync(0xffffffffu, wait(&bars.pv, (it - 1) & 1));
                 if (!alive) break;
                 tc::fence_after();
                 l *= keep;
@@ -251,12 +224,6 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                     for (int i = 0; i < 8; ++i) o[i] = __fmul2_rn(o[i], k2);
                     tc::store16(to + c, reinterpret_cast<uint32_t*>(o));
                 }
-            }
-            // The two warps of a scheduler take turns at the exponentials: side by side both
-            // would be slow here, and then both elsewhere with the unit idle.
-            if (it < turns && (a == 1 || it > 0)) {
-                alive = __all_sync(0xffffffffu, wait(&bars.turn[warp & 3][a], (it - 1 + a) & 1));
-                if (!alive) break;
             }
             const float ref = m == -INFINITY ? 0.f : -m;
             const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(ref, ref);
@@ -276,15 +243,14 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 if (REST) tc::store16(ts + 32 + 16 * c, rest);
             }
             const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
-            if (it < turns && lane == 0) mbar_arrive(&bars.turn[warp & 3][1 - a]);
             l += sum.x + sum.y;
             tc::wait_st();
             tc::fence_before();
-            mbar_arrive(&bars.p_full[a][it & 1]);
+            mbar_arrive(&bars.p_full[it & 1]);
         }
         // the row's output
-        const bool worked = lb[a] > fb[a];
-        if (alive && worked) alive = __all_sync(0xffffffffu, wait(&bars.o_full[a], 0));
+        const bool worked = j1 > j0;
+        if (alive && worked) alive = __all_sync(0xffffffffu, wait(&bars.o_full, 0));
         if (alive) {
             tc::fence_after();
             const bool none = l == 0.f;
@@ -323,68 +289,69 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
             tc::fence_before();
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 8 && lane == 0 && j0 < j1) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwdOtherRegs));
+        if (warp == 4 && lane == 0 && j0 < j1) {
             bool alive = true;
             int copies = 0;
-            mbar_arrive_expect_tx(&bars.q, 2 * S::tile);
-            load_rows<DP>(Qs, &mq, &bars.q, h0, q0, b);
-            load_rows<DP>(Qs + S::tile, &mq, &bars.q, pair ? h0 + 1 : h0, pair ? q0 : q0 + kRows, b);
-            int issued = 0;
+            mbar_arrive_expect_tx(&bars.q, S::tile);
+            load_rows<DP>(Qs, &mq, &bars.q, h, q0, b);
+            int issued = 0, k_issued = 0;   // values, keys
             for (int j = j0; j < j1; ++j, ++issued) {
                 const int s = issued % NS;
-                if (issued >= NS) alive = wait(&bars.empty[s], (issued / NS - 1) & 1);
+                if (issued >= NS) alive = wait(&bars.k_empty[s], (issued / NS - 1) & 1);
                 if (!alive) break;
                 mbar_arrive_expect_tx(&bars.k_full[s], S::block);
-                if (copies++ == bnd.skip) { ++issued; break; }
+                ++k_issued;
+                if (copies++ == bnd.skip) break;
                 load_rows<DP, kKeys>(K_at(s), &mk, &bars.k_full[s], hk, j * kKeys, b);
+                if (issued >= NS) alive = wait(&bars.v_empty[s], (issued / NS - 1) & 1);
+                if (!alive) break;
                 mbar_arrive_expect_tx(&bars.v_full[s], S::block);
                 load_rows<DP, kKeys>(V_at(s), &mv, &bars.v_full[s], hk, j * kKeys, b);
             }
             // every copy has landed before the block may end
             mbar_wait32(smem_u32(&bars.q), 0, bnd.timeouts);
-            for (int i = max(0, issued - NS); i < issued; ++i)
-                if (bnd.skip < 0 || i != bnd.skip) {
+            for (int i = max(0, k_issued - NS); i < k_issued; ++i)
+                if (bnd.skip < 0 || i != bnd.skip)
                     mbar_wait32(smem_u32(&bars.k_full[i % NS]), (i / NS) & 1, bnd.timeouts);
-                    mbar_wait32(smem_u32(&bars.v_full[i % NS]), (i / NS) & 1, bnd.timeouts);
-                }
-        } else if ((warp == 9 || warp == 10) && j0 < j1) {
-            const int x = warp - 9;
+            for (int i = max(0, issued - NS); i < issued; ++i)
+                mbar_wait32(smem_u32(&bars.v_full[i % NS]), (i / NS) & 1, bnd.timeouts);
+        } else if (warp == 5 && j0 < j1) {
             const uint32_t iqk = tc::product(kBf16, 128, kKeys, false, false);
             const uint32_t ipv = tc::product(kBf16, 128, cols, false, true);
-            const uint32_t t_s = tmem + x * 128, t_o = tmem + 256 + x * DP;
-            const uint32_t q = smem_u32(Qs + x * S::tile);
-            const int f = tc::uniform(x ? fb[1] : fb[0]), e = tc::uniform(x ? lb[1] : lb[0]);
+            const uint32_t q = smem_u32(Qs);
             const bool lead = tc::elect();
             bool fine = wait(&bars.q, 0);
-            int st = 0, phase = 0, last = 0;   // ring stage of block j + 1 and its phase; of block j
+            int st = 0, phase = 0, last = 0, last_phase = 0;   // ring stage and phase of block j + 1; of j
             for (int j = j0 - 1; j < j1; ++j) {
-                const int n = j + 1 - f, c = j - f;   // blocks of this tile so far
-                if (j + 1 < j1) fine &= wait(&bars.ok[st], phase);
-                if (j + 1 >= f && j + 1 < e) {
+                const int n = j + 1 - j0, c = j - j0;
+                if (j + 1 < j1) {
+                    // (a block that needs no guard: its keys are enough)
+                    fine &= wait(guarded(j + 1) ? &bars.ok[st] : &bars.k_full[st], phase);
                     // S(n) in the place of S and P of the block before last, once PV has read that
-                    if (n > 1) fine &= wait(&bars.pv[x], n & 1);
+                    if (n > 1) fine &= wait(&bars.pv, n & 1);
                     tc::fence_after();
                     if (lead) {
-                        scores_mma<DP, kKeys>(t_s + (n & 1) * kKeys, q, smem_u32(K_at(st)), iqk, steps);
-                        tc::commit(smem_u32(&bars.s_full[x][n & 1]));
+                        scores_mma<DP, kKeys>(tmem + (n & 1) * kKeys, q, smem_u32(K_at(st)), iqk, steps);
+                        tc::commit(smem_u32(&bars.s_full[n & 1]));
+                        tc::commit(smem_u32(&bars.k_empty[st]));
                     }
                 }
                 if (j >= j0) {
-                    if (j >= f && j < e) {
-                        fine &= wait(&bars.p_full[x][c & 1], (c >> 1) & 1);
-                        tc::fence_after();
-                        if (lead) {
-                            const uint32_t w = t_s + (c & 1) * kKeys, v = smem_u32(V_at(last));
-                            mix_mma<4, 4, 0>(t_o, w, v, S::panel, ipv, c > 0);
-                            if (REST) mix_mma<4, 4, 0>(t_o, w + 32, v, S::panel, ipv, true);
-                            tc::commit(smem_u32(&bars.pv[x]));
-                            if (j + 1 == e) tc::commit(smem_u32(&bars.o_full[x]));
-                        }
+                    fine &= wait(&bars.ok[last], last_phase);
+                    fine &= wait(&bars.p_full[c & 1], (c >> 1) & 1);
+                    tc::fence_after();
+                    if (lead) {
+                        const uint32_t w = tmem + (c & 1) * kKeys, v = smem_u32(V_at(last));
+                        mix_mma<4, 4, 0>(tmem + 128, w, v, S::panel, ipv, c > 0);
+                        if (REST) mix_mma<4, 4, 0>(tmem + 128, w + 32, v, S::panel, ipv, true);
+                        tc::commit(smem_u32(&bars.pv));
+                        tc::commit(smem_u32(&bars.v_empty[last]));
+                        if (j + 1 == j1) tc::commit(smem_u32(&bars.o_full));
                     }
-                    if (lead) tc::commit(smem_u32(&bars.empty[last]));
                 }
                 last = st;
+                last_phase = phase;
                 if (++st == NS) {
                     st = 0;
                     phase ^= 1;
@@ -392,18 +359,18 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
                 if (!__all_sync(0xffffffffu, fine)) break;
             }
             if (!__all_sync(0xffffffffu, fine)) {   // the products in flight read this block's memory
-                if (lead) tc::commit(smem_u32(&bars.drain[x]));
-                mbar_wait32(smem_u32(&bars.drain[x]), 0, bnd.timeouts);
+                if (lead) tc::commit(smem_u32(&bars.drain));
+                mbar_wait32(smem_u32(&bars.drain), 0, bnd.timeouts);
             }
-        } else if (warp == 11 && j0 < j1) {
-            // in step with the ring: every block is passed on, after the one before it in
-            // the stage was used up, so no phase of a barrier is taken for another
+        } else if (warp == 7 && j0 < j1) {
+            // Every block is passed on: PV waits for that, so no value block is replaced
+            // before it was looked at, and no phase of a barrier is taken for another.
             int i = 0;
             for (int j = j0; j < j1; ++j, ++i) {
                 const int s = i % NS;
                 const uint32_t parity = (i / NS) & 1;
-                if (i >= NS && !wait(&bars.empty[s], parity ^ 1)) break;
-                if (!wait(&bars.k_full[s], parity) || !wait(&bars.v_full[s], parity)) break;
+                if (!wait(&bars.v_full[s], parity)) break;
+                if (guarded(j) && !wait(&bars.k_full[s], parity)) break;
                 if (guarded(j)) {
                     const uint32_t bad = scrub_rows<T, DP, kKeys>(V_at(s), lane, 32);
 #pragma unroll
@@ -417,9 +384,9 @@ __global__ __launch_bounds__(kFwdThreads, 1) void tc_fwd_kernel(
         __syncwarp();
     }
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 5) {
         tc::fence_after();
-        tc::tmem_free(tmem, 512);
+        tc::tmem_free(tmem, 256);
     }
 }
 
@@ -427,11 +394,9 @@ template <typename T, int DP, bool CAP, bool BIAS, bool REST>
 nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     auto kern = tc_fwd_kernel<T, DP, CAP, BIAS, REST>;
-    const int pair = p.G % 2 == 0;
-    const int smem = FwdShape<DP>::smem + 1024 +
-                     (BIAS ? (pair ? 2 : 1) * 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0);
+    const int smem = FwdShape<DP>::smem + 1024 + (BIAS ? 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0);
     nsc_status ready = tc_ready(reinterpret_cast<const void*>(kern), smem, kFwdThreads,
-                                256 * 208 + 128 * 80);
+                                128 * kFwdMathRegs + 128 * kFwdOtherRegs);
     if (ready != NSC_OK) return ready;
     CUtensorMap mq, mk, mv;
     const char* err = nullptr;
@@ -443,10 +408,8 @@ nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     if (!bnd.timeouts)
         return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: no wait counter");
     wait_fault_settings(&bnd.skip, &bnd.budget);
-    const int rows = pair ? kRows : 2 * kRows;
-    const int64_t blocks =
-        static_cast<int64_t>((p.Lq + rows - 1) / rows) * p.B * (pair ? p.Hq / 2 : p.Hq);
-    kern<<<static_cast<unsigned>(blocks), kFwdThreads, smem, st>>>(mq, mk, mv, p, pair, bnd);
+    const int64_t blocks = static_cast<int64_t>((p.Lq + kRows - 1) / kRows) * p.B * p.Hq;
+    kern<<<static_cast<unsigned>(blocks), kFwdThreads, smem, st>>>(mq, mk, mv, p, bnd);
     return check_launch("token_attention");
 }
 
