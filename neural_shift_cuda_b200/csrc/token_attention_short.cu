@@ -1,11 +1,12 @@
-// token_attention_short.cu -- forward of token attention, fp16 / bf16, for short rows
-// of keys (windows, small grids): a block of 4 warps has 64 queries of a head, a warp 16
+// token_attention_short.cu -- forward of token attention, fp16 / bf16, for few
+// tokens (windows, small grids): a block of 4 warps has 64 queries of a head, a warp 16
 // of them, and passes the keys 64 at a time.
 //
 // Bound by latency: such a call is many small heads, each a chain of loads, two small
-// products and a softmax.  A 128-row tcgen05 tile would be half empty and costs some
-// 6 us of set-up a block with one block an SM; here a block takes 3 us or so and six or
-// more share an SM (256 windows of 64 tokens, 8 heads of 32: 90 us against 11 us).
+// products and a softmax.  A 128-row tcgen05 tile would be half empty, and has some 5 us
+// of set-up a block with two blocks an SM; here a block takes 3 us or so and three to
+// seven share an SM.  256 windows of 64 tokens, 8 heads of 32, with a bias table: 17 us
+// (33 MB, 1.9 TB/s) against 38 us; heads of 64: 25 against 40.
 // Products are those of a warp (m16n8k16); a row's statistics lie in the four lanes
 // that hold its scores.
 #include <atomic>
@@ -252,8 +253,13 @@ nsc_status run(const Params& p, cudaStream_t st) {
 
 }  // namespace
 
-// Rows of at most 128 keys, whose layout tc_fits: one or two blocks of keys.
-bool short_fits(const Params& p, int dtype) { return tc_fits(p, dtype) && p.Lk <= 128 && p.Lq <= 128; }
+// At most 64 tokens, or 128 with heads of at most 32, in a layout that tc_fits.  Measured
+// against the 128-row tiles, 8 heads: 64 tokens 17 / 38 us (heads of 32), 25 / 40 (64),
+// 52 / 51 (128; 33 tokens 40 / 46); 170 x 100 tokens 34 / 35, 48 / 37 and 91 / 49.
+bool short_fits(const Params& p, int dtype) {
+    const int most = p.D <= 32 ? 128 : 64;
+    return tc_fits(p, dtype) && p.Lk <= most && p.Lq <= most;
+}
 
 nsc_status short_fwd(const Params& p, int dtype, cudaStream_t st) {
     if (p.residue)

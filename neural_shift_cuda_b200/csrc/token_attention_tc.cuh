@@ -54,7 +54,7 @@ nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, const f
 // A query row as the backward kernels read it: the forward's statistics (m NaN
 // where delta is not finite), delta, and the norm of its output gradient.
 struct RowRec { float m, ll, delta, norm; };
-constexpr int kRecRows = 32;   // rows of a record block, and of one entry of `norms`
+constexpr int kRecRows = 128;  // rows of a record block, and of one entry of `norms`
 
 // A tile: ROWS rows from `row` of head `h`, DP / 64 panels.
 template <int DP, int ROWS = kRows>

@@ -6,17 +6,29 @@
 // that shares the key head.  It works transposed (S^T = K Q^T, dP^T = V dO^T: a
 // thread's lane is a key), so that P^T and dS^T are left in tensor memory as the
 // A operands of dV = P^T dO and dK = dS^T Q, and Q and dO serve each as both
-// kinds of operand from one landed tile.  256 threads take half a row each, in
-// two phases: P from S, then dS from dP.  The products of one phase run beside
+// kinds of operand from one landed tile.  512 threads take a quarter of a row
+// each, in two phases: P from S, then dS from dP.  The products of one phase run beside
 // the other: dV(i), S(i+1) beside phase two of i, dK(i), dP(i+1) beside phase one of
-// i+1.  Four products a tile, 16 D clocks of the tensor pipe; tensor memory is
-// full at D = 128 (S, dP, dK, dV).
+// i+1; one warp issues S and dP, another dV and dK (one warp for all was late for both:
+// 5 % of the time with heads of 64).  Tensor memory is full at D = 128 (S, dP, dK, dV);
+// with heads of 64 there are two S, so that S(i+1) need not wait for dV(i).
 //
 // tc_dq_kernel keeps 128 queries in place: S, dP, then dQ += dS K with dS in the
 // place of its S.  S has two buffers and dP is free once it is in registers, so
 // S(j+1) and dP(j+1) run beside the arithmetic of block j.  Recomputing the
 // scores here costs two of seven products and buys sums in one order without
 // an fp32 gradient in memory.
+//
+// dS is a product's operand of 16 bits twice: rounded, and what that rounding dropped
+// (grad_q and grad_k 2.7e-3 -> 1.7e-3 off in bf16, which is their own rounding, for a
+// tenth of the time).  P is rounded once, as in the forward.
+//
+// Bounded by the arithmetic between the products: 16384 scores a tile on 128 lanes, some
+// 20 instructions each (30 with a cap), against 20 D clocks (dkv) and 16 D (dq) of the
+// tensor pipe, of which only part runs beside it; a block's set-up and end are some 6 us
+// of 35.  4 x 2048 tokens, 16 heads of 64, bias table, bf16: dkv 241 us, dq 275 us (4 and 3
+// products: 142 and 94 TF/s useful).  8192 tokens in 4 documents, causal, capped, 16 / 4
+// heads of 128: dkv 410 us, dq 292 us.
 //
 // fp16: weights and score gradients of long rows lie below its normal range.
 // P is held times 2^6 and the gradient of a row divided by a power of two near

@@ -1,19 +1,19 @@
 // token_attention_tc_fwd.cuh -- forward of token attention on the tensor
 // cores, fp16 / bf16, head widths up to 128.
 //
-// A block owns two tiles of 128 queries: two heads that share a key head at the
-// same queries (one load of K and V serves both), or 256 queries of one head.
-// Roles by warp: 0-3 and 4-7 the softmax of a tile each, a thread a row; 8 loads K
-// and V blocks of 64 keys through a ring by TMA; 9 and 10 issue the products of a tile
-// each (one warp for both was late for either: its waits and issue took as long as a
-// block's softmax); 11 guards (below).
+// A block owns a tile of 128 queries of a head; two blocks share an SM, so that one's
+// set-up and output (some 5 us of a block's time) pass beside the other's products, and
+// each fills the other's waits.  (One block of two tiles an SM: 16 heads of 128, 8192 keys
+// 521 against 470 us; 16 heads of 64, 8191 packed tokens 107 against 96.)  Roles by warp:
+// 0-3 the softmax, a thread a row; 4 loads K and V blocks of 64 keys through a ring by
+// TMA; 5 issues the products; 7 guards (below).
 //
-// Tensor memory holds O of both tiles and two S of each: blocks are of 64 keys, so that
-// S(j+1) is computed beside the softmax of block j.  P takes the place of its S as 16-bit
-// pairs.  (Products of different shapes or accumulators need not complete in the order
-// of their issue: whatever overwrites an operand waits for its reader's commit.)  With
-// blocks of 128 keys and one S, a tile's warps waited a third of the time for their
-// scores: 212 against NEW us for 32 heads of 128, 4096 causal tokens, capped.
+// Tensor memory holds O and two S: S(j+1) is computed beside the softmax of block j.
+// P takes the place of its S as 16-bit pairs.  (Products of different shapes or
+// accumulators need not complete in the order of their issue: whatever overwrites an
+// operand waits for its reader's commit.)  Keys are released after their scores and values
+// after PV: heads of 128 have room for two stages only, and released together the
+// next keys came too late (669 against 470 us).
 //
 // Softmax with a running reference m: p = 2^(s2 - m); m moves, and O is
 // rescaled, only when a row's maximum passes m + 8 (p <= 256 keeps 16-bit
@@ -24,17 +24,19 @@
 // without it the score gradients of rows with few keys, and the sums of many such terms in
 // a bucket, lose digits (documents of some keys, bf16: grad_q and grad_k 2.8e-3 off
 // instead of 1.7e-3, which is their own rounding; a bucket of 8192 rows 3.1e-3 instead of
-// 1.7e-3).  It costs 15 % of a capped forward with heads of 128 (200 -> 230 us, 16 heads,
-// 8192 tokens in 4 documents).
+// 1.7e-3).  It costs some 15 % of a capped forward with heads of 128 (200 -> 230 us when
+// it came, 16 heads, 8192 tokens in 4 documents).
 //
 // Guard: in blocks that some row of a tile does not see whole, a value row
 // that is not finite would reach every row as 0 x NaN.  There the guard warp
 // looks each landed V block over; such a row becomes zero in V and NaN in K,
 // so that the rows that see it still give NaN, by their scores.
 //
-// Work per score: one exponential (16 a clock and SM) against D / 32
-// tensor-core clocks, so D = 64 is bounded by the exponentials and the FMA pipe
-// and D = 128 balances.
+// 8192 keys, 16 heads, bf16: 470 us with heads of 128 (1170 TF/s, 0.71 of a library
+// product's rate), 413 us with heads of 64 (665 TF/s).  Work per score: one exponential
+// (16 a clock and SM) against D / 32 tensor-core clocks; heads of 64 are bounded by the
+// softmax's latency at two warps a scheduler (exponential unit 0.6 busy), heads of 128
+// by that and the products about alike, capped scores by the FMA pipe (six terms).
 #pragma once
 
 #include "token_attention_tc.cuh"

@@ -590,6 +590,7 @@ __global__ __launch_bounds__(kThreads) void decode_join_kernel(const Params p, c
     const int bh = row / p.Lq, t = row - bh * p.Lq, b = bh / p.Hq, h = bh - b * p.Hq;
     const int n = keys_of(p, b), used = max(1, (n + sp.chunk - 1) / sp.chunk);
     const int64_t at = static_cast<int64_t>(row) * sp.n_chunk;
+    cudaGridDependencySynchronize();   // the chunks' parts are written
     const A* ml = part_ml<A>(p, sp) + 2 * at;
     const V4* o = reinterpret_cast<const V4*>(static_cast<const A*>(sp.part) + at * part_wide(p.D));
     const int wide = part_wide(p.D) / 4;
@@ -722,6 +723,24 @@ nsc_status run_any(const Params& p, const Split& s, unsigned blocks, cudaStream_
     return check_launch("token_attention_decode");
 }
 
+// The join's blocks come up while the last chunks are still at work and wait for them.
+template <typename T, typename A>
+nsc_status launch_join(const Params& p, const Split& s, cudaStream_t st) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hq * p.Lq));
+    c.blockDim = dim3(kThreads);
+    c.stream = st;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&c, decode_join_kernel<T, A>, p, s);
+    if (e != cudaSuccess)
+        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention_decode: %s", cudaGetErrorString(e));
+    return check_launch("token_attention_decode");
+}
+
 }  // namespace
 
 int64_t decode_workspace(const Params& p, int dtype) {
@@ -752,14 +771,12 @@ nsc_status decode(const Params& p, void* workspace, int dtype, cudaStream_t st) 
     else if (dtype == NSC_F32) r = run_any<float, float>(p, s, nb, st);
     else r = run_any<double, double>(p, s, nb, st);
     if (r != NSC_OK || s.n_chunk == 1) return r;
-    const unsigned jb = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hq * p.Lq);
     switch (dtype) {
-        case NSC_F16: decode_join_kernel<__half, float><<<jb, kThreads, 0, st>>>(p, s); break;
-        case NSC_BF16: decode_join_kernel<__nv_bfloat16, float><<<jb, kThreads, 0, st>>>(p, s); break;
-        case NSC_F32: decode_join_kernel<float, float><<<jb, kThreads, 0, st>>>(p, s); break;
-        default: decode_join_kernel<double, double><<<jb, kThreads, 0, st>>>(p, s);
+        case NSC_F16: return launch_join<__half, float>(p, s, st);
+        case NSC_BF16: return launch_join<__nv_bfloat16, float>(p, s, st);
+        case NSC_F32: return launch_join<float, float>(p, s, st);
+        default: return launch_join<double, double>(p, s, st);
     }
-    return check_launch("token_attention_decode");
 }
 
 }  // namespace tok
