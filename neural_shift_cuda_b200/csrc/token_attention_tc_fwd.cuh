@@ -35,7 +35,7 @@
 // 8192 keys, 16 heads, bf16: 470 us with heads of 128 (1170 TF/s, 0.71 of a library
 // product's rate), 413 us with heads of 64 (665 TF/s).  Work per score: one exponential
 // (16 a clock and SM) against D / 32 tensor-core clocks; heads of 64 are bounded by the
-// softmax's latency at two warps a scheduler (exponential unit 0.6 busy), heads of 128
+// softmax's latency at two warps a scheduler (exponential unit half busy), heads of 128
 // by that and the products about alike, capped scores by the FMA pipe (six terms).
 #pragma once
 
