@@ -59,6 +59,13 @@ def test_rotate_types_and_widths(cuda, dt, D, adjacent):
     _rotate(dt, 2, 17, 4, 2, D, adjacent=adjacent, given=adjacent)
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("D", [8, 24, 40, 72, 136, 264, 272, 320])
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_rotate_widths_of_eight(cuda, dt, D, adjacent):
+    _rotate(dt, 2, 11, 5, 3, D, adjacent=adjacent, given=not adjacent)
+
+
 @pytest.mark.parametrize("D,R", [(2, 2), (6, 4), (10, 10), (24, 8), (64, 32), (128, 0), (80, 48)])
 @pytest.mark.parametrize("adjacent", [False, True])
 @pytest.mark.parametrize("dt", [BF16, F32])
