@@ -14,7 +14,13 @@
 // products of a warp, statistics in fp32.  A tile of tcgen05 would be 128 rows for
 // the few there are.  Two blocks an SM (three at D <= 64): one joins its warps'
 // outputs while the other reads.
-// decode_any_kernel: any type, width and alignment, 8 rows a block, on the FMA pipes.
+// 32 ragged caches to 8192 keys, 32 / 8 heads of 128, capped, bf16: 82 us for 500 MB
+// (6.0 TB/s), the join 7; two caches of 65530 keys, 16 / 2 heads of 128, 4 new tokens,
+// fp16: 36 us (3.8 TB/s: a block's start and end beside its 450 keys), the join 7.
+// decode_f32_kernel: fp32 on the FMA pipes, 4 or 8 rows a block, in registers.
+// decode_any_kernel: any type, width and alignment, 8 rows a block, tile by tile through
+// shared memory.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -26,6 +32,7 @@ namespace {
 
 constexpr int kWarps = 4;            // of a tensor-core block
 constexpr int kMmaThreads = 32 * kWarps;
+constexpr int kF32Threads = 128;
 constexpr int kThreads = 256;        // of the others
 constexpr float kLazyMove = 8.f;
 
@@ -578,6 +585,188 @@ __global__ __launch_bounds__(kThreads) void decode_any_kernel(const Params p, co
     }
 }
 
+// fp32 rows of 16-byte units, D <= 128: eight lanes a key, D / 8 of its channels a lane, so
+// that a warp reads four keys in whole lines; each such group of lanes is a softmax of its
+// own (reference, sum and outputs in registers) until the end, so that a key costs three
+// exchanges a row and no barrier.  Values are asked for before the scores of their keys,
+// keys a step ahead.  RB rows a block.  Bound by memory with few rows: 8 caches of 8192 keys,
+// 16 / 4 heads of 128: 66 us for 268 MB (4.0 TB/s; decode_any_kernel 403 us); 32 / 4
+// heads 113 us, bound by the FMA pipe.
+template <int DP, int RB>
+__global__ __launch_bounds__(kF32Threads) void decode_f32_kernel(const Params p, const Split sp) {
+    constexpr int C = DP / 32, W = kF32Threads / 32;
+    __shared__ __align__(16) float qs[RB][DP];
+    __shared__ __align__(16) float os[W][RB][DP];
+    __shared__ float ms[W][RB], ls[W][RB];
+    __shared__ int row_pos[RB], row_head[RB];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7, slot = lane >> 3;
+    int id = blockIdx.x;
+    const int chunk = id % sp.n_chunk;
+    id /= sp.n_chunk;
+    const int group = id % sp.groups;
+    id /= sp.groups;
+    const int hk = id % p.Hkv, b = id / p.Hkv;
+    const int n = keys_of(p, b), c0 = chunk * sp.chunk, c1 = min(n, c0 + sp.chunk);
+    if (c0 >= n && chunk > 0) return;
+    const int rows = p.G * p.Lq, r0 = group * RB, nr = min(RB, rows - r0);
+    for (int i = threadIdx.x; i < RB * DP; i += kF32Threads) {
+        const int r = i / DP, d = i % DP;
+        int h = 0, t = 0;
+        if (r < nr) row_of(p, hk, r0 + r, h, t);
+        qs[r][d] = r < nr && d < p.D ? static_cast<const float*>(p.q)[b * p.qs[0] + t * p.qs[1] +
+                                                                      h * p.qs[2] + d]
+                                     : 0.f;
+        if (d == 0) {
+            row_pos[r] = n - p.Lq + t;
+            row_head[r] = h;
+        }
+    }
+    __syncthreads();
+    const float* kb = static_cast<const float*>(p.k) + b * p.ks[0] + hk * p.ks[2] + 4 * sub;
+    const float* vb = static_cast<const float*>(p.v) + b * p.vs[0] + hk * p.vs[2] + 4 * sub;
+    auto fetch = [&](const float* base, int64_t stride, int key, float4 (&x)[C]) {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            x[j] = key < c1 && 4 * sub + 32 * j < p.D
+                       ? __ldg(reinterpret_cast<const float4*>(base + key * stride + 32 * j))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
+    const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
+    float acc[RB][4 * C], m[RB], l[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4 * C; ++j) acc[r][j] = 0.f;
+    }
+    const int first = c0 + 4 * warp, steps = c1 > first ? (c1 - first + 4 * W - 1) / (4 * W) : 0;
+    float4 k[C], v[C];
+    fetch(kb, p.ks[1], first + slot, k);
+    for (int i = 0; i < steps; ++i) {
+        const int key = first + 4 * W * i + slot;
+        fetch(vb, p.vs[1], key, v);
+        float x[RB];
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            float a = 0.f, c = 0.f;
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const float4 q = *reinterpret_cast<const float4*>(&qs[r][4 * sub + 32 * j]);
+                a = fmaf(k[j].x, q.x, a);
+                c = fmaf(k[j].y, q.y, c);
+                a = fmaf(k[j].z, q.z, a);
+                c = fmaf(k[j].w, q.w, c);
+            }
+            x[r] = a + c;
+        }
+        fetch(kb, p.ks[1], key + 4 * W, k);
+#pragma unroll
+        for (int e = 1; e < 8; e <<= 1)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) x[r] += __shfl_xor_sync(0xffffffffu, x[r], e);
+        // past the oldest new token's position some row does not see a key
+        const bool tail = __any_sync(0xffffffffu, key > n - p.Lq || key >= c1);
+        bool moved = false;
+        float keep[RB];
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            x[r] = (p.cap > 0 ? tanhf(x[r] * y1) : x[r]) * unit;
+            if (p.table) {
+                const int rel = min(max(key - row_pos[r], -p.reach), 0);
+                x[r] += bias2_at<float>(p, __ldg(p.lut + rel + p.reach), row_head[r]);
+            }
+            if (tail && (key > row_pos[r] || key >= c1)) x[r] = -INFINITY;
+            keep[r] = 1.f;
+            if (x[r] > m[r] + kLazyMove || m[r] == -INFINITY) {
+                keep[r] = m[r] == -INFINITY ? 0.f : exp2f(m[r] - x[r]);
+                m[r] = fmaxf(m[r], x[r]);
+                moved = true;
+            }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                l[r] *= keep[r];
+#pragma unroll
+                for (int j = 0; j < 4 * C; ++j) acc[r][j] *= keep[r];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            x[r] = exp2f(x[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] += x[r];
+        }
+        if (tail) {   // (0 x infinity would reach a row that does not see the key)
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+                if (key <= row_pos[r] && key < c1)
+#pragma unroll
+                    for (int j = 0; j < C; ++j) {
+                        acc[r][4 * j] = fmaf(x[r], v[j].x, acc[r][4 * j]);
+                        acc[r][4 * j + 1] = fmaf(x[r], v[j].y, acc[r][4 * j + 1]);
+                        acc[r][4 * j + 2] = fmaf(x[r], v[j].z, acc[r][4 * j + 2]);
+                        acc[r][4 * j + 3] = fmaf(x[r], v[j].w, acc[r][4 * j + 3]);
+                    }
+        } else {
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    acc[r][4 * j] = fmaf(x[r], v[j].x, acc[r][4 * j]);
+                    acc[r][4 * j + 1] = fmaf(x[r], v[j].y, acc[r][4 * j + 1]);
+                    acc[r][4 * j + 2] = fmaf(x[r], v[j].z, acc[r][4 * j + 2]);
+                    acc[r][4 * j + 3] = fmaf(x[r], v[j].w, acc[r][4 * j + 3]);
+                }
+        }
+    }
+    // the four softmaxes of the warp, then the warps
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        float M = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+        const float f = m[r] == -INFINITY ? (l[r] == 0.f ? 0.f : 1.f) : exp2f(m[r] - M);
+        l[r] *= f;
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 8);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
+#pragma unroll
+        for (int j = 0; j < 4 * C; ++j) {
+            float o = acc[r][j] * f;
+            o += __shfl_xor_sync(0xffffffffu, o, 8);
+            o += __shfl_xor_sync(0xffffffffu, o, 16);
+            if (slot == 0) os[warp][r][4 * sub + 32 * (j / 4) + j % 4] = o;
+        }
+        if (lane == 0) {
+            ms[warp][r] = M;
+            ls[warp][r] = l[r];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nr * p.D; i += kF32Threads) {
+        const int r = i / p.D, d = i - r * p.D;
+        float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, ms[w][r]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = ms[w][r] == -INFINITY ? (ls[w][r] == 0.f ? 0.f : 1.f) : exp2f(ms[w][r] - M);
+            L += ls[w][r] * f;
+            o += os[w][r][d] * f;
+        }
+        int h, t;
+        row_of(p, hk, r0 + r, h, t);
+        const int64_t row = (static_cast<int64_t>(b) * p.Hq + h) * p.Lq + t;
+        if (sp.n_chunk == 1) {
+            static_cast<float*>(p.out)[((static_cast<int64_t>(b) * p.Lq + t) * p.Hq + h) * p.D + d] =
+                L == 0.f ? 0.f : o / L;
+            if (d == 0) row_stats<float>(p, row, M, log2f(L), L == 0.f);
+        } else {
+            put_part<float>(p, sp, row, chunk, d, o, M, L);
+        }
+    }
+}
+
 // A block a row, its warps side by side over the row's chunks, four channels a lane
 // at a time.  Bound by latency: the loads of a warp's chunks are independent.
 template <typename T, typename A>
@@ -649,6 +838,16 @@ bool mma_fits(const Params& p, int dtype) {
         f = f && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0 && p.qs[i] % 2 == 0;
     return f;
 }
+
+bool f32_fits(const Params& p, int dtype) {
+    auto ok16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    bool f = dtype == NSC_F32 && p.D % 4 == 0 && p.D <= 128 && ok16(p.k) && ok16(p.v);
+    for (int i = 0; i < 3; ++i) f = f && p.ks[i] % 4 == 0 && p.vs[i] % 4 == 0;
+    return f;
+}
+// Rows of a block of decode_f32_kernel: eight fill the registers of two blocks an SM, and
+// where a head has no more than four, three blocks keep more loads in flight.
+int f32_rows(const Params& p) { return p.G * p.Lq > 4 ? 8 : 4; }
 
 // Rows of a tensor-core block: two tiles of 16 where a head has more than one.
 int mma_rows(const Params& p) { return p.G * p.Lq > 16 ? 32 : 16; }
@@ -723,6 +922,15 @@ nsc_status run_any(const Params& p, const Split& s, unsigned blocks, cudaStream_
     return check_launch("token_attention_decode");
 }
 
+template <int RB>
+nsc_status run_f32(const Params& p, const Split& s, unsigned blocks, cudaStream_t st) {
+    auto kern = p.D <= 32   ? decode_f32_kernel<32, RB>
+                : p.D <= 64 ? decode_f32_kernel<64, RB>
+                            : decode_f32_kernel<128, RB>;
+    kern<<<blocks, kF32Threads, 0, st>>>(p, s);
+    return check_launch("token_attention_decode");
+}
+
 // The join's blocks come up while the last chunks are still at work and wait for them.
 template <typename T, typename A>
 nsc_status launch_join(const Params& p, const Split& s, cudaStream_t st) {
@@ -747,12 +955,13 @@ int64_t decode_workspace(const Params& p, int dtype) {
     // whichever kernel the call will take
     const int64_t a = part_bytes(p, split_of(p, mma_rows(p)), dtype);
     const int64_t b = part_bytes(p, split_of(p, kAnyRows), dtype);
-    return a > b ? a : b;
+    const int64_t c = part_bytes(p, split_of(p, f32_rows(p)), dtype);
+    return std::max(a, std::max(b, c));
 }
 
 nsc_status decode(const Params& p, void* workspace, int dtype, cudaStream_t st) {
-    const bool mma = mma_fits(p, dtype);
-    Split s = split_of(p, mma ? mma_rows(p) : kAnyRows);
+    const bool mma = mma_fits(p, dtype), f32 = f32_fits(p, dtype);
+    Split s = split_of(p, mma ? mma_rows(p) : f32 ? f32_rows(p) : kAnyRows);
     s.part = workspace;
     if (s.n_chunk > 1 && !workspace)
         return fail(NSC_ERR_INVALID_ARG, "token_attention_decode: NULL pointer");
@@ -766,6 +975,7 @@ nsc_status decode(const Params& p, void* workspace, int dtype, cudaStream_t st) 
                       : run_mma<__nv_bfloat16, 128>(p, s, nb, st);
     else if (mma)
         r = p.D <= 64 ? run_mma<__half, 64>(p, s, nb, st) : run_mma<__half, 128>(p, s, nb, st);
+    else if (f32) r = f32_rows(p) == 8 ? run_f32<8>(p, s, nb, st) : run_f32<4>(p, s, nb, st);
     else if (dtype == NSC_F16) r = run_any<__half, float>(p, s, nb, st);
     else if (dtype == NSC_BF16) r = run_any<__nv_bfloat16, float>(p, s, nb, st);
     else if (dtype == NSC_F32) r = run_any<float, float>(p, s, nb, st);
