@@ -410,9 +410,11 @@ NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
                                    const nsc_attention_grad* g, void* stream);
 
 /* The form for the newest Lq tokens of ragged sequences: k and v are caches
- * of Lk rows of which the first lengths[b] hold sequence b, the newest tokens'
- * own keys among them; causal.  Rows past lengths[b] are not read.  The long
- * axis is split over the GPU and joined.  `workspace`:
+ * of Lk rows of which the first lengths[b] (NULL: all) hold sequence b, the newest
+ * tokens' own keys among them.  causal: as above; else (and without a table) each
+ * token sees all lengths[b] keys.  Rows past lengths[b] are not read.  The long
+ * axis is split over the GPU and joined: also the form for few queries over many
+ * keys.  `workspace`:
  * nsc_token_attention_decode_workspace(a) bytes (may be 0), 256-byte aligned. */
 NSC_API int64_t nsc_token_attention_decode_workspace(const nsc_attention* a);
 NSC_API nsc_status nsc_token_attention_decode(const nsc_attention* a, void* out,

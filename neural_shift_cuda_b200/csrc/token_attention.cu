@@ -176,9 +176,10 @@ extern "C" NSC_API nsc_status nsc_token_attention_decode(const nsc_attention* a,
     nsc_status st = check(op, a, true);
     if (st != NSC_OK) return st;
     if (!a->B || !a->Lq) return ok();
-    if (!a->lengths || !out) return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
-    if (a->documents || a->prefix || !a->causal)
-        return fail(NSC_ERR_INVALID_ARG, "%s: causal, without documents or prefix", op);
+    if (!out) return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
+    if (a->documents || a->prefix || (a->table && !a->causal))
+        return fail(NSC_ERR_INVALID_ARG,
+                    "%s: without documents or prefix, and causal with a bias", op);
     Params p = params(a);
     p.out = out;
     p.lse = lse;

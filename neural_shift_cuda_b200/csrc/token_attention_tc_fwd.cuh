@@ -130,6 +130,8 @@ __global__ __launch_bounds__(kFwdThreads, 2) void tc_fwd_kernel(
             atomicMax(&span[2], v2);
             atomicMin(&span[3], v3);
         }
+        // (a row past the end is not written; it must not make a block look partly seen)
+        if (row >= p.Lq) hi = INT_MAX;
     }
     if (BIAS) load_padded_bias(p, h, E, threadIdx.x, kFwdThreads);
     __syncthreads();

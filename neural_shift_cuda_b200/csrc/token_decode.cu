@@ -64,6 +64,11 @@ __device__ __forceinline__ void row_of(const Params& p, int hk, int r, int& h, i
     t = r - r / p.Lq * p.Lq;
 }
 
+// The last key that new token t sees, of n.
+__device__ __forceinline__ int last_seen(const Params& p, int n, int t) {
+    return p.causal ? n - p.Lq + t : n - 1;
+}
+
 template <typename T, int DP, int MT, int NS, bool CAP, bool BIAS>
 __global__ __launch_bounds__(kMmaThreads, DP == 64 ? 3 : 2) void decode_mma_kernel(const Params p, const Split sp) {
     constexpr int LD = 2 * DP + 16;        // bytes of a row: rows 16 bytes apart in the banks
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(kMmaThreads, DP == 64 ? 3 : 2) void decode_mma_kern
         int h = 0, t = 0;
         const bool in = r < rows;
         if (in) row_of(p, hk, r, h, t);
-        pos[x] = in ? n - p.Lq + t : -1;
+        pos[x] = in ? last_seen(p, n, t) : -1;
         e_far[x] = 0.f;
         head[x] = 0;
         if (BIAS && in) {
@@ -513,7 +518,7 @@ __global__ __launch_bounds__(kThreads) void decode_any_kernel(const Params p, co
                 if (r + i < nr) {
                     int h, t;
                     row_of(p, hk, r0 + r + i, h, t);
-                    const int rel = k0 + key - (n - p.Lq + t);
+                    const int rel = k0 + key - last_seen(p, n, t);
                     if (rel <= 0 && k0 + key < c1) {
                         v = (p.cap > 0 ? tanh_any(x[i] * y1) : x[i]) * unit;
                         if (p.table)
@@ -617,7 +622,7 @@ __global__ __launch_bounds__(kF32Threads) void decode_f32_kernel(const Params p,
                                                                       h * p.qs[2] + d]
                                      : 0.f;
         if (d == 0) {
-            row_pos[r] = n - p.Lq + t;
+            row_pos[r] = last_seen(p, n, t);
             row_head[r] = h;
         }
     }

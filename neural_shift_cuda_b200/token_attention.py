@@ -422,14 +422,59 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
             raise RuntimeError(f"{op}: prefix must be ({B},) or ({B}, {n}); got "
                                f"{tuple(prefix.shape)}")
     scale, cap = _numbers(q, scale, softcap)
+    train = torch.is_grad_enabled() and (
+        q.requires_grad or k.requires_grad or v.requires_grad
+        or (table is not None and table.requires_grad))
+    if (Lq <= 64 and Lk >= 256 and not train and documents is None and prefix is None
+            and (causal or table is None) and _few_queries(q, k, v)):
+        out, lse = _decode(q, k, v, None, table, buckets, scale, cap, int(causal),
+                           return_lse)
+        return (out, lse) if return_lse else out
     args = (_tiled(q), _tiled(k), _tiled(v), documents, prefix, table, buckets, scale,
             cap, int(causal), return_lse)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (table is not None and table.requires_grad)):
+    if train:
         out, lse = _AttentionFn.apply(*args)
     else:
         out, lse = _attention_fwd(*args)[:2]
     return (out, lse) if return_lse else out
+
+
+def _few_queries(q, k, v) -> bool:
+    """Whether few queries over many keys take the decode form: its blocks hold the rows of
+    all heads that share a key head, 32 at a time (fp32: 8), and share out the keys.
+
+    Against a tile of 128 queries a head, us: 8 key heads of 64, 8192 keys, 1 / 32 queries:
+    83 / 83 against 11 / 18; 8 x 8 key heads of 128, 4 queries a key, 1024 keys, 1 / 8
+    queries: 22 / 23 against 12 / 27, 8192 keys: 135 / 135 against 51 / 83, 16 queries
+    137 against 156; one such sequence, 64 queries, 8192 keys: 89 against 77.  fp32 (its
+    tiles of FMA products), 8 such sequences, 256 keys, 16 / 32 queries: 76 / 78 against
+    69 / 130; one, 1024 keys, 64 queries: 203 against 143."""
+    B, Lq, Hq, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    unit = 16 // q.element_size()
+    if unit < 4 or D > 128 or D % unit or any(
+            t.data_ptr() % 16 or t.stride(3) != 1 or any(s % unit for s in t.stride()[:3])
+            for t in (q, k, v)):
+        return False
+    rows = Lq * (Hq // Hkv)
+    if unit == 4:
+        return Lq <= 16 or B * Hkv * ((rows + 7) // 8) <= 512
+    return rows <= 16 or (Lk >= 2048 and (
+        rows <= 32 or B * Hkv * ((rows + 31) // 32) <= 64))
+
+
+def _decode(q, k, v, lengths, table, buckets, scale, cap, causal, want_lse):
+    """(out, lse or None)"""
+    B, T, Hq, D = q.shape
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    out = q.new_empty((B, T, Hq, D))
+    lse = (torch.empty((B, Hq, T), dtype=_acc(q.dtype), device=q.device)
+           if want_lse else None)
+    a = _attention_args(q, k, v, None, None, lengths, table, buckets, scale, cap, causal)
+    ws = _lib.workspace("nsc_token_attention_decode_workspace", q.device, a)
+    _lib.launch(q.device, "nsc_token_attention_decode", a, out.data_ptr(), _addr(lse),
+                _addr(ws))
+    return out, lse
 
 
 def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
@@ -456,17 +501,10 @@ def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
                            f"torch.no_grad()")
     _require_cuda(op, q)
     lengths = _int32(op, "lengths", lengths, q.device)
-    B, T, Hq, D = q.shape
-    if lengths.shape != (B,):
-        raise RuntimeError(f"{op}: lengths must be ({B},); got {tuple(lengths.shape)}")
+    if lengths.shape != (q.shape[0],):
+        raise RuntimeError(f"{op}: lengths must be ({q.shape[0]},); got "
+                           f"{tuple(lengths.shape)}")
     scale, cap = _numbers(q, scale, softcap)
-    q, k_cache, v_cache = _unit(q), _unit(k_cache), _unit(v_cache)
-    out = q.new_empty((B, T, Hq, D))
-    lse = (torch.empty((B, Hq, T), dtype=_acc(q.dtype), device=q.device)
-           if return_lse else None)
-    a = _attention_args(q, k_cache, v_cache, None, None, lengths, table, buckets,
-                        scale, cap, 1)
-    ws = _lib.workspace("nsc_token_attention_decode_workspace", q.device, a)
-    _lib.launch(q.device, "nsc_token_attention_decode", a, out.data_ptr(), _addr(lse),
-                _addr(ws))
+    out, lse = _decode(q, k_cache, v_cache, lengths, table, buckets, scale, cap, 1,
+                       return_lse)
     return (out, lse) if return_lse else out

@@ -398,3 +398,41 @@ def test_score_gradients_of_rows_with_few_keys(cuda, dt, D, L):
         off = float((g.double() - w).norm() / w.norm())
         print(name, own, off)
         assert off <= 1.25 * own, f"{name}: {off:.3g}, its own rounding is {own:.3g}"
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dt,D,Lq,Lk,Hq,Hkv", [
+    (BF16, 64, 1, 256, 4, 4), (BF16, 128, 4, 300, 8, 2), (F16, 64, 16, 700, 2, 2),
+    (BF16, 128, 5, 2100, 12, 2), (F16, 96, 64, 2048, 4, 1), (BF16, 40, 33, 4097, 2, 1),
+    (F32, 64, 1, 1000, 4, 2), (F32, 128, 16, 259, 3, 1), (F32, 36, 7, 513, 8, 1)])
+def test_few_queries_over_many_keys(cuda, dt, D, Lq, Lk, Hq, Hkv, causal):
+    """Without gradients such a call shares out the keys over the GPU."""
+    for cap, buckets in ((0.0, None), (7.0, (16, 60, True) if causal else None)):
+        q = randn(1, 2, Lq, Hq, D, dtype=dt).to(cuda)
+        k = randn(2, 2, Lk, Hkv, D, dtype=dt).to(cuda)
+        v = randn(3, 2, Lk, Hkv, D, dtype=dt).to(cuda)
+        table = m = None
+        if buckets:
+            m = nsc.relative_buckets(*buckets, device=cuda)
+            table = randn(4, buckets[0], Hq, dtype=dt).to(cuda)
+        seen = T.visible(2, Lq, Lk, causal)
+        want, lse = T.attention(q, k, v, seen, D ** -0.5, cap, table, m)
+        got, gl = nsc.token_attention(q, k, v, causal=causal, softcap=cap, bias_table=table,
+                                      bias_buckets=m, return_lse=True)
+        check(got, want, dt, "out")
+        check(gl, lse, F32, "lse", 8.0)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F32, 64)])
+def test_few_queries_and_values_that_are_not_finite(cuda, dt, D):
+    """A key past a query has no influence; where a key is seen it has."""
+    q, k, v = (randn(i, 1, 3 if i == 0 else 400, 2, D, dtype=dt).to(cuda) for i in range(3))
+    want = nsc.token_attention(q, k, v, causal=True)
+    v2, k2 = v.clone(), k.clone()
+    v2[:, 398:] = math.inf
+    k2[:, 399:] = math.nan
+    got = nsc.token_attention(q, k2, v2, causal=True)
+    assert torch.equal(got[:, 0], want[:, 0])
+    assert not torch.isfinite(got[:, 1:]).any()
+    every = nsc.token_attention(q, k2, v2)
+    assert not torch.isfinite(every).any()
