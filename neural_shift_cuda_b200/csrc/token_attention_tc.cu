@@ -143,7 +143,7 @@ nsc_status tc_ready(const void* kern, int smem, int threads, int registers) {
 
 bool tc_fits(const Params& p, int dtype) {
     return (dtype == NSC_F16 || dtype == NSC_BF16) && p.D % 8 == 0 && p.D <= 128 && p.Lk > 0 &&
-           !p.lengths && p.scale > 0 && aligned(p.q) && aligned(p.k) && aligned(p.v) &&
+           !p.lengths && static_cast<float>(p.scale) > 1e-30f && aligned(p.q) && aligned(p.k) && aligned(p.v) &&
            boxable(p.qs, p.B, p.Lq, p.Hq) && boxable(p.ks, p.B, p.Lk, p.Hkv) &&
            boxable(p.vs, p.B, p.Lk, p.Hkv);
 }

@@ -64,6 +64,13 @@ __device__ __forceinline__ void load_rows(unsigned char* dst, const CUtensorMap*
     for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * ROWS * 128, map, bar, 64 * c, h, row, b);
 }
 
+// Bits [lo, hi) of 32, for any lo and hi.
+__device__ __forceinline__ uint32_t seen_bits(int lo, int hi) {
+    const int l = min(max(lo, 0), 32), h = min(max(hi, 0), 32);
+    const uint32_t below_h = h == 32 ? ~0u : (1u << h) - 1, below_l = l == 32 ? ~0u : (1u << l) - 1;
+    return below_h & ~below_l;
+}
+
 // Sees to it that rows of a landed tile that hold an infinity or NaN do not
 // reach products as anything but zero: a weight of zero does not hide them.
 // `lanes` threads, thread t has rows t, t + lanes, ...; returns a bit for each of

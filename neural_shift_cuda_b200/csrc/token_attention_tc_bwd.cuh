@@ -26,9 +26,9 @@
 // Bounded by the arithmetic between the products: 16384 scores a tile on 128 lanes, some
 // 20 instructions each (30 with a cap), against 20 D clocks (dkv) and 16 D (dq) of the
 // tensor pipe, of which only part runs beside it; a block's set-up and end are some 6 us
-// of 35.  4 x 2048 tokens, 16 heads of 64, bias table, bf16: dkv 241 us, dq 275 us (4 and 3
-// products: 142 and 94 TF/s useful).  8192 tokens in 4 documents, causal, capped, 16 / 4
-// heads of 128: dkv 410 us, dq 292 us.
+// of 35.  4 x 2048 tokens, 16 heads of 64, bias table, bf16: dkv 243 us, dq 262 us (4 and 3
+// products of 34 GF: 566 and 393 TF/s).  8192 tokens in 4 documents, causal, capped,
+// 16 / 4 heads of 128: dkv 374 us, dq 281 us.
 //
 // fp16: weights and score gradients of long rows lie below its normal range.
 // P is held times 2^6 and the gradient of a row divided by a power of two near
@@ -214,8 +214,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                 const float4* m4 = reinterpret_cast<const float4*>(rows[st][0] + 32 * part);
                 const float4* l4 = reinterpret_cast<const float4*>(rows[st][1] + 32 * part);
                 const bool whole = __all_sync(0xffffffffu, lo <= q0 && hi >= q0 + 32);
-                const uint32_t from = static_cast<uint32_t>(lo - q0);
-                const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
+                const uint32_t seen = whole ? 0 : seen_bits(lo - q0, hi - q0);
                 const int rel0 = key - (q0 + off);   // distance at column 0, one less a column
                 const int w0 = __shfl_sync(0xffffffffu, rel0, 0);
                 bool far = false;
@@ -248,10 +247,10 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     float2 p0 = make_float2(tc::ex2(x0.x), tc::ex2(x0.y));
                     float2 p1 = make_float2(tc::ex2(x1.x), tc::ex2(x1.y));
                     if (!whole) {
-                        if (4 * i - from >= len) p0.x = 0.f;
-                        if (4 * i + 1 - from >= len) p0.y = 0.f;
-                        if (4 * i + 2 - from >= len) p1.x = 0.f;
-                        if (4 * i + 3 - from >= len) p1.y = 0.f;
+                        if (!(seen >> (4 * i) & 1)) p0.x = 0.f;
+                        if (!(seen >> (4 * i + 1) & 1)) p0.y = 0.f;
+                        if (!(seen >> (4 * i + 2) & 1)) p1.x = 0.f;
+                        if (!(seen >> (4 * i + 3) & 1)) p1.y = 0.f;
                     }
                     w[2 * i] = tc::pack2<T>(p0.x, p0.y);
                     w[2 * i + 1] = tc::pack2<T>(p1.x, p1.y);
@@ -292,10 +291,10 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     a0 = __fmul2_rn(a0, s[2 * i]);
                     a1 = __fmul2_rn(a1, s[2 * i + 1]);
                     if (!whole) {   // (a hidden pair's dP need not be finite)
-                        if (4 * i - from >= len) a0.x = 0.f;
-                        if (4 * i + 1 - from >= len) a0.y = 0.f;
-                        if (4 * i + 2 - from >= len) a1.x = 0.f;
-                        if (4 * i + 3 - from >= len) a1.y = 0.f;
+                        if (!(seen >> (4 * i) & 1)) a0.x = 0.f;
+                        if (!(seen >> (4 * i + 1) & 1)) a0.y = 0.f;
+                        if (!(seen >> (4 * i + 2) & 1)) a1.x = 0.f;
+                        if (!(seen >> (4 * i + 3) & 1)) a1.y = 0.f;
                     }
                     w[2 * i] = tc::pack2<T>(a0.x, a0.y);
                     w[2 * i + 1] = tc::pack2<T>(a1.x, a1.y);
@@ -636,8 +635,16 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             if (CAP) cap(s);
             const int k0 = j * kRows + 32 * part;
             const bool whole = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 32);
-            const uint32_t from = static_cast<uint32_t>(lo - k0);
-            const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
+            const uint32_t seen = whole ? 0 : seen_bits(lo - k0, hi - k0);
+            // out of the loop where it can be: P = 2^-inf and dP = 0 give dS = 0 (a capped
+            // score would give 0 x inf by its slope)
+            if (!CAP && !whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (!(seen >> (2 * i) & 1)) s[i].x = -INFINITY, d[i].x = 0.f;
+                    if (!(seen >> (2 * i + 1) & 1)) s[i].y = -INFINITY, d[i].y = 0.f;
+                }
+            }
             const int rel0 = k0 - (row + off);   // distance at column 0, one more a column
             const int w0 = __shfl_sync(0xffffffffu, rel0, 0);   // lane r: w0 - r
             bool far = false;
@@ -661,9 +668,9 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
                 const float2 pr = make_float2(tc::ex2(x.x), tc::ex2(x.y));
                 float2 z = kBf16 ? __fadd2_rn(d[i], d2) : __ffma2_rn(d[i], g2, d2);
                 z = __fmul2_rn(z, pr);
-                if (!whole) {
-                    if (2 * i - from >= len) z.x = 0.f;
-                    if (2 * i + 1 - from >= len) z.y = 0.f;
+                if (CAP && !whole) {
+                    if (!(seen >> (2 * i) & 1)) z.x = 0.f;
+                    if (!(seen >> (2 * i + 1) & 1)) z.y = 0.f;
                 }
                 if (BIAS) d[i] = z;
                 if (CAP) {

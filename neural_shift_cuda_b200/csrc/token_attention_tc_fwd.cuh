@@ -4,7 +4,7 @@
 // A block owns a tile of 128 queries of a head; two blocks share an SM, so that one's
 // set-up and output (some 5 us of a block's time) pass beside the other's products, and
 // each fills the other's waits.  (One block of two tiles an SM: 16 heads of 128, 8192 keys
-// 521 against 470 us; 16 heads of 64, 8191 packed tokens 107 against 96.)  Roles by warp:
+// 521 against 470 us; 16 heads of 64, 8191 packed tokens 107 against 96, since 92.)  Roles by warp:
 // 0-3 the softmax, a thread a row; 4 loads K and V blocks of 64 keys through a ring by
 // TMA; 5 issues the products; 7 guards (below).
 //
@@ -192,12 +192,13 @@ __global__ __launch_bounds__(kFwdThreads, 2) void tc_fwd_kernel(
                 }
             }
             if (!__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + kKeys)) {
-                const uint32_t from = static_cast<uint32_t>(lo - k0);
-                const uint32_t len = static_cast<uint32_t>(max(hi - lo, 0));
+                // (a bit a key: an element then costs a test of a constant bit; two compares
+                // an element were 4 % of a packed call)
+                const uint32_t seen[2] = {seen_bits(lo - k0, hi - k0), seen_bits(lo - k0 - 32, hi - k0 - 32)};
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    if (2 * i - from >= len) s[i].x = -INFINITY;
-                    if (2 * i + 1 - from >= len) s[i].y = -INFINITY;
+                    if (!(seen[i / 16] >> (2 * i % 32) & 1)) s[i].x = -INFINITY;
+                    if (!(seen[i / 16] >> (2 * i % 32 + 1) & 1)) s[i].y = -INFINITY;
                 }
             }
             // (four maxima, and four sums below, side by side: one chain would wait
