@@ -243,3 +243,34 @@ def test_decode_agrees_with_attention(cuda):
         one = nsc.token_attention_decode(q[:, n - 1:n], k, v, torch.tensor([n], device=cuda),
                                          softcap=5.0)
         check(one, whole[:, n - 1:n], F32)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_a_layer_in_a_graph(cuda, dt):
+    """Prompt, few new queries and decode, captured once and replayed on new values."""
+    B, n, H, Hk, D = 2, 300, 4, 2, 64
+    x = randn(0, B, n, H + 2 * Hk, D, dtype=dt).to(cuda)
+    cos, sin = _angles(n, D, dt, cuda)
+    lengths = torch.tensor([n, 211], dtype=torch.int32, device=cuda)
+
+    def layer():
+        q, k, v = x.split((H, Hk, Hk), 2)
+        q, k = nsc.qk_norm_rotate(q, k, None, None, cos, sin)
+        return (nsc.token_attention(q, k, v, causal=True, softcap=9.0),
+                nsc.token_attention(q[:, -2:], k, v, causal=True),
+                nsc.token_attention_decode(q[:, -3:], k, v, lengths))
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layer()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = layer()
+        for seed in (1, 2):
+            x.copy_(randn(seed, *x.shape, dtype=dt))
+            graph.replay()
+            for a, b in zip(got, layer()):
+                assert torch.equal(a, b)
