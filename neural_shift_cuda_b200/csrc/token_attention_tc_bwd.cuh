@@ -28,7 +28,7 @@
 // tensor pipe, of which only part runs beside it; a block's set-up and end are some 6 us
 // of 35.  4 x 2048 tokens, 16 heads of 64, bias table, bf16: dkv 243 us, dq 262 us (4 and 3
 // products of 34 GF: 566 and 393 TF/s).  8192 tokens in 4 documents, causal, capped,
-// 16 / 4 heads of 128: dkv 374 us, dq 281 us.
+// 16 / 4 heads of 128: dkv 358 us, dq 269 us.
 //
 // fp16: weights and score gradients of long rows lie below its normal range.
 // P is held times 2^6 and the gradient of a row divided by a power of two near

@@ -36,7 +36,7 @@
 // product's rate), 413 us with heads of 64 (665 TF/s).  Work per score: one exponential
 // (16 a clock and SM) against D / 32 tensor-core clocks; heads of 64 are bounded by the
 // softmax's latency at two warps a scheduler (exponential unit half busy), heads of 128
-// by that and the products about alike, capped scores by the FMA pipe (six terms).
+// by that and the products about alike, capped scores by the FMA pipe too.
 #pragma once
 
 #include "token_attention_tc.cuh"
