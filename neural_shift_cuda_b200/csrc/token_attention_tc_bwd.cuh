@@ -412,6 +412,9 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
             bool fine = true;
             for (int i = 0; i < total; ++i) {
                 const int s = i % NS;
+                // (dO has its own barrier: P is ready as soon as Q was there.  What refills
+                // the stage waits for this warp's commit, so the phase cannot pass by)
+                fine &= wait(&bars.y_full[s], (i / NS) & 1);
                 fine &= wait(&bars.p_ready[i & 1], (i >> 1) & 1);
                 tc::fence_after();
                 if (lead) {
