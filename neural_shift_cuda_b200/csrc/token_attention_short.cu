@@ -93,8 +93,8 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
     const uint32_t va = smem_u32(Vs) + (((lane >> 3) & 1) * 8 + (lane & 7)) * LD + (lane >> 4) * 16;
 
     for (int k0 = first / kKeys * kKeys; k0 < last; k0 += kKeys) {
+        __syncthreads();   // (the last block's tiles and its odd_keys are used up)
         if (threadIdx.x == 0) odd_keys = 0;
-        __syncthreads();   // (the last block's tiles are used up)
         for (int u = threadIdx.x; u < kKeys * CH; u += kShortThreads) {
             const int r = u / CH, c = u % CH;
             const bool in = k0 + r < p.Lk && 8 * c < p.D;

@@ -38,3 +38,21 @@ def test_gradients_while_memory_is_busy(cuda, dt, D):
         torch.cuda.current_stream().wait_stream(side)
         for a, b in zip(quiet, busy):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D", [16, 32])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_short_rows_and_values_that_are_not_finite(cuda, dt, D, bad):
+    """Two blocks of keys: a bad value of the first shows in every query that sees it, in
+    every head, and in no other; so does one of the second."""
+    L, at = 128, (3, 100)
+    q, k, v = (randn(i, 16, L, 8, D, dtype=dt).to(cuda) for i in range(3))
+    want = nsc.token_attention(q, k, v, causal=True)
+    for key in at:
+        v2 = v.clone()
+        v2[:, key] = bad
+        for _ in range(10):
+            got = nsc.token_attention(q, k, v2, causal=True)
+            assert torch.equal(got[:, :key], want[:, :key])
+            assert not torch.isfinite(got[:, key:]).any()
