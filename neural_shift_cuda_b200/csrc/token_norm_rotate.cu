@@ -592,8 +592,12 @@ Args args(const nsc_norm_rotate* a) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Whether accesses of whole chunks serve this call.
-bool wide(const nsc_norm_rotate* a) {
+// Whether accesses of whole chunks serve this call: what it reads and writes lies in
+// 16-byte units (a head of all others does when the first does: D is a multiple of 8).
+bool wide(const nsc_norm_rotate* a, const Out* o, const Grad* g) {
+    if (o && !(aligned16(o->q) && aligned16(o->k))) return false;
+    if (g && !(aligned16(g->gq) && aligned16(g->gk) && aligned16(g->dq) && aligned16(g->dk)))
+        return false;
     const int64_t es = dtype_size(a->dtype);
     // (fp64 would spill its two chunks; it takes the other kernel)
     bool w = a->dtype != NSC_F64 && a->D % 8 == 0 && (a->D <= 256 || a->D % 16 == 0) && a->rot_dim == a->D && a->rows > 0 && aligned16(a->q) &&
@@ -653,7 +657,7 @@ template <typename T, typename A>
 nsc_status run(const nsc_norm_rotate* n, const Out* o, const Grad* g, int* n_part,
                cudaStream_t st) {
     Args a = args(n);
-    if constexpr (sizeof(T) < 8) if (wide(n)) {
+    if constexpr (sizeof(T) < 8) if (wide(n, o, g)) {
         switch (lanes_for(a.D)) {
             case 1: return run_wide<T, 1>(a, o, g, n_part, st);
             case 2: return run_wide<T, 2>(a, o, g, n_part, st);

@@ -101,6 +101,13 @@ def _tiled(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous from a 16-byte boundary on (what the backward of a flat
+    concatenation hands out need not start on one)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _int32(op: str, name: str, t: torch.Tensor, device) -> torch.Tensor:
     if (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device
             and t.is_contiguous()):
@@ -156,7 +163,7 @@ class _RotateFn(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         a = _rotate_args(q, k, wq, wk, cos, sin, positions, ctx.adjacent, ctx.eps)
-        gq, gk = gq.contiguous(), gk.contiguous()
+        gq, gk = _aligned(gq), _aligned(gk)
         dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None

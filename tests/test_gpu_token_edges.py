@@ -1,16 +1,20 @@
 """Edges of the token operators: what lands late, what nothing sees, what is not aligned,
 and values near the ends of their type."""
 
+import importlib
 import math
 
 import pytest
 import torch
 
 import neural_shift_cuda_b200 as nsc
+from neural_shift_cuda_b200 import _lib
 from oracle import token_oracle as T
 from token_cases import check, leaf, randn, reference
 
 pytestmark = pytest.mark.gpu
+
+A = importlib.import_module("neural_shift_cuda_b200.token_attention")
 
 F16, BF16, F32, F64 = torch.float16, torch.bfloat16, torch.float32, torch.float64
 
@@ -56,3 +60,48 @@ def test_short_rows_and_values_that_are_not_finite(cuda, dt, D, bad):
             got = nsc.token_attention(q, k, v2, causal=True)
             assert torch.equal(got[:, :key], want[:, :key])
             assert not torch.isfinite(got[:, key:]).any()
+
+
+def _shifted(t):
+    """t in storage that starts one element past an aligned address."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+    return flat.copy_(t.flatten()).view(t.shape)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("D", [64, 128, 320])
+def test_rotation_with_gradients_that_are_not_aligned(cuda, dt, D):
+    """A contiguous gradient may start anywhere: a slice by the caller, or what the
+    backward of a concatenation gives."""
+    q, k = (randn(i, 2, 9, h, D, dtype=dt).to(cuda) for i, h in ((0, 4), (1, 2)))
+    gq, gk = (randn(i, *t.shape, dtype=dt).to(cuda) for i, t in ((2, q), (3, k)))
+    w = randn(4, D, dtype=dt).to(cuda)
+    angle = torch.linspace(0, 3, 9 * D // 2, device=cuda).view(9, D // 2)
+    cos, sin = angle.cos(), angle.sin()
+    ref = [leaf(t.double()) for t in (q, k, w, w)]
+    want = torch.autograd.grad(T.qk_norm_rotate(*ref, cos, sin), ref, [gq.double(), gk.double()])
+    mine = [leaf(t) for t in (q, k, w, w)]
+    out = nsc.qk_norm_rotate(*mine, cos, sin)
+    one = torch.autograd.grad(out, mine, [_shifted(gq), _shifted(gk)], retain_graph=True)
+    flat = torch.cat([q.new_zeros(1), out[0].flatten(), out[1].flatten()])
+    two = torch.autograd.grad(flat, mine, torch.cat([q.new_zeros(1), gq.flatten(), gk.flatten()]))
+    for got in (one, two):
+        for g, x in zip(got, want):
+            check(g, x, dt)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_rotation_to_outputs_that_are_not_aligned(cuda, dt):
+    """The entry points take results and gradients at any address of their type."""
+    q, k = (randn(i, 2, 9, h, 64, dtype=dt).to(cuda) for i, h in ((0, 4), (1, 2)))
+    angle = torch.linspace(0, 3, 9 * 32, device=cuda).view(9, 32)
+    a = A._rotate_args(q, k, None, None, angle.cos(), angle.sin(), None, 0, 1e-6)
+    grads = [_shifted(k.repeat(1, 1, 2, 1)), _shifted(k)]
+    for name, odd in (("nsc_qk_norm_rotate_fwd", []), ("nsc_qk_norm_rotate_bwd", grads)):
+        tail = [None] * (3 if odd else 0)
+        even = [t.clone() for t in odd]
+        got, want = [_shifted(q), _shifted(k)], [torch.empty_like(q), torch.empty_like(k)]
+        for ins, outs in ((odd, got), (even, want)):
+            _lib.launch(q.device, name, a, *(t.data_ptr() for t in ins + outs), *tail)
+        for x, y in zip(got, want):
+            check(x, y, dt)
