@@ -84,6 +84,7 @@ Params params(const nsc_attention* a) {
 }
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255) == 0; }
 int64_t acc_size(int dtype) { return dtype == NSC_F64 ? 8 : 4; }
 
 int query_parts(const nsc_attention* a) {
@@ -138,6 +139,8 @@ extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
     if ((rows && (!g->out || !g->stats || !g->grad_out || !g->grad_q || !g->workspace)) ||
         (cols && (!g->grad_k || !g->grad_v)) || (g->grad_table && !a->table))
         return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
+    if (!aligned256(g->workspace))
+        return fail(NSC_ERR_INVALID_ARG, "%s: workspace is not 256-byte aligned", op);
     cudaStream_t s = as_stream(stream);
     Params p = params(a);
     p.out = const_cast<void*>(g->out);
@@ -180,6 +183,8 @@ extern "C" NSC_API nsc_status nsc_token_attention_decode(const nsc_attention* a,
     if (a->documents || a->prefix || (a->table && !a->causal))
         return fail(NSC_ERR_INVALID_ARG,
                     "%s: without documents or prefix, and causal with a bias", op);
+    if (!aligned256(workspace))
+        return fail(NSC_ERR_INVALID_ARG, "%s: workspace is not 256-byte aligned", op);
     Params p = params(a);
     p.out = out;
     p.lse = lse;

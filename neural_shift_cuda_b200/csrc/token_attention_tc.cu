@@ -143,7 +143,8 @@ nsc_status tc_ready(const void* kern, int smem, int threads, int registers) {
 
 bool tc_fits(const Params& p, int dtype) {
     return (dtype == NSC_F16 || dtype == NSC_BF16) && p.D % 8 == 0 && p.D <= 128 && p.Lk > 0 &&
-           !p.lengths && static_cast<float>(p.scale) > 1e-30f && aligned(p.q) && aligned(p.k) && aligned(p.v) &&
+           !p.lengths && static_cast<float>(p.scale) > 1e-30f && aligned(p.q) && aligned(p.k) &&
+           aligned(p.v) && aligned(p.out) && aligned(p.residue) &&
            boxable(p.qs, p.B, p.Lq, p.Hq) && boxable(p.ks, p.B, p.Lk, p.Hkv) &&
            boxable(p.vs, p.B, p.Lk, p.Hkv);
 }
@@ -169,9 +170,8 @@ int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t nb) {
 }
 
 bool tc_bwd_fits(const Params& p, const Grads& g, int dtype) {
-    return tc_fits(p, dtype) && p.Lq > 0 && aligned(g.dout) && aligned(p.out) &&
-           aligned(p.residue) && aligned(g.dq) && aligned(g.dk) && aligned(g.dv) &&
-           boxable(g.dos, p.B, p.Lq, p.Hq);
+    return tc_fits(p, dtype) && p.Lq > 0 && aligned(g.dout) && aligned(g.dq) && aligned(g.dk) &&
+           aligned(g.dv) && boxable(g.dos, p.B, p.Lq, p.Hq);
 }
 
 nsc_status tc_bwd(const Params& p, Grads g, void* workspace, void* grad_table, int dtype,

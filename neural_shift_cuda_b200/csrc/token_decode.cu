@@ -838,7 +838,7 @@ __global__ __launch_bounds__(kThreads) void decode_join_kernel(const Params p, c
 bool mma_fits(const Params& p, int dtype) {
     auto ok16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
     bool f = (dtype == NSC_F16 || dtype == NSC_BF16) && p.D % 8 == 0 && p.D <= 128 && ok16(p.k) &&
-             ok16(p.v) && (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;
+             ok16(p.v) && ok16(p.out) && (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;
     for (int i = 0; i < 3; ++i)
         f = f && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0 && p.qs[i] % 2 == 0;
     return f;

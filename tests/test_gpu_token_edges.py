@@ -105,3 +105,24 @@ def test_rotation_to_outputs_that_are_not_aligned(cuda, dt):
             _lib.launch(q.device, name, a, *(t.data_ptr() for t in ins + outs), *tail)
         for x, y in zip(got, want):
             check(x, y, dt)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("L,D", [(40, 32), (200, 64), (200, 128)])
+def test_attention_to_an_output_that_is_not_aligned(cuda, dt, L, D):
+    """The entry points write out and residue at any address of their type."""
+    q, k, v = (randn(i, 1, L, 2, D, dtype=dt).to(cuda) for i in range(3))
+    want = T.attention(q, k, v, T.visible(1, L, L, True), D ** -0.5)[0]
+    a = A._attention_args(q, k, v, None, None, None, None, None, D ** -0.5, 0.0, 1)
+    for residue in (None, _shifted(q)):
+        out = _shifted(q)
+        _lib.launch(q.device, "nsc_token_attention_fwd", a, out.data_ptr(), None, None,
+                    A._addr(residue))
+        check(out, want, dt, "forward")
+    n = torch.tensor([L], dtype=torch.int32, device=cuda)
+    last = q[:, -1:]
+    a = A._attention_args(last, k, v, None, None, n, None, None, D ** -0.5, 0.0, 1)
+    ws = _lib.workspace("nsc_token_attention_decode_workspace", q.device, a)
+    out = _shifted(last)
+    _lib.launch(q.device, "nsc_token_attention_decode", a, out.data_ptr(), None, A._addr(ws))
+    check(out, want[:, -1:], dt, "decode")

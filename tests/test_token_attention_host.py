@@ -121,6 +121,19 @@ def test_empty_calls_are_noops():
     assert lib.nsc_qk_norm_rotate_workspace(ctypes.byref(n)) == -1
 
 
+def test_workspaces_that_are_not_aligned_are_refused():
+    lib = _lib.load()
+    a = _att(causal=1, q=256, k=256, v=256)
+    assert lib.nsc_token_attention_decode(ctypes.byref(a), 256, None, 264, None) == 1
+    assert "aligned" in lib.nsc_last_error_string().decode()
+    g = _lib.AttentionGrad()
+    for n in ("out", "stats", "grad_out", "grad_q", "grad_k", "grad_v"):
+        setattr(g, n, 256)
+    g.workspace = 264
+    assert lib.nsc_token_attention_bwd(ctypes.byref(a), ctypes.byref(g), None) == 1
+    assert "aligned" in lib.nsc_last_error_string().decode()
+
+
 def test_relative_buckets():
     m = nsc.relative_buckets(8, 6)
     assert m.dtype == torch.int32 and m.tolist() == [3, 3, 3, 2, 2, 1, 0, 5, 6, 6, 7, 7, 7]
