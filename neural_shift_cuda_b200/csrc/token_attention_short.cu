@@ -63,6 +63,9 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
             atomicMin(&box[3], v3);
         }
     }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)   // (a row past the end is not written: no masks for its sake)
+        if (row[x] >= p.Lq) hi[x] = INT_MAX;
     uint32_t qa[KS][4];
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -129,6 +132,9 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
             }
         }
         const unsigned long long odd = odd_keys;
+        // Whether some row of this warp does not see all 64 keys.  (`part` does not tell: it
+        // is of the rows that see anything, and of the keys there are.)
+        const bool hide = __any_sync(~0u, max(lo[0], lo[1]) > k0 || min(hi[0], hi[1]) < k0 + kKeys);
         float s[8][4];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -151,11 +157,9 @@ __global__ __launch_bounds__(kShortThreads, DP == 32 ? 7 : DP == 64 ? 5 : 3) voi
                 const int x = e >> 1, c = 8 * i + 2 * sub + (e & 1), key = k0 + c;
                 float v = (CAP ? tanh_exact(s[i][e] * y1) : s[i][e]) * unit;
                 if (BIAS) v += E[min(max(key - (row[x] + off), -p.reach), p.reach) + p.reach];
-                if (part) {
+                if (hide) {
                     if (odd >> c & 1) v = NAN;
                     if (key < lo[x] || key >= hi[x]) v = -INFINITY;
-                } else if (key >= p.Lk) {
-                    v = -INFINITY;
                 }
                 s[i][e] = v;
                 top[x] = fmaxf(top[x], v);

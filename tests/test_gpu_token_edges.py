@@ -126,3 +126,30 @@ def test_attention_to_an_output_that_is_not_aligned(cuda, dt, L, D):
     out = _shifted(last)
     _lib.launch(q.device, "nsc_token_attention_decode", a, out.data_ptr(), None, A._addr(ws))
     check(out, want[:, -1:], dt, "decode")
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dt,D", [(F16, 32), (BF16, 16), (BF16, 32), (F16, 8)])
+@pytest.mark.parametrize("L,bounds", [(128, [0, 100]), (128, [28, 128]), (100, [0, 65]),
+                                      (65, [1, 64]), (128, [70, 70]), (40, [5, 30])])
+def test_short_rows_outside_all_documents(cuda, dt, D, L, bounds, causal):
+    """Queries that see nothing, in tiles whose other queries all see a whole block of
+    keys: out is 0 and lse -inf, and the gradients are those of the others."""
+    q, k, v, go = (randn(i, 2, L, 4, D, dtype=dt).to(cuda) for i in range(4))
+    m = nsc.relative_buckets(16, 40, device=cuda)
+    table = randn(5, 16, 4, dtype=dt).to(cuda)
+    rows = [bounds, [0, L]]
+    doc = torch.tensor(rows, device=cuda)
+    seen = T.visible(2, L, L, causal, None, rows)
+    for tab, cap in ((None, 0.0), (table, 12.0)):
+        kw = dict(documents=doc, causal=causal, softcap=cap, bias_table=tab,
+                  bias_buckets=None if tab is None else m, return_lse=True)
+        want = reference(q, k, v, seen, go, D ** -0.5, cap, tab, m)
+        out, lse = nsc.token_attention(q, k, v, **kw)
+        leaves = [leaf(t) for t in (q, k, v)]
+        trained, lse2 = nsc.token_attention(*leaves, **kw)
+        for o, x in ((out, lse), (trained, lse2)):
+            check(o, want[0], dt, "out")
+            check(x, want[1], F32, "lse", 8.0)
+        for g, w in zip(torch.autograd.grad(trained, leaves, go), want[2:5]):
+            check(g, w, dt)
