@@ -606,7 +606,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
         float m = -INFINITY, ll = 0.f, delta = 0.f, g = 1.f;
-        if (row < p.Lq) {
+        // (a row that sees nothing keeps its zeros, whatever its output gradient holds)
+        if (hi > lo) {
             const float4 r = __ldg(reinterpret_cast<const float4*>(
                 recs + (static_cast<int64_t>(b) * p.Hq + h) * p.Lq + row));
             if (!kBf16) g = pow2_near(r.w);
@@ -620,6 +621,9 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
         const float2 g2 = make_float2(1.f / g, 1.f / g);
         const float2 slope2 = make_float2(-1.f / (unit * unit), -1.f / (unit * unit));   // 1 - tanh^2 = 1 + s^2 slope
         const float2 m2 = make_float2(m, m), l2 = make_float2(ll, ll), d2 = make_float2(delta, delta);
+        // (a row whose output gradient is not finite has m NaN: its hidden pairs are
+        // taken out of the table's sums one by one)
+        const bool odd_row = BIAS && !CAP && __any_sync(0xffffffffu, m != m);
         float far_lo = 0.f, far_hi = 0.f;
         const float undo = kBf16 ? 1.f : g / 64.f;
         bool alive = true;
@@ -689,6 +693,13 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
             tc::fence_before();
             mbar_arrive(&bars.ds_ready[it & 1]);
             if (BIAS && gr.tab) {
+                if (!CAP && odd_row && !whole) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (!(seen >> (2 * i) & 1)) d[i].x = 0.f;
+                        if (!(seen >> (2 * i + 1) & 1)) d[i].y = 0.f;
+                    }
+                }
                 if (far) {
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll

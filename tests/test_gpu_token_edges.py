@@ -153,3 +153,33 @@ def test_short_rows_outside_all_documents(cuda, dt, D, L, bounds, causal):
             check(x, want[1], F32, "lse", 8.0)
         for g, w in zip(torch.autograd.grad(trained, leaves, go), want[2:5]):
             check(g, w, dt)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 128), (F32, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("causal", [False, True])
+def test_table_gradient_and_pairs_that_are_not_seen(cuda, dt, D, bad, cap, causal):
+    """Output gradients of padding reach no bucket; those of a query that sees some keys
+    reach the buckets of these and no other."""
+    L, H = 300, 2
+    q, k, v, go = (randn(i, 1, L, H, D, dtype=dt).to(cuda) for i in range(4))
+    m = torch.arange(61, dtype=torch.int32, device=cuda)   # a bucket a distance, -30 .. 30
+    doc = torch.tensor([[0, 140, 290]], device=cuda)
+
+    def grad(go):
+        t = leaf(randn(5, 61, H, dtype=dt).to(cuda))
+        out = nsc.token_attention(q, k, v, documents=doc, causal=causal, softcap=cap,
+                                  bias_table=t, bias_buckets=m)
+        return torch.autograd.grad(out, t, go)[0]
+
+    clean = grad(go)
+    go2 = go.clone()
+    go2[:, 290:] = bad
+    assert torch.equal(grad(go2), clean)
+    go2[:, 143] = bad     # sees keys 140 on: distances from -3
+    got = grad(go2)
+    last = 0 if causal else 30
+    assert torch.equal(got[:27], clean[:27]) and torch.equal(got[30 + last + 1:],
+                                                             clean[30 + last + 1:])
+    assert not torch.isfinite(got[27:30 + last + 1]).any()
