@@ -123,7 +123,8 @@ extern "C" NSC_API int64_t nsc_token_attention_bwd_workspace(const nsc_attention
     int64_t n = align256(a->B * a->Hq * a->Lq * acc_size(a->dtype));
     if (a->table) n += align256(a->Hq * query_parts(a) * a->n_buckets * acc_size(a->dtype));
     // whichever kernels the call will take
-    const int64_t tc = tc_bwd_workspace(a->B, a->Hq, a->Lq, a->table ? a->n_buckets : 0);
+    const int64_t tc =
+        tc_bwd_workspace(a->B, a->Hq, a->Hkv, a->Lq, a->Lk, a->table ? a->n_buckets : 0);
     return n > tc ? n : tc;
 }
 

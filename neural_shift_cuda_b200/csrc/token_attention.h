@@ -32,6 +32,10 @@ struct Grads {
     void *delta;                      // (B, Hq, Lq): sum_d dout out - dlse
     void* tab;                        // (Hq, n_part, nb) partial sums, or null
     int n_part;
+    // fp16 on the tensor cores: norms of the value rows (B, Hkv, Lk), the largest that each
+    // query sees (B, Hkv, Lq), and of each 128 query rows (B, Hq, .) the largest norm of dout
+    // and largest |delta|
+    const float *value_norms, *seen_norms, *row_norms, *row_deltas;
 };
 
 // Document [s, e) of position t: the last bound <= t opens it.  Bounds are
@@ -171,7 +175,8 @@ nsc_status tc_fwd(const Params& p, int dtype, cudaStream_t st);
 bool short_fits(const Params& p, int dtype);
 nsc_status short_fwd(const Params& p, int dtype, cudaStream_t st);
 bool tc_bwd_fits(const Params& p, const Grads& g, int dtype);
-int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t n_buckets);
+int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lq, int64_t Lk,
+                         int64_t n_buckets);
 nsc_status tc_bwd(const Params& p, Grads g, void* workspace, void* grad_table, int dtype,
                   cudaStream_t st);
 

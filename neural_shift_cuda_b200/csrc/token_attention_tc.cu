@@ -27,15 +27,18 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 // The row records, LN lanes a row, 16 bytes a lane, four rows of a lane in flight.  Bound
 // by memory: out, residue and grad_out read once (4 x 2048 tokens, 16 heads of 64: 11 us
 // for 50 MB, 4.6 TB/s; with one row in flight and half the lanes idle 19 us).
-template <typename T, int LN>
-__global__ __launch_bounds__(256) void record_kernel(Params p, Grads g, RowRec* recs, float* norms,
-                                                     int blocks_h) {
+// TOPS (fp16, for the scales of the score gradients): and the largest norm and |delta| of each
+// block's rows.  A row that is not finite does not set them: what sees it is NaN anyway.
+// (Eight blocks an SM, 32 registers: with 34 it took 26 us for 20, 8192 tokens, 16 heads of 128.)
+template <typename T, int LN, bool TOPS>
+__global__ __launch_bounds__(256, 8) void record_kernel(Params p, Grads g, RowRec* recs, float* norms,
+                                                     float* deltas, int blocks_h) {
     constexpr int RB = 256 / LN;   // rows side by side
-    __shared__ float top[RB];
+    __shared__ float top[2][RB];
     const int bh = blockIdx.x / blocks_h, blk = blockIdx.x % blocks_h;
     const int b = bh / p.Hq, h = bh % p.Hq, sub = threadIdx.x / LN, c = threadIdx.x % LN;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Lq;
-    float most = 0.f;
+    float most = 0.f, most_delta = 0.f;
 #pragma unroll 4
     for (int u = 0; u < kRecRows / RB; ++u) {
         const int l = blk * kRecRows + RB * u + sub;
@@ -70,14 +73,79 @@ __global__ __launch_bounds__(256) void record_kernel(Params p, Grads g, RowRec* 
             const float norm = sq < INFINITY ? sqrtf(sq) : 0.f;
             recs[at] = RowRec{stats[at] + (sum - sum), stats[rows + at], sum, norm};
             most = fmaxf(most, norm);
+            if (TOPS && fabsf(sum) < INFINITY) most_delta = fmaxf(most_delta, fabsf(sum));
+        }
+    }
+    if (c == 0) {
+        top[0][sub] = most;
+        if (TOPS) top[1][sub] = most_delta;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < RB; ++i) most = fmaxf(most, top[0][i]);
+        norms[blockIdx.x] = most;
+        if (TOPS) {
+            for (int i = 1; i < RB; ++i) most_delta = fmaxf(most_delta, top[1][i]);
+            deltas[blockIdx.x] = most_delta;
+        }
+    }
+}
+
+// The norms of the value rows and the largest of each 128, as above.
+template <typename T, int LN>
+__global__ __launch_bounds__(256) void value_norm_kernel(Params p, float* norms, float* tops, int blocks_h) {
+    constexpr int RB = 256 / LN;
+    __shared__ float top[RB];
+    const int bh = blockIdx.x / blocks_h, blk = blockIdx.x % blocks_h;
+    const int b = bh / p.Hkv, h = bh % p.Hkv, sub = threadIdx.x / LN, c = threadIdx.x % LN;
+    const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + h * p.vs[2] + 8 * c;
+    float most = 0.f;
+#pragma unroll 4
+    for (int u = 0; u < kRecRows / RB; ++u) {
+        const int l = blk * kRecRows + RB * u + sub;
+        float sq = 0.f;
+        if (l < p.Lk && 8 * c < p.D) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(v + l * p.vs[1]));
+            const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq += to_acc(x[i]) * to_acc(x[i]);
+        }
+#pragma unroll
+        for (int i = LN / 2; i; i >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, i);
+        if (c == 0 && l < p.Lk) {
+            const float norm = sq < INFINITY ? sqrtf(sq) : 0.f;
+            norms[static_cast<int64_t>(bh) * p.Lk + l] = norm;
+            most = fmaxf(most, norm);
         }
     }
     if (c == 0) top[sub] = most;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < RB; ++i) most = fmaxf(most, top[i]);
-        norms[blockIdx.x] = most;
+        tops[blockIdx.x] = most;
     }
+}
+
+// The largest norm of the value rows that each query sees, 512 threads a block of 128
+// queries.  (In the dq kernel itself, before its first products, it was 8 % of a call.)
+__global__ __launch_bounds__(512) void seen_norm_kernel(Params p, const float* norms, const float* tops,
+                                                        float* seen, int blocks_h) {
+    __shared__ float part_top[4][kRecRows];
+    const int bh = blockIdx.x / blocks_h, b = bh / p.Hkv, at = threadIdx.x & 127, part = threadIdx.x >> 7;
+    const int row = blockIdx.x % blocks_h * kRecRows + at, n = (p.Lk + kRecRows - 1) / kRecRows;
+    const float *one = norms + static_cast<int64_t>(bh) * p.Lk, *block = tops + static_cast<int64_t>(bh) * n;
+    int lo = 0, hi = 0;
+    if (row < p.Lq) key_span(p, b, row, p.Lk, lo, hi);
+    float top = 0.f;
+    if (hi > lo)
+        over_span(
+            lo, hi, p.Lk, part, [&](int i) { top = fmaxf(top, __ldg(one + i)); },
+            [&](int i) { top = fmaxf(top, __ldg(block + i)); });
+    part_top[part][at] = top;
+    __syncthreads();
+    if (part || row >= p.Lq) return;
+    for (int i = 1; i < 4; ++i) top = fmaxf(top, part_top[i][at]);
+    seen[static_cast<int64_t>(bh) * p.Lq + row] = top;
 }
 
 bool aligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
@@ -159,13 +227,14 @@ nsc_status tc_fwd(const Params& p, int dtype, cudaStream_t st) {
 namespace {
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t rec_bytes(int64_t B, int64_t Hq, int64_t Lq) { return round256(B * Hq * Lq * sizeof(RowRec)); }
-int64_t norm_bytes(int64_t B, int64_t Hq, int64_t Lq) {
-    return round256(B * Hq * ((Lq + kRecRows - 1) / kRecRows) * sizeof(float));
-}
+int64_t rec_blocks(int64_t L) { return (L + kRecRows - 1) / kRecRows; }
+int64_t norm_bytes(int64_t B, int64_t Hkv, int64_t L) { return round256(B * Hkv * L * sizeof(float)); }
+int64_t top_bytes(int64_t B, int64_t H, int64_t L) { return norm_bytes(B, H, rec_blocks(L)); }
 }  // namespace
 
-int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t nb) {
-    return rec_bytes(B, Hq, Lq) + norm_bytes(B, Hq, Lq) +
+int64_t tc_bwd_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t nb) {
+    return rec_bytes(B, Hq, Lq) + 2 * top_bytes(B, Hq, Lq) + norm_bytes(B, Hkv, Lk) +
+           norm_bytes(B, Hkv, Lq) + top_bytes(B, Hkv, Lk) +
            (nb ? round256(Hq * B * ((Lq + kRows - 1) / kRows) * nb * sizeof(float)) : 0);
 }
 
@@ -177,26 +246,52 @@ bool tc_bwd_fits(const Params& p, const Grads& g, int dtype) {
 nsc_status tc_bwd(const Params& p, Grads g, void* workspace, void* grad_table, int dtype,
                   cudaStream_t st) {
     char* w = static_cast<char*>(workspace);
-    RowRec* recs = reinterpret_cast<RowRec*>(w);
-    float* norms = reinterpret_cast<float*>(w + rec_bytes(p.B, p.Hq, p.Lq));
+    auto take = [&w](int64_t bytes) {
+        char* at = w;
+        w += bytes;
+        return at;
+    };
+    RowRec* recs = reinterpret_cast<RowRec*>(take(rec_bytes(p.B, p.Hq, p.Lq)));
+    float* row_norms = reinterpret_cast<float*>(take(top_bytes(p.B, p.Hq, p.Lq)));
+    float *row_deltas = nullptr, *value_norms = nullptr, *seen_norms = nullptr;
+    const int n = static_cast<int>(rec_blocks(p.Lq));
+    const unsigned blocks = static_cast<unsigned>(p.B) * p.Hq * n;
+    if (dtype == NSC_F16) {
+        row_deltas = reinterpret_cast<float*>(take(top_bytes(p.B, p.Hq, p.Lq)));
+        value_norms = reinterpret_cast<float*>(take(norm_bytes(p.B, p.Hkv, p.Lk)));
+        seen_norms = reinterpret_cast<float*>(take(norm_bytes(p.B, p.Hkv, p.Lq)));
+        float* tops = reinterpret_cast<float*>(take(top_bytes(p.B, p.Hkv, p.Lk)));
+        const int nv = static_cast<int>(rec_blocks(p.Lk));
+        auto norms = p.D <= 64 ? value_norm_kernel<__half, 8> : value_norm_kernel<__half, 16>;
+        norms<<<static_cast<unsigned>(p.B) * p.Hkv * nv, 256, 0, st>>>(p, value_norms, tops, nv);
+        nsc_status r = check_launch("token_attention backward");
+        if (r != NSC_OK) return r;
+        seen_norm_kernel<<<static_cast<unsigned>(p.B) * p.Hkv * n, 512, 0, st>>>(p, value_norms, tops,
+                                                                                seen_norms, n);
+        r = check_launch("token_attention backward");
+        if (r != NSC_OK) return r;
+    }
+    g.row_norms = row_norms;
+    g.row_deltas = row_deltas;
+    g.value_norms = value_norms;
+    g.seen_norms = seen_norms;
     if (grad_table) {
-        g.tab = w + rec_bytes(p.B, p.Hq, p.Lq) + norm_bytes(p.B, p.Hq, p.Lq);
+        g.tab = w;
         g.n_part = p.B * ((p.Lq + kRows - 1) / kRows);
     }
-    const int n = (p.Lq + kRecRows - 1) / kRecRows;
-    const unsigned blocks = static_cast<unsigned>(p.B) * p.Hq * n;
-    auto record = dtype == NSC_BF16
-                      ? (p.D <= 64 ? record_kernel<__nv_bfloat16, 8> : record_kernel<__nv_bfloat16, 16>)
-                      : (p.D <= 64 ? record_kernel<__half, 8> : record_kernel<__half, 16>);
-    record<<<blocks, 256, 0, st>>>(p, g, recs, norms, n);
+    auto record = dtype == NSC_BF16 ? (p.D <= 64 ? record_kernel<__nv_bfloat16, 8, false>
+                                                 : record_kernel<__nv_bfloat16, 16, false>)
+                                    : (p.D <= 64 ? record_kernel<__half, 8, true>
+                                                 : record_kernel<__half, 16, true>);
+    record<<<blocks, 256, 0, st>>>(p, g, recs, row_norms, row_deltas, n);
     nsc_status r = check_launch("token_attention backward");
     if (r != NSC_OK) return r;
     if (dtype == NSC_BF16)
-        r = p.D <= 64 ? tc_bwd_run<__nv_bfloat16, 64>(p, g, recs, norms, n, st)
-                      : tc_bwd_run<__nv_bfloat16, 128>(p, g, recs, norms, n, st);
+        r = p.D <= 64 ? tc_bwd_run<__nv_bfloat16, 64>(p, g, recs, st)
+                      : tc_bwd_run<__nv_bfloat16, 128>(p, g, recs, st);
     else
-        r = p.D <= 64 ? tc_bwd_run<__half, 64>(p, g, recs, norms, n, st)
-                      : tc_bwd_run<__half, 128>(p, g, recs, norms, n, st);
+        r = p.D <= 64 ? tc_bwd_run<__half, 64>(p, g, recs, st)
+                      : tc_bwd_run<__half, 128>(p, g, recs, st);
     if (r == NSC_OK && grad_table) r = launch_table_join(p, g, grad_table, st);
     return r;
 }

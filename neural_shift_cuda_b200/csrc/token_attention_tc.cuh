@@ -48,13 +48,23 @@ nsc_status tc_ready(const void* kern, int smem, int threads, int registers);
 
 template <typename T, int DP> nsc_status tc_fwd_run(const Params& p, cudaStream_t st);
 template <typename T, int DP>
-nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, const float* norms,
-                      int n_norm, cudaStream_t st);
+nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, cudaStream_t st);
 
 // A query row as the backward kernels read it: the forward's statistics (m NaN
 // where delta is not finite), delta, and the norm of its output gradient.
 struct RowRec { float m, ll, delta, norm; };
-constexpr int kRecRows = 128;  // rows of a record block, and of one entry of `norms`
+constexpr int kRecRows = 128;  // rows of a record block, and of one entry of their largest norms
+
+// Every fourth row (from the part-th) of [lo, hi) of n, rows of a whole record block at once.
+template <typename One, typename Block>
+__device__ __forceinline__ void over_span(int lo, int hi, int n, int part, One one, Block block) {
+    const int first = (lo + kRecRows - 1) / kRecRows;
+    const int last = hi == n ? (n + kRecRows - 1) / kRecRows : hi / kRecRows;   // (the end's is whole)
+    const int a = first < last ? first * kRecRows : hi, b = first < last ? last * kRecRows : hi;
+    for (int i = first + part; i < last; i += 4) block(i);
+    for (int i = lo + part; i < a; i += 4) one(i);
+    for (int i = b + part; i < hi; i += 4) one(i);
+}
 
 // A tile: ROWS rows from `row` of head `h`, DP / 64 panels.
 template <int DP, int ROWS = kRows>

@@ -30,10 +30,12 @@
 // products of 34 GF: 566 and 393 TF/s).  8192 tokens in 4 documents, causal, capped,
 // 16 / 4 heads of 128: dkv 358 us, dq 269 us.
 //
-// fp16: weights and score gradients of long rows lie below its normal range.
-// P is held times 2^6 and the gradient of a row divided by a power of two near
-// the norm of its dO (dq) or the largest such norm of the key's queries (dkv);
-// both are undone in fp32 at the end.
+// fp16: weights and score gradients of long rows lie below its normal range, and those of
+// large values or large gradients of lse above it.  P is held times 2^6, and P (dP - delta)
+// over a power of two g that bounds it: |dP - delta| <= |dO| |v| + |delta|, with the largest
+// norm of the values that the query sees (dq), or the largest |dO| and |delta| of the
+// queries that see the key (dkv).  Each lane, a query or a key, has a g of its own from
+// what it sees alone; products are then below 2^14.  Both factors are undone in fp32 at the end.
 #pragma once
 
 #include "token_attention_tc.cuh"
@@ -61,19 +63,17 @@ struct BwdBars {
     uint64_t drain[2];
 };
 
-__device__ __forceinline__ float pow2_near(float v) {   // a power of two at or above v, or 1
-    if (!(v > 0.f) || !(v < 3e38f)) return 1.f;
-    const int e = static_cast<int>((__float_as_uint(v) >> 23) & 0xFF) + 1;
-    return __uint_as_float(static_cast<uint32_t>(min(max(e, 20), 230)) << 23);
+// The g of score gradients whose factor beside P is at most v: a power of two above v, over 2^8.
+__device__ __forceinline__ float gradient_scale(float v) {
+    if (!(v > 0.f) || !(v < INFINITY)) return 1.f;
+    const int e = static_cast<int>((__float_as_uint(v) >> 23) & 0xFF) + 1 - 8;
+    return __uint_as_float(static_cast<uint32_t>(min(max(e, 20), 246)) << 23);
 }
-
 template <typename T, int DP, bool CAP, bool BIAS>
 __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mo,
     const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p,
-    const Grads gr, const RowRec* __restrict__ recs, const float* __restrict__ norms, const int n_norm,
-    const int split,
-    const Bounded bnd) {
+    const Grads gr, const RowRec* __restrict__ recs, const int split, const Bounded bnd) {
     using S = BwdShape<DP>;
     constexpr int NS = S::stages;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -82,8 +82,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag[2];
     __shared__ int span[4];
-    __shared__ unsigned top_norm;
-    // per stage: -m (or -(m + ll) without bias), -ll, delta g
+    __shared__ float2 tops[kBf16 ? 1 : 4][kRows];   // largest |dO| and |delta| of a quarter of the queries
+    // per stage: -m (or -(m + ll) without bias), -ll, -delta
     __shared__ __align__(16) float rows[NS][3][kRows];
     unsigned char* smem = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -126,7 +126,6 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         fence_mbar_init();
         abort_flag[0] = 0;
         abort_flag[1] = static_cast<int>(bnd.budget);
-        top_norm = 0;
     }
     if (warp == 17) tc::tmem_alloc(&tmem_slot, 512);
     __syncthreads();
@@ -146,24 +145,12 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         }
     }
     __syncthreads();
-    if (!kBf16 && span[1] > span[0]) {   // the largest norm of dO among the queries of this tile
-        const int n0 = span[0] / kRows * (kRows / kRecRows);
-        const int n = min((span[1] + kRows - 1) / kRows * (kRows / kRecRows), n_norm) - n0;
-        const float* src = norms + (static_cast<int64_t>(b) * p.Hq + hk * p.G) * n_norm + n0;
-        float top = 0.f;
-        for (int i = threadIdx.x; i < p.G * n; i += kBwdThreads)
-            top = fmaxf(top, src[static_cast<int64_t>(i / n) * n_norm + i % n]);
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-        if (lane == 0) atomicMax(&top_norm, __float_as_uint(top));
-    }
-    __syncthreads();
     const uint32_t tmem = tc::uniform(tmem_slot);
     const int s_lo = tc::uniform(span[0]), s_hi = tc::uniform(span[1]);
     const int all_lo = tc::uniform(span[2]), all_hi = tc::uniform(span[3]);
     const int fb = s_hi > s_lo ? s_lo / kRows : 0;
     const int lb = s_hi > s_lo ? (s_hi + kRows - 1) / kRows : 0;
     const int nq = lb - fb, total = nq * heads;
-    const float g = kBf16 ? 1.f : pow2_near(__uint_as_float(top_norm));
     // a key tail past Lk has zero rows of K and V, and sees nothing
     auto guarded = [&](int j) {
         return !(j * kRows >= all_lo && min((j + 1) * kRows, p.Lq) <= all_hi);
@@ -188,8 +175,35 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
         const Cap<T> cap(y1, unit);
         const float2 u2 = CAP ? make_float2(1.f, 1.f) : make_float2(unit, unit);
-        const float2 g2 = make_float2(1.f / g, 1.f / g);
         const float2 slope2 = make_float2(-1.f / (unit * unit), -1.f / (unit * unit));   // 1 - tanh^2 = 1 + s^2 slope
+        float g = 1.f;
+        if (!kBf16) {
+            float2 top = make_float2(0.f, 0.f);
+            const int n = (p.Lq + kRecRows - 1) / kRecRows;
+            for (int u = 0; u < heads && hi > lo; ++u) {
+                const int64_t bq = static_cast<int64_t>(b) * p.Hq + head0 + u;
+                over_span(lo, hi, p.Lq, part,
+                          [&](int i) {
+                              const float4 r = __ldg(reinterpret_cast<const float4*>(recs + bq * p.Lq + i));
+                              top.x = fmaxf(top.x, r.w);
+                              if (fabsf(r.z) < INFINITY) top.y = fmaxf(top.y, fabsf(r.z));
+                          },
+                          [&](int i) {
+                              top.x = fmaxf(top.x, __ldg(gr.row_norms + bq * n + i));
+                              top.y = fmaxf(top.y, __ldg(gr.row_deltas + bq * n + i));
+                          });
+            }
+            const int at = threadIdx.x & 127;
+            tops[part][at] = top;
+            named_sync(1, kBwdMath);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                top = make_float2(fmaxf(top.x, tops[i][at].x), fmaxf(top.y, tops[i][at].y));
+            if (hi > lo)
+                g = gradient_scale(top.x * __ldg(gr.value_norms + bh * static_cast<int64_t>(p.Lk) + key) +
+                                   top.y);
+        }
+        const float2 g2 = make_float2(1.f / g, 1.f / g);
         bool alive = true;
         int it = 0;
         for (int u = 0; u < heads && nq > 0; ++u) {
@@ -254,6 +268,10 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     }
                     w[2 * i] = tc::pack2<T>(p0.x, p0.y);
                     w[2 * i + 1] = tc::pack2<T>(p1.x, p1.y);
+                    if (!kBf16) {   // over g from here on
+                        p0 = __fmul2_rn(p0, g2);
+                        p1 = __fmul2_rn(p1, g2);
+                    }
                     if (CAP) {   // keep p (1 - tanh^2)
                         const float2 n0 = __fmul2_rn(__fmul2_rn(s[2 * i], s[2 * i]), slope2);
                         const float2 n1 = __fmul2_rn(__fmul2_rn(s[2 * i + 1], s[2 * i + 1]), slope2);
@@ -280,14 +298,8 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float4 dl = d4[i];
-                    float2 a0, a1;
-                    if (kBf16) {
-                        a0 = __fadd2_rn(d[2 * i], make_float2(dl.x, dl.y));
-                        a1 = __fadd2_rn(d[2 * i + 1], make_float2(dl.z, dl.w));
-                    } else {
-                        a0 = __ffma2_rn(d[2 * i], g2, make_float2(dl.x, dl.y));
-                        a1 = __ffma2_rn(d[2 * i + 1], g2, make_float2(dl.z, dl.w));
-                    }
+                    float2 a0 = __fadd2_rn(d[2 * i], make_float2(dl.x, dl.y));
+                    float2 a1 = __fadd2_rn(d[2 * i + 1], make_float2(dl.z, dl.w));
                     a0 = __fmul2_rn(a0, s[2 * i]);
                     a1 = __fmul2_rn(a1, s[2 * i + 1]);
                     if (!whole) {   // (a hidden pair's dP need not be finite)
@@ -466,7 +478,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dkv_kernel(
                     if (bad >> r & 1) m = NAN;
                     rows[s][0][at] = BIAS ? m : m + ll;
                     rows[s][1][at] = ll;
-                    rows[s][2][at] = -rec[r].z / g;
+                    rows[s][2][at] = -rec[r].z;
                 }
                 mbar_arrive(&bars.ok[s]);
             }
@@ -605,15 +617,20 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
         const uint32_t at_s = t_s + lane_base + 32 * part, at_dp = t_dp + lane_base + 32 * part;
         const float unit = static_cast<float>((p.cap > 0 ? p.cap : p.scale) * kLog2e);
         const float y1 = p.cap > 0 ? static_cast<float>(p.scale / p.cap) : 0.f;
-        float m = -INFINITY, ll = 0.f, delta = 0.f, g = 1.f;
+        float m = -INFINITY, ll = 0.f, delta = 0.f, norm = 0.f, g = 1.f;
         // (a row that sees nothing keeps its zeros, whatever its output gradient holds)
         if (hi > lo) {
             const float4 r = __ldg(reinterpret_cast<const float4*>(
                 recs + (static_cast<int64_t>(b) * p.Hq + h) * p.Lq + row));
-            if (!kBf16) g = pow2_near(r.w);
             m = r.x == -INFINITY ? r.x : -r.x;
             ll = -r.y + (kBf16 ? 0.f : kPShift);
-            delta = -r.z / g;
+            delta = -r.z;
+            norm = r.w;
+        }
+        if (!kBf16 && hi > lo) {
+            g = gradient_scale(norm * __ldg(gr.seen_norms + (static_cast<int64_t>(b) * p.Hkv + hk) * p.Lq + row) +
+                               fabsf(delta));
+            delta /= g;
         }
         if (!BIAS) m += ll;
         const Cap<T> cap(y1, unit);
@@ -881,8 +898,7 @@ __global__ __launch_bounds__(kBwdThreads, 1) void tc_dq_kernel(
 }
 
 template <typename T, int DP, bool CAP, bool BIAS>
-nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, const float* norms,
-                         int n_norm, cudaStream_t st) {
+nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, cudaStream_t st) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     auto kk = tc_dkv_kernel<T, DP, CAP, BIAS>;
     auto kq = tc_dq_kernel<T, DP, CAP, BIAS>;
@@ -916,7 +932,7 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, co
     const int64_t nk = tiles * split;
     const int64_t nq = static_cast<int64_t>((p.Lq + kRows - 1) / kRows) * p.B * p.Hq;
     ready = launch_cluster("token_attention backward", kk, nk, kBwdThreads, smk, split, st, mq, mo, mk,
-                           mv, p, g, recs, norms, n_norm, split, bnd);
+                           mv, p, g, recs, split, bnd);
     if (ready != NSC_OK) return ready;
     kq<<<static_cast<unsigned>(nq), kBwdThreads, smq, st>>>(mq, mo, mk, mv, p, g, recs, bnd);
     return check_launch("token_attention backward");
@@ -925,14 +941,13 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, co
 }  // namespace
 
 template <typename T, int DP>
-nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, const float* norms,
-                      int n_norm, cudaStream_t st) {
+nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, cudaStream_t st) {
     const RowRec* r = static_cast<const RowRec*>(recs);
     if (p.cap > 0)
-        return p.table ? tc_bwd_launch<T, DP, true, true>(p, g, r, norms, n_norm, st)
-                       : tc_bwd_launch<T, DP, true, false>(p, g, r, norms, n_norm, st);
-    return p.table ? tc_bwd_launch<T, DP, false, true>(p, g, r, norms, n_norm, st)
-                   : tc_bwd_launch<T, DP, false, false>(p, g, r, norms, n_norm, st);
+        return p.table ? tc_bwd_launch<T, DP, true, true>(p, g, r, st)
+                       : tc_bwd_launch<T, DP, true, false>(p, g, r, st);
+    return p.table ? tc_bwd_launch<T, DP, false, true>(p, g, r, st)
+                   : tc_bwd_launch<T, DP, false, false>(p, g, r, st);
 }
 
 }  // namespace tok

@@ -3,7 +3,7 @@
 
 namespace nsc {
 namespace tok {
-template nsc_status tc_bwd_run<__nv_bfloat16, 64>(const Params&, const Grads&, const void*, const float*, int,
+template nsc_status tc_bwd_run<__nv_bfloat16, 64>(const Params&, const Grads&, const void*,
                                          cudaStream_t);
 }  // namespace tok
 }  // namespace nsc

@@ -183,3 +183,57 @@ def test_table_gradient_and_pairs_that_are_not_seen(cuda, dt, D, bad, cap, causa
     assert torch.equal(got[:27], clean[:27]) and torch.equal(got[30 + last + 1:],
                                                              clean[30 + last + 1:])
     assert not torch.isfinite(got[27:30 + last + 1]).any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("go_mul,lse_mul", [(1e-4, 1.0), (0.0, 2000.0), (1.0, 1e-3), (1.0, 30.0)])
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+def test_fp16_gradients_of_lse(cuda, D, go_mul, lse_mul, cap):
+    """Gradients of lse far above those of the output."""
+    B, L, Hq, Hkv = 2, 300, 4, 2
+    q = randn(0, B, L, Hq, D, dtype=F16).to(cuda)
+    k, v = (randn(i, B, L, Hkv, D, dtype=F16).to(cuda) for i in (1, 2))
+    go = randn(3, B, L, Hq, D, dtype=F16, mul=go_mul).to(cuda)
+    gl = randn(4, B, Hq, L, dtype=F32, mul=lse_mul).to(cuda)
+    doc = [[0, 7, 130, 290], [0, 1, 2, 300]]
+    want = reference(q, k, v, T.visible(B, L, L, True, None, doc), go, D ** -0.5, cap, glse=gl)
+    leaves = [leaf(t) for t in (q, k, v)]
+    out, lse = nsc.token_attention(*leaves, causal=True, documents=torch.tensor(doc, device=cuda),
+                                   softcap=cap, return_lse=True)
+    got = torch.autograd.grad([out, lse], leaves, [go, gl])
+    for name, g, w in zip(("grad_q", "grad_k", "grad_v"), got, want[2:5]):
+        check(g, w, F16, name)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("v_mul", [300.0, 4000.0])
+def test_fp16_gradients_of_large_values(cuda, D, v_mul):
+    """Value rows of norms in the thousands and more."""
+    B, L, Hq, Hkv = 2, 333, 4, 2
+    q = randn(0, B, L, Hq, D, dtype=F16).to(cuda)
+    k = randn(1, B, L, Hkv, D, dtype=F16).to(cuda)
+    v = randn(2, B, L, Hkv, D, dtype=F16, mul=v_mul).to(cuda)
+    go = randn(3, B, L, Hq, D, dtype=F16).to(cuda)
+    want = reference(q, k, v, T.visible(B, L, L, True), go, D ** -0.5)
+    leaves = [leaf(t) for t in (q, k, v)]
+    out = nsc.token_attention(*leaves, causal=True)
+    got = torch.autograd.grad(out, leaves, go)
+    for name, g, w in zip(("grad_q", "grad_k", "grad_v"), got, want[2:5]):
+        check(g, w, F16, name)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_beside_a_document_of_large_values(cuda, D):
+    """The scale of one document's values and gradients is no matter of the others'."""
+    L = 300
+    q, k, v, go = (randn(i, 1, L, 2, D, dtype=F16).to(cuda) for i in range(4))
+    doc = torch.tensor([[0, 140, 290]], device=cuda)
+    leaves = [leaf(t) for t in (q, k, v)]
+    ref = torch.autograd.grad(nsc.token_attention(*leaves, documents=doc), leaves, go)
+    v2, go2 = v.clone(), go.clone()
+    v2[:, 140:] *= 3000
+    go2[:, 140:] *= 300
+    leaves = [leaf(t) for t in (q, k, v2)]
+    got = torch.autograd.grad(nsc.token_attention(*leaves, documents=doc), leaves, go2)
+    for a, b in zip(got, ref):
+        assert torch.equal(a[:, :140], b[:, :140])
