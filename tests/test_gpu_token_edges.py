@@ -237,3 +237,22 @@ def test_fp16_gradients_beside_a_document_of_large_values(cuda, D):
     got = torch.autograd.grad(nsc.token_attention(*leaves, documents=doc), leaves, go2)
     for a, b in zip(got, ref):
         assert torch.equal(a[:, :140], b[:, :140])
+
+
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("cap", [200.0, 1e3, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("form", ["short", "decode"])
+def test_large_caps_short_and_decode(cuda, dt, cap, form):
+    """Scores far below the cap are as if there was none: their digits are their own, not
+    those of the cap.  Prompt, short rows and cache agree."""
+    Lq, Lk, D = (48, 48, 32) if form == "short" else (1, 400, 64)
+    q = randn(0, 2, Lq, 4, D, dtype=dt, mul=2.0).to(cuda)
+    k, v = (randn(i, 2, Lk, 2, D, dtype=dt, mul=2.0).to(cuda) for i in (1, 2))
+    want, wl = T.attention(q, k, v, T.visible(2, Lq, Lk, True), D ** -0.5, cap)
+    if form == "short":
+        out, lse = nsc.token_attention(q, k, v, causal=True, softcap=cap, return_lse=True)
+    else:
+        n = torch.full((2,), Lk, dtype=torch.int32, device=cuda)
+        out, lse = nsc.token_attention_decode(q, k, v, n, softcap=cap, return_lse=True)
+    check(out, want, dt, "out")
+    check(lse, wl, F32, "lse", 8.0)
