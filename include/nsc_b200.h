@@ -364,7 +364,7 @@ NSC_API nsc_status nsc_qk_norm_rotate_bwd(const nsc_norm_rotate* a,
  * unit stride in D; out (B, Lq, Hq, D) contiguous, lse (B, Hq, Lq) fp32
  * (fp64).  Query i stands at position pos = i + n - Lq, n = Lk or lengths[b].
  *     s(i, j) = c tanh(scale q_i.k_j / c) + table[buckets[clamp(j - pos, -reach,
- *               reach) + reach], h]            (c = softcap; 0: no cap)
+ *               reach) + reach], h]            (c = softcap, 1e-30..1e30; 0: no cap)
  *     out_i   = sum_j softmax_j(s) v_j over the visible j,  lse_i = log sum_j e^s
  * Visible are the keys j < n of the same document (documents: `docs` + 1
  * ascending int32 bounds per batch entry, docs_stride apart, Lq == Lk; a token

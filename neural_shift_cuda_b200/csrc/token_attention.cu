@@ -26,8 +26,8 @@ nsc_status check(const char* op, const nsc_attention* a, bool need_ptrs) {
     if (a->Lq >= (1LL << 30) || a->Lk >= (1LL << 30) || a->Hq >= (1LL << 16) ||
         a->B * a->Hq >= (1LL << 31) / ((a->Lq > a->Lk ? a->Lq : a->Lk) / 32 + 2))
         return fail(NSC_ERR_INVALID_ARG, "%s: too many tokens", op);
-    if (!(a->softcap >= 0) || a->softcap > 1e30)
-        return fail(NSC_ERR_INVALID_ARG, "%s: softcap must be >= 0 and finite", op);
+    if (!(a->softcap >= 0) || a->softcap > 1e30 || (a->softcap > 0 && a->softcap < 1e-30))
+        return fail(NSC_ERR_INVALID_ARG, "%s: softcap must be 0 or in 1e-30..1e30", op);
     if (a->documents && (a->docs < 1 || a->Lq != a->Lk))
         return fail(NSC_ERR_INVALID_ARG, "%s: documents need at least two bounds and Lq == Lk", op);
     if (a->prefix && !a->causal)

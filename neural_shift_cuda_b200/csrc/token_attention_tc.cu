@@ -2,6 +2,7 @@
 // which calls they take, tensor maps, shared-memory and register checks.
 #include <cudaTypedefs.h>
 
+#include <cmath>
 #include <mutex>
 #include <unordered_map>
 
@@ -157,6 +158,13 @@ bool boxable(const int64_t* s, int B, int L, int H) {
     return true;
 }
 
+// Whether the cap's coefficients, up to scale (scale / cap)^10, and the slope's 1 / cap^2 are
+// finite in fp32 (infinite ones give NaN where a score is zero).  A cap of a thousandth of
+// the scale, or less, takes the kernels that call tanh.
+bool cap_in_range(const Params& p) {
+    return !(p.cap > 0) || (p.cap > 1e-15 && p.scale * pow(p.scale / p.cap, 10.) < 1e37);
+}
+
 }  // namespace
 
 bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, int B, int L, int H,
@@ -211,7 +219,7 @@ nsc_status tc_ready(const void* kern, int smem, int threads, int registers) {
 
 bool tc_fits(const Params& p, int dtype) {
     return (dtype == NSC_F16 || dtype == NSC_BF16) && p.D % 8 == 0 && p.D <= 128 && p.Lk > 0 &&
-           !p.lengths && static_cast<float>(p.scale) > 1e-30f && aligned(p.q) && aligned(p.k) &&
+           !p.lengths && static_cast<float>(p.scale) > 1e-30f && cap_in_range(p) && aligned(p.q) && aligned(p.k) &&
            aligned(p.v) && aligned(p.out) && aligned(p.residue) &&
            boxable(p.qs, p.B, p.Lq, p.Hq) && boxable(p.ks, p.B, p.Lk, p.Hkv) &&
            boxable(p.vs, p.B, p.Lk, p.Hkv);

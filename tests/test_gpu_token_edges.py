@@ -256,3 +256,28 @@ def test_large_caps_short_and_decode(cuda, dt, cap, form):
         out, lse = nsc.token_attention_decode(q, k, v, n, softcap=cap, return_lse=True)
     check(out, want, dt, "out")
     check(lse, wl, F32, "lse", 8.0)
+
+
+@pytest.mark.parametrize("dt,D", [(F16, 64), (BF16, 128), (F32, 64), (BF16, 32)])
+@pytest.mark.parametrize("cap", [1e-3, 1e-5, 1e-8, 1e-12, 1e-20, 1e-30])
+@pytest.mark.parametrize("L", [40, 300])
+def test_small_caps(cuda, dt, D, cap, L):
+    """Scores of zero stay zero, with a gradient, and all others are the cap's."""
+    k, v, go = (randn(i, 1, L, 2, D, dtype=dt).to(cuda) for i in range(3))
+    q = torch.zeros_like(k)
+    want = reference(q, k, v, T.visible(1, L, L, True), go, D ** -0.5, cap)
+    leaves = [leaf(t) for t in (q, k, v)]
+    out = nsc.token_attention(*leaves, causal=True, softcap=cap)
+    check(out, want[0], dt, "out")
+    for name, g, w in zip(("grad_q", "grad_k", "grad_v"),
+                          torch.autograd.grad(out, leaves, go), want[2:5]):
+        check(g, w, dt, name)
+    q = randn(5, 1, L, 2, D, dtype=dt).to(cuda)
+    leaves = [leaf(t) for t in (q, k, v)]
+    want = reference(q, k, v, T.visible(1, L, L, True), go, D ** -0.5, cap)
+    out = nsc.token_attention(*leaves, causal=True, softcap=cap)
+    check(out, want[0], dt, "out")
+    for g in torch.autograd.grad(out, leaves, go):
+        assert torch.isfinite(g).all()
+    n = torch.tensor([L], dtype=torch.int32, device=cuda)
+    check(nsc.token_attention_decode(q[:, -1:], k, v, n, softcap=cap), want[0][:, -1:], dt)

@@ -121,6 +121,16 @@ def test_empty_calls_are_noops():
     assert lib.nsc_qk_norm_rotate_workspace(ctypes.byref(n)) == -1
 
 
+@pytest.mark.parametrize("cap", [1e-31, 1e-300, 1e31, float("inf")])
+def test_caps_that_32_bits_do_not_hold_are_refused(cap):
+    lib = _lib.load()
+    a = _att(softcap=cap, causal=1)
+    for st in (lib.nsc_token_attention_fwd(ctypes.byref(a), *[None] * 5),
+               lib.nsc_token_attention_decode(ctypes.byref(a), *[None] * 4)):
+        assert st == 1 and "softcap" in lib.nsc_last_error_string().decode()
+    assert lib.nsc_token_attention_bwd_workspace(ctypes.byref(a)) == -1
+
+
 def test_workspaces_that_are_not_aligned_are_refused():
     lib = _lib.load()
     a = _att(causal=1, q=256, k=256, v=256)
