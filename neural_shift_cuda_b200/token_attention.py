@@ -23,6 +23,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -42,6 +43,16 @@ def _require_cuda(op: str, q: torch.Tensor) -> None:
             f"neural_shift_cuda_b200.{op}: expects CUDA tensors (got a "
             f"{q.device} tensor); this package has no CPU path")
     _lib.load()
+
+
+def _refuse_tangents(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A call that records no graph passes by the autograd functions, which would refuse
+    tangents: they would be dropped."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{op} has no forward-mode derivative")
 
 
 def _check_heads(op: str, name: str, t: torch.Tensor) -> None:
@@ -212,6 +223,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor,
                            f"{tuple(cos.shape)}, {tuple(sin.shape)}")
     if cos.device != q.device or sin.device != q.device:
         raise ValueError(f"{op}: cos and sin must be on {q.device}")
+    _refuse_tangents(op, q, k, q_weight, k_weight, cos, sin)
     _require_cuda(op, q)
     if positions is not None:
         positions = _int32(op, "positions", positions, q.device)
@@ -405,6 +417,7 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     table, buckets = _check_bias(op, q, bias_table, bias_buckets)
     if prefix is not None and not causal:
         raise ValueError(f"{op}: a prefix needs causal=True")
+    _refuse_tangents(op, q, k, v, table)
     _require_cuda(op, q)
     if documents is not None:
         documents = _int32(op, "documents", documents, dev)
@@ -506,6 +519,7 @@ def token_attention_decode(q: torch.Tensor, k_cache: torch.Tensor,
             or (table is not None and table.requires_grad)):
         raise RuntimeError(f"{op} has no backward; use token_attention, or "
                            f"torch.no_grad()")
+    _refuse_tangents(op, q, k_cache, v_cache, table)
     _require_cuda(op, q)
     lengths = _int32(op, "lengths", lengths, q.device)
     if lengths.shape != (q.shape[0],):

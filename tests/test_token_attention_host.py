@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad as fwd
 
 import neural_shift_cuda_b200 as nsc
 from neural_shift_cuda_b200 import _lib
@@ -56,6 +57,31 @@ def test_decode_refuses_gradients():
     q, k, v = _qkv()
     with pytest.raises(RuntimeError, match="no backward"):
         nsc.token_attention_decode(q.requires_grad_(), k, v, torch.ones(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_tangents_are_refused(no_grad):
+    """Dropped, they would give a derivative of zero without a word."""
+    q, k, v = _qkv()
+    table, m = torch.zeros(4, 2), torch.zeros(3, dtype=torch.int32)
+    n, cos, w = torch.ones(1, dtype=torch.int32), torch.zeros(4, 4), torch.zeros(8)
+    with fwd.dual_level(), torch.set_grad_enabled(not no_grad):
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        bias = dict(bias_table=dual(table), bias_buckets=m)
+        for call in (lambda: nsc.token_attention(dual(q), k, v),
+                     lambda: nsc.token_attention(q, k, dual(v)),
+                     lambda: nsc.token_attention(q, k, v, **bias),
+                     lambda: nsc.token_attention_decode(q, dual(k), v, n),
+                     lambda: nsc.token_attention_decode(q, k, v, n, **bias),
+                     lambda: nsc.qk_norm_rotate(q, dual(k), None, None, cos, cos),
+                     lambda: nsc.qk_norm_rotate(q, k, dual(w), None, cos, cos),
+                     lambda: nsc.qk_norm_rotate(q, k, None, None, cos, dual(cos))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        # (tensors without tangents pass this check inside a level too)
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            nsc.token_attention(q, k, v)
 
 
 def test_rotate_refusals():
