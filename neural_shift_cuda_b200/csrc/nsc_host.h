@@ -38,6 +38,13 @@ inline nsc_status check_launch(const char* op) {
     return ok();
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory on the current device.  The limit is
+// only ever raised, under a lock: set to each call's own size, one thread would lower it
+// between another's setting and launch.  With `registers`, refuses a kernel whose launch of
+// `threads` would hold fewer (its warps share them out, and would wait for good).
+nsc_status raise_shared(const char* op, const void* kern, size_t bytes, int threads = 0,
+                        int registers = 0);
+
 inline bool valid_dtype(int dt) { return dt >= NSC_F16 && dt <= NSC_F64; }
 
 inline size_t dtype_size(int dt) {

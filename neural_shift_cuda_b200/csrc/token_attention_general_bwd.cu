@@ -385,8 +385,10 @@ nsc_status launch(const Params& p, const Grads& g, cudaStream_t st) {
     const size_t smq = gen_smem<A, DP, TL>(4, 1, extra), smk = gen_smem<A, DP, TL>(4, 2, extra);
     auto kq = general_dq_kernel<T, A, DP, TL>;
     auto kk = general_dkv_kernel<T, A, DP, TL>;
-    cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smq));
-    cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smk));
+    const char* op = "token_attention backward";
+    nsc_status r = raise_shared(op, reinterpret_cast<const void*>(kq), smq);
+    if (r == NSC_OK) r = raise_shared(op, reinterpret_cast<const void*>(kk), smk);
+    if (r != NSC_OK) return r;
     const int64_t nq = static_cast<int64_t>((p.Lq + TL - 1) / TL) * p.B * p.Hq;
     const int64_t nk = static_cast<int64_t>((p.Lk + TL - 1) / TL) * p.B * p.Hkv;
     // blocks of a tile: up to about four an SM in all, none without a step
@@ -395,10 +397,8 @@ nsc_status launch(const Params& p, const Grads& g, cudaStream_t st) {
         while (n < 8 && tiles * n * 2 <= 4 * 148 && n * 2 <= steps) n *= 2;
         return n;
     };
-    const char* op = "token_attention backward";
     const int nqt = (p.Lq + TL - 1) / TL, nkt = (p.Lk + TL - 1) / TL;
     const int sk = share_of(nk, static_cast<int64_t>(p.G) * nqt), sq = share_of(nq, nkt);
-    nsc_status r = NSC_OK;
     if (nk) r = launch_cluster(op, kk, nk * sk, kGenThreads, smk, sk, st, p, g, sk);
     if (r == NSC_OK && nq) r = launch_cluster(op, kq, nq * sq, kGenThreads, smq, sq, st, p, g, sq);
     if (r != NSC_OK) return r;

@@ -134,8 +134,8 @@ nsc_status launch(const Params& p, cudaStream_t st) {
     const int64_t blocks = static_cast<int64_t>((p.Lq + TL - 1) / TL) * p.B * p.Hq;
     const size_t smem = gen_smem<A, DP, TL>(3, 1, p.table ? 2 * p.reach + 1 : 0);
     auto kern = general_fwd_kernel<T, A, DP, TL>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(smem));
+    const nsc_status ready = raise_shared("token_attention", reinterpret_cast<const void*>(kern), smem);
+    if (ready != NSC_OK) return ready;
     kern<<<static_cast<unsigned>(blocks), kGenThreads, smem, st>>>(p);
     return check_launch("token_attention");
 }

@@ -9,7 +9,6 @@
 // (33 MB, 1.9 TB/s) against 38 us; heads of 64: 25 against 40.
 // Products are those of a warp (m16n8k16); a row's statistics lie in the four lanes
 // that hold its scores.
-#include <atomic>
 #include <climits>
 
 #include "token_warp_mma.cuh"

@@ -3,8 +3,6 @@
 #include <cudaTypedefs.h>
 
 #include <cmath>
-#include <mutex>
-#include <unordered_map>
 
 #include "token_attention_tc.cuh"
 
@@ -191,30 +189,6 @@ bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, in
         return false;
     }
     return true;
-}
-
-nsc_status tc_ready(const void* kern, int smem, int threads, int registers) {
-    // the largest shared memory asked for so far of (device, kernel)
-    static std::mutex mu;
-    static std::unordered_map<uint64_t, int> asked;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess)
-        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: no current device");
-    const uint64_t key = reinterpret_cast<uint64_t>(kern) * 64 + static_cast<uint64_t>(dev);
-    std::lock_guard<std::mutex> lock(mu);
-    auto hit = asked.find(key);
-    if (hit != asked.end() && hit->second >= smem) return NSC_OK;
-    cudaFuncAttributes at{};
-    if (cudaFuncGetAttributes(&at, kern) != cudaSuccess)
-        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: kernel is not available");
-    if (at.numRegs * threads < registers)
-        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: kernel holds %d registers a thread",
-                    at.numRegs);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-        cudaSuccess)
-        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention: %d bytes of shared memory", smem);
-    asked[key] = smem;
-    return NSC_OK;
 }
 
 bool tc_fits(const Params& p, int dtype) {

@@ -41,11 +41,6 @@ __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, uns
 bool encode_heads(CUtensorMap* map, const void* base, const int64_t* strides, int B, int L, int H,
                   int D, bool bf16, const char** err, int rows = kRows);
 
-// Prepares a kernel's shared memory, and refuses one whose launch would hold fewer
-// registers than its warps ask for when they share them out (they would wait
-// for good).
-nsc_status tc_ready(const void* kern, int smem, int threads, int registers);
-
 template <typename T, int DP> nsc_status tc_fwd_run(const Params& p, cudaStream_t st);
 template <typename T, int DP>
 nsc_status tc_bwd_run(const Params& p, const Grads& g, const void* recs, cudaStream_t st);

@@ -906,8 +906,10 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, cu
     const int smk = BwdShape<DP>::smem + 1024 + e;
     const int smq = smk + (BIAS && g.tab ? 4 * 16 * p.nb : 0);
     const int regs = kBwdMath * kMathRegs + 128 * kOtherRegs;
-    nsc_status ready = tc_ready(reinterpret_cast<const void*>(kk), smk, kBwdThreads, regs);
-    if (ready == NSC_OK) ready = tc_ready(reinterpret_cast<const void*>(kq), smq, kBwdThreads, regs);
+    const char* op = "token_attention backward";
+    nsc_status ready = raise_shared(op, reinterpret_cast<const void*>(kk), smk, kBwdThreads, regs);
+    if (ready == NSC_OK)
+        ready = raise_shared(op, reinterpret_cast<const void*>(kq), smq, kBwdThreads, regs);
     if (ready != NSC_OK) return ready;
     CUtensorMap mq, mo, mk, mv;
     const char* err = nullptr;

@@ -400,8 +400,8 @@ nsc_status tc_fwd_launch(const Params& p, cudaStream_t st) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     auto kern = tc_fwd_kernel<T, DP, CAP, BIAS, REST>;
     const int smem = FwdShape<DP>::smem + 1024 + (BIAS ? 4 * (2 * p.reach + 2 * kBiasPad + 1) : 0);
-    nsc_status ready = tc_ready(reinterpret_cast<const void*>(kern), smem, kFwdThreads,
-                                128 * kFwdMathRegs + 128 * kFwdOtherRegs);
+    nsc_status ready = raise_shared("token_attention", reinterpret_cast<const void*>(kern), smem, kFwdThreads,
+                                    128 * kFwdMathRegs + 128 * kFwdOtherRegs);
     if (ready != NSC_OK) return ready;
     CUtensorMap mq, mk, mv;
     const char* err = nullptr;

@@ -21,7 +21,6 @@
 // decode_any_kernel: any type, width and alignment, 8 rows a block, tile by tile through
 // shared memory.
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "token_warp_mma.cuh"
@@ -890,17 +889,9 @@ nsc_status launch_mma(const Params& p, const Split& s, unsigned blocks, cudaStre
     const int ring = kWarps * NS * 2 * 16 * LD + (MT > 1 ? 16 * MT * LD : 0);
     const int heads = p.G < 16 * MT ? p.G : 16 * MT;
     const int smem = ring + (BIAS ? 4 * heads * p.nb + p.reach + 1 : 0);
-    static std::atomic<int> asked[64];   // by device: shared memory set so far
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return fail(NSC_ERR_LAUNCH_FAILED, "token_attention_decode: no current device");
-    if (asked[dev].load() < smem) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-            cudaSuccess)
-            return fail(NSC_ERR_LAUNCH_FAILED, "token_attention_decode: %d bytes of shared memory",
-                        smem);
-        asked[dev].store(smem);
-    }
+    const nsc_status ready =
+        raise_shared("token_attention_decode", reinterpret_cast<const void*>(kern), smem);
+    if (ready != NSC_OK) return ready;
     kern<<<blocks, kMmaThreads, smem, st>>>(p, s);
     return check_launch("token_attention_decode");
 }
@@ -921,9 +912,11 @@ nsc_status run_mma(const Params& p, const Split& s, unsigned blocks, cudaStream_
 template <typename T, typename A>
 nsc_status run_any(const Params& p, const Split& s, unsigned blocks, cudaStream_t st) {
     const size_t smem = AnyShape<T, A>::smem(p.D);
-    cudaFuncSetAttribute(decode_any_kernel<T, A>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(smem));
-    decode_any_kernel<T, A><<<blocks, kThreads, smem, st>>>(p, s);
+    auto kern = decode_any_kernel<T, A>;
+    const nsc_status ready =
+        raise_shared("token_attention_decode", reinterpret_cast<const void*>(kern), smem);
+    if (ready != NSC_OK) return ready;
+    kern<<<blocks, kThreads, smem, st>>>(p, s);
     return check_launch("token_attention_decode");
 }
 

@@ -677,10 +677,10 @@ nsc_status run(const nsc_norm_rotate* n, const Out* o, const Grad* g, int* n_par
         n_part[1] = static_cast<int>(2 * blocks);
     }
     const size_t smem = g ? sizeof(A) * warps * 3 * a.D : 0;
-    if (smem > 48 * 1024)
-        cudaFuncSetAttribute(any_kernel<T, A>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-    any_kernel<T, A><<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(
+    auto kern = any_kernel<T, A>;
+    const nsc_status ready = raise_shared("qk_norm_rotate", reinterpret_cast<const void*>(kern), smem);
+    if (ready != NSC_OK) return ready;
+    kern<<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(
         a, o ? *o : Out{}, g ? *g : Grad{}, g ? 1 : 0);
     return check_launch("qk_norm_rotate");
 }

@@ -3,6 +3,7 @@ and values near the ends of their type."""
 
 import importlib
 import math
+import threading
 
 import pytest
 import torch
@@ -281,3 +282,52 @@ def test_small_caps(cuda, dt, D, cap, L):
         assert torch.isfinite(g).all()
     n = torch.tensor([L], dtype=torch.int32, device=cuda)
     check(nsc.token_attention_decode(q[:, -1:], k, v, n, softcap=cap), want[0][:, -1:], dt)
+
+
+@pytest.mark.parametrize("form,dt,D,less", [
+    ("attention", F32, 96, 96), ("attention", F64, 64, 64), ("attention", BF16, 64, 64),
+    ("decode", BF16, 72, 72), ("decode", F32, 130, 70), ("rotation", F64, 502, 300)])
+def test_two_threads(cuda, form, dt, D, less):
+    """Calls of one kernel that need more and less shared memory, from two threads."""
+    def packed(width, bias):
+        """The arguments of a small call, and what keeps them alive."""
+        q = randn(0, 1, 3, 2, width, dtype=dt).to(cuda)
+        out, dk = torch.empty_like(q), torch.empty_like(q)
+        m = torch.zeros(2049, dtype=torch.int32, device=cuda)
+        table = randn(1, 256, 2, dtype=dt).to(cuda)
+        n = torch.tensor([3], dtype=torch.int32, device=cuda)
+        if form == "rotation":
+            angle = torch.zeros(3, width // 2, dtype=dt, device=cuda)
+            a = A._rotate_args(q, q, None, None, angle, angle, None, 0, 1e-6)
+            tail = (q, q, out, dk, None, None, None)
+        else:
+            a = A._attention_args(q, q, q, None, None, n if form == "decode" else None,
+                                  table if bias else None, m if bias else None, 1.0, 0.0, 1)
+            tail = (out, None, None, None) if form == "attention" else (out, None, None)
+        return (a, *(A._addr(t) for t in tail)), (q, out, dk, m, table, n, a, tail)
+
+    name = {"attention": "nsc_token_attention_fwd", "decode": "nsc_token_attention_decode",
+            "rotation": "nsc_qk_norm_rotate_bwd"}[form]
+    # (fewer channels, or no bias)
+    calls = [packed(D, True), packed(less, False)]
+    errors = []
+
+    def work(args):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            try:
+                for i in range(4000):
+                    _lib.launch(cuda_device, name, *args)
+                    if i % 500 == 499:
+                        torch.cuda.current_stream().synchronize()
+            except RuntimeError as e:
+                errors.append(e)
+
+    cuda_device = calls[0][1][0].device
+    for _ in range(3):
+        ts = [threading.Thread(target=work, args=(c[0],)) for c in calls]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[0]
