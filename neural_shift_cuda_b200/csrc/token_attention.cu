@@ -154,6 +154,8 @@ extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
     gr.dq = g->grad_q;
     gr.dk = g->grad_k;
     gr.dv = g->grad_v;
+    if (!a->B)   // no rows and no keys; a table's gradient is a sum of nothing
+        return g->grad_table ? launch_table_join(p, gr, g->grad_table, s) : ok();
     if (tc_bwd_fits(p, gr, a->dtype))
         return tc_bwd(p, gr, g->workspace, g->grad_table, a->dtype, s);
     gr.delta = g->workspace;

@@ -331,3 +331,19 @@ def test_two_threads(cuda, form, dt, D, less):
             t.join()
     torch.cuda.synchronize()
     assert not errors, errors[0]
+
+
+@pytest.mark.parametrize("dt", [F16, BF16, F32, F64])
+@pytest.mark.parametrize("D", [32, 64])
+def test_backward_of_an_empty_batch(cuda, dt, D):
+    """Empty gradients, and zeros for the table."""
+    m = nsc.relative_buckets(8, 20, device=cuda)
+    for table in (None, torch.ones(8, 2, dtype=dt, device=cuda)):
+        x = [torch.zeros(0, 70, 2, D, dtype=dt, device=cuda).requires_grad_() for _ in range(3)]
+        t = leaf(table)
+        out = nsc.token_attention(*x, bias_table=t, bias_buckets=None if t is None else m)
+        got = torch.autograd.grad(out, x + ([t] if t is not None else []), torch.zeros_like(out))
+        for g, w in zip(got, x):
+            assert g.shape == w.shape
+        if t is not None:
+            assert (got[3] == 0).all()
