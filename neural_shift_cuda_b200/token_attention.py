@@ -127,6 +127,8 @@ def _int32(op: str, name: str, t: torch.Tensor, device) -> torch.Tensor:
         raise TypeError(f"{op}: {name} must be an int32 or int64 tensor")
     if t.device != device:
         raise ValueError(f"{op}: {name} is on {t.device}, q on {device}")
+    if t.dtype == torch.int64:   # (a wrapped position would be another one)
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 
 

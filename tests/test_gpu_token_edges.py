@@ -347,3 +347,25 @@ def test_backward_of_an_empty_batch(cuda, dt, D):
             assert g.shape == w.shape
         if t is not None:
             assert (got[3] == 0).all()
+
+
+def test_whole_numbers_past_32_bits(cuda):
+    """int64 positions, lengths, bounds and prefixes are far away, not wrapped around."""
+    big = 2 ** 32
+    x = randn(0, 1, 3, 2, 64, dtype=BF16).to(cuda)
+    angle = torch.linspace(0, 3, 8 * 32, device=cuda).view(8, 32)
+    q, _ = nsc.qk_norm_rotate(x, x, None, None, angle.cos(), angle.sin(),
+                              positions=torch.tensor([[0, big + 1, -big + 2]], device=cuda))
+    assert torch.isfinite(q[:, 0]).all() and q[:, 1:].isnan().all()
+    q, k, v = (randn(i, 1, 90, 2, 64, dtype=BF16).to(cuda) for i in range(3))
+    for far in (big + 5, -big + 5):
+        near = max(-2 ** 31, min(far, 2 ** 31 - 1))
+        a = [nsc.token_attention_decode(q[:, :1], k, v, torch.tensor([n], device=cuda))
+             for n in (far, near)]
+        assert torch.equal(*a)
+        a = [nsc.token_attention(q, k, v, documents=torch.tensor(sorted([7, n]), device=cuda))
+             for n in (far, near)]
+        assert torch.equal(*a)
+        a = [nsc.token_attention(q, k, v, causal=True, prefix=torch.tensor([n], device=cuda))
+             for n in (far, near)]
+        assert torch.equal(*a)
