@@ -964,7 +964,8 @@ nsc_status decode(const Params& p, void* workspace, int dtype, cudaStream_t st) 
     if (s.n_chunk > 1 && !workspace)
         return fail(NSC_ERR_INVALID_ARG, "token_attention_decode: NULL pointer");
     const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * s.groups * s.n_chunk;
-    if (blocks >= (1LL << 31))
+    // (the join has a block a row)
+    if (blocks >= (1LL << 31) || static_cast<int64_t>(p.B) * p.Hq * p.Lq >= (1LL << 31))
         return fail(NSC_ERR_INVALID_ARG, "token_attention_decode: too many tokens");
     const unsigned nb = static_cast<unsigned>(blocks);
     nsc_status r;

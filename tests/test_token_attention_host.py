@@ -157,6 +157,14 @@ def test_caps_that_32_bits_do_not_hold_are_refused(cap):
     assert lib.nsc_token_attention_bwd_workspace(ctypes.byref(a)) == -1
 
 
+def test_decode_of_more_rows_than_a_grid_has_is_refused():
+    lib = _lib.load()
+    a = _att(B=4096, Hq=16, Hkv=16, Lq=1 << 15, Lk=4096, D=8, dtype=0, causal=1,
+             q=256, k=256, v=256)
+    assert lib.nsc_token_attention_decode(ctypes.byref(a), 256, None, 256, None) == 1
+    assert "too many" in lib.nsc_last_error_string().decode()
+
+
 def test_workspaces_that_are_not_aligned_are_refused():
     lib = _lib.load()
     a = _att(causal=1, q=256, k=256, v=256)
