@@ -26,11 +26,11 @@ template <typename A> struct Pair { A p, dz, ds; };
 
 template <typename A>
 __device__ __forceinline__ Pair<A> pair_grad(A dot, A dp, A bias, A m, A ll, A delta, bool seen,
-                                             A scale, A unit, A y1) {
+                                             A scale, A unit, bool capped, A y1) {
     Pair<A> r{0, 0, 0};
     if (!seen || m == ninf<A>()) return r;
     A x = dot, slope = scale;
-    if (y1 != A(0)) {
+    if (capped) {
         x = tanh_(dot * y1);
         slope = scale * (1 - x * x);
     }
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kGenThreads) void general_dq_kernel(Params p, Grads
                 const int key = k0 + tx + 16 * j;
                 const A bi = p.table ? bias[distance_at(p, key - (q0 + ty + 16 * i + off))] : A(0);
                 const Pair<A> r = pair_grad<A>(s[i][j], dp[i][j], bi, m[i], ll[i], delta[i],
-                                               key >= lo[i] && key < hi[i], scale, unit, y1);
+                                               key >= lo[i] && key < hi[i], scale, unit, p.cap > 0, y1);
                 s[i][j] = r.ds;
                 Ps[(ty + 16 * i) * G::LP + tx + 16 * j] = gr.tab ? r.dz : r.ds;
             }
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kGenThreads) void general_dkv_kernel(Params p, Grad
                     const int r = ty + 16 * i, c = tx + 16 * j, row = q0 + r;
                     const A bi = p.table ? bias[distance_at(p, k0 + c - (row + off))] : A(0);
                     const Pair<A> g = pair_grad<A>(s[i][j], dp[i][j], bi, ms[r], lls[r], deltas[r],
-                                                   row >= lo[j] && row < hi[j], scale, unit, y1);
+                                                   row >= lo[j] && row < hi[j], scale, unit, p.cap > 0, y1);
                     Ps[c * G::LP + r] = g.p;
                     Ss[c * G::LP + r] = g.ds;
                 }

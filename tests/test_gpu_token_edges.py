@@ -369,3 +369,21 @@ def test_whole_numbers_past_32_bits(cuda):
         a = [nsc.token_attention(q, k, v, causal=True, prefix=torch.tensor([n], device=cuda))
              for n in (far, near)]
         assert torch.equal(*a)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F32, 64), (F64, 32)])
+@pytest.mark.parametrize("scale", [0.0, -0.25])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_scales_of_zero_and_below(cuda, dt, D, scale, cap):
+    """A scale of zero leaves the bias alone, with a cap or without."""
+    q, k, v, go = (randn(i, 2, 90, 2, D, dtype=dt).to(cuda) for i in range(4))
+    m = nsc.relative_buckets(16, 40, device=cuda)
+    table = randn(5, 16, 2, dtype=dt).to(cuda)
+    want = reference(q, k, v, T.visible(2, 90, 90, True), go, scale, cap, table, m)
+    leaves = [leaf(t) for t in (q, k, v, table)]
+    out = nsc.token_attention(*leaves[:3], scale=scale, softcap=cap, causal=True,
+                              bias_table=leaves[3], bias_buckets=m)
+    check(out, want[0], dt, "out")
+    for name, g, w in zip(("grad_q", "grad_k", "grad_v", "grad_table"),
+                          torch.autograd.grad(out, leaves, go), want[2:]):
+        check(g, w, dt, name)
