@@ -382,7 +382,8 @@ NSC_API nsc_status nsc_qk_norm_rotate_bwd(const nsc_norm_rotate* a,
  * makes the backward's row sums exact to fp32 (NULL: not wanted).
  * Backward: grad_out in the dtype and shape of out (its own strides), grad_lse (B, Hq, Lq) or
  * NULL; grad_q, grad_k, grad_v contiguous in the dtype of q; grad_table
- * (n_buckets, Hq) in table_dtype, or NULL.  No atomics: the same inputs give the
+ * (n_buckets, Hq) in table_dtype, or NULL; also NULL where not wanted: grad_q without
+ * grad_table, or grad_k and grad_v.  No atomics: the same inputs give the
  * same bits.  `workspace`: nsc_token_attention_bwd_workspace(a) bytes, 256-byte aligned.
  * ------------------------------------------------------------------- */
 typedef struct nsc_attention {

@@ -137,8 +137,10 @@ extern "C" NSC_API nsc_status nsc_token_attention_bwd(const nsc_attention* a,
     if (a->lengths)
         return fail(NSC_ERR_INVALID_ARG, "%s: lengths belong to the decode form", op);
     const bool rows = a->B && a->Lq, cols = a->B && a->Lk;
-    if ((rows && (!g->out || !g->stats || !g->grad_out || !g->grad_q || !g->workspace)) ||
-        (cols && (!g->grad_k || !g->grad_v)) || (g->grad_table && !a->table))
+    // grad_q comes with grad_table, grad_k with grad_v; a pair that is not wanted is left out
+    if ((rows && (!g->out || !g->stats || !g->grad_out || !g->workspace ||
+                  (g->grad_table && !g->grad_q))) ||
+        (cols && !g->grad_k != !g->grad_v) || (g->grad_table && !a->table))
         return fail(NSC_ERR_INVALID_ARG, "%s: NULL pointer", op);
     if (!aligned256(g->workspace))
         return fail(NSC_ERR_INVALID_ARG, "%s: workspace is not 256-byte aligned", op);

@@ -399,8 +399,8 @@ nsc_status launch(const Params& p, const Grads& g, cudaStream_t st) {
     };
     const int nqt = (p.Lq + TL - 1) / TL, nkt = (p.Lk + TL - 1) / TL;
     const int sk = share_of(nk, static_cast<int64_t>(p.G) * nqt), sq = share_of(nq, nkt);
-    if (nk) r = launch_cluster(op, kk, nk * sk, kGenThreads, smk, sk, st, p, g, sk);
-    if (r == NSC_OK && nq) r = launch_cluster(op, kq, nq * sq, kGenThreads, smq, sq, st, p, g, sq);
+    if (nk && g.dk) r = launch_cluster(op, kk, nk * sk, kGenThreads, smk, sk, st, p, g, sk);
+    if (r == NSC_OK && nq && g.dq) r = launch_cluster(op, kq, nq * sq, kGenThreads, smq, sq, st, p, g, sq);
     if (r != NSC_OK) return r;
     return check_launch("token_attention backward");
 }

@@ -933,9 +933,10 @@ nsc_status tc_bwd_launch(const Params& p, const Grads& g, const RowRec* recs, cu
         if (p.G % i == 0) split = i;
     const int64_t nk = tiles * split;
     const int64_t nq = static_cast<int64_t>((p.Lq + kRows - 1) / kRows) * p.B * p.Hq;
-    ready = launch_cluster("token_attention backward", kk, nk, kBwdThreads, smk, split, st, mq, mo, mk,
+    if (g.dk)
+        ready = launch_cluster("token_attention backward", kk, nk, kBwdThreads, smk, split, st, mq, mo, mk,
                            mv, p, g, recs, split, bnd);
-    if (ready != NSC_OK) return ready;
+    if (ready != NSC_OK || !g.dq) return ready;
     kq<<<static_cast<unsigned>(nq), kBwdThreads, smq, st>>>(mq, mo, mk, mv, p, g, recs, bnd);
     return check_launch("token_attention backward");
 }

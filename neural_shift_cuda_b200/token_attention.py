@@ -144,13 +144,14 @@ def _addr(t: Optional[torch.Tensor]) -> int:
 # qk_norm_rotate
 # ---------------------------------------------------------------------------
 
-def _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps):
+def _rotate_args(q, k, wq, wk, cos, sin, positions, adjacent, eps, *, with_q=True,
+                 with_k=True):
     B, L, Hq, D = q.shape
     rows, half = cos.shape
     w = wq if wq is not None else wk
     code = _lib.dtype_code(q.dtype)
     return _lib.pack_norm_rotate(
-        B, L, Hq, k.shape[2], D, 2 * half, rows, *q.stride()[:3], *k.stride()[:3],
+        B, L, Hq * with_q, k.shape[2] * with_k, D, 2 * half, rows, *q.stride()[:3], *k.stride()[:3],
         q.data_ptr(), k.data_ptr(), _addr(wq), _addr(wk), cos.data_ptr(),
         sin.data_ptr(), _addr(positions), code,
         code if w is None else _lib.dtype_code(w.dtype), adjacent, eps)
@@ -175,16 +176,20 @@ class _RotateFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        a = _rotate_args(q, k, wq, wk, cos, sin, positions, ctx.adjacent, ctx.eps)
-        gq, gk = _aligned(gq), _aligned(gk)
-        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-        dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
-        dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
+        need = ctx.needs_input_grad
+        dwq = torch.empty_like(wq) if wq is not None and need[2] else None
+        dwk = torch.empty_like(wk) if wk is not None and need[3] else None
+        # (a side that is not wanted is one of no heads)
+        with_q, with_k = need[0] or dwq is not None, need[1] or dwk is not None
+        dq, gq = (q.new_empty(q.shape), _aligned(gq)) if with_q else (None, None)
+        dk, gk = (k.new_empty(k.shape), _aligned(gk)) if with_k else (None, None)
+        a = _rotate_args(q, k, wq, wk, cos, sin, positions, ctx.adjacent, ctx.eps,
+                         with_q=with_q, with_k=with_k)
         ws = None
         if dwq is not None or dwk is not None:
             ws = _lib.workspace("nsc_qk_norm_rotate_workspace", q.device, a)
-        _lib.launch(q.device, "nsc_qk_norm_rotate_bwd", a, gq.data_ptr(), gk.data_ptr(),
-                    dq.data_ptr(), dk.data_ptr(), _addr(dwq), _addr(dwk), _addr(ws))
+        _lib.launch(q.device, "nsc_qk_norm_rotate_bwd", a, _addr(gq), _addr(gk),
+                    _addr(dq), _addr(dk), _addr(dwq), _addr(dwk), _addr(ws))
         return dq, dk, dwq, dwk, None, None, None, None, None
 
 
@@ -342,15 +347,18 @@ class _AttentionFn(torch.autograd.Function):
         grad_out = torch.zeros_like(out) if grad_out is None else _tiled(grad_out)
         if grad_lse is not None:
             grad_lse = grad_lse.contiguous()
-        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-        dv = v.new_empty(v.shape)
-        dt = (torch.empty_like(table) if table is not None and ctx.needs_input_grad[5]
-              else None)
+        # the kernels give dq with the table's gradient, and dk with dv
+        need = ctx.needs_input_grad
+        dt = torch.empty_like(table) if table is not None and need[5] else None
+        dq = q.new_empty(q.shape) if need[0] or dt is not None else None
+        dk = dv = None
+        if need[1] or need[2]:
+            dk, dv = k.new_empty(k.shape), v.new_empty(v.shape)
         ws = _lib.workspace("nsc_token_attention_bwd_workspace", q.device, a)
         g = _lib.pack_attention_grad(
             *grad_out.stride()[:3], out.data_ptr(), stats.data_ptr(), _addr(residue),
-            grad_out.data_ptr(), _addr(grad_lse), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), _addr(dt), _addr(ws))
+            grad_out.data_ptr(), _addr(grad_lse), _addr(dq), _addr(dk), _addr(dv),
+            _addr(dt), _addr(ws))
         _lib.launch(q.device, "nsc_token_attention_bwd", a, g)
         return dq, dk, dv, None, None, dt, None, None, None, None, None
 

@@ -387,3 +387,57 @@ def test_scales_of_zero_and_below(cuda, dt, D, scale, cap):
     for name, g, w in zip(("grad_q", "grad_k", "grad_v", "grad_table"),
                           torch.autograd.grad(out, leaves, go), want[2:]):
         check(g, w, dt, name)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 128), (F32, 64)])
+@pytest.mark.parametrize("wanted", ["q", "k", "v", "kv", "t", "qv", "qkv"])
+def test_gradients_that_are_not_wanted(cuda, dt, D, wanted, monkeypatch):
+    """Frozen inputs cost no kernel, and leave the others' gradients as they are."""
+    q, k, v, go = (randn(i, 1, 300, 2, D, dtype=dt).to(cuda) for i in range(4))
+    m = nsc.relative_buckets(16, 40, device=cuda)
+    ins = dict(q=q, k=k, v=v, t=randn(5, 16, 2, dtype=dt).to(cuda))
+
+    def run(names):
+        x = {n: leaf(t) if n in names else t for n, t in ins.items()}
+        out = nsc.token_attention(x["q"], x["k"], x["v"], causal=True, bias_table=x["t"],
+                                  bias_buckets=m)
+        return dict(zip(names, torch.autograd.grad(out, [x[n] for n in names], go)))
+
+    want = run("qkvt")
+    outputs = []
+    pack = _lib.pack_attention_grad
+    monkeypatch.setattr(_lib, "pack_attention_grad",
+                        lambda *a: outputs.append(a[-5:-1]) or pack(*a))
+    got = run(wanted)
+    for n in wanted:
+        assert torch.equal(got[n], want[n])
+    dq, dk, dv, dt_ = (bool(x) for x in outputs[0])
+    assert dt_ == ("t" in wanted) and dq == ("q" in wanted or dt_)
+    assert dk == dv == ("k" in wanted or "v" in wanted)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (BF16, 40), (F64, 32)])
+@pytest.mark.parametrize("wanted", [("q",), ("k",), ("wq",), ("wk",), ("q", "wk"), ("k", "wk")])
+def test_rotation_gradients_that_are_not_wanted(cuda, dt, D, wanted, monkeypatch):
+    ins = dict(q=randn(0, 2, 9, 4, D, dtype=dt).to(cuda), k=randn(1, 2, 9, 2, D, dtype=dt).to(cuda),
+               wq=randn(2, D, dtype=dt).to(cuda), wk=randn(3, D, dtype=dt).to(cuda))
+    angle = torch.linspace(0, 3, 9 * D // 2, device=cuda).view(9, D // 2)
+    go = [randn(4, 2, 9, 4, D, dtype=dt).to(cuda), randn(5, 2, 9, 2, D, dtype=dt).to(cuda)]
+
+    def run(names):
+        x = {n: leaf(t) if n in names else t for n, t in ins.items()}
+        out = nsc.qk_norm_rotate(*x.values(), angle.cos(), angle.sin())
+        use = [i for i in (0, 1) if out[i].requires_grad]
+        return dict(zip(names, torch.autograd.grad([out[i] for i in use], [x[n] for n in names],
+                                                   [go[i] for i in use])))
+
+    want = run(("q", "k", "wq", "wk"))
+    outputs = []
+    launch = _lib.launch
+    monkeypatch.setattr(_lib, "launch", lambda *a: outputs.append(a) or launch(*a))
+    got = run(wanted)
+    for n in wanted:
+        # (a weight's sum is over the blocks that its side has, which are more on its own)
+        check(got[n], want[n], dt, n)
+    dq, dk = (bool(x) for x in outputs[-1][5:7])
+    assert dq == ("q" in wanted or "wq" in wanted) and dk == ("k" in wanted or "wk" in wanted)
