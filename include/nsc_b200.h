@@ -372,7 +372,10 @@ NSC_API nsc_status nsc_qk_norm_rotate_bwd(const nsc_norm_rotate* a,
  * those j <= pos or j < start + prefix (start: that of the document; prefix:
  * (B, docs) int32, or (B, 1) without documents, prefix_stride apart).  A query that sees nothing, or only scores
  * of -inf, gives out = 0 and lse = -inf.  What is not visible is not part of
- * any sum, whatever it holds.
+ * any sum, whatever it holds.  A visible value that is not finite makes its channel
+ * of out so, or, with 16-bit types and where not all queries nearby see its key, all
+ * of the query's out and lse NaN.  lse of 16-bit capped scores is good to 3e-6
+ * (bf16) or 3e-7 (fp16) of the cap, or 5e-5 of itself if that is less.
  * table: (n_buckets, Hq) contiguous in table_dtype (that of q, or fp32 with
  * fp16 / bf16), buckets: 2 reach + 1 int32 (values outside [0, n_buckets) are
  * taken as the nearest).  n_buckets <= 256, reach <= 1024.

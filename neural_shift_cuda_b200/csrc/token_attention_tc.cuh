@@ -135,11 +135,13 @@ __device__ __forceinline__ void fence_async_shared() {
 // The cap, f tanh(y1 s) of 32 products s, in place.  Up to |y| = 1, tanh y is an odd
 // polynomial y P(y^2), P of least maximum error of y P(y^2) against tanh y by
 // exchange: 2.4e-7 with six terms (fp16), 2.8e-6 with five (bf16: at a cap of 50,
-// 1.4e-4 of a softmax weight that is rounded to 4e-3).  Up to |y| = 0.45, where most
-// scores of a layer lie, two terms less do as well (9e-8 and 2.7e-6; 32 heads
-// of 128, 4096 causal tokens 192 -> 179 us).  It runs on the FMA pipe,
-// beside the exponentials that bound these kernels, in pairs, with y1 and f in the
-// coefficients; the hardware's tanh would be one more exponential's time, with 5e-4 of
+// 1.4e-4 of a softmax weight that is rounded to 4e-3).  Under caps in the thousands, of
+// which scores are a small part, that is 4.2e-5 of each score (its slope at zero is short by
+// it): lse is off by as much of itself, weights by as much of a difference of two scores.
+// Up to |y| = 0.45, where most scores of a layer lie, two terms less do as well (9e-8 and
+// 2.7e-6; 32 heads of 128, 4096 causal tokens 192 -> 179 us in short runs, 205 -> 193 under
+// sustained load).  It runs on the FMA pipe, beside the exponentials, in pairs, with y1 and
+// f in the coefficients; the hardware's tanh would be one more exponential's time, with 5e-4 of
 // error.  A warp with a larger |y| in the chunk takes tanh |y| = 1 - 2 / (1 + e^(2|y|)).
 template <typename T> struct Cap {
     static constexpr int N = std::is_same<T, __half>::value ? 6 : 5;

@@ -26,9 +26,9 @@
 // Bounded by the arithmetic between the products: 16384 scores a tile on 128 lanes, some
 // 20 instructions each (30 with a cap), against 20 D clocks (dkv) and 16 D (dq) of the
 // tensor pipe, of which only part runs beside it; a block's set-up and end are some 6 us
-// of 35.  4 x 2048 tokens, 16 heads of 64, bias table, bf16: dkv 243 us, dq 262 us (4 and 3
-// products of 34 GF: 566 and 393 TF/s).  8192 tokens in 4 documents, causal, capped,
-// 16 / 4 heads of 128: dkv 358 us, dq 269 us.
+// of 35.  4 x 2048 tokens, 16 heads of 64, bias table, bf16: dkv 246 us, dq 252 us (4 and 3
+// products of 34 GF: 559 and 409 TF/s).  8192 tokens in 4 documents, causal, capped,
+// 16 / 4 heads of 128: dkv 381 us, dq 268 us.
 //
 // fp16: weights and score gradients of long rows lie below its normal range, and those of
 // large values or large gradients of lse above it.  P is held times 2^6, and P (dP - delta)

@@ -929,7 +929,8 @@ nsc_status run_f32(const Params& p, const Split& s, unsigned blocks, cudaStream_
     return check_launch("token_attention_decode");
 }
 
-// The join's blocks come up while the last chunks are still at work and wait for them.
+// The join is launched before the chunks are done and its blocks start as the last of theirs
+// ends (none triggers it earlier): what is hidden is the launch's latency.
 template <typename T, typename A>
 nsc_status launch_join(const Params& p, const Split& s, cudaStream_t st) {
     cudaLaunchAttribute at{};

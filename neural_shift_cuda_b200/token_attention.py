@@ -408,8 +408,8 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     out (B, Lq, Hq, D), or (out, lse (B, Hq, Lq) fp32).
 
     Query head h reads key head h Hkv // Hq; query i stands at key position
-    i + Lk - Lq.  scale defaults to D^-0.5; softcap c turns a score s into
-    c tanh(s / c); then bias_table[bias_buckets[distance], h] is added
+    i + Lk - Lq.  scale defaults to D^-0.5; softcap c (1e-30 to 1e30; 0 or None: none)
+    turns a score s into c tanh(s / c); then bias_table[bias_buckets[distance], h] is added
     (`relative_buckets`; distances past the map's ends take the ends').
 
     causal: a query sees keys up to its own position.  prefix (an int, or an
@@ -420,7 +420,9 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     influence on it, even where it is not finite.
 
     Differentiable in q, k, v and bias_table, through out and lse; the
-    gradients are summed in a fixed order."""
+    gradients are summed in a fixed order.  What the backward keeps beside the inputs:
+    out, two numbers a row, and with fp16 / bf16 what rounding dropped of out, a second
+    tensor of its size."""
     op = "token_attention"
     _check_qkv(op, q, k, v)
     B, Lq, Lk, dev = q.shape[0], q.shape[1], k.shape[1], q.device

@@ -441,3 +441,22 @@ def test_rotation_gradients_that_are_not_wanted(cuda, dt, D, wanted, monkeypatch
         check(got[n], want[n], dt, n)
     dq, dk = (bool(x) for x in outputs[-1][5:7])
     assert dq == ("q" in wanted or "wq" in wanted) and dk == ("k" in wanted or "wk" in wanted)
+
+
+@pytest.mark.parametrize("dt,D", [(F16, 64), (BF16, 64), (BF16, 128)])
+@pytest.mark.parametrize("cap", [200.0, 500.0, 1e3, 1e4, 1e6, 1e30])
+@pytest.mark.parametrize("mul", [2.0, 8.0])
+def test_large_caps_tiles(cuda, dt, D, cap, mul):
+    """Scores far below the cap.  The polynomial's slope at zero is short by 4.2e-5 (bf16),
+    and lse, the largest score and little more, by as much: 16 times the usual bound of
+    3.8e-6 leaves half as much again."""
+    q, k, v, go = (randn(i, 1, 300, 2, D, dtype=dt, mul=mul if i < 2 else 1.0).to(cuda)
+                   for i in range(4))
+    want = reference(q, k, v, T.visible(1, 300, 300, True), go, D ** -0.5, cap)
+    leaves = [leaf(t) for t in (q, k, v)]
+    out, lse = nsc.token_attention(*leaves, causal=True, softcap=cap, return_lse=True)
+    check(out, want[0], dt, "out")
+    check(lse, want[1], F32, "lse", 16.0)
+    for name, g, w in zip(("grad_q", "grad_k", "grad_v"),
+                          torch.autograd.grad(out, leaves, go), want[2:5]):
+        check(g, w, dt, name)
